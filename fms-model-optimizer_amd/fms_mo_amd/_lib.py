@@ -25,10 +25,26 @@ F8E_SAT, F8E_PER_TENSOR, F8E_PER_ROW = 0, 1, 2
 FP8_LINEAR, FP8_FPXACC, FP8_FPXACC_DL8 = 0, 1, 2
 WQ_MUL, WQ_DIV = 0, 1
 MS_PER_TOKEN, MS_SYMM, MS_ASYMM = 0, 1, 2
+KV_E4M3 = 16
 ABI_VERSION = 2
 PLAN_DECODE, PLAN_TILE_REGISTER_STAGED, PLAN_TILE_LDS_DMA, PLAN_GENERIC = 0, 1, 2, 3
 
 _P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
+
+
+class KvCache(ctypes.Structure):
+    """fmsmo_kv_cache_t"""
+
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("k_strides", _L * 3), ("v_strides", _L * 3),
+                ("k_scale_strides", _L * 2), ("v_scale_strides", _L * 2), ("pages", _L), ("page_size", _I), ("heads", _I),
+                ("dim", _I), ("dtype", _I)]
+
+
+class KvBatch(ctypes.Structure):
+    """fmsmo_kv_batch_t"""
+
+    _fields_ = [("block_table", _P), ("table_stride", _L), ("table_width", _L), ("seq_lens", _P), ("query_start", _P), ("seqs", _L)]
+
 
 # name -> argument types (all functions return int except the three below)
 SIGNATURES = {
@@ -89,6 +105,8 @@ SIGNATURES = {
     "fmsmo_bmm_qa_i8": [_P, _I, _L, _L, _F, _F, _I, _P, _L, _L, _F, _P, _I, _P, _L, _L, _L, _L, _L, _P],
     "fmsmo_bmm_i8_dq": [_P, _L, _P, _L, _L, _P, _P, _P, _P, _I, _L, _L, _L, _L, _L, _P],
     "fmsmo_bmm_fp8_dq": [_P, _L, _P, _L, _L, _P, _P, _P, _P, _I, _L, _L, _L, _L, _L, _P],
+    "fmsmo_kv_store": [_P, _P, _I, _L, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _F, _P, _P, _L, _I, _I, _I, _P],
+    "fmsmo_paged_attn": [_P, _P, _I, _L, _I, _P, _L, _L, _P, _L, _L, _F, _L, _L, _L, _L, _I, _P, _L, _P],
     "fmsmo_zero_shift_bias": [_P, _L, _P, _L, _P, _F, _P, _I, _P, _L, _L, _P],
     "fmsmo_debug_clock_probe": [_P],
     "fmsmo_debug_stream_read": [_P, _L, _P, _P],
@@ -108,6 +126,7 @@ OTHER = {
     "fmsmo_gemm_workspace_bytes": ([c_int64, c_int64, c_int64], c_int64),
     "fmsmo_gemm_fp8_workspace_bytes": ([c_int64, c_int64, c_int64], c_int64),
     "fmsmo_matmul_chunk_workspace_bytes": ([c_int, c_int64, c_int64, c_int64, c_int, c_int], c_int64),
+    "fmsmo_paged_attn_workspace_bytes": ([c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64], c_int64),
     "fmsmo_decode_linear_ok": ([c_int64, c_int64], c_int),
     "fmsmo_decode_linear_f32s_ok": ([c_int64, c_int64], c_int),
     "fmsmo_small_linear_static_ok": ([c_int64, c_int64, c_int64, _F, _F, _F, _F], c_int),

@@ -3,6 +3,8 @@ torch's caching allocator, the current HIP stream of the tensors' device.  No ar
 here; torch is only the owner of device memory and streams."""
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib as L
@@ -1119,3 +1121,231 @@ def decode_linear_fp8(x, w, w_scale, bias=None, out_dtype=torch.bfloat16):
     if _eager(x, w, bias) and (not torch.is_tensor(w_scale) or _eager(w_scale)):
         return _decode_linear_fp8_impl(x, w, w_scale, bias, out_dtype)
     return torch.ops.fms_mo_amd.decode_linear_fp8(x, w, _as_scale(w_scale, x.device), bias, out_dtype)
+
+
+# ------------------------------------------------------------------ paged key-value cache
+def _strides(t, dims):
+    """Strides of the first `dims` dimensions; 0 where a dimension of one element leaves them open."""
+    return [0 if t.shape[i] == 1 else t.stride(i) for i in range(dims)]
+
+
+def _paged_cache(k_cache, v_cache, k_scale, v_scale):
+    """Checks a cache; the structure the entry points take."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [pages, kv heads, page size, head dim], got {tuple(t.shape)}")
+        if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * t.element_size() % 16 for s in _strides(t, 3)):
+            raise ValueError(f"every key of {name} must be contiguous and 16-byte aligned")
+    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError("k_cache and v_cache must have one shape and dtype")
+    pages, heads, size, dim = k_cache.shape
+    if dim not in (64, 128, 256):
+        raise ValueError(f"head dim must be 64, 128 or 256, got {dim}")
+    if size < 16 or size > 65536 or size & (size - 1):
+        raise ValueError(f"page size must be a power of two from 16 to 65536, got {size}")
+    if pages < 1 or heads < 1:
+        raise ValueError("a cache has at least one page and one head")
+    e4m3 = k_cache.dtype == torch.float8_e4m3fn
+    if not e4m3 and k_cache.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported cache dtype {k_cache.dtype}")
+    if (k_scale is None) == e4m3 or (v_scale is None) == e4m3:
+        raise ValueError("an e4m3 cache takes k_scale and v_scale, any other none")
+    c = L.KvCache(k=k_cache.data_ptr(), v=v_cache.data_ptr(), k_scale=_ptr(k_scale), v_scale=_ptr(v_scale), pages=pages, page_size=size,
+                  heads=heads, dim=dim, dtype=L.KV_E4M3 if e4m3 else _DT[k_cache.dtype])
+    c.k_strides[:] = _strides(k_cache, 3)
+    c.v_strides[:] = _strides(v_cache, 3)
+    if e4m3:
+        for name, t, to in (("k_scale", k_scale, c.k_scale_strides), ("v_scale", v_scale, c.v_scale_strides)):
+            if t.dtype != torch.float32 or t.shape != (pages, heads, size):
+                raise ValueError(f"{name} must be float32 [pages, kv heads, page size]")
+            to[:] = _strides(t, 2)
+            if t.stride(2) != 1 or t.data_ptr() % 16 or any(s % 4 for s in to):
+                raise ValueError(f"the scales of a page's keys in {name} must be contiguous and 16-byte aligned")
+    return c
+
+
+def _paged_batch(block_table, seq_lens, query_start, rows):
+    """Checks a batch; the structure the entry points take and what has to live until the launch."""
+    if block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.shape[0] != seq_lens.shape[0] or block_table.shape[1] < 1:
+        raise ValueError("block_table must be [sequences, pages of a sequence] and seq_lens [sequences]")
+    for name, t in (("block_table", block_table), ("seq_lens", seq_lens), ("query_start", query_start)):
+        if t is not None and t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+    seqs = seq_lens.shape[0]
+    if query_start is None:
+        if rows != seqs:
+            raise ValueError(f"without query_start every sequence has one new token: {rows} rows, {seqs} sequences")
+    else:
+        if query_start.dim() != 1 or query_start.shape[0] != seqs + 1:
+            raise ValueError("query_start must be [sequences + 1]")
+        query_start = query_start.contiguous()
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        block_table = block_table.contiguous()
+    seq_lens = seq_lens.contiguous()
+    b = L.KvBatch(block_table=block_table.data_ptr(), table_stride=_strides(block_table, 1)[0], table_width=block_table.shape[1],
+                  seq_lens=seq_lens.data_ptr(), query_start=_ptr(query_start), seqs=seqs)
+    return b, (block_table, seq_lens, query_start)
+
+
+def _same_gpu(first, *ts):
+    _need_gpu(first, *ts)
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"all tensors of a call must lie on one GPU: {first.device} and {t.device}")
+
+
+def _head_rows(t, name, rows, heads, dim, dtype):
+    """[rows, heads, dim] with contiguous, 16-byte aligned heads (copied where they are not)."""
+    if t.shape != (rows, heads, dim):
+        raise ValueError(f"{name} must be {(rows, heads, dim)}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.stride(2) != 1 or t.data_ptr() % 16 or any(s % 8 for s in _strides(t, 2)):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _paged_out(out, q):
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device), True
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"out must be {q.dtype} {tuple(q.shape)}")
+    if out.stride(2) != 1 or out.data_ptr() % 16 or any(s % 8 or (s == 0 and n > 1) for s, n in zip(_strides(out, 2), out.shape)):
+        raise ValueError("the heads of out must be contiguous, 16-byte aligned and apart")
+    return out, False
+
+
+def _qk_norm_rope_store_impl(q, k, v, k_cache, v_cache, block_table, seq_lens, query_start, cos, sin, interleaved, q_weight, k_weight,
+                             eps, k_scale, v_scale, out, zero_rest):
+    _same_gpu(q, k, v, k_cache, v_cache, block_table, seq_lens, query_start, cos, sin, q_weight, k_weight, k_scale, v_scale, out)
+    cache = _paged_cache(k_cache, v_cache, k_scale, v_scale)
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{name} is written to: its elements must not share memory")
+    rows, heads, dim = q.shape
+    if dim != cache.dim or heads % cache.heads or heads == 0:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.heads} heads of {cache.dim}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {q.dtype}")
+    if cache.dtype != L.KV_E4M3 and k_cache.dtype != q.dtype:
+        raise TypeError(f"a {k_cache.dtype} cache does not take {q.dtype}")
+    q = _head_rows(q, "q", rows, heads, dim, q.dtype)
+    k = _head_rows(k, "k", rows, cache.heads, dim, q.dtype)
+    v = _head_rows(v, "v", rows, cache.heads, dim, q.dtype)
+    batch, held = _paged_batch(block_table, seq_lens, query_start, rows)
+    rotary = table_rows = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise ValueError("cos and sin must be float32 [positions, rotary dim / 2]")
+        table_rows, rotary = cos.shape[0], 2 * cos.shape[1]
+        if rotary % 16 or rotary > dim or rotary == 0 or table_rows == 0:
+            raise ValueError(f"the rotary dim must be a multiple of 16 up to {dim}, and the tables hold a position: {tuple(cos.shape)}")
+        cos, sin = (t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 or not t.is_contiguous() else t
+                    for t in (cos, sin))
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        if w.shape != (dim,) or w.dtype not in (q.dtype, torch.float32) or w.dtype != weights[0].dtype:
+            raise ValueError(f"norm weights must be [{dim}], both {q.dtype} or both float32")
+    q_weight, k_weight = (w.clone(memory_format=torch.contiguous_format) if w is not None and (w.data_ptr() % 16 or not w.is_contiguous())
+                          else w for w in (q_weight, k_weight))
+    with _dev(q):
+        L.call("fmsmo_kv_store", ctypes.byref(cache), ctypes.byref(batch), _DT[q.dtype], rows, heads, q.data_ptr(), *_strides(q, 2),
+               k.data_ptr(), *_strides(k, 2), v.data_ptr(), *_strides(v, 2), out.data_ptr(), *_strides(out, 2), _ptr(q_weight),
+               _ptr(k_weight), _DT[weights[0].dtype] if weights else 0, float(eps), _ptr(cos), _ptr(sin), table_rows, rotary,
+               int(bool(interleaved)), int(bool(zero_rest)), _stream(q))
+    del held
+
+
+def _paged_attention_impl(q, k_cache, v_cache, block_table, seq_lens, query_start, scale, window, sinks, k_scale, v_scale, max_query_len,
+                          max_seq_len, out, zero_rest):
+    _same_gpu(q, k_cache, v_cache, block_table, seq_lens, query_start, k_scale, v_scale, out)
+    cache = _paged_cache(k_cache, v_cache, k_scale, v_scale)
+    rows, heads, dim = q.shape
+    if dim != cache.dim or heads % cache.heads or heads == 0:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.heads} heads of {cache.dim}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {q.dtype}")
+    if cache.dtype != L.KV_E4M3 and k_cache.dtype != q.dtype:
+        raise TypeError(f"queries of {q.dtype} over a {k_cache.dtype} cache")
+    q = _head_rows(q, "q", rows, heads, dim, q.dtype)
+    batch, held = _paged_batch(block_table, seq_lens, query_start, rows)
+    keys = batch.table_width * cache.page_size
+    max_rows = 1 if query_start is None else min(max_query_len or rows, rows)
+    max_keys = min(max_seq_len or keys, keys)
+    nbytes = L.load().fmsmo_paged_attn_workspace_bytes(heads, cache.heads, dim, batch.seqs, rows, max_rows, max_keys)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes > 0 else None
+    with _dev(q):
+        L.call("fmsmo_paged_attn", ctypes.byref(cache), ctypes.byref(batch), _DT[q.dtype], rows, heads, q.data_ptr(), *_strides(q, 2),
+               out.data_ptr(), *_strides(out, 2), float(scale), window, sinks, max_rows, max_keys, int(bool(zero_rest)), _ptr(ws), nbytes,
+               _stream(q))
+    del held
+
+
+_register(
+    "qk_norm_rope_store",
+    "(Tensor q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor seq_lens, Tensor? query_start, "
+    "Tensor? cos, Tensor? sin, bool interleaved, Tensor? q_weight, Tensor? k_weight, float eps, Tensor(c!)? k_scale, "
+    "Tensor(d!)? v_scale, Tensor(e!) out, bool zero_rest) -> ()",
+    lambda *a: _qk_norm_rope_store_impl(*a),
+    lambda *a: None,
+)
+_register(
+    "paged_attention",
+    "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor? query_start, float scale, int window, "
+    "int sinks, Tensor? k_scale, Tensor? v_scale, int max_query_len, int max_seq_len, Tensor(a!) out, bool zero_rest) -> ()",
+    lambda *a: _paged_attention_impl(*a),
+    lambda *a: None,
+)
+
+
+def qk_norm_rope_store(q, k, v, k_cache, v_cache, block_table, seq_lens, query_start=None, *, cos=None, sin=None, interleaved=False,
+                       q_weight=None, k_weight=None, eps=1e-6, k_scale=None, v_scale=None, out=None):
+    """New tokens of a batch of sequences, in one launch: q [T, heads, dim] and k [T, kv heads, dim] normalized per head (RMS, with
+    ``q_weight`` / ``k_weight``; None: no norm) and rotated by their positions (``cos`` / ``sin`` fp32 [positions, rotary dim / 2];
+    None: no rotation), k and v [T, kv heads, dim] written to their places in the cache, as e4m3 codes with a scale per key
+    (``k_scale`` / ``v_scale`` fp32 [pages, kv heads, page size]) where that is the cache's dtype.  Returns the rotated q: ``out``
+    (which may be q), or a new tensor, in which rows of no sequence are zero.
+
+    k_cache, v_cache [pages, kv heads, page size, dim]; block_table int32 [B, pages], seq_lens int32 [B] with the new tokens,
+    query_start int32 [B + 1] (None: one token per sequence).  See fmsmo_kv_store and fmsmo_kv_batch_t."""
+    _need_gpu(q)
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, heads, head dim]")
+    out, fresh = _paged_out(out, q)
+    if q.shape[0] == 0 or seq_lens.shape[0] == 0:
+        return out.zero_() if fresh else out
+    args = (q, k, v, k_cache, v_cache, block_table, seq_lens, query_start, cos, sin, bool(interleaved), q_weight, k_weight, float(eps),
+            k_scale, v_scale, out, fresh)
+    if _eager(*(t for t in args if torch.is_tensor(t))):
+        _qk_norm_rope_store_impl(*args)
+    else:
+        torch.ops.fms_mo_amd.qk_norm_rope_store(*args)
+    return out
+
+
+def paged_attention(q, k_cache, v_cache, block_table, seq_lens, query_start=None, *, scale=None, window=0, sinks=0, k_scale=None,
+                    v_scale=None, max_query_len=None, max_seq_len=None, out=None):
+    """Attention of new tokens q [T, heads, dim] over a paged cache that holds their keys and values already (see
+    ``qk_norm_rope_store`` for the cache and the batch): every token sees the keys up to its own, with ``window`` > 0 only the last
+    ``window`` of them and the first ``sinks``.  ``scale`` defaults to dim ** -0.5.  ``max_query_len`` / ``max_seq_len``: the longest
+    sequence's new tokens and keys, where the host knows them; the work is laid out for them (any length is right).  Returns
+    [T, heads, dim] in ``out`` or a new tensor; tokens that see nothing, and in a new tensor rows of no sequence, are zero.
+    No gradients.  See fmsmo_paged_attn."""
+    _need_gpu(q)
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, heads, head dim]")
+    window, sinks, rows, keys = int(window or 0), int(sinks or 0), int(max_query_len or 0), int(max_seq_len or 0)
+    if window < 0 or sinks < 0 or rows < 0 or keys < 0:
+        raise ValueError("window, sinks, max_query_len and max_seq_len must not be negative")
+    out, fresh = _paged_out(out, q)
+    if q.shape[0] == 0 or seq_lens.shape[0] == 0:
+        return out.zero_() if fresh else out
+    args = (q, k_cache, v_cache, block_table, seq_lens, query_start, q.shape[2] ** -0.5 if scale is None else float(scale), window, sinks,
+            k_scale, v_scale, rows, keys, out, fresh)
+    if _eager(*(t for t in args if torch.is_tensor(t))):
+        _paged_attention_impl(*args)
+    else:
+        torch.ops.fms_mo_amd.paged_attention(*args)
+    return out

@@ -826,6 +826,87 @@ int fmsmo_bmm_qa_i8(const void* x, int x_dtype, int64_t ldx, int64_t stride_x, f
                     const int32_t* sums, int parts, void* y, int64_t ldy, int64_t batch, int64_t M,
                     int64_t N, int64_t K, fmsmo_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * 8. Paged key-value cache: norm, rotation and store of new tokens, and attention over it.  The
+ *    reference's FP8 attention (fms_mo/aiu_addons/fp8/fp8_attn.py) keeps such a cache for an accelerator
+ *    that is not this one; its host kernels are the batched matmuls of section 7.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Cache type beside FMSMO_F16 and FMSMO_BF16: e4m3 codes with an fp32 scale per key and head. */
+enum { FMSMO_KV_E4M3 = 16 };
+
+/*
+ * A cache: `pages` pages of `page_size` (a power of two, 16 .. 65536) keys and values of `heads` heads of `dim`
+ * (64, 128 or 256) elements.  k and v have strides of their own, in elements, for page, head and key; the
+ * elements of a key are contiguous, every key 16-byte aligned.  A head's keys of a page should lie together (a key stride of
+ * `dim`): they are read as one piece.  dtype FMSMO_KV_E4M3: k = code * k_scale, one fp32 scale per
+ * key with strides for page and head (multiples of 4), the scales of a page's keys contiguous.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t k_scale_strides[2];
+  int64_t v_scale_strides[2];
+  int64_t pages;
+  int page_size, heads, dim, dtype;
+} fmsmo_kv_cache_t;
+
+/*
+ * A batch of `seqs` sequences, all arrays on the device.  Sequence b has the rows query_start[b] .. query_start[b + 1] - 1 of
+ * the call's rows (ascending; query_start NULL: row b alone, and as many rows as sequences) and seq_lens[b] keys with
+ * those of its rows, so its i-th of n rows stands at position seq_lens[b] - n + i.  Key j lies in row j % page_size of
+ * page block_table[b * table_stride + j / page_size].  A page number outside of the cache's pages names no page: such keys are
+ * neither written nor seen.  So are keys beyond the table's row.  Rows before position 0 see nothing.
+ */
+typedef struct {
+  const int32_t* block_table;
+  int64_t table_stride, table_width;
+  const int32_t* seq_lens;
+  const int32_t* query_start;
+  int64_t seqs;
+} fmsmo_kv_batch_t;
+
+/*
+ * New tokens: q [rows, q_heads, dim] and k [rows, cache heads, dim] are normalized per head, rotated by their position, q
+ * written to q_out (which may be q), k and v to their places in the cache.  dtype (FMSMO_F16 or FMSMO_BF16) is that of q,
+ * k, v and q_out, and of a cache that is not e4m3; strides in elements, multiples of 8.
+ *   y = x / sqrt(mean(x^2) + eps) * weight[dim]              (q_weight, k_weight: NULL for none; weight_dtype dtype or FMSMO_F32)
+ *   (a, b) -> (a cos - b sin, b cos + a sin)   over the first `rotary` elements (0 or a multiple of 16), pairs (i, i + rotary / 2),
+ *                                              interleaved: (2i, 2i + 1), angles cos / sin [table_rows, rotary / 2] fp32
+ *   16-bit results are rounded once; e4m3: scale = max(max |y| / 448, 1e-12), code = e4m3(clamp(y / scale, -448, 448)) of
+ *   the fp32 y, the recipe of fmsmo_quant_act_fp8_pertoken.
+ * A position that the angle tables don't hold gives NaN; a row of q before position 0 is zero.  Rows of q_out
+ * that belong to no sequence (behind the last one's) become zero with zero_rest, else they are left as they are.  A place in the cache that two rows of a call name holds one of them or a mixture.
+ */
+int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, int dtype, int64_t rows, int q_heads,
+                   const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                   int64_t v_row, int64_t v_head, void* q_out, int64_t o_row, int64_t o_head, const void* q_weight,
+                   const void* k_weight, int weight_dtype, float eps, const float* cos, const float* sin, int64_t table_rows,
+                   int rotary, int interleaved, int zero_rest, fmsmo_stream_t stream);
+
+/*
+ * out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j over the keys j that a row at position p sees:
+ *   j <= p,  and with a window > 0 also j > p - window or j < sinks.
+ * q heads h * g .. share key head h (g = q_heads / heads).  A row that sees nothing is zero; what a row doesn't see has no
+ * influence on it, whatever it holds.  Sums are fp32; the probabilities are rounded to dtype before they meet the values
+ * (e4m3 caches: times the values' scales, to bf16, for dtype fp16 to the sum of two bf16 numbers).  Rows of no
+ * sequence: zero with zero_rest, else left as they are.
+ * max_rows, max_keys: upper bounds of a sequence's rows and keys that the host knows (0: none); they choose the kernel and how
+ * the work is split, and a sequence that exceeds them is still computed in full.
+ * workspace: fmsmo_paged_attn_workspace_bytes(q_heads, heads, dim, seqs, rows, max_rows, max_keys) bytes, 16-byte aligned, private to the
+ * call until it has finished; max_rows and max_keys as given there, at least 1 and at most rows and table_width * page_size.
+ */
+int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, int dtype, int64_t rows, int q_heads,
+                     const void* q, int64_t q_row, int64_t q_head, void* out, int64_t o_row, int64_t o_head, float scale,
+                     int64_t window, int64_t sinks, int64_t max_rows, int64_t max_keys, int zero_rest, void* workspace,
+                     int64_t workspace_bytes, fmsmo_stream_t stream);
+int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int heads, int dim, int64_t seqs, int64_t rows, int64_t max_rows,
+                                         int64_t max_keys);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,289 @@
+"""Attention over a paged key-value cache against a 64-bit reference: types, heads, lengths, pages, windows, what unseen places
+hold, and the calls around it (streams, graphs, strides, devices)."""
+import pytest
+import torch
+
+import paged_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def K():
+    from fms_mo_amd import kernels
+
+    return kernels
+
+
+def starts(new):
+    s = [0]
+    for n in new:
+        s.append(s[-1] + n)
+    return s
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def on(dev, *ts):
+    return [None if t is None else t.to(dev) for t in ts]  # (keeps strides)
+
+
+def compare(dev, dt, e4m3, heads, kv, D, size, lens, new=None, window=0, sinks=0, layout="heads", seed=0, spare_rows=0, edit=None, hints=True):
+    g = gen(seed)
+    table, pages = R.make_pages(g, lens, size)
+    k, v, ks, vs = R.make_cache(g, pages, kv, size, D, dt, e4m3, layout)
+    start = None if new is None else starts(new)
+    T = len(lens) if new is None else start[-1] + spare_rows
+    q = (1.5 * torch.randn(T, heads, D, generator=g)).to(dt)
+    if edit:
+        table = edit(table, k, v, ks, vs)
+    ref, bound = R.attention(q, k, v, table, lens, start, None, window, sinks, ks, vs)
+    qd, kd, vd, td, ksd, vsd = on(dev, q, k, v, table, ks, vs)
+    kw = dict(max_query_len=max(new) if new else None, max_seq_len=max(lens)) if hints else {}
+    y = K().paged_attention(qd, kd, vd, td, i32(lens, dev), None if start is None else i32(start, dev), window=window, sinks=sinks,
+                            k_scale=ksd, v_scale=vsd, **kw)
+    torch.cuda.synchronize()
+    assert y.shape == q.shape and y.dtype == dt
+    assert R.worst(y, ref, bound) <= 1.0
+    return y
+
+
+TYPES = [(torch.bfloat16, False), (torch.float16, False), (torch.bfloat16, True), (torch.float16, True)]
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("heads,kv,D", [(8, 2, 128), (3, 3, 64), (6, 1, 256), (20, 1, 128), (34, 2, 64)])
+def test_one_token(dev, dt, e4m3, heads, kv, D):
+    compare(dev, dt, e4m3, heads, kv, D, 16, [1, 0, 15, 16, 17, 31, 32, 33, 127, 129, 300, 700], seed=D + heads)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("size", [16, 32, 64, 256])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (7, 3), (40, 40), (64, 1), (1000, 5)])
+def test_one_token_window_and_pages(dev, dt, e4m3, size, window, sinks):
+    compare(dev, dt, e4m3, 4, 2, 64, size, [5, 64, 65, 97, 333, 410], window=window, sinks=sinks, seed=size + window)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("lens", [[3000], [1] * 70 + [1500], [2000, 1, 900], [0, 0, 0]])
+def test_one_token_split(dev, dt, e4m3, lens):
+    compare(dev, dt, e4m3, 4, 2, 128, 64, lens, seed=len(lens))
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("heads,kv,D,new", [(4, 2, 128, 3), (8, 2, 128, 5), (2, 2, 64, 9), (8, 1, 256, 4), (6, 2, 64, 17), (8, 2, 128, 16)])
+def test_few_tokens(dev, dt, e4m3, heads, kv, D, new):
+    compare(dev, dt, e4m3, heads, kv, D, 32, [new, 40, 100, 333, new + 1], [new, 1, new, 2, 0], spare_rows=3, seed=new)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("heads,kv,D", [(4, 2, 128), (3, 3, 64), (4, 1, 256), (10, 2, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (33, 5), (1, 0), (200, 70)])
+def test_prompts(dev, dt, e4m3, heads, kv, D, window, sinks):
+    compare(dev, dt, e4m3, heads, kv, D, 16, [100, 65, 1, 0, 333, 130], [100, 64, 1, 0, 130, 2], window=window, sinks=sinks, seed=window + D)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+def test_prompts_larger_pages(dev, dt, e4m3):
+    compare(dev, dt, e4m3, 4, 2, 128, 128, [129, 500, 257], [129, 100, 257], layout="keys", spare_rows=5)
+    compare(dev, dt, e4m3, 4, 2, 128, 64, [129, 400], [129, 100], hints=False)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_layout_of_keys(dev, dt, e4m3, new):
+    compare(dev, dt, e4m3, 4, 2, 64, 32, [200, 101], None if new == 1 else [new, new], layout="keys", seed=3)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_pages_that_are_not_there(dev, dt, e4m3, new):
+    """Page numbers outside of the cache name no keys, also within a sequence; a sequence longer than its table's row ends there."""
+    def edit(table, k, v, ks, vs):
+        t = table.clone()
+        t[0, 1] = -1
+        t[1, 0] = 1 << 30
+        t[1, 3] = -(1 << 31)
+        return t
+    compare(dev, dt, e4m3, 4, 2, 128, 32, [300, 200], None if new == 1 else [new, new], edit=edit, seed=5)
+
+    def cut(table, k, v, ks, vs):
+        return table[:, :4].contiguous()
+    compare(dev, dt, e4m3, 4, 2, 128, 32, [300, 200], None if new == 1 else [new, new], edit=cut, seed=6)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("new", [1, 4, 70])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("window", [0, 24])
+def test_what_is_not_seen_may_hold_anything(dev, dt, e4m3, new, bad, window):
+    """Infinities and NaN behind the sequence, in pages of nobody, in keys that the window hides, and in the last token's own key, which
+    the tokens before it do not see: every row is what it is with zeros there."""
+    g = gen(new)
+    lens, size, heads, kv, D, sinks = [150, 77], 16, 4, 2, 128, 2 if window else 0
+    table, pages = R.make_pages(g, lens, size)
+    k, v, ks, vs = R.make_cache(g, pages, kv, size, D, dt, e4m3)
+    start = None if new == 1 else starts([new, new])
+    T = 2 if new == 1 else 2 * new
+    q = torch.randn(T, heads, D, generator=g).to(dt)
+    seen = torch.zeros(pages, size, dtype=torch.bool)
+    for r, b, p in R.rows_of(lens, start, T):
+        for j in range(lens[b]):
+            if j <= p and (not window or j > p - window or j < sinks):
+                seen[int(table[b, j // size]), j % size] = True
+    clean = [None if t is None else t.clone() for t in (k, v, ks, vs)]
+    hidden = ~seen[:, None].expand(pages, kv, size)
+    raw = 0x7f if e4m3 else None
+
+    def spoil(where):
+        for c in (k, v):
+            if e4m3:
+                c.view(torch.uint8)[where] = raw
+            else:
+                c[where] = bad
+        for s in (ks, vs):
+            if s is not None:
+                s[where] = bad
+
+    def wipe(where):
+        for c in clean[:2]:
+            (c.view(torch.uint8) if e4m3 else c)[where] = 0
+        for s in clean[2:]:
+            if s is not None:
+                s[where] = 1
+    spoil(hidden)
+    wipe(hidden)
+    whole = torch.arange(T)
+    if new > 1:  # the last token of sequence 0: seen by its own row only
+        p = int(table[0, (lens[0] - 1) // size])
+        where = torch.zeros(pages, kv, size, dtype=torch.bool)
+        where[p, :, (lens[0] - 1) % size] = True
+        spoil(where)
+        wipe(where)
+        whole = torch.tensor([r for r in range(T) if r != new - 1])
+    ref, bound = R.attention(q, clean[0], clean[1], table, lens, start, None, window, sinks, clean[2], clean[3])
+    qd, kd, vd, td, ksd, vsd = on(dev, q, k, v, table, ks, vs)
+    y = K().paged_attention(qd, kd, vd, td, i32(lens, dev), None if start is None else i32(start, dev), window=window, sinks=sinks,
+                            k_scale=ksd, v_scale=vsd, max_query_len=new, max_seq_len=150).cpu()
+    assert R.worst(y[whole], ref[whole], bound[whole]) <= 1.0
+    if new > 1:
+        assert not torch.isfinite(y[new - 1].float()).any()  # its own key is not a number
+
+
+def test_large_scores_and_scales(dev):
+    """Scores far apart (one key takes all) and e4m3 scales over the whole range of fp32's normals that a product leaves finite."""
+    g = gen(1)
+    lens, size = [260, 100], 32
+    for dt in (torch.bfloat16, torch.float16):
+        for e4m3 in (False, True):
+            table, pages = R.make_pages(g, lens, size)
+            k, v, ks, vs = R.make_cache(g, pages, 2, size, 128, dt, e4m3)
+            if e4m3:
+                vs *= 2.0 ** torch.randint(-30, 3, vs.shape, generator=g)
+            q = (60 * torch.randn(2, 4, 128, generator=g)).to(dt)
+            ref, bound = R.attention(q, k, v, table, lens, None, None, 0, 0, ks, vs)
+            qd, kd, vd, td, ksd, vsd = on(dev, q, k, v, table, ks, vs)
+            y = K().paged_attention(qd, kd, vd, td, i32(lens, dev), k_scale=ksd, v_scale=vsd)
+            assert R.worst(y, ref, bound) <= 1.0
+
+
+@pytest.mark.parametrize("new", [1, 4, 100])
+def test_rows_of_no_sequence(dev, new):
+    g = gen(2)
+    lens = [150, 120]
+    table, pages = R.make_pages(g, lens, 16)
+    k, v, _, _ = R.make_cache(g, pages, 2, 16, 64, torch.float16, False)
+    q = torch.randn(2 * new + 7, 4, 64, generator=g).half().to(dev)
+    args = (k.to(dev), v.to(dev), table.to(dev), i32(lens, dev), i32([0, new, 2 * new], dev))
+    y = K().paged_attention(q, *args, max_query_len=new)
+    assert (y[2 * new:] == 0).all() and (y[:2 * new] != 0).any()
+    out = torch.full_like(q, 7.0)
+    z = K().paged_attention(q, *args, max_query_len=new, out=out)
+    assert z is out and (out[2 * new:] == 7).all() and torch.equal(out[:2 * new], y[:2 * new])
+
+
+@pytest.mark.parametrize("new", [1, 4, 100])
+def test_strided_operands_and_hints(dev, new):
+    """q as a slice of a fused projection, out with padding, a table with a wide row stride; wrong hints change the speed only; the
+    same call gives the same bits."""
+    g = gen(4)
+    lens = [700, 333, 501]
+    table, pages = R.make_pages(g, lens, 64)
+    wide = torch.full((3, table.shape[1] + 5), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    k, v, ks, vs = R.make_cache(g, pages, 2, 64, 128, torch.bfloat16, True)
+    T = 3 * new
+    qkv = torch.randn(T, 12, 128, generator=g).bfloat16().to(dev)
+    q = qkv[:, 2:10]
+    args = [t.to(dev) for t in (k, v)] + [wide.to(dev)[:, :table.shape[1]], i32(lens, dev), None if new == 1 else i32([0, new, 2 * new, 3 * new], dev)]
+    kw = dict(k_scale=ks.to(dev), v_scale=vs.to(dev))
+    y = K().paged_attention(q, *args, max_query_len=new, max_seq_len=700, **kw)
+    ref, bound = R.attention(q.cpu(), k, v, table, lens, None if new == 1 else [0, new, 2 * new, 3 * new], None, 0, 0, ks, vs)
+    assert R.worst(y, ref, bound) <= 1.0
+    assert torch.equal(y, K().paged_attention(q, *args, max_query_len=new, max_seq_len=700, **kw))
+    for hint in (dict(max_query_len=1, max_seq_len=1), dict(max_query_len=T, max_seq_len=10 ** 7), {}):
+        assert R.worst(K().paged_attention(q, *args, **hint, **kw), ref, bound) <= 1.0
+    room = torch.zeros(T, 8, 160, dtype=torch.bfloat16, device=dev)
+    K().paged_attention(q, *args, max_query_len=new, max_seq_len=700, out=room[:, :, :128], **kw)
+    assert torch.equal(room[:, :, :128], y) and (room[:, :, 128:] == 0).all()
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_streams_and_graphs(dev, new):
+    """A captured call replays on new lengths, tables and caches; two streams at once do not share a workspace."""
+    g = gen(8)
+    lens = [900, 640]
+    table, pages = R.make_pages(g, lens, 32)
+    k, v, _, _ = R.make_cache(g, pages, 2, 32, 64, torch.float16, False)
+    T = 2 * new
+    start = None if new == 1 else i32([0, new, 2 * new], dev)
+    kd, vd, td, ld = k.to(dev), v.to(dev), table.to(dev), i32(lens, dev)
+    q = torch.randn(T, 4, 64, generator=g).half().to(dev)
+
+    def call():
+        return K().paged_attention(q, kd, vd, td, ld, start, max_query_len=new, max_seq_len=900)
+    want = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = call()
+    b = call()
+    torch.cuda.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call()
+    for i in range(4):
+        new_lens = [900 - 37 * i, 640 - 100 * i]
+        ld.copy_(i32(new_lens, dev))
+        q.normal_()
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        ref, bound = R.attention(q.cpu(), k, v, table, new_lens, None if new == 1 else [0, new, 2 * new])
+        assert R.worst(y, ref, bound) <= 1.0
+
+
+def test_far_offsets(dev):
+    """A cache of more than 4 GiB: places beyond 32 bits, with a stride of its own between pages."""
+    size, D, kv = 16, 64, 1
+    pages = (5 << 30) // (size * D * 2 * 2)
+    both = torch.zeros(pages, 2, kv, size, D, dtype=torch.float16, device=dev)
+    lens = [100]
+    g = gen(3)
+    order = torch.tensor([pages - 1, pages - 3, 5, pages // 2, pages - 7, 0, pages - 2], dtype=torch.int32)
+    k, v, _, _ = R.make_cache(g, 7, kv, size, D, torch.float16, False)
+    both[order.long().to(dev), 0] = k.to(dev)
+    both[order.long().to(dev), 1] = v.to(dev)
+    for new in (1, 70):
+        q = torch.randn(new, 2, D, generator=g).half()
+        start = None if new == 1 else [0, new]
+        ref, bound = R.attention(q, k, v, torch.arange(7, dtype=torch.int32)[None], lens, start)
+        y = K().paged_attention(q.to(dev), both[:, 0], both[:, 1], order[None].to(dev), i32(lens, dev), None if new == 1 else i32(start, dev))
+        assert R.worst(y, ref, bound) <= 1.0
