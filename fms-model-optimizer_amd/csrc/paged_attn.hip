@@ -13,7 +13,7 @@
 //                 free: element 4 t + i of lane group g is key 16 t + 4 g + i), and lane c reads elements ND c .. of those eight keys,
 //                 from which v_perm makes columns ND c + n of V^T for the ND instructions n.
 //
-// Shares: all tiles of all sequences and heads in a row, cut into `workers` equal parts on the device from seq_lens, so a batch of
+// Work: all tiles of all sequences and heads in a row, cut into `workers` equal parts on the device from seq_lens, so a batch of
 // uneven lengths keeps every block busy for the same time and nothing about the lengths has to be known on the host.
 #include "paged_kv.hpp"
 
@@ -22,25 +22,28 @@
 
 namespace fmsmo {
 
-constexpr int TILE = 32, WAVES = 4;
+constexpr int TILE = 32, WAVES = 4, WAVES_SHIFT = 2;
+constexpr int MAX_WORKERS = 512;  // two blocks per compute unit
 
 struct SplitArgs {
   PagedArgs p;
   float* ws;
-  int workers, unit;  // unit: tiles that are never divided between blocks (a multiple of WAVES)
+  int workers, unit_shift;  // 1 << unit_shift tiles are never divided between blocks
+  int splits;               // pairs may be cut: the workspace is there
 };
 
-// A sequence's share of the work: (heads x groups of rows) x units
-struct Share {
+// A sequence's part of the work: (heads x groups of rows) x units
+struct Part {
   int groups, units, pairs;
 };
 template <int ROWS>
-__device__ __forceinline__ Share share_of(const PagedArgs& a, const Seq& s, int unit) {
-  Share w{0, 0, 0};
+__device__ __forceinline__ Part part_of(const PagedArgs& a, const Seq& s, int unit_shift) {
+  Part w{0, 0, 0};
   if (s.n > 0) {
     const Tiles t = tiles_of<TILE>(a, s.len, s.pos0, s.pos0 + s.n - 1);
     w.groups = (s.n * a.group + ROWS - 1) / ROWS;
-    w.units = t.count > unit ? (t.count + unit - 1) / unit : 1;  // (no keys: one that writes zeros)
+    const int units = (t.count + (1 << unit_shift) - 1) >> unit_shift;
+    w.units = units > 1 ? units : 1;  // (no keys: one that writes zeros)
     w.pairs = a.kv_heads * w.groups;
   }
   return w;
@@ -53,83 +56,133 @@ __device__ __forceinline__ int scan_lanes(int v, int lane) {  // inclusive
   }
   return v;
 }
-// sum over the sequences of f(its share)
-template <int ROWS, class F>
-__device__ __forceinline__ int total_of(const PagedArgs& a, int unit, int lane, F f) {
-  int sum = 0;
-  for (int c = 0; c < a.seqs; c += 64) {
-    int v = 0;
-    if (c + lane < a.seqs) v = f(share_of<ROWS>(a, seq_of(a, c + lane), unit));
-    sum += __shfl(scan_lanes(v, lane), 63);
-  }
-  return uniform(sum);
-}
-// the sequence in which the at-th of all f(share)'s lies (at < their sum); base: the sums before it; also_base: those of g
-template <int ROWS, class F, class G>
-__device__ __forceinline__ int find_of(const PagedArgs& a, int unit, int lane, int at, F f, G g, int& base, int& also_base) {
-  int sum = 0, also = 0;
-  for (int c = 0; c < a.seqs; c += 64) {
-    int v = 0, w = 0;
-    if (c + lane < a.seqs) {
-      const Share s = share_of<ROWS>(a, seq_of(a, c + lane), unit);
-      v = f(s);
-      w = g(s);
-    }
-    const int iv = scan_lanes(v, lane), iw = scan_lanes(w, lane);
-    const uint64_t m = __ballot(sum + iv > at);
-    if (m) {
-      const int l = __ffsll((unsigned long long)m) - 1;
-      base = uniform(sum + __shfl(iv - v, l));
-      also_base = uniform(also + __shfl(iw - w, l));
-      return c + l;
-    }
-    sum += __shfl(iv, 63);
-    also += __shfl(iw, 63);
-  }
-  base = also_base = 0;
-  return -1;
-}
 
-// ws: [2 workers] x { o[ROWS][D], (m, l)[ROWS] }, slot 0 of a worker its first share, slot 1 its last
+// The units of each worker: `each` of them, one more for the first `more`
+struct Deal {
+  unsigned each, more;
+  __device__ __forceinline__ int first(unsigned w) const { return (int)(w * each + (w < more ? w : more)); }
+  __device__ __forceinline__ int worker(unsigned u) const {
+    const unsigned big = more * (each + 1);
+    return (int)(u < big ? u / (each + 1) : more + (u - big) / each);
+  }
+};
+
+// What the join needs to know of a cut pair: written by the pair's second worker.
+struct Cut {
+  int rows;             // 0: nothing to join
+  int first, last;      // workers
+  int first_slot;       // of the first worker (the others hold the pair's part in slot 0)
+  int row0, pair_row0;  // q row of the sequence, row of the pair's group in it
+  int head, pad;        // key head
+};
+// workspace: Cut[workers], then per worker two slots of { o[ROWS][D], (m, l)[ROWS] }: its first part, its last
 template <int ROWS, int D>
-__device__ __forceinline__ float* slot_of(float* ws, int worker, int slot) {
-  return ws + (int64_t)(2 * worker + slot) * (ROWS * (D + 2));
+__device__ __forceinline__ float* slot_of(const SplitArgs& a, int worker, int slot) {
+  return (float*)((Cut*)a.ws + a.workers) + (int64_t)(2 * worker + slot) * (ROWS * (D + 2));
 }
 
-template <int QT, bool E4M3, int D, int RT>
-__global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
+// Rows of a lane's keys that may be seen, as bounds of their offsets 16 h + i in the tile (from which 4 g is taken away):
+// offset <= hi and (offset > lo or offset < sink)
+struct Bounds {
+  int hi, lo, sink;
+};
+__device__ __forceinline__ Bounds bounds_of(const PagedArgs& a, int p_lo, int p_hi, int len, int at) {
+  Bounds b;
+  b.hi = (p_hi < len - 1 ? p_hi : len - 1) - at;
+  b.lo = a.window ? p_lo - a.window - at : -(1 << 30);
+  b.sink = a.sinks - at;
+  return b;
+}
+__device__ __forceinline__ bool inside(const Bounds& b, int off) { return off <= b.hi && (off > b.lo || off < b.sink); }
+
+// MULTI: rows of a group may stand at different positions
+template <int QT, bool E4M3, int D, int RT, bool MULTI>
+__global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(SplitArgs sa) {
   constexpr int ROWS = 16 * RT, ND = D / 16;
-  // Type of the probabilities and the values in the product.  e4m3 caches: the probabilities are multiplied by the values'
-  // scales before they are rounded, which takes the exponents of bf16; for an fp16 output, of which bf16 would lose three bits, they
-  // are the sum of two bf16 numbers, and the product is made twice.
+  // Type of the probabilities and the values in the product.  e4m3 caches: the probabilities are multiplied by the values' scales before
+  // they are rounded, which takes the exponents of bf16.  A bf16 probability has lost as much as the rounded result may, so it
+  // enters as the sum of two bf16 numbers and the product is made twice: the matrix units have nothing else to do.
   constexpr int PT = E4M3 ? FMSMO_BF16 : QT;
-  constexpr bool TWO = E4M3 && QT == FMSMO_F16;
-  constexpr int KW = E4M3 ? D / 64 : D / 32;           // 16-byte loads per key and lane group
-  constexpr int QS = D / 32;                           // steps of the reduction over D
-  constexpr int VW = E4M3 ? ND / 4 : ND / 2;           // words of a lane's values per key
+  constexpr bool TWO = PT == FMSMO_BF16;
+  constexpr int KW = E4M3 ? D / 64 : D / 32;  // 16-byte loads per key and lane group
+  constexpr int QS = D / 32;                  // steps of the reduction over D
+  constexpr int VW = E4M3 ? ND / 4 : ND / 2;  // words of a lane's values per key
   __shared__ float join[2][(RT * ND * 4 + 2 * RT) * 64];
   const PagedArgs& a = sa.p;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
+  if (MULTI && a.zero_rest) zero_rest(a, D / 8);
 
-  if (a.zero_rest) zero_rest(a, D / 8);
-  const auto work = [](const Share& s) { return s.pairs * s.units; };
-  const auto none = [](const Share&) { return 0; };
-  const int total = total_of<ROWS>(a, sa.unit, lane, work);
-  int u = (int)((int64_t)blockIdx.x * total / sa.workers);
-  const int u_end = (int)((int64_t)(blockIdx.x + 1) * total / sa.workers);
+  // The sequences, one per lane, 64 at a time: the last 64 stay in registers (all of them, as a rule).
+  Seq seq{};
+  Part part{};
+  int scan = 0, kept = 0;
+  const auto look = [&](int c) {
+    seq = Seq{};
+    if (c + lane < a.seqs) seq = seq_of(a, c + lane);
+    part = part_of<ROWS>(a, seq, sa.unit_shift);
+    scan = scan_lanes(part.pairs * part.units, lane);
+    kept = c;
+  };
+  int total = 0;
+  for (int c = 0; c < a.seqs; c += 64) {
+    look(c);
+    total += __builtin_amdgcn_readlane(scan, 63);
+  }
+  const int workers = sa.workers < total ? sa.workers : total;  // (so that no worker is without work)
+  const bool idle = (int)blockIdx.x >= workers;
+  Cut* cut = (Cut*)sa.ws + blockIdx.x;
+  if (idle) {
+    if (threadIdx.x == 0 && sa.splits) cut->rows = 0;
+    return;
+  }
+  Deal deal;
+  deal.each = (unsigned)total / (unsigned)workers;
+  deal.more = (unsigned)total - deal.each * (unsigned)workers;
+  int u = deal.first(blockIdx.x);
+  const int u_end = deal.first(blockIdx.x + 1);
   for (bool first = true; u < u_end; first = false) {
-    int base, unused;
-    const int b = find_of<ROWS>(a, sa.unit, lane, u, work, none, base, unused);
-    if (b < 0) return;
-    const Seq s = seq_of(a, b);
-    const Share w = share_of<ROWS>(a, s, sa.unit);
+    // the sequence, head and group of rows that unit u belongs to
+    int base = 0, at = 0;
+    if (a.seqs > 64) {
+      for (int c = 0; c < a.seqs; c += 64) {
+        look(c);
+        const int sum = __builtin_amdgcn_readlane(scan, 63);
+        if (base + sum > u) break;
+        base += sum;
+      }
+    }
+    const uint64_t behind = __ballot(base + scan > u);
+    at = behind ? __ffsll((unsigned long long)behind) - 1 : 0;
+    const auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+    const int b = kept + at;
+    Seq s;
+    s.n = pick(seq.n);
+    s.row0 = pick(seq.row0);
+    s.pos0 = pick(seq.pos0);
+    s.len = pick(seq.len);
+    const int units = pick(part.units), groups = pick(part.groups);
+    base += pick(scan) - units * pick(part.pairs);
     const Tiles t = tiles_of<TILE>(a, s.len, s.pos0, s.pos0 + s.n - 1);
-    const int pair = (u - base) / w.units, u0 = (u - base) % w.units;
-    const int u1 = w.units - u0 < u_end - u ? w.units : u0 + (u_end - u);
-    const int hk = pair / w.groups, r0 = pair % w.groups * ROWS;
+    const int pair = (int)((unsigned)(u - base) / (unsigned)units), u0 = u - base - pair * units;
+    const int u1 = units - u0 < u_end - u ? units : u0 + (u_end - u);
+    const int hk = groups == 1 ? pair : pair / groups, r0 = groups == 1 ? 0 : pair % groups * ROWS;
     const int nrows = s.n * a.group - r0 < ROWS ? s.n * a.group - r0 : ROWS;
-    const int p_lo = s.pos0 + r0 / a.group, p_hi = s.pos0 + (r0 + nrows - 1) / a.group;
+    const int p_lo = MULTI ? s.pos0 + r0 / a.group : s.pos0, p_hi = MULTI ? s.pos0 + (r0 + nrows - 1) / a.group : s.pos0;
+    if (first && sa.splits && threadIdx.x == 0) {
+      Cut d{};
+      if (u0 > 0) {
+        const int from = u - u0;
+        d.first = deal.worker(from);
+        d.last = deal.worker(from + units - 1);
+        d.first_slot = from <= deal.first(d.first) ? 0 : 1;
+        d.rows = d.first == (int)blockIdx.x - 1 ? nrows : 0;
+        d.row0 = s.row0;
+        d.pair_row0 = r0;
+        d.head = hk;
+      }
+      *cut = d;
+    }
 
     // the rows: operand of the scores, and each lane's position
     v4i q[RT][QS];
@@ -138,14 +191,15 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
     for (int rt = 0; rt < RT; ++rt) {
       const int r = r0 + rt * 16 + c16;
       const bool in = rt * 16 + c16 < nrows;
-      const int i = in ? r / a.group : 0, h = in ? r - i * a.group : 0;
+      const int i = MULTI && in ? r / a.group : 0, h = in ? r - i * a.group : 0;
       pos[rt] = in ? s.pos0 + i : -1;
       const char* src = a.q + (s.row0 + i) * a.q_row + (hk * a.group + h) * a.q_head;
 #pragma unroll
       for (int x = 0; x < QS; ++x) {
         // element order of the reduction: that in which the keys come (e4m3: 16 bytes are two steps)
-        const int at = E4M3 ? (x / 2) * 64 + g * 16 + (x % 2) * 8 : x * 32 + g * 8;
-        q[rt][x] = in ? *(const v4i*)(src + at * 2) : v4i{0, 0, 0, 0};
+        const int el = E4M3 ? (x / 2) * 64 + g * 16 + (x % 2) * 8 : x * 32 + g * 8;
+        q[rt][x] = *(const v4i*)(src + el * 2);
+        q[rt][x] = in ? q[rt][x] : v4i{0, 0, 0, 0};
       }
     }
     v4f o[RT][ND];
@@ -158,35 +212,44 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
       for (int n = 0; n < ND; ++n) o[rt][n] = v4f{0, 0, 0, 0};
     }
 
-    const int end = u1 * sa.unit < t.count ? u1 * sa.unit : t.count;
+    const int end = u1 << sa.unit_shift < t.count ? u1 << sa.unit_shift : t.count;
     const int in_page = (1 << a.page_shift) - 1;
-    const int* row = a.table + b * a.table_stride;
+    const auto row = (const __attribute__((address_space(4))) int*)(uintptr_t)(a.table + b * a.table_stride);
     const auto key_of = [&](int tile) { return (tile < t.sink_tiles ? tile : tile + t.skip) * TILE; };
     // page numbers of a tile's two halves; -1: no such page, or behind the sequence
     const auto pages_of = [&](int tile, int* pg) {
       const int k0 = key_of(tile);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = k0 + 16 * h;
-        pg[h] = tile < end && k < s.len ? row[k >> a.page_shift] : -1;
-        if ((unsigned)pg[h] >= (unsigned)a.pages) pg[h] = -1;
+        const int k = k0 + 16 * h, n = row[(k < s.len ? k : 0) >> a.page_shift];
+        pg[h] = tile < end && k < s.len && (unsigned)n < (unsigned)a.pages ? n : -1;
       }
+    };
+    // Every iteration makes the same loads, so that the wait for one of them never waits for those after it; of a half that is
+    // not there (behind the end, too) they come back as zeros without a request: a buffer of no bytes.
+    const auto buffer = [&](const char* at, bool there) {
+      return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, there ? 0x7fffffff : 0, 0x00020000);
     };
     v4i kr[2][KW];
     uint32_t vr[8][VW];
     v4f ksr[2], vsr[2];
-    const int k_lane = c16 * a.k_slot + g * 16, v_lane = 4 * g * a.v_slot + c16 * (VW * 4);
+    const int k_lane = c16 * a.k_slot + g * 16;
+    int v_lane[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v_lane[j] = (4 * g + j) * a.v_slot + c16 * (VW * 4);
     const auto load_k = [&](int tile, const int* pg) {
       const int k0 = key_of(tile);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int page = uniform(pg[h] < 0 ? 0 : pg[h]), slot = (k0 + 16 * h) & in_page;
-        const char* at = a.k + page * a.k_page + hk * a.k_head + (int64_t)slot * a.k_slot;
+        const int64_t page = pg[h] < 0 ? 0 : pg[h], slot = (k0 + 16 * h) & in_page;
+        const auto src = buffer(a.k + page * a.k_page + hk * a.k_head + slot * a.k_slot, pg[h] >= 0);
 #pragma unroll
-        for (int x = 0; x < KW; ++x) kr[h][x] = *(const v4i*)(at + k_lane + x * 64);
+        for (int x = 0; x < KW; ++x) kr[h][x] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(src, k_lane + x * 64, 0, 0));
         if constexpr (E4M3) {
-          ksr[h] = *(const v4f*)(a.ks + page * a.ks_page + hk * a.ks_head + slot + 4 * g);
-          vsr[h] = *(const v4f*)(a.vs + page * a.vs_page + hk * a.vs_head + slot + 4 * g);
+          const auto ks = buffer((const char*)(a.ks + page * a.ks_page + hk * a.ks_head + slot), pg[h] >= 0);
+          const auto vs = buffer((const char*)(a.vs + page * a.vs_page + hk * a.vs_head + slot), pg[h] >= 0);
+          ksr[h] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(ks, 16 * g, 0, 0));
+          vsr[h] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(vs, 16 * g, 0, 0));
         }
       }
     };
@@ -194,14 +257,27 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
       const int k0 = key_of(tile);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int page = uniform(pg[h] < 0 ? 0 : pg[h]), slot = (k0 + 16 * h) & in_page;
-        const char* at = a.v + page * a.v_page + hk * a.v_head + (int64_t)slot * a.v_slot;
+        const int64_t page = pg[h] < 0 ? 0 : pg[h], slot = (k0 + 16 * h) & in_page;
+        const auto src = buffer(a.v + page * a.v_page + hk * a.v_head + slot * a.v_slot, pg[h] >= 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) __builtin_memcpy(vr[4 * h + j], at + v_lane + j * a.v_slot, VW * 4);
+        for (int j = 0; j < 4; ++j) {
+          uint32_t* to = vr[4 * h + j];
+          if constexpr (VW == 1) to[0] = __builtin_amdgcn_raw_buffer_load_b32(src, v_lane[j], 0, 0);
+          else if constexpr (VW == 2) {
+            const auto u = __builtin_amdgcn_raw_buffer_load_b64(src, v_lane[j], 0, 0);
+            __builtin_memcpy(to, &u, 8);
+          } else {
+#pragma unroll
+            for (int x = 0; x < VW / 4; ++x) {
+              const auto u = __builtin_amdgcn_raw_buffer_load_b128(src, v_lane[j] + 16 * x, 0, 0);
+              __builtin_memcpy(to + 4 * x, &u, 16);
+            }
+          }
+        }
       }
     };
 
-    int tile = u0 * sa.unit + wave;
+    int tile = (u0 << sa.unit_shift) + wave;
     int pg[2], pg_next[2];
     if (tile < end) {
       pages_of(tile, pg);
@@ -246,12 +322,8 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
       const int more = tile + WAVES;
       pg[0] = pg_next[0];
       pg[1] = pg_next[1];
-      if (more < end) {
-        load_k(more, pg);
-        pages_of(more + WAVES, pg_next);
-      }
-      // the keys a lane holds scores of: 16 h + 4 g + i
-      const auto there = [&](int h, int i) { return (h ? there1 : there0) && k0 + 16 * h + 4 * g + i < s.len; };
+      load_k(more, pg);
+      pages_of(more + WAVES, pg_next);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -260,14 +332,14 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
           for (int i = 0; i < 4; ++i) st[rt][h][i] *= E4M3 ? ks[h][i] : a.c;
       if (!whole) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int rt = 0; rt < RT; ++rt) {
+          const Bounds bd = bounds_of(a, pos[rt], pos[rt], s.len, k0 + 4 * g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool in = there(h, i);
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              st[rt][h][i] = in && sees(a, pos[rt], k0 + 16 * h + 4 * g + i) ? st[rt][h][i] : -__builtin_inff();
-          }
+            for (int i = 0; i < 4; ++i)
+              st[rt][h][i] = (h ? there1 : there0) && inside(bd, 16 * h + i) ? st[rt][h][i] : -__builtin_inff();
+        }
       }
       v4i pb[RT], pl[RT];
 #pragma unroll
@@ -276,13 +348,13 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
                           fmaxf(fmaxf(st[rt][1][0], st[rt][1][1]), fmaxf(st[rt][1][2], st[rt][1][3])));
         top = max_x32(max_x16(top));
         const float m_new = fmaxf(m[rt], top), ms = safe_max(m_new);
-        const float f = exp2_hw(m[rt] - ms);
         if (__any(m_new > m[rt])) {
+          const float f = exp2_hw(m[rt] - ms);
 #pragma unroll
           for (int n = 0; n < ND; ++n) o[rt][n] *= f;
+          l[rt] *= f;
+          m[rt] = m_new;
         }
-        l[rt] *= f;
-        m[rt] = m_new;
         float pr[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -317,29 +389,26 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
       if (!whole) {
         // what no row sees may hold anything, and 0 * inf is not 0: such values count as zero.  Where rows see different keys, a
         // value that is not finite goes to those only that see it (below).
+        const Bounds bd = bounds_of(a, p_lo, p_hi, s.len, k0 + 4 * g);
         uint32_t fine = 0x80008000u;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool in = there(j / 4, j % 4) && sees_one(a, p_lo, p_hi, k0 + 16 * (j / 4) + 4 * g + j % 4);
+          const bool in = (j / 4 ? there1 : there0) && inside(bd, 16 * (j / 4) + j % 4);
 #pragma unroll
           for (int x = 0; x < ND / 2; ++x) {
             vw[j][x] = in ? vw[j][x] : 0u;
-            fine &= finite2<PT>(vw[j][x]);
+            if constexpr (MULTI) fine &= finite2<PT>(vw[j][x]);
           }
         }
-        apart = p_lo != p_hi && __any(fine != 0x80008000u);
+        if constexpr (MULTI) apart = p_lo != p_hi && __any(fine != 0x80008000u);
       }
-      const auto column = [&](int n) {
-        const uint32_t sel = n % 2 ? 0x07060302u : 0x05040100u;
-        v4i f;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) f[x] = (int)__builtin_amdgcn_perm(vw[2 * x + 1][n / 2], vw[2 * x][n / 2], sel);
-        return f;
+      const auto column = [&](int n, int x) {  // words x of column n: keys 2 x and 2 x + 1 of the lane's eight
+        return (int)__builtin_amdgcn_perm(vw[2 * x + 1][n / 2], vw[2 * x][n / 2], n % 2 ? 0x07060302u : 0x05040100u);
       };
-      if (!apart) {
+      if (!MULTI || !apart) {
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
-          const v4i f = column(n);
+          const v4i f = {column(n, 0), column(n, 1), column(n, 2), column(n, 3)};
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
             o[rt][n] = mfma16<PT>(f, pb[rt], o[rt][n]);
@@ -347,18 +416,19 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
           }
         }
       } else {
+#pragma unroll 1
         for (int r = 0; r < nrows; ++r) {  // one row at a time, with the values it sees
           const int p = s.pos0 + (r0 + r) / a.group;
-          uint32_t keep[8];
+          const Bounds bd = bounds_of(a, p, p, s.len, k0 + 4 * g);
+          uint32_t keep[4];  // halves: keys 2 x and 2 x + 1
 #pragma unroll
-          for (int j = 0; j < 8; ++j) keep[j] = sees(a, p, k0 + 16 * (j / 4) + 4 * g + j % 4) ? ~0u : 0u;
+          for (int x = 0; x < 4; ++x)
+            keep[x] = (inside(bd, 16 * (x / 2) + 2 * (x % 2)) ? 0xffffu : 0u) | (inside(bd, 16 * (x / 2) + 2 * (x % 2) + 1) ? 0xffff0000u : 0u);
 #pragma unroll
           for (int n = 0; n < ND; ++n) {
-            const uint32_t sel = n % 2 ? 0x07060302u : 0x05040100u;
             v4i f;
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              f[x] = (int)__builtin_amdgcn_perm(vw[2 * x + 1][n / 2] & keep[2 * x + 1], vw[2 * x][n / 2] & keep[2 * x], sel);
+            for (int x = 0; x < 4; ++x) f[x] = column(n, x) & (int)keep[x];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
               v4f d = mfma16<PT>(f, pb[rt], o[rt][n]);
@@ -368,7 +438,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
           }
         }
       }
-      if (more < end) load_v(more, pg);
+      load_v(more, pg);
     }
 
     // the four waves' shares: 2 and 3 into 0 and 1, then 1 into 0
@@ -407,14 +477,14 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
       __syncthreads();
     }
     if (wave == 0) {
-      const bool complete = u0 == 0 && u1 == w.units;
-      float* part = slot_of<ROWS, D>(sa.ws, blockIdx.x, first ? 0 : 1);
+      const bool complete = u0 == 0 && u1 == units;
+      float* share = slot_of<ROWS, D>(sa, blockIdx.x, first ? 0 : 1);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const int r = rt * 16 + c16;
         if (r >= nrows) continue;
         if (complete) {
-          const int i = (r0 + r) / a.group, h = r0 + r - i * a.group;
+          const int i = MULTI ? (r0 + r) / a.group : 0, h = r0 + r - i * a.group;
           char* to = a.out + (s.row0 + i) * a.o_row + (hk * a.group + h) * a.o_head;
           const float inv = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
 #pragma unroll
@@ -431,11 +501,11 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
             float y[ND];
 #pragma unroll
             for (int n = 0; n < ND; ++n) y[n] = o[rt][n][i4];
-            __builtin_memcpy(part + r * D + (4 * g + i4) * ND, y, ND * 4);
+            __builtin_memcpy(share + r * D + (4 * g + i4) * ND, y, ND * 4);
           }
           if (g == 0) {
-            part[ROWS * D + 2 * r] = m[rt];
-            part[ROWS * D + 2 * r + 1] = l[rt];
+            share[ROWS * D + 2 * r] = m[rt];
+            share[ROWS * D + 2 * r + 1] = l[rt];
           }
         }
       }
@@ -444,70 +514,57 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(SplitArgs sa) {
   }
 }
 
-// Joins the shares of the heads and groups of rows that were cut: one block per row, its waves take every fourth share.
+// Joins the shares of the pairs that were cut: a block per cut and row.  The weights of all shares first (a share per thread), then
+// every group of D / 4 threads adds up every (1024 / D)-th share: loads that wait for nothing but the weights.
 template <int QT, int D, int ROWS>
 __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
-  constexpr int W = D / 64;
-  __shared__ float om[WAVES][D + 2];
+  constexpr int LG = D / 4, GROUPS = 256 / LG;
+  __shared__ float weight[MAX_WORKERS];
+  __shared__ float red[8];
+  __shared__ __attribute__((aligned(16))) float sum[GROUPS][D];
   const PagedArgs& a = sa.p;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const auto work = [](const Share& s) { return s.pairs * s.units; };
-  const auto rows = [](const Share& s) { return s.pairs * ROWS; };
-  const int total = total_of<ROWS>(a, sa.unit, lane, work), jobs = total_of<ROWS>(a, sa.unit, lane, rows);
-  for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
-    int base, unit_base;
-    const int b = find_of<ROWS>(a, sa.unit, lane, job, rows, work, base, unit_base);
-    if (b < 0) return;
-    const Seq s = seq_of(a, b);
-    const Share w = share_of<ROWS>(a, s, sa.unit);
-    const int pair = (job - base) / ROWS, r = (job - base) % ROWS;
-    const int row = pair % w.groups * ROWS + r;
-    if (row >= s.n * a.group) continue;
-    const int64_t u0 = unit_base + pair * w.units, u1 = u0 + w.units;
-    // the workers of the first and the last unit
-    const int w0 = (int)(((u0 + 1) * sa.workers - 1) / total), w1 = (int)((u1 * sa.workers - 1) / total);
-    if (w0 == w1) continue;  // whole: written by its block
-    float m = -__builtin_inff(), l = 0.0f, o[W];
-#pragma unroll
-    for (int x = 0; x < W; ++x) o[x] = 0.0f;
-    for (int k = w0 + wave; k <= w1; k += WAVES) {
-      const int64_t start = (int64_t)k * total / sa.workers, stop = (int64_t)(k + 1) * total / sa.workers;
-      if (start == stop) continue;  // a worker without work
-      const float* part = slot_of<ROWS, D>(sa.ws, k, u0 <= start ? 0 : 1);
-      const float m2 = part[ROWS * D + 2 * r], l2 = part[ROWS * D + 2 * r + 1];
-      const float mx = fmaxf(m, m2), ms = safe_max(mx), f1 = exp2_hw(m - ms), f2 = exp2_hw(m2 - ms);
-      m = mx;
-      l = l * f1 + l2 * f2;
-#pragma unroll
-      for (int x = 0; x < W; ++x) o[x] = o[x] * f1 + part[r * D + lane * W + x] * f2;
+  const Cut d = ((const Cut*)sa.ws)[blockIdx.x];
+  const int shares = d.last - d.first + 1, tid = threadIdx.x, wave = tid >> 6;
+  for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
+    const auto share = [&](int k) { return slot_of<ROWS, D>(sa, d.first + k, k == 0 ? d.first_slot : 0); };
+    float top = -__builtin_inff();
+    for (int k = tid; k < shares; k += 256) {
+      weight[k] = share(k)[ROWS * D + 2 * r];
+      top = fmaxf(top, weight[k]);
     }
-#pragma unroll
-    for (int x = 0; x < W; ++x) om[wave][lane * W + x] = o[x];
-    if (lane == 0) {
-      om[wave][D] = m;
-      om[wave][D + 1] = l;
-    }
+    top = wave_max(top);
+    if ((tid & 63) == 0) red[wave] = top;
     __syncthreads();
-    if (wave == 0) {
-      float mx = om[0][D];
+    const float ms = safe_max(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    float l = 0.0f;
+    for (int k = tid; k < shares; k += 256) {
+      const float f = exp2_hw(weight[k] - ms);
+      weight[k] = f;
+      l += share(k)[ROWS * D + 2 * r + 1] * f;
+    }
 #pragma unroll
-      for (int k = 1; k < WAVES; ++k) mx = fmaxf(mx, om[k][D]);
-      const float ms = safe_max(mx);
-      l = 0.0f;
+    for (int o = 1; o < 64; o *= 2) l += __shfl_xor(l, o);
+    if ((tid & 63) == 0) red[4 + wave] = l;
+    __syncthreads();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    const int c = tid % LG;
+    v4f o = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int k = tid / LG; k < shares; k += GROUPS) o += *(const v4f*)(share(k) + r * D + 4 * c) * weight[k];
+    *(v4f*)&sum[tid / LG][4 * c] = o;
+    __syncthreads();
+    if (tid < LG) {
 #pragma unroll
-      for (int x = 0; x < W; ++x) o[x] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < WAVES; ++k) {
-        const float f = exp2_hw(om[k][D] - ms);
-        l += om[k][D + 1] * f;
-#pragma unroll
-        for (int x = 0; x < W; ++x) o[x] += om[k][lane * W + x] * f;
-      }
+      for (int k = 1; k < GROUPS; ++k) o += *(const v4f*)&sum[k][4 * c];
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int i = row / a.group, h = row - i * a.group;
-      u16* to = (u16*)(a.out + (s.row0 + i) * a.o_row + (pair / w.groups * a.group + h) * a.o_head) + lane * W;
-#pragma unroll
-      for (int x = 0; x < W; ++x) store_from_f32<QT>(to, x, l == 0.0f ? 0.0f : o[x] * inv);
+      const int row = d.pair_row0 + r, i = row / a.group, h = row - i * a.group;
+      char* to = a.out + (d.row0 + i) * a.o_row + (d.head * a.group + h) * a.o_head;
+      uint32_t y[2] = {0, 0};
+      if (l != 0.0f) {
+        y[0] = pack2<QT>(o[0] * inv, o[1] * inv);
+        y[1] = pack2<QT>(o[2] * inv, o[3] * inv);
+      }
+      __builtin_memcpy(to + 8 * c, y, 8);
     }
     __syncthreads();
   }
@@ -596,7 +653,7 @@ int fmsmo_paged_args(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batc
 struct Plan {
   bool prompt;   // the kernel of many rows
   int row_tiles; // of the split kernel
-  int workers, unit;
+  int workers, unit_shift;
 };
 static Plan plan_of(int group, int kv_heads, int dim, int64_t seqs, int64_t rows, int64_t max_rows, int64_t max_keys) {
   Plan p{};
@@ -605,14 +662,16 @@ static Plan plan_of(int group, int kv_heads, int dim, int64_t seqs, int64_t rows
   p.row_tiles = most <= 16 ? 1 : 2;
   const int64_t tiles = std::max<int64_t>(1, (max_keys + TILE - 1) / TILE);
   const int64_t pairs = std::max<int64_t>(1, std::min(seqs, rows)) * kv_heads * ((most + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
-  p.unit = WAVES;
-  if (tiles <= 2 * WAVES) p.unit = 1 << 24;  // nothing to split: one launch
-  const int64_t units = pairs * ((tiles + p.unit - 1) / p.unit);
-  p.workers = (int)std::min<int64_t>(p.unit > WAVES ? 65536 : 512, units);
+  p.unit_shift = WAVES_SHIFT;
+  if (tiles <= 2 * WAVES) p.unit_shift = 26;  // nothing to split: one launch
+  const int64_t units = pairs * (((tiles - 1) >> p.unit_shift) + 1);
+  // as many as are resident: the kernels whose registers leave room for one block per compute unit get half
+  const int resident = p.row_tiles * dim > 128 ? MAX_WORKERS / 2 : MAX_WORKERS;
+  p.workers = (int)std::min<int64_t>(p.unit_shift > WAVES_SHIFT ? 65536 : resident, units);
   return p;
 }
 static int64_t plan_bytes(const Plan& p, int dim) {
-  return p.prompt || p.unit > WAVES ? 0 : (int64_t)p.workers * 2 * 16 * p.row_tiles * (dim + 2) * 4;
+  return p.prompt || p.unit_shift > WAVES_SHIFT ? 0 : p.workers * ((int64_t)sizeof(Cut) + 2 * 16 * p.row_tiles * (dim + 2) * 4);
 }
 static void bounds(int64_t& max_rows, int64_t& max_keys, int64_t rows, int64_t cap, bool ragged) {
   if (!ragged) max_rows = 1;
@@ -650,17 +709,19 @@ extern "C" int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_ba
   if (((uintptr_t)workspace) & 15) return FMSMO_ERR_ALIGN;
   // (units are counted in 31 bits: heads x groups of rows x units of a sequence, summed)
   const int64_t pairs = (rows * a.group / (16 * p.row_tiles) + a.seqs) * a.kv_heads;
-  if (pairs > 0x7fffffffll / 32 || pairs * (a.cap / TILE / p.unit + 2) > 0x7fffffffll) return FMSMO_ERR_UNSUPPORTED;
+  if (pairs > 0x7fffffffll / 32 || pairs * ((a.cap / TILE >> p.unit_shift) + 2) > 0x7fffffffll) return FMSMO_ERR_UNSUPPORTED;
   sa.ws = (float*)workspace;
   sa.workers = p.workers;
-  sa.unit = p.unit;
+  sa.unit_shift = p.unit_shift;
+  sa.splits = need > 0;
   const auto go = [&](auto t, auto e, auto d, auto r) {
     constexpr int T = decltype(t)::value, D = decltype(d)::value, RT = decltype(r)::value;
-    hipLaunchKernelGGL((paged_split_kernel<T, decltype(e)::value, D, RT>), dim3(p.workers), dim3(256), 0, (hipStream_t)stream, sa);
+    constexpr bool E = decltype(e)::value;
+    if (a.starts) hipLaunchKernelGGL((paged_split_kernel<T, E, D, RT, true>), dim3(p.workers), dim3(256), 0, (hipStream_t)stream, sa);
+    else hipLaunchKernelGGL((paged_split_kernel<T, E, D, RT, false>), dim3(p.workers), dim3(256), 0, (hipStream_t)stream, sa);
     if (need) {
-      const int64_t jobs = (rows * a.group + (int64_t)a.seqs * 16 * RT) * a.kv_heads;
-      hipLaunchKernelGGL((paged_join_kernel<T, D, 16 * RT>), dim3((unsigned)std::min<int64_t>(jobs, 2048)), dim3(256), 0,
-                         (hipStream_t)stream, sa);
+      const unsigned per = (unsigned)std::min<int64_t>(max_rows * a.group, 16 * RT);  // rows of a group, as a rule
+      hipLaunchKernelGGL((paged_join_kernel<T, D, 16 * RT>), dim3(p.workers, per), dim3(256), 0, (hipStream_t)stream, sa);
     }
   };
   const auto tiles = [&](auto t, auto e, auto d) {
