@@ -4,7 +4,7 @@
 // over the keys that a row sees, with the running maximum m and sum l of each wave's share; shares are joined as
 //   m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), o likewise (everything in powers of two, fp32).
 //
-// What bounds it is reading the cache once.  Up to 16 RT rows (tokens x the query heads that share a key head) are the columns of
+// What bounds it is reading the cache once.  Up to 16 rows (tokens x the query heads that share a key head) are the columns of
 // one matrix instruction, so the arithmetic is 1 / 10 of what the units could do in that time; the kernel is made of loads
 // in flight: every wave owns tiles of 32 keys, from memory straight into the operands' registers -- no shared memory, no barrier --
 // and asks for the keys of its next tile before the softmax of the present one, for its values after them.
@@ -22,13 +22,14 @@
 
 namespace fmsmo {
 
-constexpr int TILE = 32, WAVES = 4, WAVES_SHIFT = 2;
+constexpr int TILE = 32, WAVES = 4;
 constexpr int MAX_WORKERS = 512;  // two blocks per compute unit
 
 struct SplitArgs {
   PagedArgs p;
   float* ws;
   int workers, unit_shift;  // 1 << unit_shift tiles are never divided between blocks
+  int row_shift;            // 1 << row_shift waves of a block take the same keys, 16 rows each
   int splits;               // pairs may be cut: the workspace is there
 };
 
@@ -36,24 +37,27 @@ struct SplitArgs {
 struct Part {
   int groups, units, pairs;
 };
-template <int ROWS>
-__device__ __forceinline__ Part part_of(const PagedArgs& a, const Seq& s, int unit_shift) {
+__device__ __forceinline__ Part part_of(const PagedArgs& a, const Seq& s, int unit_shift, int row_shift) {
   Part w{0, 0, 0};
   if (s.n > 0) {
     const Tiles t = tiles_of<TILE>(a, s.len, s.pos0, s.pos0 + s.n - 1);
-    w.groups = (s.n * a.group + ROWS - 1) / ROWS;
+    w.groups = (s.n * a.group + (16 << row_shift) - 1) >> (4 + row_shift);
     const int units = (t.count + (1 << unit_shift) - 1) >> unit_shift;
     w.units = units > 1 ? units : 1;  // (no keys: one that writes zeros)
     w.pairs = a.kv_heads * w.groups;
   }
   return w;
 }
-__device__ __forceinline__ int scan_lanes(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int w = __shfl_up(v, o);
-    if (lane >= o) v += w;
-  }
+// inclusive sums over the lanes of the wave: within rows of 16, then the rows before
+__device__ __forceinline__ int scan_lanes(int v) {
+#define FMSMO_DPP_ADD(ctrl, rows) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, true)
+  FMSMO_DPP_ADD(0x111, 0xf);  // row_shr 1, 2, 4, 8
+  FMSMO_DPP_ADD(0x112, 0xf);
+  FMSMO_DPP_ADD(0x114, 0xf);
+  FMSMO_DPP_ADD(0x118, 0xf);
+  FMSMO_DPP_ADD(0x142, 0xa);  // row_bcast15 into rows 1 and 3
+  FMSMO_DPP_ADD(0x143, 0xc);  // row_bcast31 into rows 2 and 3
+#undef FMSMO_DPP_ADD
   return v;
 }
 
@@ -75,10 +79,10 @@ struct Cut {
   int row0, pair_row0;  // q row of the sequence, row of the pair's group in it
   int head, pad;        // key head
 };
-// workspace: Cut[workers], then per worker two slots of { o[ROWS][D], (m, l)[ROWS] }: its first part, its last
-template <int ROWS, int D>
+// workspace: Cut[workers], then per worker two slots of { o[rows][D], (m, l)[rows] }: its first part, its last
+template <int D>
 __device__ __forceinline__ float* slot_of(const SplitArgs& a, int worker, int slot) {
-  return (float*)((Cut*)a.ws + a.workers) + (int64_t)(2 * worker + slot) * (ROWS * (D + 2));
+  return (float*)((Cut*)a.ws + a.workers) + (((int64_t)(2 * worker + slot) * 16 * (D + 2)) << a.row_shift);
 }
 
 // Rows of a lane's keys that may be seen, as bounds of their offsets 16 h + i in the tile (from which 4 g is taken away):
@@ -95,10 +99,10 @@ __device__ __forceinline__ Bounds bounds_of(const PagedArgs& a, int p_lo, int p_
 }
 __device__ __forceinline__ bool inside(const Bounds& b, int off) { return off <= b.hi && (off > b.lo || off < b.sink); }
 
-// MULTI: rows of a group may stand at different positions
-template <int QT, bool E4M3, int D, int RT, bool MULTI>
-__global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(SplitArgs sa) {
-  constexpr int ROWS = 16 * RT, ND = D / 16;
+// MULTI: rows of a group may stand at different positions.  SHARED: row_shift > 0
+template <int QT, bool E4M3, int D, bool MULTI, bool SHARED>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(SplitArgs sa) {
+  constexpr int ND = D / 16;
   // Type of the probabilities and the values in the product.  e4m3 caches: the probabilities are multiplied by the values' scales before
   // they are rounded, which takes the exponents of bf16.  A bf16 probability has lost as much as the rounded result may, so it
   // enters as the sum of two bf16 numbers and the product is made twice: the matrix units have nothing else to do.
@@ -107,10 +111,12 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
   constexpr int KW = E4M3 ? D / 64 : D / 32;  // 16-byte loads per key and lane group
   constexpr int QS = D / 32;                  // steps of the reduction over D
   constexpr int VW = E4M3 ? ND / 4 : ND / 2;  // words of a lane's values per key
-  __shared__ float join[2][(RT * ND * 4 + 2 * RT) * 64];
+  __shared__ float join[2][(ND * 4 + 2) * 64];
   const PagedArgs& a = sa.p;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
+  const int row_shift = SHARED ? sa.row_shift : 0, rows = 16 << row_shift;
+  const int waves = WAVES >> row_shift, sub = wave & (waves - 1), row_tile = SHARED ? wave / waves : 0;  // of a row tile
   if (MULTI && a.zero_rest) zero_rest(a, D / 8);
 
   // The sequences, one per lane, 64 at a time: the last 64 stay in registers (all of them, as a rule).
@@ -120,8 +126,8 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
   const auto look = [&](int c) {
     seq = Seq{};
     if (c + lane < a.seqs) seq = seq_of(a, c + lane);
-    part = part_of<ROWS>(a, seq, sa.unit_shift);
-    scan = scan_lanes(part.pairs * part.units, lane);
+    part = part_of(a, seq, sa.unit_shift, row_shift);
+    scan = scan_lanes(part.pairs * part.units);
     kept = c;
   };
   int total = 0;
@@ -166,53 +172,11 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
     const Tiles t = tiles_of<TILE>(a, s.len, s.pos0, s.pos0 + s.n - 1);
     const int pair = (int)((unsigned)(u - base) / (unsigned)units), u0 = u - base - pair * units;
     const int u1 = units - u0 < u_end - u ? units : u0 + (u_end - u);
-    const int hk = groups == 1 ? pair : pair / groups, r0 = groups == 1 ? 0 : pair % groups * ROWS;
-    const int nrows = s.n * a.group - r0 < ROWS ? s.n * a.group - r0 : ROWS;
+    const int hk = groups == 1 ? pair : pair / groups, g0 = groups == 1 ? 0 : pair % groups * rows;
+    const int grows = s.n * a.group - g0 < rows ? s.n * a.group - g0 : rows;  // rows of the group, and of them this wave's
+    const int r0 = g0 + 16 * row_tile, nrows = grows - 16 * row_tile < 16 ? grows - 16 * row_tile : 16;
     const int p_lo = MULTI ? s.pos0 + r0 / a.group : s.pos0, p_hi = MULTI ? s.pos0 + (r0 + nrows - 1) / a.group : s.pos0;
-    if (first && sa.splits && threadIdx.x == 0) {
-      Cut d{};
-      if (u0 > 0) {
-        const int from = u - u0;
-        d.first = deal.worker(from);
-        d.last = deal.worker(from + units - 1);
-        d.first_slot = from <= deal.first(d.first) ? 0 : 1;
-        d.rows = d.first == (int)blockIdx.x - 1 ? nrows : 0;
-        d.row0 = s.row0;
-        d.pair_row0 = r0;
-        d.head = hk;
-      }
-      *cut = d;
-    }
-
-    // the rows: operand of the scores, and each lane's position
-    v4i q[RT][QS];
-    int pos[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = r0 + rt * 16 + c16;
-      const bool in = rt * 16 + c16 < nrows;
-      const int i = MULTI && in ? r / a.group : 0, h = in ? r - i * a.group : 0;
-      pos[rt] = in ? s.pos0 + i : -1;
-      const char* src = a.q + (s.row0 + i) * a.q_row + (hk * a.group + h) * a.q_head;
-#pragma unroll
-      for (int x = 0; x < QS; ++x) {
-        // element order of the reduction: that in which the keys come (e4m3: 16 bytes are two steps)
-        const int el = E4M3 ? (x / 2) * 64 + g * 16 + (x % 2) * 8 : x * 32 + g * 8;
-        q[rt][x] = *(const v4i*)(src + el * 2);
-        q[rt][x] = in ? q[rt][x] : v4i{0, 0, 0, 0};
-      }
-    }
-    v4f o[RT][ND];
-    float m[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      m[rt] = -__builtin_inff();
-      l[rt] = 0.0f;
-#pragma unroll
-      for (int n = 0; n < ND; ++n) o[rt][n] = v4f{0, 0, 0, 0};
-    }
-
-    const int end = u1 << sa.unit_shift < t.count ? u1 << sa.unit_shift : t.count;
+    const int end = SHARED && nrows <= 0 ? 0 : u1 << sa.unit_shift < t.count ? u1 << sa.unit_shift : t.count;
     const int in_page = (1 << a.page_shift) - 1;
     const auto row = (const __attribute__((address_space(4))) int*)(uintptr_t)(a.table + b * a.table_stride);
     const auto key_of = [&](int tile) { return (tile < t.sink_tiles ? tile : tile + t.skip) * TILE; };
@@ -225,6 +189,30 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
         pg[h] = tile < end && k < s.len && (unsigned)n < (unsigned)a.pages ? n : -1;
       }
     };
+    int tile = (u0 << sa.unit_shift) + sub;
+    int pg[2], pg_next[2];
+    pages_of(tile, pg);
+    // the rows: operand of the scores, and each lane's position
+    v4i q[QS];
+    const bool valid = c16 < nrows;
+    int pos;
+    {
+      const int r = r0 + c16, i = MULTI && valid ? r / a.group : 0, h = valid ? r - i * a.group : 0;
+      pos = valid ? s.pos0 + i : -1;
+      const char* src = a.q + (s.row0 + i) * a.q_row + (hk * a.group + h) * a.q_head;
+#pragma unroll
+      for (int x = 0; x < QS; ++x) {
+        // element order of the reduction: that in which the keys come (e4m3: 16 bytes are two steps)
+        const int el = E4M3 ? (x / 2) * 64 + g * 16 + (x % 2) * 8 : x * 32 + g * 8;
+        q[x] = *(const v4i*)(src + el * 2);
+        q[x] = valid ? q[x] : v4i{0, 0, 0, 0};
+      }
+    }
+    v4f o[ND];
+    float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+    for (int n = 0; n < ND; ++n) o[n] = v4f{0, 0, 0, 0};
+
     // Every iteration makes the same loads, so that the wait for one of them never waits for those after it; of a half that is
     // not there (behind the end, too) they come back as zeros without a request: a buffer of no bytes.
     const auto buffer = [&](const char* at, bool there) {
@@ -237,6 +225,8 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
     int v_lane[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v_lane[j] = (4 * g + j) * a.v_slot + c16 * (VW * 4);
+    // (NT: read once, kept from pushing other things out of the caches.  64 sequences of up to 8000 keys 197 us without, 182 with)
+    constexpr int NT = SHARED ? 0 : 2;
     const auto load_k = [&](int tile, const int* pg) {
       const int k0 = key_of(tile);
 #pragma unroll
@@ -244,12 +234,12 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
         const int64_t page = pg[h] < 0 ? 0 : pg[h], slot = (k0 + 16 * h) & in_page;
         const auto src = buffer(a.k + page * a.k_page + hk * a.k_head + slot * a.k_slot, pg[h] >= 0);
 #pragma unroll
-        for (int x = 0; x < KW; ++x) kr[h][x] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(src, k_lane + x * 64, 0, 0));
+        for (int x = 0; x < KW; ++x) kr[h][x] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(src, k_lane + x * 64, 0, NT));
         if constexpr (E4M3) {
           const auto ks = buffer((const char*)(a.ks + page * a.ks_page + hk * a.ks_head + slot), pg[h] >= 0);
           const auto vs = buffer((const char*)(a.vs + page * a.vs_page + hk * a.vs_head + slot), pg[h] >= 0);
-          ksr[h] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(ks, 16 * g, 0, 0));
-          vsr[h] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(vs, 16 * g, 0, 0));
+          ksr[h] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(ks, 16 * g, 0, NT));
+          vsr[h] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(vs, 16 * g, 0, NT));
         }
       }
     };
@@ -262,14 +252,14 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t* to = vr[4 * h + j];
-          if constexpr (VW == 1) to[0] = __builtin_amdgcn_raw_buffer_load_b32(src, v_lane[j], 0, 0);
+          if constexpr (VW == 1) to[0] = __builtin_amdgcn_raw_buffer_load_b32(src, v_lane[j], 0, NT);
           else if constexpr (VW == 2) {
-            const auto u = __builtin_amdgcn_raw_buffer_load_b64(src, v_lane[j], 0, 0);
+            const auto u = __builtin_amdgcn_raw_buffer_load_b64(src, v_lane[j], 0, NT);
             __builtin_memcpy(to, &u, 8);
           } else {
 #pragma unroll
             for (int x = 0; x < VW / 4; ++x) {
-              const auto u = __builtin_amdgcn_raw_buffer_load_b128(src, v_lane[j] + 16 * x, 0, 0);
+              const auto u = __builtin_amdgcn_raw_buffer_load_b128(src, v_lane[j] + 16 * x, 0, NT);
               __builtin_memcpy(to + 4 * x, &u, 16);
             }
           }
@@ -277,22 +267,32 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
       }
     };
 
-    int tile = (u0 << sa.unit_shift) + wave;
-    int pg[2], pg_next[2];
     if (tile < end) {
-      pages_of(tile, pg);
       load_k(tile, pg);
       load_v(tile, pg);
-      pages_of(tile + WAVES, pg_next);
+      pages_of(tile + waves, pg_next);
     }
-    for (; tile < end; tile += WAVES) {
+    if (first && sa.splits && threadIdx.x == 0) {
+      Cut d{};
+      if (u0 > 0) {
+        const int from = u - u0;
+        d.first = deal.worker(from);
+        d.last = deal.worker(from + units - 1);
+        d.first_slot = from <= deal.first(d.first) ? 0 : 1;
+        d.rows = d.first == (int)blockIdx.x - 1 ? grows : 0;
+        d.row0 = s.row0;
+        d.pair_row0 = g0;
+        d.head = hk;
+      }
+      *cut = d;
+    }
+    for (; tile < end; tile += waves) {
       const int k0 = key_of(tile);
       // S^T
-      v4f st[RT][2];
+      v4f st[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) st[rt][h] = v4f{0, 0, 0, 0};
+        st[h] = v4f{0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < QS; ++x) {
           v4i kx;
@@ -305,8 +305,7 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
           } else {
             kx = kr[h][x];
           }
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) st[rt][h] = mfma16<QT>(kx, q[rt][x], st[rt][h]);
+          st[h] = mfma16<QT>(kx, q[x], st[h]);
         }
       }
       v4f ks[2], vs[2];
@@ -319,59 +318,50 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
       }
       const bool there0 = pg[0] >= 0, there1 = pg[1] >= 0;
       const bool whole = there0 && there1 && k0 + TILE <= s.len && sees_all(a, p_lo, p_hi, k0, k0 + TILE - 1);
-      const int more = tile + WAVES;
+      const int more = tile + waves;
       pg[0] = pg_next[0];
       pg[1] = pg_next[1];
       load_k(more, pg);
-      pages_of(more + WAVES, pg_next);
+      pages_of(more + waves, pg_next);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) st[rt][h][i] *= E4M3 ? ks[h][i] : a.c;
+        for (int i = 0; i < 4; ++i) st[h][i] *= E4M3 ? ks[h][i] : a.c;
       if (!whole) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const Bounds bd = bounds_of(a, pos[rt], pos[rt], s.len, k0 + 4 * g);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              st[rt][h][i] = (h ? there1 : there0) && inside(bd, 16 * h + i) ? st[rt][h][i] : -__builtin_inff();
-        }
-      }
-      v4i pb[RT], pl[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float top = fmaxf(fmaxf(fmaxf(st[rt][0][0], st[rt][0][1]), fmaxf(st[rt][0][2], st[rt][0][3])),
-                          fmaxf(fmaxf(st[rt][1][0], st[rt][1][1]), fmaxf(st[rt][1][2], st[rt][1][3])));
-        top = max_x32(max_x16(top));
-        const float m_new = fmaxf(m[rt], top), ms = safe_max(m_new);
-        if (__any(m_new > m[rt])) {
-          const float f = exp2_hw(m[rt] - ms);
-#pragma unroll
-          for (int n = 0; n < ND; ++n) o[rt][n] *= f;
-          l[rt] *= f;
-          m[rt] = m_new;
-        }
-        float pr[8];
+        const Bounds bd = bounds_of(a, pos, pos, s.len, k0 + 4 * g);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = exp2_hw(st[rt][h][i] - ms);
-            l[rt] += x;
-            // (a key that the row does not see counts nothing, whatever its scale holds)
-            pr[4 * h + i] = E4M3 ? (whole || st[rt][h][i] != -__builtin_inff() ? x * vs[h][i] : 0.0f) : x;
-          }
+          for (int i = 0; i < 4; ++i) st[h][i] = (h ? there1 : there0) && inside(bd, 16 * h + i) ? st[h][i] : -__builtin_inff();
+      }
+      float top = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
+                        fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
+      top = max_x32(max_x16(top));
+      const float m_new = fmaxf(m, top), ms = safe_max(m_new);
+      if (__any(m_new > m)) {
+        const float f = exp2_hw(m - ms);
+#pragma unroll
+        for (int n = 0; n < ND; ++n) o[n] *= f;
+        l *= f;
+        m = m_new;
+      }
+      float pr[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t hi = pack2<PT>(pr[2 * i], pr[2 * i + 1]);
-          pb[rt][i] = (int)hi;
-          if constexpr (TWO)
-            pl[rt][i] = (int)pack2<PT>(pr[2 * i] - __uint_as_float(hi << 16), pr[2 * i + 1] - __uint_as_float(hi & 0xffff0000u));
+          const float x = exp2_hw(st[h][i] - ms);
+          l += x;
+          // (a key that the row does not see counts nothing, whatever its scale holds)
+          pr[4 * h + i] = E4M3 ? (whole || st[h][i] != -__builtin_inff() ? x * vs[h][i] : 0.0f) : x;
         }
+      v4i pb, pl;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t hi = pack2<PT>(pr[2 * i], pr[2 * i + 1]);
+        pb[i] = (int)hi;
+        if constexpr (TWO)
+          pl[i] = (int)pack2<PT>(pr[2 * i] - __uint_as_float(hi << 16), pr[2 * i + 1] - __uint_as_float(hi & 0xffff0000u));
       }
       // O^T
       uint32_t vw[8][ND / 2];
@@ -409,11 +399,8 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           const v4i f = {column(n, 0), column(n, 1), column(n, 2), column(n, 3)};
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            o[rt][n] = mfma16<PT>(f, pb[rt], o[rt][n]);
-            if constexpr (TWO) o[rt][n] = mfma16<PT>(f, pl[rt], o[rt][n]);
-          }
+          o[n] = mfma16<PT>(f, pb, o[n]);
+          if constexpr (TWO) o[n] = mfma16<PT>(f, pl, o[n]);
         }
       } else {
 #pragma unroll 1
@@ -429,84 +416,67 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
             v4i f;
 #pragma unroll
             for (int x = 0; x < 4; ++x) f[x] = column(n, x) & (int)keep[x];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              v4f d = mfma16<PT>(f, pb[rt], o[rt][n]);
-              if constexpr (TWO) d = mfma16<PT>(f, pl[rt], d);
-              if (rt * 16 + c16 == r) o[rt][n] = d;
-            }
+            v4f y = mfma16<PT>(f, pb, o[n]);
+            if constexpr (TWO) y = mfma16<PT>(f, pl, y);
+            if (c16 == r) o[n] = y;
           }
         }
       }
       load_v(more, pg);
     }
 
-    // the four waves' shares: 2 and 3 into 0 and 1, then 1 into 0
+    // the shares of the waves of a row tile: the upper half into the lower one, until one is left
+    l = sum_x32(sum_x16(l));
+    for (int half = waves / 2; half >= 1; half /= 2) {
+      if (sub >= half && sub < 2 * half) {
+        float* to = join[row_tile * half + sub - half] + lane;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) l[rt] = sum_x32(sum_x16(l[rt]));
+        for (int n = 0; n < ND; ++n)
 #pragma unroll
-    for (int half = 2; half >= 1; half /= 2) {
-      if (wave >= half && wave < 2 * half) {
-        float* to = join[wave - half] + lane;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-          for (int n = 0; n < ND; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[((rt * ND + n) * 4 + i) * 64] = o[rt][n][i];
-          to[(RT * ND * 4 + 2 * rt) * 64] = m[rt];
-          to[(RT * ND * 4 + 2 * rt + 1) * 64] = l[rt];
-        }
+          for (int i = 0; i < 4; ++i) to[(n * 4 + i) * 64] = o[n][i];
+        to[ND * 4 * 64] = m;
+        to[(ND * 4 + 1) * 64] = l;
       }
       __syncthreads();
-      if (wave < half) {
-        const float* from = join[wave] + lane;
+      if (sub < half) {
+        const float* from = join[row_tile * half + sub] + lane;
+        const float m2 = from[ND * 4 * 64], l2 = from[(ND * 4 + 1) * 64];
+        const float mx = fmaxf(m, m2), ms = safe_max(mx);
+        const float f1 = exp2_hw(m - ms), f2 = exp2_hw(m2 - ms);
+        m = mx;
+        l = l * f1 + l2 * f2;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const float m2 = from[(RT * ND * 4 + 2 * rt) * 64], l2 = from[(RT * ND * 4 + 2 * rt + 1) * 64];
-          const float mx = fmaxf(m[rt], m2), ms = safe_max(mx);
-          const float f1 = exp2_hw(m[rt] - ms), f2 = exp2_hw(m2 - ms);
-          m[rt] = mx;
-          l[rt] = l[rt] * f1 + l2 * f2;
+        for (int n = 0; n < ND; ++n)
 #pragma unroll
-          for (int n = 0; n < ND; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[rt][n][i] = o[rt][n][i] * f1 + from[((rt * ND + n) * 4 + i) * 64] * f2;
-        }
+          for (int i = 0; i < 4; ++i) o[n][i] = o[n][i] * f1 + from[(n * 4 + i) * 64] * f2;
       }
       __syncthreads();
     }
-    if (wave == 0) {
-      const bool complete = u0 == 0 && u1 == units;
-      float* share = slot_of<ROWS, D>(sa, blockIdx.x, first ? 0 : 1);
+    if (sub == 0 && valid) {
+      if (u0 == 0 && u1 == units) {
+        const int r = r0 + c16, i = MULTI ? r / a.group : 0, h = r - i * a.group;
+        char* to = a.out + (s.row0 + i) * a.o_row + (hk * a.group + h) * a.o_head;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const int r = rt * 16 + c16;
-        if (r >= nrows) continue;
-        if (complete) {
-          const int i = MULTI ? (r0 + r) / a.group : 0, h = r0 + r - i * a.group;
-          char* to = a.out + (s.row0 + i) * a.o_row + (hk * a.group + h) * a.o_head;
-          const float inv = l[rt] == 0.0f ? 0.0f : 1.0f / l[rt];
+        for (int i4 = 0; i4 < 4; ++i4) {
+          uint32_t y[ND / 2];
 #pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            uint32_t y[ND / 2];
+          for (int n = 0; n < ND; n += 2) y[n / 2] = l == 0.0f ? 0u : pack2<QT>(o[n][i4] * inv, o[n + 1][i4] * inv);
+          __builtin_memcpy(to + (4 * g + i4) * ND * 2, y, ND * 2);
+        }
+      } else {
+        const int r = 16 * row_tile + c16;
+        float* share = slot_of<D>(sa, blockIdx.x, first ? 0 : 1);
 #pragma unroll
-            for (int n = 0; n < ND; n += 2)
-              y[n / 2] = l[rt] == 0.0f ? 0u : pack2<QT>(o[rt][n][i4] * inv, o[rt][n + 1][i4] * inv);
-            __builtin_memcpy(to + (4 * g + i4) * ND * 2, y, ND * 2);
-          }
-        } else {
+        for (int i4 = 0; i4 < 4; ++i4) {
+          float y[ND];
 #pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            float y[ND];
-#pragma unroll
-            for (int n = 0; n < ND; ++n) y[n] = o[rt][n][i4];
-            __builtin_memcpy(share + r * D + (4 * g + i4) * ND, y, ND * 4);
-          }
-          if (g == 0) {
-            share[ROWS * D + 2 * r] = m[rt];
-            share[ROWS * D + 2 * r + 1] = l[rt];
-          }
+          for (int n = 0; n < ND; ++n) y[n] = o[n][i4];
+          __builtin_memcpy(share + r * D + (4 * g + i4) * ND, y, ND * 4);
+        }
+        if (g == 0) {
+          share[rows * D + 2 * r] = m;
+          share[rows * D + 2 * r + 1] = l;
         }
       }
     }
@@ -516,21 +486,21 @@ __global__ __launch_bounds__(256, RT * D > 128 ? 1 : 2) void paged_split_kernel(
 
 // Joins the shares of the pairs that were cut: a block per cut and row.  The weights of all shares first (a share per thread), then
 // every group of D / 4 threads adds up every (1024 / D)-th share: loads that wait for nothing but the weights.
-template <int QT, int D, int ROWS>
+template <int QT, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
   constexpr int LG = D / 4, GROUPS = 256 / LG;
-  __shared__ float weight[MAX_WORKERS];
+  __shared__ float2 weight[MAX_WORKERS];
   __shared__ float red[8];
   __shared__ __attribute__((aligned(16))) float sum[GROUPS][D];
   const PagedArgs& a = sa.p;
   const Cut d = ((const Cut*)sa.ws)[blockIdx.x];
-  const int shares = d.last - d.first + 1, tid = threadIdx.x, wave = tid >> 6;
+  const int shares = d.last - d.first + 1, rows = 16 << sa.row_shift, tid = threadIdx.x, wave = tid >> 6;
   for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
-    const auto share = [&](int k) { return slot_of<ROWS, D>(sa, d.first + k, k == 0 ? d.first_slot : 0); };
+    const auto share = [&](int k) { return slot_of<D>(sa, d.first + k, k == 0 ? d.first_slot : 0); };
     float top = -__builtin_inff();
     for (int k = tid; k < shares; k += 256) {
-      weight[k] = share(k)[ROWS * D + 2 * r];
-      top = fmaxf(top, weight[k]);
+      weight[k] = *(const float2*)(share(k) + rows * D + 2 * r);
+      top = fmaxf(top, weight[k].x);
     }
     top = wave_max(top);
     if ((tid & 63) == 0) red[wave] = top;
@@ -538,9 +508,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
     const float ms = safe_max(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
     float l = 0.0f;
     for (int k = tid; k < shares; k += 256) {
-      const float f = exp2_hw(weight[k] - ms);
-      weight[k] = f;
-      l += share(k)[ROWS * D + 2 * r + 1] * f;
+      const float f = exp2_hw(weight[k].x - ms);
+      weight[k].x = f;
+      l += weight[k].y * f;
     }
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) l += __shfl_xor(l, o);
@@ -550,7 +520,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
     const int c = tid % LG;
     v4f o = {0, 0, 0, 0};
 #pragma unroll 4
-    for (int k = tid / LG; k < shares; k += GROUPS) o += *(const v4f*)(share(k) + r * D + 4 * c) * weight[k];
+    for (int k = tid / LG; k < shares; k += GROUPS) o += *(const v4f*)(share(k) + r * D + 4 * c) * weight[k].x;
     *(v4f*)&sum[tid / LG][4 * c] = o;
     __syncthreads();
     if (tid < LG) {
@@ -651,27 +621,29 @@ int fmsmo_paged_args(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batc
 
 // How a call is run, from what the host knows of it: bounds of the new rows and of the keys of a sequence.
 struct Plan {
-  bool prompt;   // the kernel of many rows
-  int row_tiles; // of the split kernel
-  int workers, unit_shift;
+  bool prompt;  // the kernel of many rows
+  int row_shift, unit_shift, workers;
+  bool splits;
 };
 static Plan plan_of(int group, int kv_heads, int dim, int64_t seqs, int64_t rows, int64_t max_rows, int64_t max_keys) {
   Plan p{};
   const int64_t most = max_rows * group;
-  p.prompt = most > 64;
-  p.row_tiles = most <= 16 ? 1 : 2;
-  const int64_t tiles = std::max<int64_t>(1, (max_keys + TILE - 1) / TILE);
-  const int64_t pairs = std::max<int64_t>(1, std::min(seqs, rows)) * kv_heads * ((most + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
-  p.unit_shift = WAVES_SHIFT;
-  if (tiles <= 2 * WAVES) p.unit_shift = 26;  // nothing to split: one launch
+  p.prompt = most > 16 * WAVES;
+  p.row_shift = most <= 16 ? 0 : most <= 32 ? 1 : 2;
+  const int64_t tiles = std::max<int64_t>(1, (max_keys + TILE - 1) / TILE), waves = WAVES >> p.row_shift;
+  const int64_t pairs = std::max<int64_t>(1, std::min(seqs, rows)) * kv_heads;
+  // One launch where a block per pair is through as early as the second launch would be: it takes 4 us, an iteration of
+  // all waves 1.5 to 2 us while memory is not busy.  Single tokens, 8 key heads of 128 elements, one launch / two: 1 sequence of 400 keys
+  // 11.6 / 9.6 us, 8 of them 13.1 / 10.9, 32 of them 15.4 / 18.6.
+  p.splits = tiles > waves && !(pairs >= 192 && tiles <= 4 * waves);
+  p.unit_shift = p.splits ? 2 - p.row_shift : 26;
   const int64_t units = pairs * (((tiles - 1) >> p.unit_shift) + 1);
-  // as many as are resident: the kernels whose registers leave room for one block per compute unit get half
-  const int resident = p.row_tiles * dim > 128 ? MAX_WORKERS / 2 : MAX_WORKERS;
-  p.workers = (int)std::min<int64_t>(p.unit_shift > WAVES_SHIFT ? 65536 : resident, units);
+  // as many as are resident: two blocks per compute unit, one where the registers leave room for one
+  p.workers = (int)std::min<int64_t>(!p.splits ? 65536 : dim > 128 ? MAX_WORKERS / 2 : MAX_WORKERS, units);
   return p;
 }
 static int64_t plan_bytes(const Plan& p, int dim) {
-  return p.prompt || p.unit_shift > WAVES_SHIFT ? 0 : p.workers * ((int64_t)sizeof(Cut) + 2 * 16 * p.row_tiles * (dim + 2) * 4);
+  return p.prompt || !p.splits ? 0 : p.workers * ((int64_t)sizeof(Cut) + (2 * 16 * (dim + 2) * 4ll << p.row_shift));
 }
 static void bounds(int64_t& max_rows, int64_t& max_keys, int64_t rows, int64_t cap, bool ragged) {
   if (!ragged) max_rows = 1;
@@ -708,30 +680,31 @@ extern "C" int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_ba
   if (need > workspace_bytes || (need && !workspace)) return FMSMO_ERR_SCRATCH;
   if (((uintptr_t)workspace) & 15) return FMSMO_ERR_ALIGN;
   // (units are counted in 31 bits: heads x groups of rows x units of a sequence, summed)
-  const int64_t pairs = (rows * a.group / (16 * p.row_tiles) + a.seqs) * a.kv_heads;
-  if (pairs > 0x7fffffffll / 32 || pairs * ((a.cap / TILE >> p.unit_shift) + 2) > 0x7fffffffll) return FMSMO_ERR_UNSUPPORTED;
+  const int64_t pairs = ((rows * a.group >> (4 + p.row_shift)) + a.seqs) * a.kv_heads;
+  if (pairs * ((a.cap / TILE >> p.unit_shift) + 2) > 0x7fffffffll) return FMSMO_ERR_UNSUPPORTED;
   sa.ws = (float*)workspace;
   sa.workers = p.workers;
   sa.unit_shift = p.unit_shift;
-  sa.splits = need > 0;
-  const auto go = [&](auto t, auto e, auto d, auto r) {
-    constexpr int T = decltype(t)::value, D = decltype(d)::value, RT = decltype(r)::value;
+  sa.splits = p.splits;
+  sa.row_shift = p.row_shift;
+  const auto go = [&](auto t, auto e, auto d) {
+    constexpr int T = decltype(t)::value, D = decltype(d)::value;
     constexpr bool E = decltype(e)::value;
-    if (a.starts) hipLaunchKernelGGL((paged_split_kernel<T, E, D, RT, true>), dim3(p.workers), dim3(256), 0, (hipStream_t)stream, sa);
-    else hipLaunchKernelGGL((paged_split_kernel<T, E, D, RT, false>), dim3(p.workers), dim3(256), 0, (hipStream_t)stream, sa);
-    if (need) {
-      const unsigned per = (unsigned)std::min<int64_t>(max_rows * a.group, 16 * RT);  // rows of a group, as a rule
-      hipLaunchKernelGGL((paged_join_kernel<T, D, 16 * RT>), dim3(p.workers, per), dim3(256), 0, (hipStream_t)stream, sa);
+    const dim3 grid(p.workers), threads(64 * WAVES);
+    const hipStream_t s = (hipStream_t)stream;
+    if (a.starts && p.row_shift) hipLaunchKernelGGL((paged_split_kernel<T, E, D, true, true>), grid, threads, 0, s, sa);
+    else if (a.starts) hipLaunchKernelGGL((paged_split_kernel<T, E, D, true, false>), grid, threads, 0, s, sa);
+    else if (p.row_shift) hipLaunchKernelGGL((paged_split_kernel<T, E, D, false, true>), grid, threads, 0, s, sa);
+    else hipLaunchKernelGGL((paged_split_kernel<T, E, D, false, false>), grid, threads, 0, s, sa);
+    if (p.splits) {
+      const unsigned per = (unsigned)std::min<int64_t>(max_rows * a.group, 16 << p.row_shift);  // rows of a group, as a rule
+      hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(p.workers, per), dim3(256), 0, s, sa);
     }
   };
-  const auto tiles = [&](auto t, auto e, auto d) {
-    if (p.row_tiles == 1) go(t, e, d, std::integral_constant<int, 1>{});
-    else go(t, e, d, std::integral_constant<int, 2>{});
-  };
   const auto dims = [&](auto t, auto e) {
-    if (cache->dim == 64) tiles(t, e, std::integral_constant<int, 64>{});
-    else if (cache->dim == 128) tiles(t, e, std::integral_constant<int, 128>{});
-    else tiles(t, e, std::integral_constant<int, 256>{});
+    if (cache->dim == 64) go(t, e, std::integral_constant<int, 64>{});
+    else if (cache->dim == 128) go(t, e, std::integral_constant<int, 128>{});
+    else go(t, e, std::integral_constant<int, 256>{});
   };
   const auto types = [&](auto t) {
     if (e4m3) dims(t, std::true_type{});
