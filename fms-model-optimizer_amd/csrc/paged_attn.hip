@@ -85,20 +85,6 @@ __device__ __forceinline__ float* slot_of(const SplitArgs& a, int worker, int sl
   return (float*)((Cut*)a.ws + a.workers) + (((int64_t)(2 * worker + slot) * 16 * (D + 2)) << a.row_shift);
 }
 
-// Rows of a lane's keys that may be seen, as bounds of their offsets 16 h + i in the tile (from which 4 g is taken away):
-// offset <= hi and (offset > lo or offset < sink)
-struct Bounds {
-  int hi, lo, sink;
-};
-__device__ __forceinline__ Bounds bounds_of(const PagedArgs& a, int p_lo, int p_hi, int len, int at) {
-  Bounds b;
-  b.hi = (p_hi < len - 1 ? p_hi : len - 1) - at;
-  b.lo = a.window ? p_lo - a.window - at : -(1 << 30);
-  b.sink = a.sinks - at;
-  return b;
-}
-__device__ __forceinline__ bool inside(const Bounds& b, int off) { return off <= b.hi && (off > b.lo || off < b.sink); }
-
 // MULTI: rows of a group may stand at different positions.  SHARED: row_shift > 0
 template <int QT, bool E4M3, int D, bool MULTI, bool SHARED>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(SplitArgs sa) {
@@ -210,6 +196,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
     }
     v4f o[ND];
     float m = -__builtin_inff(), l = 0.0f;
+    bool odd = false;  // (MULTI) infinities or NaN among the values of keys that some rows see
 #pragma unroll
     for (int n = 0; n < ND; ++n) o[n] = v4f{0, 0, 0, 0};
 
@@ -375,54 +362,61 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
           for (int x = 0; x < VW; ++x) vw[j][x] = vr[j][x];
         }
       }
-      bool apart = false;
       if (!whole) {
-        // what no row sees may hold anything, and 0 * inf is not 0: such values count as zero.  Where rows see different keys, a
-        // value that is not finite goes to those only that see it (below).
+        // what no row sees may hold anything
         const Bounds bd = bounds_of(a, p_lo, p_hi, s.len, k0 + 4 * g);
-        uint32_t fine = 0x80008000u;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool in = (j / 4 ? there1 : there0) && inside(bd, 16 * (j / 4) + j % 4);
 #pragma unroll
           for (int x = 0; x < ND / 2; ++x) {
             vw[j][x] = in ? vw[j][x] : 0u;
-            if constexpr (MULTI) fine &= finite2<PT>(vw[j][x]);
+            if constexpr (MULTI) {
+              const uint32_t u = finite_only<PT>(vw[j][x]);
+              odd = odd || u != vw[j][x];
+              vw[j][x] = u;
+            }
           }
         }
-        if constexpr (MULTI) apart = p_lo != p_hi && __any(fine != 0x80008000u);
       }
       const auto column = [&](int n, int x) {  // words x of column n: keys 2 x and 2 x + 1 of the lane's eight
         return (int)__builtin_amdgcn_perm(vw[2 * x + 1][n / 2], vw[2 * x][n / 2], n % 2 ? 0x07060302u : 0x05040100u);
       };
-      if (!MULTI || !apart) {
 #pragma unroll
-        for (int n = 0; n < ND; ++n) {
-          const v4i f = {column(n, 0), column(n, 1), column(n, 2), column(n, 3)};
-          o[n] = mfma16<PT>(f, pb, o[n]);
-          if constexpr (TWO) o[n] = mfma16<PT>(f, pl, o[n]);
-        }
-      } else {
+      for (int n = 0; n < ND; ++n) {
+        const v4i f = {column(n, 0), column(n, 1), column(n, 2), column(n, 3)};
+        o[n] = mfma16<PT>(f, pb, o[n]);
+        if constexpr (TWO) o[n] = mfma16<PT>(f, pl, o[n]);
+      }
+      load_v(more, pg);
+    }
+    if (MULTI && __any(odd)) {
 #pragma unroll 1
-        for (int r = 0; r < nrows; ++r) {  // one row at a time, with the values it sees
-          const int p = s.pos0 + (r0 + r) / a.group;
-          const Bounds bd = bounds_of(a, p, p, s.len, k0 + 4 * g);
-          uint32_t keep[4];  // halves: keys 2 x and 2 x + 1
+      for (int again = (u0 << sa.unit_shift) + sub; again < end; again += waves) {
+        const int k0 = key_of(again);
+        int pages[2];
+        pages_of(again, pages);
+        if (pages[0] >= 0 && pages[1] >= 0 && k0 + TILE <= s.len && sees_all(a, p_lo, p_hi, k0, k0 + TILE - 1)) continue;
+#pragma unroll 1
+        for (int i = 0; i < TILE; ++i) {
+          const int key = k0 + i, page = i < 16 ? pages[0] : pages[1];
+          if (page < 0 || key >= s.len) continue;
+          const bool seen = valid && inside(bounds_of(a, pos, pos, s.len, key), 0);
+          const char* src = a.v + page * a.v_page + hk * a.v_head + (int64_t)(key & in_page) * a.v_slot;
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            keep[x] = (inside(bd, 16 * (x / 2) + 2 * (x % 2)) ? 0xffffu : 0u) | (inside(bd, 16 * (x / 2) + 2 * (x % 2) + 1) ? 0xffff0000u : 0u);
+          for (int i4 = 0; i4 < 4; ++i4) {
+            uint32_t u[ND / 2];
+            if constexpr (E4M3) {
 #pragma unroll
-          for (int n = 0; n < ND; ++n) {
-            v4i f;
+              for (int x = 0; x < ND / 4; ++x) widen4<PT>(*(const uint32_t*)(src + (4 * g + i4) * ND + 4 * x), u[2 * x], u[2 * x + 1]);
+            } else {
+              __builtin_memcpy(u, src + (4 * g + i4) * ND * 2, ND * 2);
+            }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) f[x] = column(n, x) & (int)keep[x];
-            v4f y = mfma16<PT>(f, pb, o[n]);
-            if constexpr (TWO) y = mfma16<PT>(f, pl, y);
-            if (c16 == r) o[n] = y;
+            for (int n = 0; n < ND; ++n) o[n][i4] = add_odd<PT>(o[n][i4], (u16)(u[n / 2] >> 16 * (n % 2)), seen);
           }
         }
       }
-      load_v(more, pg);
     }
 
     // the shares of the waves of a row tile: the upper half into the lower one, until one is left

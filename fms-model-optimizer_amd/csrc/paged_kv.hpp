@@ -95,17 +95,24 @@ __device__ __forceinline__ Tiles tiles_of(const PagedArgs& a, int len, int p_lo,
   t.count = all - t.skip > t.sink_tiles ? all - t.skip : t.sink_tiles;
   return t;
 }
-__device__ __forceinline__ bool sees(const PagedArgs& a, int p, int j) {
-  return j <= p && (a.window == 0 || j > p - a.window || j < a.sinks);
-}
-// some row of positions p_lo .. p_hi sees key j
-__device__ __forceinline__ bool sees_one(const PagedArgs& a, int p_lo, int p_hi, int j) {
-  return j <= p_hi && (a.window == 0 || j > p_lo - a.window || j < a.sinks);
-}
 // every row of positions p_lo .. p_hi sees every key of j0 .. j1
 __device__ __forceinline__ bool sees_all(const PagedArgs& a, int p_lo, int p_hi, int j0, int j1) {
   return j1 <= p_lo && (a.window == 0 || j0 > p_hi - a.window || j1 < a.sinks);
 }
+
+// The keys that rows at positions p_lo .. p_hi may see (some of them, p_lo < p_hi), as bounds of their offsets from key `at`:
+// offset <= hi and (offset > lo or offset < sink)
+struct Bounds {
+  int hi, lo, sink;
+};
+__device__ __forceinline__ Bounds bounds_of(const PagedArgs& a, int p_lo, int p_hi, int len, int at) {
+  Bounds b;
+  b.hi = (p_hi < len - 1 ? p_hi : len - 1) - at;
+  b.lo = a.window ? p_lo - a.window - at : -(1 << 30);
+  b.sink = a.sinks - at;
+  return b;
+}
+__device__ __forceinline__ bool inside(const Bounds& b, int off) { return off <= b.hi && (off > b.lo || off < b.sink); }
 
 // ------------------------------------------------------------------ cross-lane
 // a maximum (sum) over the lanes that differ in bit 5, and in bits 5 and 4: v_permlane*_swap, no LDS round trip
@@ -126,6 +133,11 @@ __device__ __forceinline__ float sum_x16(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// 16 bytes a lane from `at` + off into 1 KiB of shared memory, lane after lane
+__device__ __forceinline__ void to_shared(const char* at, char* lds, int off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)at, 0, 0x7fffffff, 0x00020000), FMSMO_LPTR(lds), 16, off, 0, 0, 0);
+}
 
 // ------------------------------------------------------------------ 16-bit operands
 // two fp32 values rounded to nearest even, packed
@@ -158,11 +170,17 @@ __device__ __forceinline__ void widen4(uint32_t u, uint32_t& lo, uint32_t& hi) {
     __builtin_memcpy(&hi, &b, 4);
   }
 }
-// bits 15 and 31 stay set while both halves of every word it was folded over are finite
+// Infinities and NaN among the values of keys that some rows see and others don't: 0 * inf is not 0, so they leave the product
+// (finite_only), and are added to the rows that see them behind the loop over the keys (add_odd) -- to which they are all that matters.
 template <int T>
-__device__ __forceinline__ uint32_t finite2(uint32_t u) {
-  constexpr uint32_t E = T == FMSMO_F16 ? 0x7c007c00u : 0x7f807f80u;
-  return ((u & E) ^ E) + 0x7fff7fffu;
+__device__ __forceinline__ uint32_t finite_only(uint32_t u) {
+  constexpr uint32_t E = T == FMSMO_F16 ? 0x7c00u : 0x7f80u;
+  return ((u & E) == E ? 0u : u & 0xffffu) | ((u >> 16 & E) == E ? 0u : u & 0xffff0000u);
+}
+template <int T>
+__device__ __forceinline__ float add_odd(float o, u16 h, bool seen) {
+  constexpr u16 E = T == FMSMO_F16 ? 0x7c00 : 0x7f80;
+  return seen && (h & E) == E ? o + (T == FMSMO_F16 ? f16_to_f32(h) : bf16_to_f32(h)) : o;
 }
 
 // D[16 x 16] += A[16 x 32] . B[32 x 16]: lane l holds row (column) l % 16 of A (B), elements 8 (l / 16) .. + 7 of the reduction;

@@ -6,8 +6,8 @@
 //                 (lane l with l + 32) for the maximum and none for anything else,
 //   O^T = V^T P^T the scores as they stand are the second operand (the reduction's order is free), and what rescales O is a
 //                 number per lane.  V^T comes out of row-major shared memory by ds_read_b64_tr_b16.
-// Keys and values go through registers into the other of two buffers while the present one is used: the pages are looked up on
-// the way, e4m3 codes become 16-bit numbers once per block, and what nobody may see becomes zero.
+// Each wave brings 16 of a tile's keys, one page, into the other of two buffers while the present one is used: a 16-bit cache straight
+// from memory, e4m3 codes through registers, where they become 16-bit numbers once per block.
 #include "paged_kv.hpp"
 
 #include <algorithm>
@@ -19,22 +19,26 @@ constexpr int BM = 128, BN = 64;
 
 template <int QT, bool E4M3, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(PagedArgs a, int tiles_x) {
-  constexpr int PT = E4M3 ? FMSMO_BF16 : QT;  // (see the split kernel: e4m3 scales are multiplied in before the rounding)
+  // e4m3 caches: the values' scales are multiplied in before the probabilities are rounded, which takes the exponents of bf16; for
+  // an fp16 result, of which bf16 would lose three bits, they are the sum of two bf16 numbers
+  constexpr int PT = E4M3 ? FMSMO_BF16 : QT;
   constexpr bool TWO = E4M3 && QT == FMSMO_F16;
   constexpr int QS = D / 16, NV = D / 32;
-  // Strides in 16-bit elements.  Keys are read 16 bytes a lane from 32 rows, values four rows by 64 bytes an instruction: 16 and 64
-  // bytes more than a row spread both over all banks.
-  constexpr int KLD = D + 8, VLD = D + 32;
-  constexpr int CH = D * (E4M3 ? 1 : 2) / 16;  // 16-byte chunks of a row
-  constexpr int NJ = BN * CH / 256;            // of them per thread
-  __shared__ __attribute__((aligned(16))) u16 kl[2][BN * KLD];
-  __shared__ __attribute__((aligned(16))) u16 vl[2][BN * VLD];
+  // Shared memory holds rows as they are in memory, D elements; 16-byte piece c of row r lies at place c ^ f(r), by which neither the keys
+  // (16 bytes of 32 rows per instruction) nor the values (64 bytes of 8 rows) ask a bank for two things at once.
+  constexpr int ROW = 2 * D, WRAP = ROW < 256 ? 256 / ROW : 1;  // bytes of a row; rows in a turn of the banks
+  const auto key_place = [](int r) { return r / WRAP % (D == 64 ? 8 : 16); };
+  const auto value_place = [](int r) { return r / WRAP % (D == 64 ? 4 : 8) * 2; };
+  constexpr int LOADS = 16 * ROW / 1024;              // of 1 KiB for 16 rows of 16-bit numbers
+  constexpr int CODES = 16 * D / 1024;                // of e4m3
+  __shared__ __attribute__((aligned(1024))) char kl[2][BN * ROW];
+  __shared__ __attribute__((aligned(1024))) char vl[2][BN * ROW];
   __shared__ __attribute__((aligned(16))) float sc[2][2][E4M3 ? BN : 4];
   __shared__ int odd;  // values of a tile that some rows see in part held infinities or NaN
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int c32 = lane & 31, hl = lane >> 5;
-
   if (a.zero_rest) zero_rest(a, D / 8);
+
   // the tile of rows: sequence b's start at tile query_start[b] group / BM + b, which leaves room for all of them
   const int hk = blockIdx.x % a.kv_heads, x = tiles_x - 1 - blockIdx.x / a.kv_heads;
   int before = 0;
@@ -48,7 +52,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   }
   const int b = uniform(before) - 1;
   if (b < 0) return;
-  const Seq s = seq_of(a, b);
+  Seq s = seq_of(a, b);
+  s.n = uniform(s.n);
+  s.row0 = uniform(s.row0);
+  s.pos0 = uniform(s.pos0);
+  s.len = uniform(s.len);
   const int r0 = (x - (int)((int64_t)s.row0 * a.group / BM) - b) * BM;
   if (s.n == 0 || r0 < 0 || r0 >= s.n * a.group) return;
   const int nrows = s.n * a.group - r0 < BM ? s.n * a.group - r0 : BM;
@@ -60,11 +68,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   const int row = r0 + wr + c32, tok = mine ? row / a.group : 0, head = hk * a.group + (mine ? row - tok * a.group : 0);
   const int pos = mine ? s.pos0 + tok : -1;
   const int w_lo = s.pos0 + (r0 + wr) / a.group, w_hi = wn > 0 ? s.pos0 + (r0 + wr + wn - 1) / a.group : w_lo;
+  // exp2(c s - m) with c > 0, so that the maximum of c s is that of s: a negative scale turns the queries' sign
+  const float c = fmaxf(fabsf(a.c), 0x1p-126f);
   v4i q[QS];
   {
     const char* src = a.q + (s.row0 + tok) * a.q_row + head * a.q_head;
+    const int turn = a.c < 0.0f ? (int)0x80008000u : 0;
 #pragma unroll
-    for (int k = 0; k < QS; ++k) q[k] = mine ? *(const v4i*)(src + (k * 16 + hl * 8) * 2) : v4i{0, 0, 0, 0};
+    for (int k = 0; k < QS; ++k) {
+      q[k] = *(const v4i*)(src + (k * 16 + hl * 8) * 2);
+      q[k] = mine ? q[k] ^ turn : v4i{0, 0, 0, 0};
+    }
   }
   v16f o[NV];
 #pragma unroll
@@ -75,141 +89,192 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
 
   const auto key_of = [&](int tile) { return (tile < t.sink_tiles ? tile : tile + t.skip) * BN; };
   const int in_page = (1 << a.page_shift) - 1;
-  const int* table = a.table + b * a.table_stride;
-  // lane i holds the page of the tile's i-th 16 keys; -1: not there
-  const auto pages_of = [&](int tile) {
-    const int k = key_of(tile) + 16 * (lane & 3);
-    int pg = tile < t.count && k < s.len ? table[k >> a.page_shift] : -1;
-    return (unsigned)pg < (unsigned)a.pages ? pg : -1;
+  const auto table = (const __attribute__((address_space(4))) int*)(uintptr_t)(a.table + b * a.table_stride);
+  // page of a tile's i-th 16 keys; -1: not there
+  const auto page_of = [&](int tile, int i) {
+    const int k = key_of(tile) + 16 * i, n = table[(k < s.len ? k : 0) >> a.page_shift];
+    return tile < t.count && k < s.len && (unsigned)n < (unsigned)a.pages ? n : -1;
   };
-  v4i kr[NJ], vr[NJ];
-  float sr = 0.0f;
-  const auto load = [&](int tile, int pgs) {
+  const auto there_of = [&](int tile) {
+    return (page_of(tile, 0) >= 0 ? 1 : 0) | (page_of(tile, 1) >= 0 ? 2 : 0) | (page_of(tile, 2) >= 0 ? 4 : 0) | (page_of(tile, 3) >= 0 ? 8 : 0);
+  };
+  // a tile that some rows see in part
+  const auto partial = [&](int tile, int there) {
     const int k0 = key_of(tile);
+    return there != 15 || k0 + BN > s.len || !sees_all(a, p_lo, p_hi, k0, k0 + BN - 1);
+  };
+
+  // This wave's 16 keys of a tile.  16-bit caches: instruction j brings 1 KiB, lane i the 16-byte piece that belongs at its end.
+  constexpr int PIECES = ROW / 16;       // of a row
+  constexpr int RPL = 64 / PIECES;       // rows of an instruction
+  int k_off[E4M3 ? 1 : LOADS], v_off[E4M3 ? 1 : LOADS];
+  if constexpr (!E4M3) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int at = threadIdx.x + 256 * j, r = at / CH, ch = at % CH;
-      const int sub = uniform(r >> 4), page = __builtin_amdgcn_readlane(pgs, sub);
-      kr[j] = vr[j] = v4i{0, 0, 0, 0};
-      if (page >= 0 && k0 + r < s.len) {  // (anything else has to read as zero: 0 * NaN is not 0)
-        const int64_t slot = (k0 + r) & in_page;
-        kr[j] = *(const v4i*)(a.k + page * a.k_page + hk * a.k_head + slot * a.k_slot + ch * 16);
-        vr[j] = *(const v4i*)(a.v + page * a.v_page + hk * a.v_head + slot * a.v_slot + ch * 16);
-      }
+    for (int j = 0; j < LOADS; ++j) {
+      const int r = j * RPL + lane / PIECES, at = lane % PIECES;  // (16 rows further the places are the same)
+      k_off[j] = r * a.k_slot + (at ^ key_place(r)) * 16;
+      v_off[j] = r * a.v_slot + (at ^ value_place(r)) * 16;
     }
-    if constexpr (E4M3) {
-      if (wave < 2) {  // one lane per key: wave 0 the scales of the keys, wave 1 those of the values
-        const int page = __shfl(pgs, lane >> 4), slot = (k0 + lane) & in_page;
-        sr = 0.0f;
-        if (page >= 0 && k0 + lane < s.len)
-          sr = wave == 0 ? a.ks[page * a.ks_page + hk * a.ks_head + slot] * a.c : a.vs[page * a.vs_page + hk * a.vs_head + slot];
+  }
+  v4i kr[E4M3 ? CODES : 1], vr[E4M3 ? CODES : 1];
+  float sr = 0.0f;
+  const auto load = [&](int tile, int pg, int buf) {
+    const int k0 = key_of(tile) + 16 * wave;
+    const int64_t page = pg < 0 ? 0 : pg, slot = k0 & in_page;
+    const char* ks = a.k + page * a.k_page + hk * a.k_head + slot * a.k_slot;
+    const char* vs = a.v + page * a.v_page + hk * a.v_head + slot * a.v_slot;
+    if constexpr (!E4M3) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        to_shared(ks, &kl[buf][16 * wave * ROW + j * 1024], k_off[j]);
+        to_shared(vs, &vl[buf][16 * wave * ROW + j * 1024], v_off[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CODES; ++j) {
+        const int r = (j * 64 + lane) / (D / 16), at = lane % (D / 16);
+        kr[j] = *(const v4i*)(ks + (unsigned)(r * a.k_slot + at * 16));
+        vr[j] = *(const v4i*)(vs + (unsigned)(r * a.v_slot + at * 16));
+      }
+      if (lane < 32) {
+        const float* src = lane < 16 ? a.ks + page * a.ks_page + hk * a.ks_head : a.vs + page * a.vs_page + hk * a.vs_head;
+        sr = src[slot + (lane & 15)];
+        sr = lane < 16 ? sr * c : sr;
       }
     }
   };
-  const auto put = [&](int buf, bool look) {
-    uint32_t fine = 0x80008000u;
+  // In a tile that is not seen as a whole: what nobody may see becomes zero, and so do infinities and NaN (see finite_only).
+  const auto settle = [&](int tile, int buf, int there, bool part) {
+    bool fine = true;
+    const int k0 = key_of(tile) + 16 * wave;
+    if constexpr (E4M3) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int at = threadIdx.x + 256 * j, r = at / CH, ch = at % CH;
-      if constexpr (E4M3) {
+      for (int j = 0; j < CODES; ++j) {
+        const int r = (j * 64 + lane) / (D / 16), at = lane % (D / 16);
+        if (part && !((there >> wave & 1) && k0 + r < s.len)) kr[j] = vr[j] = v4i{0, 0, 0, 0};
         uint32_t y[8], z[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           widen4<QT>((uint32_t)kr[j][i], y[2 * i], y[2 * i + 1]);
           widen4<PT>((uint32_t)vr[j][i], z[2 * i], z[2 * i + 1]);
         }
-        __builtin_memcpy(&kl[buf][r * KLD + ch * 16], y, 32);
-        __builtin_memcpy(&vl[buf][r * VLD + ch * 16], z, 32);
-        if (look) {
+        if (part) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) fine &= finite2<PT>(z[i]);
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t u = finite_only<PT>(z[i]);
+            fine = fine && u == z[i];
+            z[i] = u;
+          }
         }
-      } else {
-        *(v4i*)&kl[buf][r * KLD + ch * 8] = kr[j];
-        *(v4i*)&vl[buf][r * VLD + ch * 8] = vr[j];
-        if (look) {
+        char* kt = kl[buf] + (16 * wave + r) * ROW;
+        char* vt = vl[buf] + (16 * wave + r) * ROW;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) fine &= finite2<PT>((uint32_t)vr[j][i]);
+        for (int h = 0; h < 2; ++h) {
+          *(v4i*)(kt + ((2 * at + h) ^ key_place(r)) * 16) = v4i{(int)y[4 * h], (int)y[4 * h + 1], (int)y[4 * h + 2], (int)y[4 * h + 3]};
+          *(v4i*)(vt + ((2 * at + h) ^ value_place(r)) * 16) = v4i{(int)z[4 * h], (int)z[4 * h + 1], (int)z[4 * h + 2], (int)z[4 * h + 3]};
         }
       }
+      if (lane < 32) sc[buf][lane >> 4][16 * wave + (lane & 15)] = sr;
+    } else if (part) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int r = j * RPL + lane / PIECES;
+        v4i* vt = (v4i*)(vl[buf] + 16 * wave * ROW + j * 1024 + lane * 16);
+        v4i u = {0, 0, 0, 0};
+        if ((there >> wave & 1) && k0 + r < s.len) {
+          const v4i v = *vt;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            u[i] = (int)finite_only<PT>((uint32_t)v[i]);
+            fine = fine && u[i] == v[i];
+          }
+        }
+        *vt = u;
+      }
     }
-    if constexpr (E4M3) {
-      if (wave < 2) sc[buf][wave][lane] = sr;
-    }
-    if (look && __any(fine != 0x80008000u) && lane == 0) odd = 1;
-  };
-  // a tile that some rows see in part
-  const auto partial = [&](int tile) {
-    const int k0 = key_of(tile);
-    return !(k0 + BN <= s.len && sees_all(a, p_lo, p_hi, k0, k0 + BN - 1));
+    if (part && __any(!fine) && lane == 0) odd = 1;
   };
 
-  if (threadIdx.x == 0) odd = 0;
-  __syncthreads();
-  int pgs = pages_of(0), pgs_next = pages_of(1);
-  uint64_t there = 0;
-  if (t.count > 0) {
-    load(0, pgs);
-    put(0, partial(0));
+  // places of this lane's operands: keys per step of the reduction, values per 32 elements
+  int k_at[QS], v_at[NV];
+#pragma unroll
+  for (int k = 0; k < QS; ++k) k_at[k] = c32 * ROW + ((2 * k + hl) ^ key_place(c32)) * 16;
+  {
+    const int l16 = lane & 15, r = 4 * hl + l16 / 4;  // (8 rows further the place is the same)
+#pragma unroll
+    for (int d = 0; d < NV; ++d)
+      v_at[d] = r * ROW + ((d * 4 + (lane >> 4 & 1) * 2 + l16 % 4 / 2) ^ value_place(r)) * 16 + l16 % 2 * 8;
   }
-  there = __ballot(pgs >= 0) & 15;
+
+  if (threadIdx.x == 0) odd = 0;
+  int there = 0, pg = page_of(0, wave);
+  if (t.count > 0) {
+    load(0, pg, 0);
+    there = there_of(0);
+    pg = page_of(1, wave);
+  }
   __syncthreads();
+  if (E4M3 && t.count > 0) settle(0, 0, there, partial(0, there));
   for (int tile = 0; tile < t.count; ++tile) {
     const int buf = tile & 1, k0 = key_of(tile);
-    const bool whole = there == 15 && k0 + BN <= s.len && sees_all(a, w_lo, w_hi, k0, k0 + BN - 1);
-    const uint64_t there_now = there;
+    const bool part = partial(tile, there);
+    if constexpr (!E4M3) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (part) settle(tile, buf, there, true);
+    }
+    // this tile is here, and nobody reads the one before it any more
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int there_now = there;
     const bool more = tile + 1 < t.count;
     if (more) {
-      pgs = pgs_next;
-      there = __ballot(pgs >= 0) & 15;
-      load(tile + 1, pgs);
-      pgs_next = pages_of(tile + 2);
+      load(tile + 1, pg, buf ^ 1);
+      there = there_of(tile + 1);
+      pg = page_of(tile + 2, wave);
     }
+    const bool whole = !part || (there_now == 15 && k0 + BN <= s.len && sees_all(a, w_lo, w_hi, k0, k0 + BN - 1));
     // S^T
     v16f st[2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int i = 0; i < 16; ++i) st[0][i] = st[1][i] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) st[kt][i] = 0.0f;
+    for (int k = 0; k < QS; ++k)
 #pragma unroll
-      for (int k = 0; k < QS; ++k)
-        st[kt] = mfma32<QT>(*(const v4i*)&kl[buf][(kt * 32 + c32) * KLD + k * 16 + hl * 8], q[k], st[kt]);
-    }
+      for (int kt = 0; kt < 2; ++kt) st[kt] = mfma32<QT>(*(const v4i*)(kl[buf] + k_at[k] + kt * 32 * ROW), q[k], st[kt]);
     // register 4 i + j of st[kt]: key kt * 32 + 8 i + 4 hl + j
+    if constexpr (E4M3) {
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (E4M3) {
+        for (int i = 0; i < 4; ++i) {
           const v4f ks = *(const v4f*)&sc[buf][0][kt * 32 + 8 * i + 4 * hl];
 #pragma unroll
           for (int j = 0; j < 4; ++j) st[kt][4 * i + j] *= ks[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) st[kt][4 * i + j] *= a.c;
         }
-      }
+    }
     if (!whole) {
+      const Bounds bd = bounds_of(a, pos, pos, s.len, k0 + 4 * hl);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int at = kt * 32 + 8 * (i / 4) + 4 * hl + i % 4, key = k0 + at;
-          const bool in = (there_now >> (at >> 4) & 1) && key < s.len && sees(a, pos, key);
-          st[kt][i] = in ? st[kt][i] : -__builtin_inff();
+          const int at = kt * 32 + 8 * (i / 4) + i % 4;
+          st[kt][i] = (there_now >> (at >> 4) & 1) && inside(bd, at) ? st[kt][i] : -__builtin_inff();
         }
     }
-    float top = st[0][0];
+    const float by = E4M3 ? 1.0f : c;
+    float top = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(st[0][i], st[1][i]));
-    top = max_x32(top);
-    const float m_new = fmaxf(m, top), ms = safe_max(m_new), f = exp2_hw(m - ms);
-    if (__any(m_new > m)) {
+    for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, st[0][i]), st[1][i]);
+    top = max_x32(top) * by;
+    // The maximum is held back: powers up to 2^8 are as good as powers up to 1, and O is rescaled a few times at all.
+    if (__any(top > m + 8.0f || (m == -__builtin_inff() && top > m))) {
+      const float m_new = fmaxf(m, top), f = exp2_hw(m - safe_max(m_new));
 #pragma unroll
       for (int d = 0; d < NV; ++d) o[d] *= f;
+      l *= f;
+      m = m_new;
     }
-    l *= f;
-    m = m_new;
+    const float ms = safe_max(m);
     v4i pb[4], pl[4];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -218,11 +283,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
         float pr[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          pr[j] = exp2_hw(st[kt][4 * i + j] - ms);
+          const float y = st[kt][4 * i + j];
+          pr[j] = exp2_hw(E4M3 ? y - ms : __fmaf_rn(y, by, -ms));
           l += pr[j];
         }
         if constexpr (E4M3) {
           const v4f vs = *(const v4f*)&sc[buf][1][kt * 32 + 8 * i + 4 * hl];
+          // (a key that the row does not see counts nothing, whatever its scale holds)
 #pragma unroll
           for (int j = 0; j < 4; ++j) pr[j] = whole || st[kt][4 * i + j] != -__builtin_inff() ? pr[j] * vs[j] : 0.0f;
         }
@@ -236,55 +303,50 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       }
     // O^T: step k of the reduction has keys 16 k + 4 hl + (0..3) and those + 8, as the scores lie
     const auto values = [&](int d, int k) {
-      const int l16 = lane & 15, r = 16 * k + 4 * hl + l16 / 4, col = d * 32 + (lane >> 4 & 1) * 16 + l16 % 4 * 4;
-      const s4v u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)&vl[buf][r * VLD + col]);
-      const s4v w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)&vl[buf][(r + 8) * VLD + col]);
+      const char* at = vl[buf] + v_at[d] + 16 * k * ROW;
+      const s4v u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)at);
+      const s4v w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(at + 8 * ROW));
       v4i f;
       __builtin_memcpy(&f, &u, 8);
       __builtin_memcpy((char*)&f + 8, &w, 8);
       return f;
     };
-    if (whole || !uniform(odd)) {
 #pragma unroll
-      for (int d = 0; d < NV; ++d)
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const v4i f = values(d, k);
-          o[d] = mfma32<PT>(f, pb[k], o[d]);
-          if constexpr (TWO) o[d] = mfma32<PT>(f, pl[k], o[d]);
-        }
-    } else {
-      // infinities or NaN among the values: one row at a time, with the values it sees (0 * inf is not 0)
-      for (int r = 0; r < wn; ++r) {
-        const int p = s.pos0 + (r0 + wr + r) / a.group;
-        for (int d = 0; d < NV; ++d) {
-          v16f acc = o[0];
-#pragma unroll
-          for (int e = 1; e < NV; ++e)
-            if (e == d) acc = o[e];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            v4i f = values(d, k);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int key = k0 + 16 * k + 4 * hl + (i / 2) * 8 + (i % 2) * 2;
-              const uint32_t keep = (sees(a, p, key) ? 0xffffu : 0u) | (sees(a, p, key + 1) ? 0xffff0000u : 0u);
-              f[i] = (int)((uint32_t)f[i] & keep);
-            }
-            acc = mfma32<PT>(f, pb[k], acc);
-            if constexpr (TWO) acc = mfma32<PT>(f, pl[k], acc);
-          }
-#pragma unroll
-          for (int e = 0; e < NV; ++e)
-            if (e == d && c32 == r) o[e] = acc;
-        }
+      for (int d = 0; d < NV; ++d) {
+        const v4i f = values(d, k);
+        o[d] = mfma32<PT>(f, pb[k], o[d]);
+        if constexpr (TWO) o[d] = mfma32<PT>(f, pl[k], o[d]);
       }
-    }
-    if (more) put(buf ^ 1, partial(tile + 1));
-    __syncthreads();
+    if (E4M3 && more) settle(tile + 1, buf ^ 1, there, partial(tile + 1, there));
   }
 
   l = sum_x32(l);
+  if (uniform(odd)) {
+#pragma unroll 1
+    for (int tile = 0; tile < t.count; ++tile) {
+      if (!partial(tile, there_of(tile))) continue;
+#pragma unroll 1
+      for (int i = 0; i < BN; ++i) {
+        const int key = key_of(tile) + i, page = page_of(tile, i >> 4);
+        if (page < 0 || key >= s.len) continue;
+        const bool seen = mine && inside(bounds_of(a, pos, pos, s.len, key), 0);
+        const char* src = a.v + page * a.v_page + hk * a.v_head + (int64_t)(key & in_page) * a.v_slot;
+#pragma unroll
+        for (int d = 0; d < NV; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int at = d * 32 + 8 * k + 4 * hl;
+            uint32_t u[2];
+            if constexpr (E4M3) widen4<PT>(*(const uint32_t*)(src + at), u[0], u[1]);
+            else __builtin_memcpy(u, src + 2 * at, 8);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) o[d][4 * k + n] = add_odd<PT>(o[d][4 * k + n], (u16)(u[n / 2] >> 16 * (n % 2)), seen);
+          }
+      }
+    }
+  }
   if (!mine) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   char* to = a.out + (s.row0 + tok) * a.o_row + head * a.o_head;
