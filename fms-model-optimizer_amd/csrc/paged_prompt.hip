@@ -104,6 +104,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     return there != 15 || k0 + BN > s.len || !sees_all(a, p_lo, p_hi, k0, k0 + BN - 1);
   };
 
+  // Places of this lane's operands, and of its codes: piece c of a row is piece 0 with c's bits turned over.
+  int k_base = c32 * ROW + (hl ^ key_place(c32)) * 16, v_base;
+  {
+    const int l16 = lane & 15, r = 4 * hl + l16 / 4;  // (8 rows further the place is the same)
+    v_base = r * ROW + (((lane >> 4 & 1) * 2 + l16 % 4 / 2) ^ value_place(r)) * 16 + l16 % 2 * 8;
+  }
+  constexpr int RPC = 1024 / D;  // rows of a load of codes
+  int kw_base, vw_base, k_from, v_from;
+  {
+    const int r = lane / (D / 16), at = lane % (D / 16);
+    kw_base = (16 * wave + r) * ROW + (2 * at ^ key_place(r)) * 16;
+    vw_base = (16 * wave + r) * ROW + (2 * at ^ value_place(r)) * 16;
+    k_from = r * a.k_slot + at * 16;
+    v_from = r * a.v_slot + at * 16;
+  }
+
   // This wave's 16 keys of a tile.  16-bit caches: instruction j brings 1 KiB, lane i the 16-byte piece that belongs at its end.
   constexpr int PIECES = ROW / 16;       // of a row
   constexpr int RPL = 64 / PIECES;       // rows of an instruction
@@ -132,9 +148,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     } else {
 #pragma unroll
       for (int j = 0; j < CODES; ++j) {
-        const int r = (j * 64 + lane) / (D / 16), at = lane % (D / 16);
-        kr[j] = *(const v4i*)(ks + (unsigned)(r * a.k_slot + at * 16));
-        vr[j] = *(const v4i*)(vs + (unsigned)(r * a.v_slot + at * 16));
+        kr[j] = *(const v4i*)(ks + j * RPC * a.k_slot + (unsigned)k_from);
+        vr[j] = *(const v4i*)(vs + j * RPC * a.v_slot + (unsigned)v_from);
       }
       if (lane < 32) {
         const float* src = lane < 16 ? a.ks + page * a.ks_page + hk * a.ks_head : a.vs + page * a.vs_page + hk * a.vs_head;
@@ -150,7 +165,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     if constexpr (E4M3) {
 #pragma unroll
       for (int j = 0; j < CODES; ++j) {
-        const int r = (j * 64 + lane) / (D / 16), at = lane % (D / 16);
+        const int r = j * RPC + lane / (D / 16);
         if (part && !((there >> wave & 1) && k0 + r < s.len)) kr[j] = vr[j] = v4i{0, 0, 0, 0};
         uint32_t y[8], z[8];
 #pragma unroll
@@ -166,12 +181,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
             z[i] = u;
           }
         }
-        char* kt = kl[buf] + (16 * wave + r) * ROW;
-        char* vt = vl[buf] + (16 * wave + r) * ROW;
+        // (rows j RPC + r with r < RPC, a power of two: their places are those of r with the bits of j RPC turned over)
+        char* kt = kl[buf] + j * RPC * ROW;
+        char* vt = vl[buf] + j * RPC * ROW;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          *(v4i*)(kt + ((2 * at + h) ^ key_place(r)) * 16) = v4i{(int)y[4 * h], (int)y[4 * h + 1], (int)y[4 * h + 2], (int)y[4 * h + 3]};
-          *(v4i*)(vt + ((2 * at + h) ^ value_place(r)) * 16) = v4i{(int)z[4 * h], (int)z[4 * h + 1], (int)z[4 * h + 2], (int)z[4 * h + 3]};
+          *(v4i*)(kt + (kw_base ^ (h ^ key_place(j * RPC)) * 16)) = v4i{(int)y[4 * h], (int)y[4 * h + 1], (int)y[4 * h + 2], (int)y[4 * h + 3]};
+          *(v4i*)(vt + (vw_base ^ (h ^ value_place(j * RPC)) * 16)) = v4i{(int)z[4 * h], (int)z[4 * h + 1], (int)z[4 * h + 2], (int)z[4 * h + 3]};
         }
       }
       if (lane < 32) sc[buf][lane >> 4][16 * wave + (lane & 15)] = sr;
@@ -194,17 +210,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     }
     if (part && __any(!fine) && lane == 0) odd = 1;
   };
-
-  // places of this lane's operands: keys per step of the reduction, values per 32 elements
-  int k_at[QS], v_at[NV];
-#pragma unroll
-  for (int k = 0; k < QS; ++k) k_at[k] = c32 * ROW + ((2 * k + hl) ^ key_place(c32)) * 16;
-  {
-    const int l16 = lane & 15, r = 4 * hl + l16 / 4;  // (8 rows further the place is the same)
-#pragma unroll
-    for (int d = 0; d < NV; ++d)
-      v_at[d] = r * ROW + ((d * 4 + (lane >> 4 & 1) * 2 + l16 % 4 / 2) ^ value_place(r)) * 16 + l16 % 2 * 8;
-  }
 
   if (threadIdx.x == 0) odd = 0;
   int there = 0, pg = page_of(0, wave);
@@ -231,6 +236,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       there = there_of(tile + 1);
       pg = page_of(tile + 2, wave);
     }
+    // (computed anew in every iteration instead of being kept in registers that are needed)
+    if constexpr (E4M3 || D == 256) asm volatile("" : "+v"(k_base), "+v"(v_base), "+v"(kw_base), "+v"(vw_base));
     const bool whole = !part || (there_now == 15 && k0 + BN <= s.len && sees_all(a, w_lo, w_hi, k0, k0 + BN - 1));
     // S^T
     v16f st[2];
@@ -239,7 +246,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
 #pragma unroll
     for (int k = 0; k < QS; ++k)
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) st[kt] = mfma32<QT>(*(const v4i*)(kl[buf] + k_at[k] + kt * 32 * ROW), q[k], st[kt]);
+      for (int kt = 0; kt < 2; ++kt) st[kt] = mfma32<QT>(*(const v4i*)(kl[buf] + (k_base ^ k * 32) + kt * 32 * ROW), q[k], st[kt]);
     // register 4 i + j of st[kt]: key kt * 32 + 8 i + 4 hl + j
     if constexpr (E4M3) {
 #pragma unroll
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       }
     // O^T: step k of the reduction has keys 16 k + 4 hl + (0..3) and those + 8, as the scores lie
     const auto values = [&](int d, int k) {
-      const char* at = vl[buf] + v_at[d] + 16 * k * ROW;
+      const char* at = vl[buf] + (v_base ^ d * 64) + 16 * k * ROW;
       const s4v u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)at);
       const s4v w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(at + 8 * ROW));
       v4i f;
