@@ -166,18 +166,25 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
     const int in_page = (1 << a.page_shift) - 1;
     const auto row = (const __attribute__((address_space(4))) int*)(uintptr_t)(a.table + b * a.table_stride);
     const auto key_of = [&](int tile) { return (tile < t.sink_tiles ? tile : tile + t.skip) * TILE; };
-    // page numbers of a tile's two halves; -1: no such page, or behind the sequence
+    // page numbers of a tile's two halves as the table has them, asked for an iteration before they are looked at
     const auto pages_of = [&](int tile, int* pg) {
       const int k0 = key_of(tile);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = k0 + 16 * h, n = row[(k < s.len ? k : 0) >> a.page_shift];
-        pg[h] = tile < end && k < s.len && (unsigned)n < (unsigned)a.pages ? n : -1;
+        const int k = k0 + 16 * h;
+        pg[h] = row[(k < s.len ? k : 0) >> a.page_shift];
       }
+    };
+    // -1: no such page, or behind the sequence
+    const auto check = [&](int tile, const int* from, int* pg) {
+      const int k0 = key_of(tile);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        pg[h] = tile < end && k0 + 16 * h < s.len && (unsigned)from[h] < (unsigned)a.pages ? from[h] : -1;
     };
     int tile = (u0 << sa.unit_shift) + sub;
     int pg[2], pg_next[2];
-    pages_of(tile, pg);
+    pages_of(tile, pg_next);
     // the rows: operand of the scores, and each lane's position
     v4i q[QS];
     const bool valid = c16 < nrows;
@@ -255,6 +262,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
     };
 
     if (tile < end) {
+      check(tile, pg_next, pg);
       load_k(tile, pg);
       load_v(tile, pg);
       pages_of(tile + waves, pg_next);
@@ -306,8 +314,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
       const bool there0 = pg[0] >= 0, there1 = pg[1] >= 0;
       const bool whole = there0 && there1 && k0 + TILE <= s.len && sees_all(a, p_lo, p_hi, k0, k0 + TILE - 1);
       const int more = tile + waves;
-      pg[0] = pg_next[0];
-      pg[1] = pg_next[1];
+      check(more, pg_next, pg);
       load_k(more, pg);
       pages_of(more + waves, pg_next);
 #pragma unroll
@@ -396,6 +403,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
         const int k0 = key_of(again);
         int pages[2];
         pages_of(again, pages);
+        check(again, pages, pages);
         if (pages[0] >= 0 && pages[1] >= 0 && k0 + TILE <= s.len && sees_all(a, p_lo, p_hi, k0, k0 + TILE - 1)) continue;
 #pragma unroll 1
         for (int i = 0; i < TILE; ++i) {

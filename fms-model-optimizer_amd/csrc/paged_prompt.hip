@@ -89,14 +89,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
 
   const auto key_of = [&](int tile) { return (tile < t.sink_tiles ? tile : tile + t.skip) * BN; };
   const int in_page = (1 << a.page_shift) - 1;
-  const auto table = (const __attribute__((address_space(4))) int*)(uintptr_t)(a.table + b * a.table_stride);
-  // page of a tile's i-th 16 keys; -1: not there
-  const auto page_of = [&](int tile, int i) {
-    const int k = key_of(tile) + 16 * i, n = table[(k < s.len ? k : 0) >> a.page_shift];
-    return tile < t.count && k < s.len && (unsigned)n < (unsigned)a.pages ? n : -1;
+  const int* table = a.table + b * a.table_stride;
+  // lane i (of four) holds the page of a tile's i-th 16 keys, as the table has it; checked when it is used, an iteration later
+  const auto pages_of = [&](int tile) {
+    const int k = key_of(tile) + 16 * (lane & 3);
+    return table[(k < s.len && k >= 0 ? k : 0) >> a.page_shift];
   };
-  const auto there_of = [&](int tile) {
-    return (page_of(tile, 0) >= 0 ? 1 : 0) | (page_of(tile, 1) >= 0 ? 2 : 0) | (page_of(tile, 2) >= 0 ? 4 : 0) | (page_of(tile, 3) >= 0 ? 8 : 0);
+  // which of them are there
+  const auto there_of = [&](int tile, int pages) {
+    return (int)__ballot(tile < t.count && key_of(tile) + 16 * (lane & 3) < s.len && (unsigned)pages < (unsigned)a.pages) & 15;
   };
   // a tile that some rows see in part
   const auto partial = [&](int tile, int there) {
@@ -134,9 +135,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   }
   v4i kr[E4M3 ? CODES : 1], vr[E4M3 ? CODES : 1];
   float sr = 0.0f;
-  const auto load = [&](int tile, int pg, int buf) {
+  const auto load = [&](int tile, int pages, int there, int buf) {
     const int k0 = key_of(tile) + 16 * wave;
-    const int64_t page = pg < 0 ? 0 : pg, slot = k0 & in_page;
+    const int64_t page = there >> wave & 1 ? __builtin_amdgcn_readlane(pages, wave) : 0, slot = k0 & in_page;
     const char* ks = a.k + page * a.k_page + hk * a.k_head + slot * a.k_slot;
     const char* vs = a.v + page * a.v_page + hk * a.v_head + slot * a.v_slot;
     if constexpr (!E4M3) {
@@ -212,11 +213,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   };
 
   if (threadIdx.x == 0) odd = 0;
-  int there = 0, pg = page_of(0, wave);
+  int pages = pages_of(0), there = there_of(0, pages);
   if (t.count > 0) {
-    load(0, pg, 0);
-    there = there_of(0);
-    pg = page_of(1, wave);
+    load(0, pages, there, 0);
+    pages = pages_of(1);
   }
   __syncthreads();
   if (E4M3 && t.count > 0) settle(0, 0, there, partial(0, there));
@@ -232,9 +232,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     const int there_now = there;
     const bool more = tile + 1 < t.count;
     if (more) {
-      load(tile + 1, pg, buf ^ 1);
-      there = there_of(tile + 1);
-      pg = page_of(tile + 2, wave);
+      there = there_of(tile + 1, pages);
+      load(tile + 1, pages, there, buf ^ 1);
+      pages = pages_of(tile + 2);
     }
     // (computed anew in every iteration instead of being kept in registers that are needed)
     if constexpr (E4M3 || D == 256) asm volatile("" : "+v"(k_base), "+v"(v_base), "+v"(kw_base), "+v"(vw_base));
@@ -247,6 +247,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     for (int k = 0; k < QS; ++k)
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) st[kt] = mfma32<QT>(*(const v4i*)(kl[buf] + (k_base ^ k * 32) + kt * 32 * ROW), q[k], st[kt]);
+    // (six reads ahead of the products)
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int k = 0; k < 2 * QS - 6; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     // register 4 i + j of st[kt]: key kt * 32 + 8 i + 4 hl + j
     if constexpr (E4M3) {
 #pragma unroll
@@ -298,7 +306,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
           const v4f vs = *(const v4f*)&sc[buf][1][kt * 32 + 8 * i + 4 * hl];
           // (a key that the row does not see counts nothing, whatever its scale holds)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) pr[j] = whole || st[kt][4 * i + j] != -__builtin_inff() ? pr[j] * vs[j] : 0.0f;
+          for (int j = 0; j < 4; ++j) pr[j] *= vs[j];
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pr[j] = st[kt][4 * i + j] != -__builtin_inff() ? pr[j] : 0.0f;
+          }
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -333,11 +345,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   if (uniform(odd)) {
 #pragma unroll 1
     for (int tile = 0; tile < t.count; ++tile) {
-      if (!partial(tile, there_of(tile))) continue;
+      const int pages = pages_of(tile), there = there_of(tile, pages);
+      if (!partial(tile, there)) continue;
 #pragma unroll 1
       for (int i = 0; i < BN; ++i) {
-        const int key = key_of(tile) + i, page = page_of(tile, i >> 4);
-        if (page < 0 || key >= s.len) continue;
+        const int key = key_of(tile) + i;
+        if (!(there >> (i >> 4) & 1) || key >= s.len) continue;
+        const int page = __builtin_amdgcn_readlane(pages, i >> 4);
         const bool seen = mine && inside(bounds_of(a, pos, pos, s.len, key), 0);
         const char* src = a.v + page * a.v_page + hk * a.v_head + (int64_t)(key & in_page) * a.v_slot;
 #pragma unroll
