@@ -31,7 +31,8 @@ namespace {
   X(fmsmo_decode_linear_ok) X(fmsmo_decode_linear_f32s_ok) X(fmsmo_small_linear_better) X(fmsmo_small_linear_i8) X(fmsmo_small_linear_fp8) X(fmsmo_small_linear_static_ok) X(fmsmo_small_linear_i8_static_scale) X(fmsmo_grouped_gemm_i8_dq)                   \
   X(fmsmo_matmul_chunk_i8_dq_ws) X(fmsmo_matmul_chunk_fp_dq) X(fmsmo_matmul_chunk_workspace_bytes)    \
   X(fmsmo_quant_i8_affine_sums) X(fmsmo_quant_i8_affine_pair) X(fmsmo_affine_sum_parts) X(fmsmo_affine_parts_first) X(fmsmo_affine_add_parts) X(fmsmo_bmm_qa_ok)   \
-  X(fmsmo_bmm_qa_i8) X(fmsmo_bmm_i8_zp)
+  X(fmsmo_bmm_qa_i8) X(fmsmo_bmm_i8_zp)                                                                 \
+  X(fmsmo_kv_store) X(fmsmo_paged_attn) X(fmsmo_paged_attn_workspace_bytes)
 #define DECLARE(f) decltype(&::f) p_##f = nullptr;
 ENTRIES(DECLARE)
 #undef DECLARE
@@ -779,6 +780,184 @@ PyObject* fp8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------ paged key-value cache
+int64_t step(const at::Tensor& t, int i) { return t.size(i) == 1 ? 0 : t.stride(i); }  // (one element leaves it open)
+bool apart(const at::Tensor& t) {  // no two elements share memory by a stride of nothing
+  for (int i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) return false;
+  return true;
+}
+// [rows, heads, dim] of a 16-bit type, heads contiguous and 16-byte aligned
+struct Heads {
+  const at::Tensor* t = nullptr;
+  int64_t rows = 0, heads = 0, dim = 0, row = 0, head = 0;
+  char* p = nullptr;
+  explicit operator bool() const { return t != nullptr; }
+};
+Heads heads_of(const at::Tensor* t) {
+  if (!t || t->dim() != 3 || (t->scalar_type() != at::kHalf && t->scalar_type() != at::kBFloat16) || t->stride(2) != 1) return Heads{};
+  const Heads h{t, t->size(0), t->size(1), t->size(2), step(*t, 0), step(*t, 1), (char*)t->data_ptr()};
+  if (h.row % 8 || h.head % 8 || (uintptr_t)h.p % 16) return Heads{};
+  return h;
+}
+// the cache of (k, v, k_scale | None, v_scale | None)
+struct Cache {
+  fmsmo_kv_cache_t c{};
+  const at::Tensor *k = nullptr, *v = nullptr, *ks = nullptr, *vs = nullptr;
+  bool ok = false;
+};
+Cache cache_of(PyObject* ok, PyObject* ov, PyObject* oks, PyObject* ovs, at::ScalarType q) {
+  Cache r;
+  r.k = plain(ok);
+  r.v = plain(ov);
+  if (!r.k || !r.v || r.k->dim() != 4 || r.k->sizes() != r.v->sizes() || r.k->scalar_type() != r.v->scalar_type()) return r;
+  const at::ScalarType st = r.k->scalar_type();
+  const bool e4m3 = st == at::kFloat8_e4m3fn;
+  if (!e4m3 && st != q) return r;
+  fmsmo_kv_cache_t& c = r.c;
+  c.pages = r.k->size(0);
+  c.heads = (int)r.k->size(1);
+  c.page_size = (int)r.k->size(2);
+  c.dim = (int)r.k->size(3);
+  c.dtype = e4m3 ? FMSMO_KV_E4M3 : code_of(st);
+  if ((c.dim != 64 && c.dim != 128 && c.dim != 256) || r.k->size(2) > 65536 || c.page_size < 16 || (c.page_size & (c.page_size - 1)) || c.pages < 1 ||
+      c.heads < 1 || r.k->stride(3) != 1 || r.v->stride(3) != 1)
+    return r;
+  c.k = r.k->data_ptr();
+  c.v = r.v->data_ptr();
+  for (int i = 0; i < 3; ++i) {
+    c.k_strides[i] = step(*r.k, i);
+    c.v_strides[i] = step(*r.v, i);
+    if (c.k_strides[i] * (e4m3 ? 1 : 2) % 16 || c.v_strides[i] * (e4m3 ? 1 : 2) % 16) return r;
+  }
+  if ((uintptr_t)c.k % 16 || (uintptr_t)c.v % 16) return r;
+  if (!e4m3) {
+    r.ok = oks == Py_None && ovs == Py_None;
+    return r;
+  }
+  r.ks = plain(oks);
+  r.vs = plain(ovs);
+  for (const at::Tensor* t : {r.ks, r.vs})
+    if (!t || t->scalar_type() != at::kFloat || t->dim() != 3 || t->size(0) != c.pages || t->size(1) != c.heads || t->size(2) != c.page_size ||
+        t->stride(2) != 1 || (uintptr_t)t->data_ptr() % 16 || step(*t, 0) % 4 || step(*t, 1) % 4)
+      return r;
+  c.k_scale = (float*)r.ks->data_ptr();
+  c.v_scale = (float*)r.vs->data_ptr();
+  for (int i = 0; i < 2; ++i) {
+    c.k_scale_strides[i] = step(*r.ks, i);
+    c.v_scale_strides[i] = step(*r.vs, i);
+  }
+  r.ok = true;
+  return r;
+}
+// the batch of (block_table, seq_lens, query_start | None)
+struct Batch {
+  fmsmo_kv_batch_t b{};
+  const at::Tensor *table = nullptr, *lens = nullptr, *start = nullptr;
+  bool ok = false;
+};
+Batch batch_of(PyObject* ot, PyObject* ol, PyObject* os, int64_t rows) {
+  Batch r;
+  r.table = plain(ot);
+  r.lens = plain(ol);
+  r.start = os == Py_None ? nullptr : plain(os);
+  const at::Tensor *t = r.table, *l = r.lens, *s = r.start;
+  if (!t || !l || (!s && os != Py_None) || t->dim() != 2 || l->dim() != 1 || t->scalar_type() != at::kInt || l->scalar_type() != at::kInt) return r;
+  const int64_t seqs = l->size(0);
+  if (seqs == 0 || t->size(0) != seqs || t->size(1) < 1 || (t->size(1) > 1 && t->stride(1) != 1) || !l->is_contiguous()) return r;
+  if (s ? s->dim() != 1 || s->size(0) != seqs + 1 || s->scalar_type() != at::kInt || !s->is_contiguous() : rows != seqs) return r;
+  r.b = fmsmo_kv_batch_t{(const int32_t*)t->data_ptr(), step(*t, 0), t->size(1), (const int32_t*)l->data_ptr(),
+                         s ? (const int32_t*)s->data_ptr() : nullptr, seqs};
+  r.ok = true;
+  return r;
+}
+// what a call writes: `given`, or a new tensor like q
+bool result_of(PyObject* given, const Heads& q, at::Tensor* out, Heads* h) {
+  if (given == Py_None) {
+    *out = empty({q.rows, q.heads, q.dim}, q.t->scalar_type(), *q.t);
+    *h = heads_of(out);
+    return true;
+  }
+  const at::Tensor* t = plain(given);
+  *h = heads_of(t);
+  if (!*h || t->sizes() != q.t->sizes() || t->scalar_type() != q.t->scalar_type() || !apart(*t)) return false;
+  *out = *t;
+  return true;
+}
+// (q, k_cache, v_cache, block_table, seq_lens, query_start | None, scale | None, window, sinks, k_scale | None, v_scale | None,
+//  max_query_len, max_seq_len, out | None) -> out
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  WANT(14);
+  const Heads q = heads_of(plain(args[0]));
+  if (!q || q.rows == 0 || q.heads == 0) return none();
+  const Cache c = cache_of(args[1], args[2], args[9], args[10], q.t->scalar_type());
+  if (!c.ok || c.c.dim != q.dim || q.heads % c.c.heads) return none();
+  const Batch b = batch_of(args[3], args[4], args[5], q.rows);
+  if (!b.ok) return none();
+  const float scale = args[6] == Py_None ? (float)(1.0 / std::sqrt((double)q.dim)) : (float)REAL(6);
+  const int64_t window = WHOLE(7), sinks = WHOLE(8), most_rows = WHOLE(11), most_keys = WHOLE(12);
+  NUMBERS_OK;
+  if (window < 0 || sinks < 0 || most_rows < 0 || most_keys < 0) return none();
+  at::Tensor out;
+  Heads o;
+  if (!result_of(args[13], q, &out, &o) || !here(q.t, c.k, c.v, c.ks, c.vs, b.table, b.lens, b.start, &out)) return none();
+  const int64_t keys = b.b.table_width * c.c.page_size;
+  const int64_t max_rows = b.start ? std::min(most_rows ? most_rows : q.rows, q.rows) : 1, max_keys = std::min(most_keys ? most_keys : keys, keys);
+  const at::Tensor ws = workspace(p_fmsmo_paged_attn_workspace_bytes((int)q.heads, c.c.heads, c.c.dim, b.b.seqs, q.rows, max_rows, max_keys), *q.t);
+  if (!LAUNCH(fmsmo_paged_attn, &c.c, &b.b, code_of(q.t->scalar_type()), q.rows, (int)q.heads, q.p, q.row, q.head, o.p, o.row, o.head, scale,
+              window, sinks, max_rows, max_keys, (int)(args[13] == Py_None), ws.defined() ? ws.data_ptr() : nullptr,
+              ws.defined() ? ws.numel() : 0, stream_of(*q.t)))
+    return nullptr;
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+// (q, k, v, k_cache, v_cache, block_table, seq_lens, query_start | None, cos | None, sin | None, interleaved, q_weight | None,
+//  k_weight | None, eps, k_scale | None, v_scale | None, out | None) -> out
+PyObject* kv_store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  WANT(17);
+  const Heads q = heads_of(plain(args[0])), k = heads_of(plain(args[1])), v = heads_of(plain(args[2]));
+  if (!q || !k || !v || q.rows == 0 || q.heads == 0) return none();
+  const at::ScalarType st = q.t->scalar_type();
+  const Cache c = cache_of(args[3], args[4], args[14], args[15], st);
+  if (!c.ok || c.c.dim != q.dim || q.heads % c.c.heads || !apart(*c.k) || !apart(*c.v) || (c.ks && (!apart(*c.ks) || !apart(*c.vs)))) return none();
+  for (const Heads* h : {&k, &v})
+    if (h->rows != q.rows || h->heads != c.c.heads || h->dim != q.dim || h->t->scalar_type() != st) return none();
+  const Batch b = batch_of(args[5], args[6], args[7], q.rows);
+  if (!b.ok) return none();
+  const at::Tensor *cs = nullptr, *sn = nullptr;
+  if (args[8] != Py_None) {
+    cs = plain(args[8]);
+    sn = plain(args[9]);
+    if (!cs || !sn || cs->dim() != 2 || cs->sizes() != sn->sizes() || cs->scalar_type() != at::kFloat || sn->scalar_type() != at::kFloat ||
+        !cs->is_contiguous() || !sn->is_contiguous() || cs->size(0) < 1 || cs->size(1) % 8 || cs->size(1) < 8 || 2 * cs->size(1) > q.dim ||
+        (uintptr_t)cs->data_ptr() % 16 || (uintptr_t)sn->data_ptr() % 16)
+      return none();
+  } else if (args[9] != Py_None) {
+    return none();
+  }
+  const Opt qw = opt_vec(args[11], q.dim, 16), kw = opt_vec(args[12], q.dim, 16);
+  if (!qw.ok || !kw.ok || (qw.p && kw.p && qw.st != kw.st)) return none();
+  const at::ScalarType wt = qw.p ? qw.st : kw.st;
+  if ((qw.p || kw.p) && wt != st && wt != at::kFloat) return none();
+  const int turned = PyObject_IsTrue(args[10]);
+  const double eps = REAL(13);
+  NUMBERS_OK;
+  at::Tensor out;
+  Heads o;
+  if (!result_of(args[16], q, &out, &o) ||
+      !here(q.t, k.t, v.t, c.k, c.v, c.ks, c.vs, b.table, b.lens, b.start, cs, sn, qw.t, kw.t, &out))
+    return none();
+  if (!LAUNCH(fmsmo_kv_store, &c.c, &b.b, code_of(st), q.rows, (int)q.heads, q.p, q.row, q.head, k.p, k.row, k.head, v.p, v.row, v.head, o.p,
+              o.row, o.head, qw.p, kw.p, qw.p || kw.p ? code_of(wt) : 0, (float)eps, cs ? (const float*)cs->data_ptr() : nullptr,
+              sn ? (const float*)sn->data_ptr() : nullptr, cs ? cs->size(0) : 0, cs ? (int)(2 * cs->size(1)) : 0, turned,
+              (int)(args[16] == Py_None), stream_of(*q.t)))
+    return nullptr;
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // ------------------------------------------------------------------ module
 // bind({entry point: address}, raise_status)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -812,7 +991,7 @@ PyObject* entries(PyObject*, PyObject*) {
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(quant_i8), FAST(quant_i8_clips), FAST(quant_i8_static), FAST(quant_i8_static_t), FAST(quant_fp8), FAST(gemm_dq),
                          FAST(decode_i8), FAST(decode_fp8), FAST(grouped_i8), FAST(chunk_dq), FAST(bmm_quantized),
-                         FAST(deploy_i8), FAST(fp8_linear), FAST(bind), {"entries", entries, METH_NOARGS, nullptr},
+                         FAST(deploy_i8), FAST(fp8_linear), FAST(paged_attention), FAST(kv_store), FAST(bind), {"entries", entries, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fmsmo_host", nullptr, -1, methods};
 

@@ -27,65 +27,77 @@ struct StoreArgs {
   int heads;             // of q
 };
 
-__device__ __forceinline__ void load8(const char* p, int dt, float* x) {
-  const v4i u = *(const v4i*)p;
-  if (dt == FMSMO_F16) {
+// eight elements of 16 bits
+template <int T>
+__device__ __forceinline__ void widen8(v4i u, float* x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = T == FMSMO_F16 ? f16_to_f32((u16)u[i]) : __uint_as_float((uint32_t)u[i] << 16);
+    x[2 * i + 1] = T == FMSMO_F16 ? f16_to_f32((u16)((uint32_t)u[i] >> 16)) : __uint_as_float((uint32_t)u[i] & 0xffff0000u);
+  }
+}
+template <int WT>
+__device__ __forceinline__ void load_weight(const void* w, int piece, float* x) {
+  if constexpr (WT == FMSMO_F32) {
+    const v4f a = ((const v4f*)w)[2 * piece], b = ((const v4f*)w)[2 * piece + 1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[2 * i] = f16_to_f32((u16)u[i]);
-      x[2 * i + 1] = f16_to_f32((u16)((uint32_t)u[i] >> 16));
-    }
-  } else if (dt == FMSMO_BF16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float((uint32_t)u[i] << 16);
-      x[2 * i + 1] = __uint_as_float((uint32_t)u[i] & 0xffff0000u);
+      x[i] = a[i];
+      x[4 + i] = b[i];
     }
   } else {
-    const v4i w = *(const v4i*)(p + 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = __int_as_float(u[i]);
-      x[4 + i] = __int_as_float(w[i]);
-    }
+    widen8<WT>(((const v4i*)w)[piece], x);
   }
 }
 
-// over the LG lanes that hold a row
+// over the LG lanes that hold a row, the same result in all of them: moves inside rows of 16 lanes, then one between rows
+#define FMSMO_DPP(v, ctrl) __builtin_amdgcn_update_dpp((int)(v), (int)(v), ctrl, 0xf, 0xf, false)
 template <int LG>
 __device__ __forceinline__ float sum_lanes(float v) {
-#pragma unroll
-  for (int o = 1; o < LG; o *= 2) v += __shfl_xor(v, o);
+  v += __int_as_float(FMSMO_DPP(__float_as_int(v), 0xb1));   // quad_perm [1,0,3,2]
+  v += __int_as_float(FMSMO_DPP(__float_as_int(v), 0x4e));   // quad_perm [2,3,0,1]
+  v += __int_as_float(FMSMO_DPP(__float_as_int(v), 0x141));  // row_half_mirror
+  if constexpr (LG >= 16) v += __int_as_float(FMSMO_DPP(__float_as_int(v), 0x140));  // row_mirror
+  if constexpr (LG >= 32) v = sum_x16(v);
   return v;
 }
 template <int LG>
 __device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
-#pragma unroll
-  for (int o = 1; o < LG; o *= 2) {
-    const uint32_t w = __shfl_xor(v, o);
-    v = v > w ? v : w;
+  const auto max2 = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  v = max2(v, (uint32_t)FMSMO_DPP(v, 0xb1));
+  v = max2(v, (uint32_t)FMSMO_DPP(v, 0x4e));
+  v = max2(v, (uint32_t)FMSMO_DPP(v, 0x141));
+  if constexpr (LG >= 16) v = max2(v, (uint32_t)FMSMO_DPP(v, 0x140));
+  if constexpr (LG >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max2(r[0], r[1]);
   }
   return v;
 }
+#undef FMSMO_DPP
 
-// One block per token and group of heads, one lane per eight elements of a row: the token, its position and its page are
-// the same for the whole block, and a row's sums stay inside a wave.  The other half of a pair is loaded again (it is
-// in the cache lines that the row's lanes just fetched) instead of being passed between lanes.
+// One block per token and `per` groups of heads, one lane per eight elements of a row: the token, its position, its angles and its
+// page are the same for the whole block, and a row's sums stay inside a wave.  The other half of a pair is loaded again (it is
+// in the cache lines that the row's lanes just fetched) instead of being passed between lanes.  Bound by the latency of a token's
+// chain of loads (sequence, length, page, row), so where tokens are many a block goes through all of its heads, the next group's rows on
+// their way meanwhile: 4 uneven prompts of up to 4095 tokens, 32 + 8 + 8 heads of 128, e4m3: 105 us with a block per group of heads.
 template <int T, bool E4M3, int D, int WT, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
+__global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a, int per) {
   constexpr int LG = D / 8, ROWS = 256 / LG;
   const PagedArgs& p = a.p;
   const int t = blockIdx.x, lane = threadIdx.x & 63;
   // the token's sequence: as many as start at or before it
   int b = t;
-  const int h = blockIdx.y * ROWS + threadIdx.x / LG, c = threadIdx.x % LG;
+  const int h0 = blockIdx.y * per * ROWS + threadIdx.x / LG, c = threadIdx.x % LG;
+  const int kv = p.kv_heads, all = a.heads + 2 * kv;
   const auto none = [&] {  // a row of no sequence
-    if (p.zero_rest && h < a.heads) *(v4i*)(p.out + t * p.o_row + h * p.o_head + c * 16) = v4i{0, 0, 0, 0};
+    if (!p.zero_rest) return;
+    for (int h = h0; h < h0 + per * ROWS && h < a.heads; h += ROWS) *(v4i*)(p.out + t * p.o_row + h * p.o_head + c * 16) = v4i{0, 0, 0, 0};
   };
   if (p.starts) {
     int before = 0;
-    for (int c = 0; c < p.seqs; c += 64) {
-      const bool yes = c + lane < p.seqs && p.starts[c + lane] <= t;
+    for (int i = 0; i < p.seqs; i += 64) {
+      const bool yes = i + lane < p.seqs && p.starts[i + lane] <= t;
       before += __popcll(__ballot(yes));
     }
     b = uniform(before) - 1;
@@ -94,108 +106,126 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
   const Seq s = seq_of(p, b);
   if (t >= s.row0 + s.n) return none();
   const int pos = s.pos0 + (t - s.row0);
+  int page = pos >= 0 && pos < p.cap ? p.table[b * p.table_stride + (pos >> p.page_shift)] : -1;
+  if ((unsigned)page >= (unsigned)p.pages) page = -1;
+  const int64_t slot = pos & ((1 << p.page_shift) - 1);
 
-  const int kv = p.kv_heads;
-  if (h >= a.heads + 2 * kv) return;  // (whole lane groups: the others of a wave go on)
-  const int kind = h < a.heads ? 0 : h < a.heads + kv ? 1 : 2;
-  const int hh = kind == 0 ? h : kind == 1 ? h - a.heads : h - a.heads - kv;
-  const char* src = kind == 0 ? p.q + t * p.q_row + hh * p.q_head
-                  : kind == 1 ? a.xk + t * a.xk_row + hh * a.xk_head
-                              : a.xv + t * a.xv_row + hh * a.xv_head;
-  const void* w = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
-  float x[8];
-  load8(src + c * 16, T, x);
-  const bool turn = kind < 2 && a.cos && 8 * c < 2 * a.half;
-  const bool far = turn && pos >= a.table_rows;  // a position that the tables don't hold
-  const int other = 8 * c < a.half ? c + a.half / 8 : c - a.half / 8;
-  float y[8];
-  if (!INTERLEAVED && turn) load8(src + other * 16, T, y);
-  if (w) {
-    float ss = 0.0f;
+  const bool paired = a.cos && 8 * c < 2 * a.half;  // this lane's piece is turned
+  const bool far = paired && pos >= a.table_rows;   // by a position that the tables don't hold
+  const bool first = 8 * c < a.half;
+  const int other = first ? c + a.half / 8 : c - a.half / 8;
+  // angles: of eight pairs across the halves, or of four neighbours
+  constexpr int PAIRS = INTERLEAVED ? 4 : 8;
+  float cs[PAIRS], sn[PAIRS];
+  if (paired) {
+    const int64_t at = (int64_t)(far || pos < 0 ? 0 : pos) * a.half + (INTERLEAVED ? 4 * c : first ? 8 * c : 8 * c - a.half);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = __fmaf_rn(x[i], x[i], ss);
-    const float r = 1.0f / sqrtf(sum_lanes<LG>(ss) * (1.0f / D) + a.eps);
-    constexpr int WB = WT == FMSMO_F32 ? 4 : 2;
-    float g[8];
-    load8((const char*)w + c * 8 * WB, WT, g);
+    for (int i = 0; i < PAIRS; i += 4) {
+      const v4f u = *(const v4f*)(a.cos + at + i), v = *(const v4f*)(a.sin + at + i);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * g[i];
-    if (!INTERLEAVED && turn) {
-      load8((const char*)w + other * 8 * WB, WT, g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * r * g[i];
+      for (int k = 0; k < 4; ++k) {
+        cs[i + k] = u[k];
+        sn[i + k] = INTERLEAVED || !first ? v[k] : -v[k];
+      }
     }
   }
-  if (turn) {
-    const int at = far || pos < 0 ? 0 : pos;
-    const float* cs = a.cos + (int64_t)at * a.half;
-    const float* sn = a.sin + (int64_t)at * a.half;
-    if constexpr (INTERLEAVED) {
+  v4i own = {0, 0, 0, 0}, far_half = {0, 0, 0, 0};
+  const auto fetch = [&](int h) {
+    if (h >= all) return;
+    const char* src = h < a.heads        ? p.q + t * p.q_row + h * p.q_head
+                      : h < a.heads + kv ? a.xk + t * a.xk_row + (h - a.heads) * a.xk_head
+                                         : a.xv + t * a.xv_row + (h - a.heads - kv) * a.xv_head;
+    own = *(const v4i*)(src + c * 16);
+    if (!INTERLEAVED && paired && h < a.heads + kv) far_half = *(const v4i*)(src + other * 16);
+  };
+  fetch(h0);
+  for (int i = 0; i < per; ++i) {
+    const int h = h0 + i * ROWS;
+    if (h >= all) break;  // (whole lane groups: the others of a wave go on)
+    const int kind = h < a.heads ? 0 : h < a.heads + kv ? 1 : 2;
+    const int hh = kind == 0 ? h : kind == 1 ? h - a.heads : h - a.heads - kv;
+    const void* w = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
+    const bool turn = kind < 2 && paired;
+    float x[8], y[8];
+    widen8<T>(own, x);
+    if (!INTERLEAVED) widen8<T>(far_half, y);
+    // (before any of this row's is written: q_out may be q)
+    if (i + 1 < per) fetch(h + ROWS);
+    if (w) {
+      float ss = 0.0f, g[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float u = cs[4 * c + i], v = sn[4 * c + i], e = x[2 * i], o = x[2 * i + 1];
-        x[2 * i] = e * u - o * v;
-        x[2 * i + 1] = o * u + e * v;
+      for (int k = 0; k < 8; ++k) ss = __fmaf_rn(x[k], x[k], ss);
+      const float r = 1.0f / sqrtf(sum_lanes<LG>(ss) * (1.0f / D) + a.eps);
+      load_weight<WT>(w, c, g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = x[k] * r * g[k];
+      if (!INTERLEAVED && turn) {
+        load_weight<WT>(w, other, g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = y[k] * r * g[k];
+      }
+    }
+    if (turn) {
+      if constexpr (INTERLEAVED) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float e = x[2 * k], o = x[2 * k + 1];
+          x[2 * k] = e * cs[k] - o * sn[k];
+          x[2 * k + 1] = o * cs[k] + e * sn[k];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = x[k] * cs[k] + y[k] * sn[k];
+      }
+      if (far) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = __builtin_nanf("");
+      }
+    }
+    if (kind == 0) {
+      v4i o;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = pos < 0 ? 0 : (int)pack2<T>(x[2 * k], x[2 * k + 1]);
+      *(v4i*)(p.out + t * p.o_row + hh * p.o_head + c * 16) = o;
+      continue;
+    }
+    float scale = 1.0f;
+    if constexpr (E4M3) {
+      uint32_t m = 0;  // (as integers: a NaN is larger than everything)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t u = __float_as_uint(x[k]) & 0x7fffffffu;
+        m = m > u ? m : u;
+      }
+      scale = __uint_as_float(max_lanes<LG>(m)) / 448.0f;
+      scale = scale < 1e-12f ? 1e-12f : scale;
+    }
+    if (page < 0) continue;
+    char* to = kind == 1 ? (char*)p.k + page * p.k_page + hh * p.k_head + slot * p.k_slot
+                         : (char*)p.v + page * p.v_page + hh * p.v_head + slot * p.v_slot;
+    if constexpr (E4M3) {
+      int lo = 0, hi = 0;
+      float q[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        q[k] = x[k] / scale;
+        q[k] = q[k] != q[k] ? q[k] : fminf(fmaxf(q[k], -448.0f), 448.0f);
+      }
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], hi, false);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
+      *(int2*)(to + c * 8) = make_int2(lo, hi);
+      if (c == 0) {
+        if (kind == 1) ((float*)p.ks)[page * p.ks_page + hh * p.ks_head + slot] = scale;
+        else ((float*)p.vs)[page * p.vs_page + hh * p.vs_head + slot] = scale;
       }
     } else {
-      const bool first = 8 * c < a.half;
-      const int i0 = first ? 8 * c : 8 * c - a.half;
+      v4i o;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float u = cs[i0 + i], v = sn[i0 + i];
-        x[i] = first ? x[i] * u - y[i] * v : x[i] * u + y[i] * v;
-      }
+      for (int k = 0; k < 4; ++k) o[k] = (int)pack2<T>(x[2 * k], x[2 * k + 1]);
+      *(v4i*)(to + c * 16) = o;
     }
-  }
-  if (far) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __builtin_nanf("");
-  }
-  if (kind == 0) {
-    v4i o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = pos < 0 ? 0 : (int)pack2<T>(x[2 * i], x[2 * i + 1]);
-    *(v4i*)(p.out + t * p.o_row + hh * p.o_head + c * 16) = o;
-    return;
-  }
-  float scale = 1.0f;
-  if constexpr (E4M3) {
-    uint32_t m = 0;  // (as integers: a NaN is larger than everything)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
-      m = m > u ? m : u;
-    }
-    scale = __uint_as_float(max_lanes<LG>(m)) / 448.0f;
-    scale = scale < 1e-12f ? 1e-12f : scale;
-  }
-  if (pos < 0 || pos >= p.cap) return;
-  const int page = p.table[b * p.table_stride + (pos >> p.page_shift)], slot = pos & ((1 << p.page_shift) - 1);
-  if ((unsigned)page >= (unsigned)p.pages) return;
-  char* to = kind == 1 ? (char*)p.k + page * p.k_page + hh * p.k_head + (int64_t)slot * p.k_slot
-                       : (char*)p.v + page * p.v_page + hh * p.v_head + (int64_t)slot * p.v_slot;
-  if constexpr (E4M3) {
-    int lo = 0, hi = 0;
-    float q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      q[i] = x[i] / scale;
-      q[i] = q[i] != q[i] ? q[i] : fminf(fmaxf(q[i], -448.0f), 448.0f);
-    }
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], hi, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
-    *(int2*)(to + c * 8) = make_int2(lo, hi);
-    if (c == 0) {
-      if (kind == 1) ((float*)p.ks)[page * p.ks_page + hh * p.ks_head + slot] = scale;
-      else ((float*)p.vs)[page * p.vs_page + hh * p.vs_head + slot] = scale;
-    }
-  } else {
-    v4i o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = (int)pack2<T>(x[2 * i], x[2 * i + 1]);
-    *(v4i*)(to + c * 16) = o;
   }
 }
 
@@ -209,9 +239,11 @@ int fmsmo_paged_args(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batc
 
 template <int T, bool E4M3, int D, int WT>
 static void run_store(const StoreArgs& a, bool interleaved, int64_t rows, hipStream_t s) {
-  const dim3 grid((unsigned)rows, (unsigned)div_up(a.heads + 2 * a.p.kv_heads, 2048 / D));
-  if (interleaved) hipLaunchKernelGGL((kv_store_kernel<T, E4M3, D, WT, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((kv_store_kernel<T, E4M3, D, WT, false>), grid, dim3(256), 0, s, a);
+  // groups of 2048 elements; a block takes all of them where there are blocks enough without
+  const int groups = div_up(a.heads + 2 * a.p.kv_heads, 2048 / D), per = rows >= 2048 ? (groups < 8 ? groups : 8) : 1;
+  const dim3 grid((unsigned)rows, (unsigned)div_up(groups, per));
+  if (interleaved) hipLaunchKernelGGL((kv_store_kernel<T, E4M3, D, WT, true>), grid, dim3(256), 0, s, a, per);
+  else hipLaunchKernelGGL((kv_store_kernel<T, E4M3, D, WT, false>), grid, dim3(256), 0, s, a, per);
 }
 
 extern "C" int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, int dtype, int64_t rows, int q_heads,

@@ -112,101 +112,87 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     v_base = r * ROW + (((lane >> 4 & 1) * 2 + l16 % 4 / 2) ^ value_place(r)) * 16 + l16 % 2 * 8;
   }
   constexpr int RPC = 1024 / D;  // rows of a load of codes
-  int kw_base, vw_base, k_from, v_from;
+  int kw_base, vw_base;
   {
     const int r = lane / (D / 16), at = lane % (D / 16);
     kw_base = (16 * wave + r) * ROW + (2 * at ^ key_place(r)) * 16;
     vw_base = (16 * wave + r) * ROW + (2 * at ^ value_place(r)) * 16;
-    k_from = r * a.k_slot + at * 16;
-    v_from = r * a.v_slot + at * 16;
   }
 
-  // This wave's 16 keys of a tile.  16-bit caches: instruction j brings 1 KiB, lane i the 16-byte piece that belongs at its end.
-  constexpr int PIECES = ROW / 16;       // of a row
-  constexpr int RPL = 64 / PIECES;       // rows of an instruction
-  int k_off[E4M3 ? 1 : LOADS], v_off[E4M3 ? 1 : LOADS];
-  if constexpr (!E4M3) {
+  // This wave's 16 keys of a tile, straight from memory, 1 KiB an instruction.  16 bits: lane i brings the 16-byte piece that belongs
+  // at its end.  Codes, half as many bytes: into the second half of their place, from which they are widened when they are there.
+  constexpr int PIECES = (E4M3 ? D : ROW) / 16;  // of a row
+  constexpr int RPL = 64 / PIECES;               // rows of an instruction
+  constexpr int N = E4M3 ? CODES : LOADS;
+  int k_off[N], v_off[N];
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int r = j * RPL + lane / PIECES, at = lane % PIECES;  // (16 rows further the places are the same)
-      k_off[j] = r * a.k_slot + (at ^ key_place(r)) * 16;
-      v_off[j] = r * a.v_slot + (at ^ value_place(r)) * 16;
-    }
+  for (int j = 0; j < N; ++j) {
+    const int r = j * RPL + lane / PIECES, at = lane % PIECES;  // (16 rows further the places are the same)
+    k_off[j] = r * a.k_slot + (E4M3 ? at : at ^ key_place(r)) * 16;
+    v_off[j] = r * a.v_slot + (E4M3 ? at : at ^ value_place(r)) * 16;
   }
-  v4i kr[E4M3 ? CODES : 1], vr[E4M3 ? CODES : 1];
-  float sr = 0.0f;
+  constexpr int RAW = E4M3 ? CODES * 1024 : 0;
+  float sr = 0.0f;  // scales: of the keys in lanes 0 .. 15, of the values in lanes 16 .. 31
   const auto load = [&](int tile, int pages, int there, int buf) {
-    const int k0 = key_of(tile) + 16 * wave;
-    const int64_t page = there >> wave & 1 ? __builtin_amdgcn_readlane(pages, wave) : 0, slot = k0 & in_page;
+    const int64_t page = there >> wave & 1 ? __builtin_amdgcn_readlane(pages, wave) : 0, slot = (key_of(tile) + 16 * wave) & in_page;
     const char* ks = a.k + page * a.k_page + hk * a.k_head + slot * a.k_slot;
     const char* vs = a.v + page * a.v_page + hk * a.v_head + slot * a.v_slot;
-    if constexpr (!E4M3) {
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        to_shared(ks, &kl[buf][16 * wave * ROW + j * 1024], k_off[j]);
-        to_shared(vs, &vl[buf][16 * wave * ROW + j * 1024], v_off[j]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < CODES; ++j) {
-        kr[j] = *(const v4i*)(ks + j * RPC * a.k_slot + (unsigned)k_from);
-        vr[j] = *(const v4i*)(vs + j * RPC * a.v_slot + (unsigned)v_from);
-      }
-      if (lane < 32) {
-        const float* src = lane < 16 ? a.ks + page * a.ks_page + hk * a.ks_head : a.vs + page * a.vs_page + hk * a.vs_head;
-        sr = src[slot + (lane & 15)];
-        sr = lane < 16 ? sr * c : sr;
-      }
+    for (int j = 0; j < N; ++j) {
+      to_shared(ks, &kl[buf][16 * wave * ROW + RAW + j * 1024], k_off[j]);
+      to_shared(vs, &vl[buf][16 * wave * ROW + RAW + j * 1024], v_off[j]);
+    }
+    if constexpr (E4M3) {
+      const float* src = (lane & 16) ? a.vs + page * a.vs_page + hk * a.vs_head : a.ks + page * a.ks_page + hk * a.ks_head;
+      sr = src[slot + (lane & 15)] * ((lane & 16) ? 1.0f : c);
     }
   };
-  // In a tile that is not seen as a whole: what nobody may see becomes zero, and so do infinities and NaN (see finite_only).
+  // What a tile that has arrived still needs.  Codes become 16-bit numbers.  In a tile that is not seen as a whole, values that nobody
+  // may see become zero, and so do infinities and NaN (see finite_only).
   const auto settle = [&](int tile, int buf, int there, bool part) {
     bool fine = true;
     const int k0 = key_of(tile) + 16 * wave;
+    const auto clean = [&](uint32_t u, int r) {
+      const bool in = (there >> wave & 1) && k0 + r < s.len;
+      const uint32_t v = in ? finite_only<PT>(u) : 0u;
+      fine = fine && (v == u || !in);
+      return v;
+    };
     if constexpr (E4M3) {
+      v4i ku[CODES], vu[CODES];
 #pragma unroll
       for (int j = 0; j < CODES; ++j) {
-        const int r = j * RPC + lane / (D / 16);
-        if (part && !((there >> wave & 1) && k0 + r < s.len)) kr[j] = vr[j] = v4i{0, 0, 0, 0};
-        uint32_t y[8], z[8];
+        ku[j] = *(const v4i*)(kl[buf] + 16 * wave * ROW + RAW + j * 1024 + lane * 16);
+        vu[j] = *(const v4i*)(vl[buf] + 16 * wave * ROW + RAW + j * 1024 + lane * 16);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (all of them are read before the first is written over)
+      // (rows j RPC + r with r < RPC, a power of two: their places are those of r with the bits of j RPC turned over)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          widen4<QT>((uint32_t)kr[j][i], y[2 * i], y[2 * i + 1]);
-          widen4<PT>((uint32_t)vr[j][i], z[2 * i], z[2 * i + 1]);
-        }
-        if (part) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t u = finite_only<PT>(z[i]);
-            fine = fine && u == z[i];
-            z[i] = u;
-          }
-        }
-        // (rows j RPC + r with r < RPC, a power of two: their places are those of r with the bits of j RPC turned over)
-        char* kt = kl[buf] + j * RPC * ROW;
-        char* vt = vl[buf] + j * RPC * ROW;
+      for (int j = 0; j < CODES; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          *(v4i*)(kt + (kw_base ^ (h ^ key_place(j * RPC)) * 16)) = v4i{(int)y[4 * h], (int)y[4 * h + 1], (int)y[4 * h + 2], (int)y[4 * h + 3]};
-          *(v4i*)(vt + (vw_base ^ (h ^ value_place(j * RPC)) * 16)) = v4i{(int)z[4 * h], (int)z[4 * h + 1], (int)z[4 * h + 2], (int)z[4 * h + 3]};
+          uint32_t y[4], z[4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            widen4<QT>((uint32_t)ku[j][2 * h + i], y[2 * i], y[2 * i + 1]);
+            widen4<PT>((uint32_t)vu[j][2 * h + i], z[2 * i], z[2 * i + 1]);
+          }
+          if (part) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = clean(z[i], j * RPC + lane / (D / 16));
+          }
+          __builtin_memcpy(kl[buf] + j * RPC * ROW + (kw_base ^ (h ^ key_place(j * RPC)) * 16), y, 16);
+          __builtin_memcpy(vl[buf] + j * RPC * ROW + (vw_base ^ (h ^ value_place(j * RPC)) * 16), z, 16);
         }
-      }
       if (lane < 32) sc[buf][lane >> 4][16 * wave + (lane & 15)] = sr;
     } else if (part) {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
-        const int r = j * RPL + lane / PIECES;
-        v4i* vt = (v4i*)(vl[buf] + 16 * wave * ROW + j * 1024 + lane * 16);
-        v4i u = {0, 0, 0, 0};
-        if ((there >> wave & 1) && k0 + r < s.len) {
-          const v4i v = *vt;
+        v4i* at = (v4i*)(vl[buf] + 16 * wave * ROW + j * 1024 + lane * 16);
+        v4i u = *at;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            u[i] = (int)finite_only<PT>((uint32_t)v[i]);
-            fine = fine && u[i] == v[i];
-          }
-        }
-        *vt = u;
+        for (int i = 0; i < 4; ++i) u[i] = (int)clean((uint32_t)u[i], j * RPL + lane / PIECES);
+        *at = u;
       }
     }
     if (part && __any(!fine) && lane == 0) odd = 1;
@@ -219,14 +205,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     pages = pages_of(1);
   }
   __syncthreads();
-  if (E4M3 && t.count > 0) settle(0, 0, there, partial(0, there));
   for (int tile = 0; tile < t.count; ++tile) {
     const int buf = tile & 1, k0 = key_of(tile);
     const bool part = partial(tile, there);
-    if constexpr (!E4M3) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (part) settle(tile, buf, there, true);
-    }
+    if (!E4M3 || tile == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (E4M3 ? tile == 0 : part) settle(tile, buf, there, part);
     // this tile is here, and nobody reads the one before it any more
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int there_now = there;
@@ -281,9 +264,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, st[0][i]), st[1][i]);
     top = max_x32(top) * by;
-    // The maximum is held back: powers up to 2^8 are as good as powers up to 1, and O is rescaled a few times at all.
-    if (__any(top > m + 8.0f || (m == -__builtin_inff() && top > m))) {
-      const float m_new = fmaxf(m, top), f = exp2_hw(m - safe_max(m_new));
+    // The maximum is held back: powers up to 2^8 are as good as powers up to 1, and O is rescaled a few times at all.  (e4m3 keeps too
+    // much in registers for a branch around O, which copies it: 2900 us with, 2833 without for 2 x 2048 tokens behind 30000 keys; 16-bit
+    // caches 560 with, 600 without for 8192 tokens)
+    const bool grow = top > m + 8.0f || (m == -__builtin_inff() && top > m);
+    if (E4M3 || __any(grow)) {
+      const float m_new = grow ? fmaxf(m, top) : m, f = grow ? exp2_hw(m - safe_max(m_new)) : 1.0f;
 #pragma unroll
       for (int d = 0; d < NV; ++d) o[d] *= f;
       l *= f;
@@ -338,7 +324,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
         o[d] = mfma32<PT>(f, pb[k], o[d]);
         if constexpr (TWO) o[d] = mfma32<PT>(f, pl[k], o[d]);
       }
-    if (E4M3 && more) settle(tile + 1, buf ^ 1, there, partial(tile + 1, there));
+    if (E4M3 && more) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      settle(tile + 1, buf ^ 1, there, partial(tile + 1, there));
+    }
   }
 
   l = sum_x32(l);

@@ -1310,6 +1310,11 @@ def qk_norm_rope_store(q, k, v, k_cache, v_cache, block_table, seq_lens, query_s
 
     k_cache, v_cache [pages, kv heads, page size, dim]; block_table int32 [B, pages], seq_lens int32 [B] with the new tokens,
     query_start int32 [B + 1] (None: one token per sequence).  See fmsmo_kv_store and fmsmo_kv_batch_t."""
+    if not _COMPILING():
+        r = (_H or _host()).kv_store(q, k, v, k_cache, v_cache, block_table, seq_lens, query_start, cos, sin, interleaved, q_weight, k_weight,
+                                     eps, k_scale, v_scale, out)
+        if r is not None:
+            return r if out is None else out
     _need_gpu(q)
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, head dim]")
@@ -1333,6 +1338,11 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, query_start=None
     sequence's new tokens and keys, where the host knows them; the work is laid out for them (any length is right).  Returns
     [T, heads, dim] in ``out`` or a new tensor; tokens that see nothing, and in a new tensor rows of no sequence, are zero.
     No gradients.  See fmsmo_paged_attn."""
+    if not _COMPILING():
+        r = (_H or _host()).paged_attention(q, k_cache, v_cache, block_table, seq_lens, query_start, scale, window or 0, sinks or 0, k_scale,
+                                            v_scale, max_query_len or 0, max_seq_len or 0, out)
+        if r is not None:
+            return r if out is None else out
     _need_gpu(q)
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, head dim]")

@@ -102,7 +102,7 @@ def test_workspace_grows_with_what_is_split():
     assert f(4, 2, 128, 3, 3, 1, 64) == 0            # one launch
     assert f(4, 2, 128, 3, 3000, 1000, 1000) == 0    # prompts
     n = f(4, 2, 128, 3, 3, 1, 100000)
-    assert n > 0 and n % 16 == 0 and f(4, 2, 256, 3, 3, 1, 100000) > n
+    assert n > 0 and n % 16 == 0 and n > f(4, 2, 64, 3, 3, 1, 100000) > 0 and n == f(4, 2, 128, 3, 3, 1, 200000)
     assert f(3, 2, 128, 3, 3, 1, 100) == 0 and f(0, 0, 128, 0, 0, 0, 0) == 0
 
 
