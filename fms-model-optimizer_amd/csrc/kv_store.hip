@@ -240,7 +240,7 @@ int fmsmo_paged_args(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batc
 template <int T, bool E4M3, int D, int WT>
 static void run_store(const StoreArgs& a, bool interleaved, int64_t rows, hipStream_t s) {
   // groups of 2048 elements; a block takes all of them where there are blocks enough without
-  const int groups = div_up(a.heads + 2 * a.p.kv_heads, 2048 / D), per = rows >= 2048 ? (groups < 8 ? groups : 8) : 1;
+  const int groups = div_up(a.heads + 2 * a.p.kv_heads, 2048 / D), per = rows >= 768 ? (groups < 8 ? groups : 8) : 1;
   const dim3 grid((unsigned)rows, (unsigned)div_up(groups, per));
   if (interleaved) hipLaunchKernelGGL((kv_store_kernel<T, E4M3, D, WT, true>), grid, dim3(256), 0, s, a, per);
   else hipLaunchKernelGGL((kv_store_kernel<T, E4M3, D, WT, false>), grid, dim3(256), 0, s, a, per);

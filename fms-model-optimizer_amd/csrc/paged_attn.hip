@@ -25,14 +25,6 @@ namespace fmsmo {
 constexpr int TILE = 32, WAVES = 4;
 constexpr int MAX_WORKERS = 512;  // two blocks per compute unit
 
-struct SplitArgs {
-  PagedArgs p;
-  float* ws;
-  int workers, unit_shift;  // 1 << unit_shift tiles are never divided between blocks
-  int row_shift;            // 1 << row_shift waves of a block take the same keys, 16 rows each
-  int splits;               // pairs may be cut: the workspace is there
-};
-
 // A sequence's part of the work: (heads x groups of rows) x units
 struct Part {
   int groups, units, pairs;
@@ -70,20 +62,6 @@ struct Deal {
     return (int)(u < big ? u / (each + 1) : more + (u - big) / each);
   }
 };
-
-// What the join needs to know of a cut pair: written by the pair's second worker.
-struct Cut {
-  int rows;             // 0: nothing to join
-  int first, last;      // workers
-  int first_slot;       // of the first worker (the others hold the pair's part in slot 0)
-  int row0, pair_row0;  // q row of the sequence, row of the pair's group in it
-  int head, pad;        // key head
-};
-// workspace: Cut[workers], then per worker two slots of { o[rows][D], (m, l)[rows] }: its first part, its last
-template <int D>
-__device__ __forceinline__ float* slot_of(const SplitArgs& a, int worker, int slot) {
-  return (float*)((Cut*)a.ws + a.workers) + (((int64_t)(2 * worker + slot) * 16 * (D + 2)) << a.row_shift);
-}
 
 // MULTI: rows of a group may stand at different positions.  SHARED: row_shift > 0
 template <int QT, bool E4M3, int D, bool MULTI, bool SHARED>
@@ -271,10 +249,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
       Cut d{};
       if (u0 > 0) {
         const int from = u - u0;
-        d.first = deal.worker(from);
-        d.last = deal.worker(from + units - 1);
-        d.first_slot = from <= deal.first(d.first) ? 0 : 1;
-        d.rows = d.first == (int)blockIdx.x - 1 ? grows : 0;
+        const int worker = deal.worker(from);
+        d.first = 2 * worker + (from <= deal.first(worker) ? 0 : 1);
+        d.last = 2 * deal.worker(from + units - 1);
+        d.rows = worker == (int)blockIdx.x - 1 ? grows : 0;
         d.row0 = s.row0;
         d.pair_row0 = g0;
         d.head = hk;
@@ -468,7 +446,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
         }
       } else {
         const int r = 16 * row_tile + c16;
-        float* share = slot_of<D>(sa, blockIdx.x, first ? 0 : 1);
+        float* share = share_of<D>(sa, 2 * blockIdx.x + (first ? 0 : 1));
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
           float y[ND];
@@ -486,7 +464,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
   }
 }
 
-// Joins the shares of the pairs that were cut: a block per cut and row.  The weights of all shares first (a share per thread), then
+// Joins the shares of the pairs that were cut: a block per cut and row, rows side by side, since neighbouring blocks go to different parts
+// of the chip and cuts may come in steps of eight (with the cuts side by side 32 pairs of 32 rows in 16 shares took 23 us, not 8).  The weights of all shares first (a share per thread), then
 // every group of D / 4 threads adds up every (1024 / D)-th share: loads that wait for nothing but the weights.
 template <int QT, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
@@ -495,10 +474,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
   __shared__ float red[8];
   __shared__ __attribute__((aligned(16))) float sum[GROUPS][D];
   const PagedArgs& a = sa.p;
-  const Cut d = ((const Cut*)sa.ws)[blockIdx.x];
-  const int shares = d.last - d.first + 1, rows = 16 << sa.row_shift, tid = threadIdx.x, wave = tid >> 6;
-  for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
-    const auto share = [&](int k) { return slot_of<D>(sa, d.first + k, k == 0 ? d.first_slot : 0); };
+  const Cut d = ((const Cut*)sa.ws)[blockIdx.y];
+  // split kernel: every worker has two shares, and but for the first one it is its first part that belongs here
+  const int step = sa.parts ? 1 : 2, shares = sa.parts ? sa.parts : d.last / 2 - d.first / 2 + 1;
+  const int rows = 16 << sa.row_shift, tid = threadIdx.x, wave = tid >> 6;
+  for (int r = blockIdx.x; r < d.rows; r += gridDim.x) {
+    const auto share = [&](int k) { return share_of<D>(sa, k == 0 ? d.first : (d.first / step + k) * step); };
     float top = -__builtin_inff();
     for (int k = tid; k < shares; k += 256) {
       weight[k] = *(const float2*)(share(k) + rows * D + 2 * r);
@@ -522,7 +503,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
     const int c = tid % LG;
     v4f o = {0, 0, 0, 0};
 #pragma unroll 4
-    for (int k = tid / LG; k < shares; k += GROUPS) o += *(const v4f*)(share(k) + r * D + 4 * c) * weight[k].x;
+    for (int k = tid / LG; k < shares; k += GROUPS) {
+      const v4f x = *(const v4f*)(share(k) + r * D + 4 * c);
+      const float f = weight[k].x;
+      o += f == 0.0f && weight[k].y == 0.0f ? v4f{0, 0, 0, 0} : x * f;  // (a share without keys holds no sums)
+    }
     *(v4f*)&sum[tid / LG][4 * c] = o;
     __syncthreads();
     if (tid < LG) {
@@ -547,7 +532,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
 using namespace fmsmo;
 
 int fmsmo_check_launch();
-int fmsmo_paged_prompt(const PagedArgs& a, int dtype, bool e4m3, int dim, fmsmo_stream_t stream);
+int fmsmo_paged_prompt(const SplitArgs& a, int dtype, bool e4m3, int dim, fmsmo_stream_t stream);
 
 // Checks a call's arguments and puts them into the kernels' form.
 int fmsmo_paged_args(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, const void* q, int64_t q_row, int64_t q_head,
@@ -626,26 +611,44 @@ struct Plan {
   bool prompt;  // the kernel of many rows
   int row_shift, unit_shift, workers;
   bool splits;
+  int tiles, parts;  // prompt kernel
+  int64_t cuts, shares;
 };
-static Plan plan_of(int group, int kv_heads, int dim, int64_t seqs, int64_t rows, int64_t max_rows, int64_t max_keys) {
+static Plan plan_of(int group, int kv_heads, int dim, bool e4m3, int64_t seqs, int64_t rows, int64_t max_rows, int64_t max_keys) {
   Plan p{};
-  const int64_t most = max_rows * group;
-  p.prompt = most > 16 * WAVES;
-  p.row_shift = most <= 16 ? 0 : most <= 32 ? 1 : 2;
+  const int64_t most = max_rows * group, tokens = std::max<int64_t>(1, std::min(seqs, rows));
+  // Up to 16 rows are one tile of the split kernel; up to 32 rows of an e4m3 cache, whose codes it widens on the way to the products,
+  // two waves take the same keys.  5 tokens x 4 heads, 16 sequences of 16000 keys: 16 bits 229 us so and 221 by the prompt kernel,
+  // e4m3 157 and 260.
+  p.prompt = most > (e4m3 ? 32 : 16);
+  if (p.prompt) {
+    p.row_shift = 3;
+    p.tiles = (int)(rows * group / PROMPT_ROWS + seqs);
+    // Few tiles of rows: several blocks for each, as many as leave every one eight tiles of keys, up to two for a compute unit
+    const int64_t blocks = std::max<int64_t>(rows * group / PROMPT_ROWS, 1) * kv_heads, key_tiles = (max_keys + PROMPT_KEYS - 1) / PROMPT_KEYS;
+    p.cuts = (int64_t)p.tiles * kv_heads;  // (counted with the room between sequences: at most 2048 shares, 64 KiB each at 128 elements)
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({(dim > 128 ? 256 : 512) / blocks, key_tiles / 8, 2048 / p.cuts, 64}));
+    p.splits = p.parts > 1;
+    p.shares = p.cuts * p.parts;
+    return p;
+  }
+  p.row_shift = most <= 16 ? 0 : 1;
   const int64_t tiles = std::max<int64_t>(1, (max_keys + TILE - 1) / TILE), waves = WAVES >> p.row_shift;
-  const int64_t pairs = std::max<int64_t>(1, std::min(seqs, rows)) * kv_heads;
+  const int64_t pairs = tokens * kv_heads;
   // One launch where a block per pair is through as early as the second launch would be: it takes 4 us, an iteration of
   // all waves 1.5 to 2 us while memory is not busy.  Single tokens, 8 key heads of 128 elements, one launch / two: 1 sequence of 400 keys
-  // 11.6 / 9.6 us, 8 of them 13.1 / 10.9, 32 of them 15.4 / 18.6.
+  // 11.6 / 9.6 us, 8 of them 13.1 / 10.9, 32 of them 13.3 / 18.6.
   p.splits = tiles > waves && !(pairs >= 192 && tiles <= 4 * waves);
   p.unit_shift = p.splits ? 2 - p.row_shift : 26;
   const int64_t units = pairs * (((tiles - 1) >> p.unit_shift) + 1);
   // as many as are resident: two blocks per compute unit, one where the registers leave room for one
   p.workers = (int)std::min<int64_t>(!p.splits ? 65536 : dim > 128 ? MAX_WORKERS / 2 : MAX_WORKERS, units);
+  p.cuts = p.workers;
+  p.shares = 2 * p.workers;
   return p;
 }
 static int64_t plan_bytes(const Plan& p, int dim) {
-  return p.prompt || !p.splits ? 0 : p.workers * ((int64_t)sizeof(Cut) + (2 * 16 * (dim + 2) * 4ll << p.row_shift));
+  return p.splits ? p.cuts * (int64_t)sizeof(Cut) + (p.shares * 16 * (dim + 2) * 4 << p.row_shift) : 0;
 }
 static void bounds(int64_t& max_rows, int64_t& max_keys, int64_t rows, int64_t cap, bool ragged) {
   if (!ragged) max_rows = 1;
@@ -653,11 +656,11 @@ static void bounds(int64_t& max_rows, int64_t& max_keys, int64_t rows, int64_t c
   if (max_keys < 1 || max_keys > cap) max_keys = std::max<int64_t>(1, cap);
 }
 
-extern "C" int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int64_t seqs, int64_t rows, int64_t max_rows,
+extern "C" int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int cache_dtype, int64_t seqs, int64_t rows, int64_t max_rows,
                                                     int64_t max_keys) {
   if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || rows < 1 || seqs < 1) return 0;
   bounds(max_rows, max_keys, rows, 1ll << 30, true);
-  return plan_bytes(plan_of(q_heads / kv_heads, kv_heads, dim, seqs, rows, max_rows, max_keys), dim);
+  return plan_bytes(plan_of(q_heads / kv_heads, kv_heads, dim, cache_dtype == FMSMO_KV_E4M3, seqs, rows, max_rows, max_keys), dim);
 }
 
 extern "C" int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, int dtype, int64_t rows, int q_heads,
@@ -676,32 +679,48 @@ extern "C" int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_ba
   a.zero_rest = zero_rest && batch->query_start;
   bounds(max_rows, max_keys, rows, a.cap, batch->query_start != nullptr);
   const bool e4m3 = cache->dtype == FMSMO_KV_E4M3;
-  const Plan p = plan_of(a.group, a.kv_heads, cache->dim, a.seqs, rows, max_rows, max_keys);
-  if (p.prompt) return fmsmo_paged_prompt(a, dtype, e4m3, cache->dim, stream);
+  const Plan p = plan_of(a.group, a.kv_heads, cache->dim, e4m3, a.seqs, rows, max_rows, max_keys);
   const int64_t need = plan_bytes(p, cache->dim);
   if (need > workspace_bytes || (need && !workspace)) return FMSMO_ERR_SCRATCH;
   if (((uintptr_t)workspace) & 15) return FMSMO_ERR_ALIGN;
-  // (units are counted in 31 bits: heads x groups of rows x units of a sequence, summed)
-  const int64_t pairs = ((rows * a.group >> (4 + p.row_shift)) + a.seqs) * a.kv_heads;
-  if (pairs * ((a.cap / TILE >> p.unit_shift) + 2) > 0x7fffffffll) return FMSMO_ERR_UNSUPPORTED;
   sa.ws = (float*)workspace;
-  sa.workers = p.workers;
-  sa.unit_shift = p.unit_shift;
+  sa.cuts = (int)p.cuts;
   sa.splits = p.splits;
   sa.row_shift = p.row_shift;
+  sa.tiles = p.tiles;
+  sa.parts = p.parts;
+  const hipStream_t s = (hipStream_t)stream;
+  const auto join = [&](auto t, auto d) {
+    if (!p.splits) return;
+    // rows of a pair, as a rule; of a prompt's a block takes every 32nd
+    const unsigned per = (unsigned)std::min<int64_t>(max_rows * a.group, p.prompt ? 32 : 16 << p.row_shift);
+    hipLaunchKernelGGL((paged_join_kernel<decltype(t)::value, decltype(d)::value>), dim3(per, (unsigned)p.cuts), dim3(256), 0, s, sa);
+  };
+  if (p.prompt) {
+    if (p.cuts * p.parts > 0x7fffffffll / 256) return FMSMO_ERR_UNSUPPORTED;
+    const int done = fmsmo_paged_prompt(sa, dtype, e4m3, cache->dim, stream);
+    if (done) return done;
+  }
+  // (units are counted in 31 bits: heads x groups of rows x units of a sequence, summed)
+  const int64_t pairs = ((rows * a.group >> (4 + p.row_shift)) + a.seqs) * a.kv_heads;
+  if (!p.prompt && pairs * ((a.cap / TILE >> p.unit_shift) + 2) > 0x7fffffffll) return FMSMO_ERR_UNSUPPORTED;
+  sa.workers = p.workers;
+  sa.unit_shift = p.unit_shift;
   const auto go = [&](auto t, auto e, auto d) {
     constexpr int T = decltype(t)::value, D = decltype(d)::value;
     constexpr bool E = decltype(e)::value;
     const dim3 grid(p.workers), threads(64 * WAVES);
-    const hipStream_t s = (hipStream_t)stream;
-    if (a.starts && p.row_shift) hipLaunchKernelGGL((paged_split_kernel<T, E, D, true, true>), grid, threads, 0, s, sa);
-    else if (a.starts) hipLaunchKernelGGL((paged_split_kernel<T, E, D, true, false>), grid, threads, 0, s, sa);
-    else if (p.row_shift) hipLaunchKernelGGL((paged_split_kernel<T, E, D, false, true>), grid, threads, 0, s, sa);
-    else hipLaunchKernelGGL((paged_split_kernel<T, E, D, false, false>), grid, threads, 0, s, sa);
-    if (p.splits) {
-      const unsigned per = (unsigned)std::min<int64_t>(max_rows * a.group, 16 << p.row_shift);  // rows of a group, as a rule
-      hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(p.workers, per), dim3(256), 0, s, sa);
+    if (p.prompt) return join(t, d);
+    if constexpr (E) {
+      if (p.row_shift) {
+        if (a.starts) hipLaunchKernelGGL((paged_split_kernel<T, E, D, true, true>), grid, threads, 0, s, sa);
+        else hipLaunchKernelGGL((paged_split_kernel<T, E, D, false, true>), grid, threads, 0, s, sa);
+        return join(t, d);
+      }
     }
+    if (a.starts) hipLaunchKernelGGL((paged_split_kernel<T, E, D, true, false>), grid, threads, 0, s, sa);
+    else hipLaunchKernelGGL((paged_split_kernel<T, E, D, false, false>), grid, threads, 0, s, sa);
+    join(t, d);
   };
   const auto dims = [&](auto t, auto e) {
     if (cache->dim == 64) go(t, e, std::integral_constant<int, 64>{});

@@ -12,6 +12,8 @@ namespace fmsmo {
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
+constexpr int PROMPT_ROWS = 128, PROMPT_KEYS = 64;  // tiles of the prompt kernel
+
 constexpr float LOG2E = 1.44269504088896340736f;
 
 struct PagedArgs {
@@ -113,6 +115,32 @@ __device__ __forceinline__ Bounds bounds_of(const PagedArgs& a, int p_lo, int p_
   return b;
 }
 __device__ __forceinline__ bool inside(const Bounds& b, int off) { return off <= b.hi && (off > b.lo || off < b.sink); }
+
+// ------------------------------------------------------------------ work split over a sequence's keys
+struct SplitArgs {
+  PagedArgs p;
+  float* ws;
+  int cuts;                 // entries that tell the join of a head and rows that several blocks share
+  int workers, unit_shift;  // split kernel: 1 << unit_shift tiles are never divided between blocks
+  int row_shift;            // 16 << row_shift rows in a share; split kernel: 1 << row_shift waves of a block take the same keys
+  int splits;               // the workspace is there
+  int tiles, parts;         // prompt kernel: tiles of rows, blocks for each
+};
+// Shares first .. last of rows row0 .. of a key head's queries (counted as tokens x heads of the group)
+struct Cut {
+  int rows;         // 0: nothing to join
+  int first, last;  // shares
+  int pad;
+  int row0;       // q row of the sequence
+  int pair_row0;  // first row in it
+  int head;       // key head
+  int pad2;
+};
+// workspace: Cut[cuts], then shares of { o[rows][D], (m, l)[rows] }
+template <int D>
+__device__ __forceinline__ float* share_of(const SplitArgs& a, int share) {
+  return (float*)((Cut*)a.ws + a.cuts) + (((int64_t)share * 16 * (D + 2)) << a.row_shift);
+}
 
 // ------------------------------------------------------------------ cross-lane
 // a maximum (sum) over the lanes that differ in bit 5, and in bits 5 and 4: v_permlane*_swap, no LDS round trip

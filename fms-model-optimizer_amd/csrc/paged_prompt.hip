@@ -15,10 +15,11 @@
 
 namespace fmsmo {
 
-constexpr int BM = 128, BN = 64;
+constexpr int BM = PROMPT_ROWS, BN = PROMPT_KEYS;
 
 template <int QT, bool E4M3, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(PagedArgs a, int tiles_x) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(SplitArgs sa) {
+  const PagedArgs& a = sa.p;
   // e4m3 caches: the values' scales are multiplied in before the probabilities are rounded, which takes the exponents of bf16; for
   // an fp16 result, of which bf16 would lose three bits, they are the sum of two bf16 numbers
   constexpr int PT = E4M3 ? FMSMO_BF16 : QT;
@@ -40,7 +41,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   if (a.zero_rest) zero_rest(a, D / 8);
 
   // the tile of rows: sequence b's start at tile query_start[b] group / BM + b, which leaves room for all of them
-  const int hk = blockIdx.x % a.kv_heads, x = tiles_x - 1 - blockIdx.x / a.kv_heads;
+  const int hk = blockIdx.x % a.kv_heads, y = blockIdx.x / a.kv_heads, part_no = sa.splits ? y % sa.parts : 0;
+  const int x = sa.tiles - 1 - (sa.splits ? y / sa.parts : y), pair = x * a.kv_heads + hk;
+  const auto nothing = [&] {
+    if (sa.splits && part_no == 0 && threadIdx.x == 0) ((Cut*)sa.ws)[pair].rows = 0;
+  };
   int before = 0;
   for (int c = 0; c < a.seqs; c += 64) {
     bool yes = false;
@@ -51,17 +56,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     before += __popcll(__ballot(yes));
   }
   const int b = uniform(before) - 1;
-  if (b < 0) return;
+  if (b < 0) return nothing();
   Seq s = seq_of(a, b);
   s.n = uniform(s.n);
   s.row0 = uniform(s.row0);
   s.pos0 = uniform(s.pos0);
   s.len = uniform(s.len);
   const int r0 = (x - (int)((int64_t)s.row0 * a.group / BM) - b) * BM;
-  if (s.n == 0 || r0 < 0 || r0 >= s.n * a.group) return;
+  if (s.n == 0 || r0 < 0 || r0 >= s.n * a.group) return nothing();
   const int nrows = s.n * a.group - r0 < BM ? s.n * a.group - r0 : BM;
   const int p_lo = s.pos0 + r0 / a.group, p_hi = s.pos0 + (r0 + nrows - 1) / a.group;
   const Tiles t = tiles_of<BN>(a, s.len, p_lo, p_hi);
+  // this block's tiles of keys
+  const int begin = sa.splits ? t.count * part_no / sa.parts : 0, end = sa.splits ? t.count * (part_no + 1) / sa.parts : t.count;
   // this wave's rows
   const int wr = wave * 32, wn = nrows - wr < 32 ? nrows - wr : 32;
   const bool mine = wr + c32 < nrows;
@@ -97,7 +104,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   };
   // which of them are there
   const auto there_of = [&](int tile, int pages) {
-    return (int)__ballot(tile < t.count && key_of(tile) + 16 * (lane & 3) < s.len && (unsigned)pages < (unsigned)a.pages) & 15;
+    return (int)__ballot(tile < end && key_of(tile) + 16 * (lane & 3) < s.len && (unsigned)pages < (unsigned)a.pages) & 15;
   };
   // a tile that some rows see in part
   const auto partial = [&](int tile, int there) {
@@ -199,21 +206,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   };
 
   if (threadIdx.x == 0) odd = 0;
-  int pages = pages_of(0), there = there_of(0, pages);
-  if (t.count > 0) {
-    load(0, pages, there, 0);
-    pages = pages_of(1);
+  int pages = pages_of(begin), there = there_of(begin, pages);
+  if (begin < end) {
+    load(begin, pages, there, begin & 1);
+    pages = pages_of(begin + 1);
   }
   __syncthreads();
-  for (int tile = 0; tile < t.count; ++tile) {
+  for (int tile = begin; tile < end; ++tile) {
     const int buf = tile & 1, k0 = key_of(tile);
     const bool part = partial(tile, there);
-    if (!E4M3 || tile == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (E4M3 ? tile == 0 : part) settle(tile, buf, there, part);
+    if (!E4M3 || tile == begin) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (E4M3 ? tile == begin : part) settle(tile, buf, there, part);
     // this tile is here, and nobody reads the one before it any more
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int there_now = there;
-    const bool more = tile + 1 < t.count;
+    const bool more = tile + 1 < end;
     if (more) {
       there = there_of(tile + 1, pages);
       load(tile + 1, pages, there, buf ^ 1);
@@ -250,14 +257,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
         }
     }
     if (!whole) {
+      // (one test at a time, and only those that the tile needs)
       const Bounds bd = bounds_of(a, pos, pos, s.len, k0 + 4 * hl);
+      const auto keep = [&](auto seen) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int at = kt * 32 + 8 * (i / 4) + i % 4;
-          st[kt][i] = (there_now >> (at >> 4) & 1) && inside(bd, at) ? st[kt][i] : -__builtin_inff();
-        }
+          for (int i = 0; i < 16; ++i) st[kt][i] = seen(kt * 32 + 8 * (i / 4) + i % 4) ? st[kt][i] : -__builtin_inff();
+      };
+      if (k0 + BN > s.len || k0 + BN - 1 > w_lo) keep([&](int at) { return at <= bd.hi; });
+      if (a.window && k0 <= w_hi - a.window) keep([&](int at) { return at > bd.lo || at < bd.sink; });
+      if (there_now != 15) keep([&](int at) { return (there_now >> (at >> 4) & 1) != 0; });
+      if (!mine) keep([&](int) { return false; });
     }
     const float by = E4M3 ? 1.0f : c;
     float top = fmaxf(st[0][0], st[1][0]);
@@ -333,7 +344,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   l = sum_x32(l);
   if (uniform(odd)) {
 #pragma unroll 1
-    for (int tile = 0; tile < t.count; ++tile) {
+    for (int tile = begin; tile < end; ++tile) {
       const int pages = pages_of(tile), there = there_of(tile, pages);
       if (!partial(tile, there)) continue;
 #pragma unroll 1
@@ -357,6 +368,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       }
     }
   }
+  if (sa.splits) {
+    if (part_no == 0 && threadIdx.x == 0) {
+      Cut d{};
+      d.rows = nrows;
+      d.first = pair * sa.parts;
+      d.last = d.first + sa.parts - 1;
+      d.row0 = s.row0;
+      d.pair_row0 = r0;
+      d.head = hk;
+      ((Cut*)sa.ws)[pair] = d;
+    }
+    if (!mine) return;
+    float* share = share_of<D>(sa, pair * sa.parts + part_no);
+    const int r = wr + c32;
+#pragma unroll
+    for (int d = 0; d < NV; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(v4f*)(share + r * D + d * 32 + 8 * i + 4 * hl) = v4f{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+    if (hl == 0) *(float2*)(share + BM * D + 2 * r) = make_float2(m, l);
+    return;
+  }
   if (!mine) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   char* to = a.out + (s.row0 + tok) * a.o_row + head * a.o_head;
@@ -378,12 +411,11 @@ using namespace fmsmo;
 
 int fmsmo_check_launch();
 
-int fmsmo_paged_prompt(const PagedArgs& a, int dtype, bool e4m3, int dim, fmsmo_stream_t stream) {
-  const int64_t tiles = (int64_t)a.rows * a.group / BM + a.seqs;
-  if (tiles * a.kv_heads > 0x7fffffffll / 256) return FMSMO_ERR_UNSUPPORTED;
+int fmsmo_paged_prompt(const SplitArgs& sa, int dtype, bool e4m3, int dim, fmsmo_stream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)sa.tiles * sa.p.kv_heads * sa.parts);
   const auto go = [&](auto t, auto e, auto d) {
-    hipLaunchKernelGGL((paged_prompt_kernel<decltype(t)::value, decltype(e)::value, decltype(d)::value>),
-                       dim3((unsigned)(tiles * a.kv_heads)), dim3(256), 0, (hipStream_t)stream, a, (int)tiles);
+    hipLaunchKernelGGL((paged_prompt_kernel<decltype(t)::value, decltype(e)::value, decltype(d)::value>), dim3(blocks), dim3(256), 0,
+                       (hipStream_t)stream, sa);
   };
   const auto dims = [&](auto t, auto e) {
     if (dim == 64) go(t, e, std::integral_constant<int, 64>{});

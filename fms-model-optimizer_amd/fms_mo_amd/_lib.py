@@ -126,7 +126,7 @@ OTHER = {
     "fmsmo_gemm_workspace_bytes": ([c_int64, c_int64, c_int64], c_int64),
     "fmsmo_gemm_fp8_workspace_bytes": ([c_int64, c_int64, c_int64], c_int64),
     "fmsmo_matmul_chunk_workspace_bytes": ([c_int, c_int64, c_int64, c_int64, c_int, c_int], c_int64),
-    "fmsmo_paged_attn_workspace_bytes": ([c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64], c_int64),
+    "fmsmo_paged_attn_workspace_bytes": ([c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64], c_int64),
     "fmsmo_decode_linear_ok": ([c_int64, c_int64], c_int),
     "fmsmo_decode_linear_f32s_ok": ([c_int64, c_int64], c_int),
     "fmsmo_small_linear_static_ok": ([c_int64, c_int64, c_int64, _F, _F, _F, _F], c_int),

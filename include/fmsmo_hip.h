@@ -897,14 +897,14 @@ int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch,
  * sequence: zero with zero_rest, else left as they are.
  * max_rows, max_keys: upper bounds of a sequence's rows and keys that the host knows (0: none); they choose the kernel and how
  * the work is split, and a sequence that exceeds them is still computed in full.
- * workspace: fmsmo_paged_attn_workspace_bytes(q_heads, heads, dim, seqs, rows, max_rows, max_keys) bytes, 16-byte aligned, private to the
+ * workspace: fmsmo_paged_attn_workspace_bytes(q_heads, heads, dim, dtype of the cache, seqs, rows, max_rows, max_keys) bytes, 16-byte aligned, private to the
  * call until it has finished; max_rows and max_keys as given there, at least 1 and at most rows and table_width * page_size.
  */
 int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, int dtype, int64_t rows, int q_heads,
                      const void* q, int64_t q_row, int64_t q_head, void* out, int64_t o_row, int64_t o_head, float scale,
                      int64_t window, int64_t sinks, int64_t max_rows, int64_t max_keys, int zero_rest, void* workspace,
                      int64_t workspace_bytes, fmsmo_stream_t stream);
-int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int heads, int dim, int64_t seqs, int64_t rows, int64_t max_rows,
+int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int heads, int dim, int cache_dtype, int64_t seqs, int64_t rows, int64_t max_rows,
                                          int64_t max_keys);
 
 #ifdef __cplusplus

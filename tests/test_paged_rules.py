@@ -99,11 +99,15 @@ def test_workspace_grows_with_what_is_split():
     from fms_mo_amd import _lib as L
 
     f = L.load().fmsmo_paged_attn_workspace_bytes
-    assert f(4, 2, 128, 3, 3, 1, 64) == 0            # one launch
-    assert f(4, 2, 128, 3, 3000, 1000, 1000) == 0    # prompts
-    n = f(4, 2, 128, 3, 3, 1, 100000)
-    assert n > 0 and n % 16 == 0 and n > f(4, 2, 64, 3, 3, 1, 100000) > 0 and n == f(4, 2, 128, 3, 3, 1, 200000)
-    assert f(3, 2, 128, 3, 3, 1, 100) == 0 and f(0, 0, 128, 0, 0, 0, 0) == 0
+    F16, E4M3 = L.F16, L.KV_E4M3
+    assert f(4, 2, 128, F16, 3, 3, 1, 64) == 0              # one launch
+    n = f(4, 2, 128, F16, 3, 3, 1, 100000)
+    assert n > 0 and n % 16 == 0 and n > f(4, 2, 64, F16, 3, 3, 1, 100000) > 0 and n == f(4, 2, 128, F16, 3, 3, 1, 200000)
+    assert f(4, 2, 128, F16, 1, 20000, 20000, 20000) == 0   # prompts: tiles of rows enough for the chip
+    m = f(4, 2, 128, F16, 1, 100, 100, 100000)              # a few tokens behind many: several blocks for a tile of rows
+    assert m > 0 and m % 16 == 0 and m < 1 << 28
+    assert f(64, 8, 256, E4M3, 300, 400, 200, 1 << 20) < 1 << 30
+    assert f(3, 2, 128, F16, 3, 3, 1, 100) == 0 and f(0, 0, 128, F16, 0, 0, 0, 0) == 0
 
 
 def meta(*shape, dtype=torch.float16):
