@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = k0 + 16 * h;
-        pg[h] = row[(k < s.len ? k : 0) >> a.page_shift];
+        pg[h] = row[((unsigned)k < (unsigned)s.len ? k : 0) >> a.page_shift];
       }
     };
     // -1: no such page, or behind the sequence

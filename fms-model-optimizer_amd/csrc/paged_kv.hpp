@@ -68,7 +68,8 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int b) {
     r1 = a.starts[b + 1];
   }
   const int len = a.lens[b];
-  const int n = r1 > r0 && r0 >= 0 ? r1 - r0 : 0;
+  int n = r1 > r0 && r0 >= 0 ? r1 - r0 : 0;
+  n = n < a.rows ? n : a.rows;
   s.pos0 = (len < 0 ? 0 : len) - n;
   s.row0 = r0;
   s.n = r0 >= a.rows ? 0 : n < a.rows - r0 ? n : a.rows - r0;

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Spl
   // lane i (of four) holds the page of a tile's i-th 16 keys, as the table has it; checked when it is used, an iteration later
   const auto pages_of = [&](int tile) {
     const int k = key_of(tile) + 16 * (lane & 3);
-    return table[(k < s.len && k >= 0 ? k : 0) >> a.page_shift];
+    return table[((unsigned)k < (unsigned)s.len ? k : 0) >> a.page_shift];
   };
   // which of them are there
   const auto there_of = [&](int tile, int pages) {

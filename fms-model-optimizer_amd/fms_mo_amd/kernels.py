@@ -1210,7 +1210,7 @@ def _paged_out(out, q):
         return torch.empty(q.shape, dtype=q.dtype, device=q.device), True
     if out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError(f"out must be {q.dtype} {tuple(q.shape)}")
-    if out.stride(2) != 1 or out.data_ptr() % 16 or any(s % 8 or (s == 0 and n > 1) for s, n in zip(_strides(out, 2), out.shape)):
+    if out.stride(2) != 1 or (not _COMPILING() and out.data_ptr() % 16) or any(s % 8 or (s == 0 and n > 1) for s, n in zip(_strides(out, 2), out.shape)):
         raise ValueError("the heads of out must be contiguous, 16-byte aligned and apart")
     return out, False
 
@@ -1336,7 +1336,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, query_start=None
     ``qk_norm_rope_store`` for the cache and the batch): every token sees the keys up to its own, with ``window`` > 0 only the last
     ``window`` of them and the first ``sinks``.  ``scale`` defaults to dim ** -0.5.  ``max_query_len`` / ``max_seq_len``: the longest
     sequence's new tokens and keys, where the host knows them; the work is laid out for them (any length is right).  Returns
-    [T, heads, dim] in ``out`` or a new tensor; tokens that see nothing, and in a new tensor rows of no sequence, are zero.
+    [T, heads, dim] in ``out`` (which may be q) or a new tensor; tokens that see nothing, and in a new tensor rows of no sequence, are zero.
     No gradients.  See fmsmo_paged_attn."""
     if not _COMPILING():
         r = (_H or _host()).paged_attention(q, k_cache, v_cache, block_table, seq_lens, query_start, scale, window or 0, sinks or 0, k_scale,

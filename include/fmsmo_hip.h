@@ -892,13 +892,13 @@ int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch,
  * out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j over the keys j that a row at position p sees:
  *   j <= p,  and with a window > 0 also j > p - window or j < sinks.
  * q heads h * g .. share key head h (g = q_heads / heads).  A row that sees nothing is zero; what a row doesn't see has no
- * influence on it, whatever it holds.  Sums are fp32; the probabilities are rounded to dtype before they meet the values
+ * influence on it, whatever it holds.  out may be q.  Sums are fp32; the probabilities are rounded to dtype before they meet the values
  * (e4m3 caches: times the values' scales, to bf16, for dtype fp16 to the sum of two bf16 numbers).  Rows of no
  * sequence: zero with zero_rest, else left as they are.
  * max_rows, max_keys: upper bounds of a sequence's rows and keys that the host knows (0: none); they choose the kernel and how
  * the work is split, and a sequence that exceeds them is still computed in full.
  * workspace: fmsmo_paged_attn_workspace_bytes(q_heads, heads, dim, dtype of the cache, seqs, rows, max_rows, max_keys) bytes, 16-byte aligned, private to the
- * call until it has finished; max_rows and max_keys as given there, at least 1 and at most rows and table_width * page_size.
+ * call until it has finished; max_rows and max_keys as given there, at least 1 (max_rows 1 without query_start) and at most rows and table_width * page_size.
  */
 int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, int dtype, int64_t rows, int q_heads,
                      const void* q, int64_t q_row, int64_t q_head, void* out, int64_t o_row, int64_t o_head, float scale,

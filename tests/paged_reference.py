@@ -69,7 +69,7 @@ def attention(q, kc, vc, table, lens, start=None, scale=None, window=0, sinks=0,
             w = torch.softmax(s, 0)
             out[r, h] = w @ v
             # scores: D products and sums in fp32, and the scale's and the exponent's own roundings; twice (numerator, denominator)
-            ds = float((scale * (k.abs() @ x.abs())).max()) * (D + 8) * 2.0 ** -24 + 2.0 ** -20
+            ds = float((abs(scale) * (k.abs() @ x.abs())).max()) * (D + 8) * 2.0 ** -24 + 2.0 ** -20
             mean = w @ v.abs()
             more = int(seen.sum()) * 2.0 ** -25 * float(v.abs().max()) if q.dtype == torch.float16 and ks is None else 0.0  # fp16 below its normals
             bound[r, h] = u * out[r, h].abs() + (up + 2 * ds + (int(seen.sum()) + 64) * 2.0 ** -23) * (1 + u) * mean + more + 2.0 ** -24

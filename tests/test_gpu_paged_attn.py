@@ -175,6 +175,82 @@ def test_what_is_not_seen_may_hold_anything(dev, dt, e4m3, new, bad, window):
         assert not torch.isfinite(y[new - 1].float()).any()  # its own key is not a number
 
 
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("heads,kv,D", [(4, 2, 128), (6, 2, 64), (4, 1, 256)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 5)])
+def test_few_rows_behind_many_keys(dev, dt, e4m3, heads, kv, D, window, sinks):
+    """Tiles of rows that several blocks share."""
+    compare(dev, dt, e4m3, heads, kv, D, 32, [2500, 40, 900, 0], [40, 3, 33, 0], window=window, sinks=sinks, seed=D, spare_rows=2)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+def test_many_sequences(dev, dt, e4m3):
+    g = gen(9)
+    lens = [int(x) for x in torch.randint(0, 90, (150,), generator=g)]
+    for most in (1, 3, 40):
+        new = [min(n, int(x)) for n, x in zip(lens, torch.randint(0, most + 1, (150,), generator=g))]
+        compare(dev, dt, e4m3, 4, 2, 64, 16, lens, new, seed=most)
+    compare(dev, dt, e4m3, 4, 2, 64, 16, lens, None, window=20, sinks=1)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 70])
+@pytest.mark.parametrize("scale", [0.0, -0.25, 1.5])
+def test_other_scales(dev, dt, e4m3, new, scale):
+    g = gen(12)
+    lens, start = [300, 77], None if new == 1 else [0, new, 2 * new]
+    table, pages = R.make_pages(g, lens, 16)
+    k, v, ks, vs = R.make_cache(g, pages, 2, 16, 64, dt, e4m3)
+    q = torch.randn(2 * new, 4, 64, generator=g).to(dt)
+    ref, bound = R.attention(q, k, v, table, lens, start, scale, 0, 0, ks, vs)
+    qd, kd, vd, td, ksd, vsd = on(dev, q, k, v, table, ks, vs)
+    args = (kd, vd, td, i32(lens, dev), None if start is None else i32(start, dev))
+    y = K().paged_attention(qd, *args, scale=scale, k_scale=ksd, v_scale=vsd, max_query_len=new)
+    assert R.worst(y, ref, bound) <= 1.0
+    K().paged_attention(qd, *args, scale=scale, k_scale=ksd, v_scale=vsd, max_query_len=new, out=qd)  # in place
+    assert torch.equal(qd, y)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_through_the_registered_operators_and_a_compiler(dev, new):
+    g = gen(13)
+    lens, start = [200, 77], None if new == 1 else i32([0, new, 2 * new], dev)
+    table, pages = R.make_pages(g, lens, 16)
+    k, v, ks, vs = R.make_cache(g, pages, 2, 16, 64, torch.bfloat16, True)
+    kd, vd, td, ksd, vsd = on(dev, k, v, table, ks, vs)
+    x = torch.randn(2 * new, 8, 64, generator=g).bfloat16().to(dev)
+    ld = i32(lens, dev)
+
+    def step(x, kd, vd, ksd, vsd):
+        q = K().qk_norm_rope_store(x[:, :4], x[:, 4:6], x[:, 6:], kd, vd, td, ld, start, k_scale=ksd, v_scale=vsd)
+        return K().paged_attention(q, kd, vd, td, ld, start, k_scale=ksd, v_scale=vsd, max_query_len=new) * 2
+    a, b = [[t.clone() for t in (kd, vd, ksd, vsd)] for _ in range(2)]
+    want = step(x, *a)
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(x, *b)
+    assert torch.equal(got, want)
+    for s, t in zip(a, b):
+        assert torch.equal(s.view(torch.uint8), t.view(torch.uint8))
+
+
+def test_nonsense_in_the_batch_stays_inside_of_the_tensors(dev):
+    """Rows and lengths that the operands don't have, and descending starts: rows that are given are computed from what is there, nothing
+    outside of the tensors is touched."""
+    g = gen(14)
+    table, pages = R.make_pages(g, [64, 64], 16)
+    k, v, _, _ = R.make_cache(g, pages, 2, 16, 64, torch.float16, False)
+    kd, vd, td = on(dev, k, v, table)
+    q = torch.randn(40, 4, 64, generator=g).half().to(dev)
+    room = torch.full((44, 4, 64), 3.0, dtype=torch.float16, device=dev)
+    big = 2 ** 31 - 1
+    for lens, start in (([big, -5], [0, 20, 40]), ([64, 64], [0, big, big]), ([64, 64], [30, 10, 40]), ([big, big], [-9, 5, -1]), ([64, 0], [60, 70, 80])):
+        for hint in (1, 8, 40):
+            for w in (0, 5, big):
+                y = K().paged_attention(q, kd, vd, td, i32(lens, dev), i32(start, dev), max_query_len=hint, out=room[2:42], window=w, sinks=2)
+                K().qk_norm_rope_store(q, q[:, :2], q[:, 2:], kd.clone(), vd.clone(), td, i32(lens, dev), i32(start, dev))
+                torch.cuda.synchronize()
+    assert (room[:2] == 3).all() and (room[42:] == 3).all() and y.shape == q.shape
+
+
 def test_large_scores_and_scales(dev):
     """Scores far apart (one key takes all) and e4m3 scales over the whole range of fp32's normals that a product leaves finite."""
     g = gen(1)
