@@ -18,7 +18,7 @@ namespace fmsmo {
 constexpr int BM = PROMPT_ROWS, BN = PROMPT_KEYS;
 
 template <int QT, bool E4M3, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(SplitArgs sa) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_prompt_kernel(SplitArgs sa) {
   const PagedArgs& a = sa.p;
   // e4m3 caches: the values' scales are multiplied in before the probabilities are rounded, which takes the exponents of bf16; for
   // an fp16 result, of which bf16 would lose three bits, they are the sum of two bf16 numbers
@@ -245,17 +245,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Spl
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
-    // register 4 i + j of st[kt]: key kt * 32 + 8 i + 4 hl + j
-    if constexpr (E4M3) {
+    // register 4 i + j of st[kt]: key kt * 32 + 8 i + 4 hl + j.  From here on as the exponents that the present maximum leaves.
+    const float ms = safe_max(m);
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4f ks = *(const v4f*)&sc[buf][0][kt * 32 + 8 * i + 4 * hl];
+      for (int i = 0; i < 4; ++i) {
+        v4f by = {c, c, c, c};
+        if constexpr (E4M3) by = *(const v4f*)&sc[buf][0][kt * 32 + 8 * i + 4 * hl];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) st[kt][4 * i + j] *= ks[j];
-        }
-    }
+        for (int j = 0; j < 4; ++j) st[kt][4 * i + j] = __fmaf_rn(st[kt][4 * i + j], by[j], -ms);
+      }
     if (!whole) {
       // (one test at a time, and only those that the tile needs)
       const Bounds bd = bounds_of(a, pos, pos, s.len, k0 + 4 * hl);
@@ -270,23 +270,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Spl
       if (there_now != 15) keep([&](int at) { return (there_now >> (at >> 4) & 1) != 0; });
       if (!mine) keep([&](int) { return false; });
     }
-    const float by = E4M3 ? 1.0f : c;
     float top = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, st[0][i]), st[1][i]);
-    top = max_x32(top) * by;
+    top = max_x32(top);
     // The maximum is held back: powers up to 2^8 are as good as powers up to 1, and O is rescaled a few times at all.  (e4m3 keeps too
     // much in registers for a branch around O, which copies it: 2900 us with, 2833 without for 2 x 2048 tokens behind 30000 keys; 16-bit
     // caches 560 with, 600 without for 8192 tokens)
-    const bool grow = top > m + 8.0f || (m == -__builtin_inff() && top > m);
-    if (E4M3 || __any(grow)) {
-      const float m_new = grow ? fmaxf(m, top) : m, f = grow ? exp2_hw(m - safe_max(m_new)) : 1.0f;
+    const bool grow = top > 8.0f || (m == -__builtin_inff() && top > m);
+    const bool any = __any(grow);
+    const float step = grow ? top : 0.0f;
+    if (any) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        st[0][i] -= step;
+        st[1][i] -= step;
+      }
+    }
+    if (E4M3 || any) {
+      const float m_new = grow ? ms + top : m, f = grow ? exp2_hw(m - m_new) : 1.0f;
 #pragma unroll
       for (int d = 0; d < NV; ++d) o[d] *= f;
       l *= f;
       m = m_new;
     }
-    const float ms = safe_max(m);
     v4i pb[4], pl[4];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -295,8 +302,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Spl
         float pr[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float y = st[kt][4 * i + j];
-          pr[j] = exp2_hw(E4M3 ? y - ms : __fmaf_rn(y, by, -ms));
+          pr[j] = exp2_hw(st[kt][4 * i + j]);
           l += pr[j];
         }
         if constexpr (E4M3) {
