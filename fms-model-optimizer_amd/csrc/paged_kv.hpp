@@ -11,6 +11,7 @@ namespace fmsmo {
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 
 constexpr int PROMPT_ROWS = 128, PROMPT_KEYS = 64;  // tiles of the prompt kernel
 

@@ -9,9 +9,10 @@
 // Each wave brings 16 of a tile's keys, one page, straight from memory into the other of two buffers while the present one is used;
 // e4m3 codes become 16-bit numbers there, once per block.
 //
-// What bounds it: the matrix instructions and the softmax of two blocks share a compute unit, 46 % of the first's cycles in use at the
+// What bounds it: the matrix instructions and the softmax of two blocks share a compute unit, 51 % of the first's cycles in use at the
 // 1.8 GHz that the power limit leaves; one prompt of 8192 tokens, 32 + 8 heads of 128, bf16: 560 us, 980 TFLOP/s, where a large library
-// product reaches 1409.  Tried and slower there: the scores of the next tile beside the softmax of this one (649 us; a third of the
+// product reaches 1409.  e4m3 has 290 vector instructions for a tile and wave instead of 210, codes widened and scales multiplied in:
+// 2 x 2048 tokens behind 30000 keys 2440 us, 850 TFLOP/s.  Tried and slower, one prompt: the scores of the next tile beside the softmax of this one (649 us; a third of the
 // registers more and no better order), the values' reads ahead of their products (621), s_setprio around the products (571),
 // sums of the probabilities by dot products (587).
 #include "paged_kv.hpp"
@@ -24,7 +25,7 @@ namespace fmsmo {
 constexpr int BM = PROMPT_ROWS, BN = PROMPT_KEYS;
 
 template <int QT, bool E4M3, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_prompt_kernel(SplitArgs sa) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) void paged_prompt_kernel(SplitArgs sa) {
   const PagedArgs& a = sa.p;
   // e4m3 caches: the values' scales are multiplied in before the probabilities are rounded, which takes the exponents of bf16; for
   // an fp16 result, of which bf16 would lose three bits, they are the sum of two bf16 numbers
@@ -35,7 +36,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
   // (16 bytes of 32 rows per instruction) nor the values (64 bytes of 8 rows) ask a bank for two things at once.
   constexpr int ROW = 2 * D, WRAP = ROW < 256 ? 256 / ROW : 1;  // bytes of a row; rows in a turn of the banks
   const auto key_place = [](int r) { return r / WRAP % (D == 64 ? 8 : 16); };
-  const auto value_place = [](int r) { return r / WRAP % (D == 64 ? 4 : 8) * 2; };
+  // (by turns of the bits: any four rows that follow each other, and any eight of which 32 bytes are read, lie apart)
+  const auto value_place = [](int r) { return ((r & 1) << 3 | (r & 2) << 1 | (r & 4) >> 1) & (D == 64 ? 7 : 15); };
   constexpr int LOADS = 16 * ROW / 1024;              // of 1 KiB for 16 rows of 16-bit numbers
   constexpr int CODES = 16 * D / 1024;                // of e4m3
   __shared__ __attribute__((aligned(1024))) char kl[2][BN * ROW];
@@ -124,12 +126,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
     const int l16 = lane & 15, r = 4 * hl + l16 / 4;  // (8 rows further the place is the same)
     v_base = r * ROW + (((lane >> 4 & 1) * 2 + l16 % 4 / 2) ^ value_place(r)) * 16 + l16 % 2 * 8;
   }
-  constexpr int RPC = 1024 / D;  // rows of a load of codes
+  constexpr int RPC = 512 / D, WIDEN = 16 / RPC;  // rows that are widened at once, 8 codes a lane; turns for 16
   int kw_base, vw_base;
   {
-    const int r = lane / (D / 16), at = lane % (D / 16);
-    kw_base = (16 * wave + r) * ROW + (2 * at ^ key_place(r)) * 16;
-    vw_base = (16 * wave + r) * ROW + (2 * at ^ value_place(r)) * 16;
+    const int r = lane / (D / 8), at = lane % (D / 8);
+    kw_base = (16 * wave + r) * ROW + (at ^ key_place(r)) * 16;
+    vw_base = (16 * wave + r) * ROW + (at ^ value_place(r)) * 16;
   }
 
   // This wave's 16 keys of a tile, straight from memory, 1 KiB an instruction.  16 bits: lane i brings the 16-byte piece that belongs
@@ -157,12 +159,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
     }
     if constexpr (E4M3) {
       const float* src = (lane & 16) ? a.vs + page * a.vs_page + hk * a.vs_head : a.ks + page * a.ks_page + hk * a.ks_head;
-      sr = src[slot + (lane & 15)] * ((lane & 16) ? 1.0f : c);
+      sr = src[slot + (lane & 15)];  // (looked at when the codes are, an iteration later)
+    }
+  };
+  // (256 elements, whose block has its compute unit to itself, read them before the second product and widen them behind it: 608 us
+  // for one prompt of 6000 tokens with 16 + 4 heads, else 643; 128, with 19 registers more for it, 2500 us instead of 2440 as below)
+  constexpr bool EARLY = E4M3 && D == 256;
+  v2i ku[E4M3 ? WIDEN : 1], vu[E4M3 ? WIDEN : 1];
+  const auto codes = [&](int buf) __attribute__((always_inline)) {
+    if constexpr (E4M3) {
+#pragma unroll
+      for (int j = 0; j < WIDEN; ++j) {
+        ku[j] = *(const v2i*)(kl[buf] + 16 * wave * ROW + RAW + j * 512 + lane * 8);
+        vu[j] = *(const v2i*)(vl[buf] + 16 * wave * ROW + RAW + j * 512 + lane * 8);
+      }
     }
   };
   // What a tile that has arrived still needs.  Codes become 16-bit numbers.  In a tile that is not seen as a whole, values that nobody
   // may see become zero, and so do infinities and NaN (see finite_only).
-  const auto settle = [&](int tile, int buf, int there, bool part) {
+  const auto settle_as = [&](int tile, int buf, int there, auto part_of) __attribute__((always_inline)) {
+    const bool part = part_of;
     bool fine = true;
     const int k0 = key_of(tile) + 16 * wave;
     const auto clean = [&](uint32_t u, int r) {
@@ -172,32 +188,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
       return v;
     };
     if constexpr (E4M3) {
-      v4i ku[CODES], vu[CODES];
-#pragma unroll
-      for (int j = 0; j < CODES; ++j) {
-        ku[j] = *(const v4i*)(kl[buf] + 16 * wave * ROW + RAW + j * 1024 + lane * 16);
-        vu[j] = *(const v4i*)(vl[buf] + 16 * wave * ROW + RAW + j * 1024 + lane * 16);
-      }
+      if constexpr (!EARLY) codes(buf);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (all of them are read before the first is written over)
       // (rows j RPC + r with r < RPC, a power of two: their places are those of r with the bits of j RPC turned over)
 #pragma unroll
-      for (int j = 0; j < CODES; ++j)
+      for (int j = 0; j < WIDEN; ++j) {
+        uint32_t y[4], z[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t y[4], z[4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            widen4<QT>((uint32_t)ku[j][2 * h + i], y[2 * i], y[2 * i + 1]);
-            widen4<PT>((uint32_t)vu[j][2 * h + i], z[2 * i], z[2 * i + 1]);
-          }
-          if (part) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = clean(z[i], j * RPC + lane / (D / 16));
-          }
-          __builtin_memcpy(kl[buf] + j * RPC * ROW + (kw_base ^ (h ^ key_place(j * RPC)) * 16), y, 16);
-          __builtin_memcpy(vl[buf] + j * RPC * ROW + (vw_base ^ (h ^ value_place(j * RPC)) * 16), z, 16);
+        for (int i = 0; i < 2; ++i) {
+          widen4<QT>((uint32_t)ku[j][i], y[2 * i], y[2 * i + 1]);
+          widen4<PT>((uint32_t)vu[j][i], z[2 * i], z[2 * i + 1]);
         }
-      if (lane < 32) sc[buf][lane >> 4][16 * wave + (lane & 15)] = sr;
+        if (part) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z[i] = clean(z[i], j * RPC + lane / (D / 8));
+        }
+        __builtin_memcpy(kl[buf] + j * RPC * ROW + (kw_base ^ key_place(j * RPC) * 16), y, 16);
+        __builtin_memcpy(vl[buf] + j * RPC * ROW + (vw_base ^ value_place(j * RPC) * 16), z, 16);
+      }
+      if (lane < 32) sc[buf][lane >> 4][16 * wave + (lane & 15)] = (lane & 16) ? sr : sr * c;
     } else if (part) {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
@@ -209,6 +218,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
       }
     }
     if (part && __any(!fine) && lane == 0) odd = 1;
+  };
+  // (e4m3: both forms of this and of `powers` are written out, since a test inside waits for each read from shared memory by itself:
+  // 2 x 2048 tokens behind 30000 keys 2440 us, else 2650)
+  const auto settle = [&](int tile, int buf, int there, bool part) __attribute__((always_inline)) {
+    if (!E4M3) settle_as(tile, buf, there, part);
+    else if (part) settle_as(tile, buf, there, std::true_type{});
+    else settle_as(tile, buf, there, std::false_type{});
   };
 
   if (threadIdx.x == 0) odd = 0;
@@ -222,6 +238,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
     const int buf = tile & 1, k0 = key_of(tile);
     const bool part = partial(tile, there);
     if (!E4M3 || tile == begin) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (EARLY && tile == begin) codes(buf);
     if (E4M3 ? tile == begin : part) settle(tile, buf, there, part);
     // this tile is here, and nobody reads the one before it any more
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -280,9 +297,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, st[0][i]), st[1][i]);
     top = max_x32(top);
-    // The maximum is held back: powers up to 2^8 are as good as powers up to 1, and O is rescaled a few times at all.  (e4m3 keeps too
-    // much in registers for a branch around O, which copies it: 2900 us with, 2833 without for 2 x 2048 tokens behind 30000 keys; 16-bit
-    // caches 560 with, 600 without for 8192 tokens)
+    // The maximum is held back: powers up to 2^8 are as good as powers up to 1, and O is rescaled a few times at all (8192 tokens 560 us,
+    // 600 with O rescaled for every tile; e4m3, 2 x 2048 tokens behind 30000 keys, 2707 and 2795)
     const bool grow = top > 8.0f || (m == -__builtin_inff() && top > m);
     const bool any = __any(grow);
     const float step = grow ? top : 0.0f;
@@ -293,7 +309,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
         st[1][i] -= step;
       }
     }
-    if (E4M3 || any) {
+    if (any) {
       const float m_new = grow ? ms + top : m, f = grow ? exp2_hw(m - m_new) : 1.0f;
 #pragma unroll
       for (int d = 0; d < NV; ++d) o[d] *= f;
@@ -301,34 +317,34 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
       m = m_new;
     }
     v4i pb[4], pl[4];
+    const auto powers = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float pr[4];
+        for (int i = 0; i < 4; ++i) {
+          float pr[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          pr[j] = exp2_hw(st[kt][4 * i + j]);
-          l += pr[j];
-        }
-        if constexpr (E4M3) {
-          const v4f vs = *(const v4f*)&sc[buf][1][kt * 32 + 8 * i + 4 * hl];
-          // (a key that the row does not see counts nothing, whatever its scale holds)
+          for (int j = 0; j < 4; ++j) {
+            pr[j] = exp2_hw(st[kt][4 * i + j]);
+            l += pr[j];
+          }
+          if constexpr (E4M3) {
+            const v4f vs = *(const v4f*)&sc[buf][1][kt * 32 + 8 * i + 4 * hl];
+            // (a key that the row does not see counts nothing, whatever its scale holds)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) pr[j] *= vs[j];
-          if (!whole) {
+            for (int j = 0; j < 4; ++j) pr[j] = !masked || st[kt][4 * i + j] != -__builtin_inff() ? pr[j] * vs[j] : 0.0f;
+          }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) pr[j] = st[kt][4 * i + j] != -__builtin_inff() ? pr[j] : 0.0f;
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t hi = pack2<PT>(pr[2 * j], pr[2 * j + 1]);
+            pb[kt * 2 + i / 2][i % 2 * 2 + j] = (int)hi;
+            if constexpr (TWO)
+              pl[kt * 2 + i / 2][i % 2 * 2 + j] = (int)pack2<PT>(pr[2 * j] - __uint_as_float(hi << 16), pr[2 * j + 1] - __uint_as_float(hi & 0xffff0000u));
           }
         }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t hi = pack2<PT>(pr[2 * j], pr[2 * j + 1]);
-          pb[kt * 2 + i / 2][i % 2 * 2 + j] = (int)hi;
-          if constexpr (TWO)
-            pl[kt * 2 + i / 2][i % 2 * 2 + j] = (int)pack2<PT>(pr[2 * j] - __uint_as_float(hi << 16), pr[2 * j + 1] - __uint_as_float(hi & 0xffff0000u));
-        }
-      }
+    };
+    if (E4M3 && !whole) powers(std::true_type{});
+    else powers(std::false_type{});
     // O^T: step k of the reduction has keys 16 k + 4 hl + (0..3) and those + 8, as the scores lie
     const auto values = [&](int d, int k) {
       const char* at = vl[buf] + (v_base ^ d * 64) + 16 * k * ROW;
@@ -339,6 +355,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
       __builtin_memcpy((char*)&f + 8, &w, 8);
       return f;
     };
+    if (EARLY && more) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      codes(buf ^ 1);
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -348,7 +368,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_pro
         if constexpr (TWO) o[d] = mfma32<PT>(f, pl[k], o[d]);
       }
     if (E4M3 && more) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (!EARLY) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       settle(tile + 1, buf ^ 1, there, partial(tile + 1, there));
     }
   }
