@@ -80,7 +80,9 @@ __device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
 // page are the same for the whole block, and a row's sums stay inside a wave.  The other half of a pair is loaded again (it is
 // in the cache lines that the row's lanes just fetched) instead of being passed between lanes.  Bound by the latency of a token's
 // chain of loads (sequence, length, page, row), so where tokens are many a block goes through all of its heads, the next group's rows on
-// their way meanwhile: 4 uneven prompts of up to 4095 tokens, 32 + 8 + 8 heads of 128, e4m3: 105 us with a block per group of heads.
+// their way meanwhile: 4 uneven prompts of up to 4095 tokens, 32 + 8 + 8 heads of 128, e4m3: 79 us (262 MB in and out, 3.3 TB/s; a
+// large copy reaches 4.9), 105 with a block per group of heads.  It pays from about 768 tokens on: 512 tokens 6.9 us so and 6.6 with a
+// block per group, 1024 tokens 9.7 and 11.1.  A few tokens are the launch: 3 us on the device for one.
 template <int T, bool E4M3, int D, int WT, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a, int per) {
   constexpr int LG = D / 8, ROWS = 256 / LG;
@@ -239,7 +241,7 @@ int fmsmo_paged_args(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batc
 
 template <int T, bool E4M3, int D, int WT>
 static void run_store(const StoreArgs& a, bool interleaved, int64_t rows, hipStream_t s) {
-  // groups of 2048 elements; a block takes all of them where there are blocks enough without
+  // groups of 2048 elements; a block takes all of them where there are blocks enough without (figures at the kernel)
   const int groups = div_up(a.heads + 2 * a.p.kv_heads, 2048 / D), per = rows >= 768 ? (groups < 8 ? groups : 8) : 1;
   const dim3 grid((unsigned)rows, (unsigned)div_up(groups, per));
   if (interleaved) hipLaunchKernelGGL((kv_store_kernel<T, E4M3, D, WT, true>), grid, dim3(256), 0, s, a, per);

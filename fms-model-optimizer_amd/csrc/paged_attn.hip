@@ -6,12 +6,15 @@
 //
 // What bounds it is reading the cache once.  Up to 16 rows (tokens x the query heads that share a key head) are the columns of
 // one matrix instruction, so the arithmetic is 1 / 10 of what the units could do in that time; the kernel is made of loads
-// in flight: every wave owns tiles of 32 keys, from memory straight into the operands' registers -- no shared memory, no barrier --
-// and asks for the keys of its next tile before the softmax of the present one, for its values after them.
+// in flight: every wave owns tiles of 32 keys, from memory straight into the operands' registers -- no shared memory and no barrier
+// before the waves' shares are joined -- and asks for the keys of its next tile before the softmax of the present one, for its values after them.
 //   S^T = K Q^T   16 x 16 x 32: lane l has key l % 16, and 16 bytes of it; the scores of row l % 16 for keys 4 (l / 16) .. + 3
 //   O^T = V^T P^T the same instruction over 32 keys: the scores are the second operand as they stand (the reduction's order is
 //                 free: element 4 t + i of lane group g is key 16 t + 4 g + i), and lane c reads elements ND c .. of those eight keys,
 //                 from which v_perm makes columns ND c + n of V^T for the ND instructions n.
+//
+// 64 sequences of up to 8000 keys, 32 + 8 heads of 128, bf16: 180 us, 6.1 TB/s, where a launch that only reads reaches 6.9.  Tried without
+// gain: tiles asked for two ahead, three waves per SIMD, eight waves a block, more blocks.
 //
 // Work: all tiles of all sequences and heads in a row, cut into `workers` equal parts on the device from seq_lens, so a batch of
 // uneven lengths keeps every block busy for the same time and nothing about the lengths has to be known on the host.
@@ -465,8 +468,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
 }
 
 // Joins the shares of the pairs that were cut: a block per cut and row, rows side by side, since neighbouring blocks go to different parts
-// of the chip and cuts may come in steps of eight (with the cuts side by side 32 pairs of 32 rows in 16 shares took 23 us, not 8).  The weights of all shares first (a share per thread), then
-// every group of D / 4 threads adds up every (1024 / D)-th share: loads that wait for nothing but the weights.
+// of the chip and cuts may come in steps of eight (with the cuts side by side 32 pairs of 32 rows in 16 shares took 23 us, not 8).  The
+// weights of all shares first (a share per thread), then every group of D / 4 threads adds up every (1024 / D)-th share: loads that wait
+// for nothing but the weights.  Bound by those two dependent rounds of loads: 4 us for single tokens, 7 for 512 shares a row.
 template <int QT, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
   constexpr int LG = D / 4, GROUPS = 256 / LG;
@@ -545,8 +549,8 @@ int fmsmo_paged_args(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batc
   if (cache->dim != 64 && cache->dim != 128 && cache->dim != 256) return FMSMO_ERR_UNSUPPORTED;
   const int size = cache->page_size;
   if (size < 16 || size > 65536 || (size & (size - 1))) return FMSMO_ERR_UNSUPPORTED;
-  if (rows < 0 || rows > 0x7fffffff || batch->seqs < 0 || cache->pages < 1 || cache->heads < 1 || q_heads < 1 || q_heads % cache->heads || batch->table_width < 1 ||
-      batch->table_stride < 0 || q_row < 0 || q_head < 0 || o_row < 0 || o_head < 0)
+  if (rows < 0 || rows > 0x7fffffff || batch->seqs < 0 || cache->pages < 1 || cache->heads < 1 || q_heads < 1 || q_heads % cache->heads ||
+      batch->table_width < 1 || batch->table_stride < 0 || q_row < 0 || q_head < 0 || o_row < 0 || o_head < 0)
     return FMSMO_ERR_SHAPE;
   if (!batch->query_start && rows != batch->seqs) return FMSMO_ERR_SHAPE;
   if (rows * q_heads > 0x7fffffff / 2 || batch->seqs > (1 << 20) || cache->pages > 0x7fffffff || q_heads > 4096 ||
@@ -619,7 +623,8 @@ static Plan plan_of(int group, int kv_heads, int dim, bool e4m3, int64_t seqs, i
   const int64_t most = max_rows * group, tokens = std::max<int64_t>(1, std::min(seqs, rows));
   // Up to 16 rows are one tile of the split kernel; up to 32 rows of an e4m3 cache, whose codes it widens on the way to the products,
   // two waves take the same keys.  5 tokens x 4 heads, 16 sequences of 16000 keys: 16 bits 229 us so and 221 by the prompt kernel,
-  // e4m3 157 and 260.
+  // e4m3 157 and 260.  (One wave taking both tiles of rows through its keys, codes widened once, has half as many waves to wait with: 8
+  // sequences of 4000 keys 29 us instead of 26, 32 of 16000 124 instead of 134.)
   p.prompt = most > (e4m3 ? 32 : 16);
   if (p.prompt) {
     p.row_shift = 3;

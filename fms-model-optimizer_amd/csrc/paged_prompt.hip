@@ -10,11 +10,11 @@
 // e4m3 codes become 16-bit numbers there, once per block.
 //
 // What bounds it: the matrix instructions and the softmax of two blocks share a compute unit, 51 % of the first's cycles in use at the
-// 1.8 GHz that the power limit leaves; one prompt of 8192 tokens, 32 + 8 heads of 128, bf16: 560 us, 980 TFLOP/s, where a large library
+// 1.8 GHz that the power limit leaves; one prompt of 8192 tokens, 32 + 8 heads of 128, bf16: 545 us, 1010 TFLOP/s, where a large library
 // product reaches 1409.  e4m3 has 290 vector instructions for a tile and wave instead of 210, codes widened and scales multiplied in:
-// 2 x 2048 tokens behind 30000 keys 2440 us, 850 TFLOP/s.  Tried and slower, one prompt: the scores of the next tile beside the softmax of this one (649 us; a third of the
-// registers more and no better order), the values' reads ahead of their products (621), s_setprio around the products (571),
-// sums of the probabilities by dot products (587).
+// 2 x 2048 tokens behind 30000 keys 2415 us, 860 TFLOP/s.  Tried and slower, the one prompt (560 us then): the scores of the next tile
+// beside the softmax of this one (649; a third of the registers more and no better order), the values' reads ahead of their products
+// (621), s_setprio around the products (571), sums of the probabilities by dot products (587).
 #include "paged_kv.hpp"
 
 #include <algorithm>
@@ -339,7 +339,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
             const uint32_t hi = pack2<PT>(pr[2 * j], pr[2 * j + 1]);
             pb[kt * 2 + i / 2][i % 2 * 2 + j] = (int)hi;
             if constexpr (TWO)
-              pl[kt * 2 + i / 2][i % 2 * 2 + j] = (int)pack2<PT>(pr[2 * j] - __uint_as_float(hi << 16), pr[2 * j + 1] - __uint_as_float(hi & 0xffff0000u));
+              pl[kt * 2 + i / 2][i % 2 * 2 + j] =
+                  (int)pack2<PT>(pr[2 * j] - __uint_as_float(hi << 16), pr[2 * j + 1] - __uint_as_float(hi & 0xffff0000u));
           }
         }
     };
