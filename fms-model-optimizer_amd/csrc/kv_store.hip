@@ -5,7 +5,7 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin)   (the first `rotary` elements, in pairs (i, i + rotary / 2) or (2i, 2i + 1))
 //   16 bit: rounded once.   e4m3: s = max(max|y| / 448, 1e-12), code = e4m3(clamp(y / s, +-448)) of the fp32 y.
 //
-// Everything is fp32 between the load and the one rounding.  The scale and the quotient are IEEE divisions: the recipe of
+// Everything is fp32 between the load and the one rounding.  The scale and the quotient are those of IEEE divisions: the recipe of
 // the linears' dynamic per-token quantizer.
 #include "paged_kv.hpp"
 
@@ -80,9 +80,11 @@ __device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
 // page are the same for the whole block, and a row's sums stay inside a wave.  The other half of a pair is loaded again (it is
 // in the cache lines that the row's lanes just fetched) instead of being passed between lanes.  Bound by the latency of a token's
 // chain of loads (sequence, length, page, row), so where tokens are many a block goes through all of its heads, the next group's rows on
-// their way meanwhile: 4 uneven prompts of up to 4095 tokens, 32 + 8 + 8 heads of 128, e4m3: 79 us (262 MB in and out, 3.3 TB/s; a
-// large copy reaches 4.9), 105 with a block per group of heads.  It pays from about 768 tokens on: 512 tokens 6.9 us so and 6.6 with a
-// block per group, 1024 tokens 9.7 and 11.1.  A few tokens are the launch: 3 us on the device for one.
+// their way meanwhile: 4 uneven prompts of up to 4095 tokens, 32 + 8 + 8 heads of 128, e4m3: 79 us, 105 with a block per group of heads.
+// It pays from about 768 tokens on: 512 tokens 6.9 us so and 6.6 with a block per group, 1024 tokens 9.7 and 11.1.  With the quotients and
+// the norm below (IEEE divisions before) the prompts take 75 us: 262 MB in and out, 3.5 TB/s, a large copy reaches 4.9.  A few tokens are
+// the launch: 3 us on the device for one.  Tried without gain: the first rows asked for before the sequence is looked up (79), weights and
+// angles multiplied once for all heads of a kind and places counted on from head to head (104: more registers, longer before the first row).
 template <int T, bool E4M3, int D, int WT, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a, int per) {
   constexpr int LG = D / 8, ROWS = 256 / LG;
@@ -153,18 +155,19 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a, int per) {
     if (!INTERLEAVED) widen8<T>(far_half, y);
     // (before any of this row's is written: q_out may be q)
     if (i + 1 < per) fetch(h + ROWS);
+    float r = 1.0f;  // (multiplied in at the end, once for a pair)
     if (w) {
       float ss = 0.0f, g[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) ss = __fmaf_rn(x[k], x[k], ss);
-      const float r = 1.0f / sqrtf(sum_lanes<LG>(ss) * (1.0f / D) + a.eps);
+      r = rsqrtf(sum_lanes<LG>(ss) * (1.0f / D) + a.eps);
       load_weight<WT>(w, c, g);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = x[k] * r * g[k];
+      for (int k = 0; k < 8; ++k) x[k] *= g[k];
       if (!INTERLEAVED && turn) {
         load_weight<WT>(w, other, g);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = y[k] * r * g[k];
+        for (int k = 0; k < 8; ++k) y[k] *= g[k];
       }
     }
     if (turn) {
@@ -177,12 +180,16 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a, int per) {
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = x[k] * cs[k] + y[k] * sn[k];
+        for (int k = 0; k < 8; ++k) x[k] = __fmaf_rn(x[k], cs[k], y[k] * sn[k]);
       }
       if (far) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = __builtin_nanf("");
       }
+    }
+    if (w) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= r;
     }
     if (kind == 0) {
       v4i o;
@@ -206,12 +213,17 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a, int per) {
     char* to = kind == 1 ? (char*)p.k + page * p.k_page + hh * p.k_head + slot * p.k_slot
                          : (char*)p.v + page * p.v_page + hh * p.v_head + slot * p.v_slot;
     if constexpr (E4M3) {
+      // x / scale as IEEE division has it: the reciprocal's product and two corrections, each with an exact remainder; zeros, infinities
+      // and NaN by the fixup.  No clamp: of a finite row no quotient leaves 448 by more than a rounding.
+      const float inverse = 1.0f / scale;
       int lo = 0, hi = 0;
       float q[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        q[k] = x[k] / scale;
-        q[k] = q[k] != q[k] ? q[k] : fminf(fmaxf(q[k], -448.0f), 448.0f);
+        q[k] = x[k] * inverse;
+        q[k] = __fmaf_rn(__fmaf_rn(-q[k], scale, x[k]), inverse, q[k]);
+        q[k] = __fmaf_rn(__fmaf_rn(-q[k], scale, x[k]), inverse, q[k]);
+        q[k] = __builtin_amdgcn_div_fixupf(q[k], scale, x[k]);
       }
       lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
       lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);

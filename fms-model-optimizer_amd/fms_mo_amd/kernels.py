@@ -1306,7 +1306,7 @@ def qk_norm_rope_store(q, k, v, k_cache, v_cache, block_table, seq_lens, query_s
     ``q_weight`` / ``k_weight``; None: no norm) and rotated by their positions (``cos`` / ``sin`` fp32 [positions, rotary dim / 2];
     None: no rotation), k and v [T, kv heads, dim] written to their places in the cache, as e4m3 codes with a scale per key
     (``k_scale`` / ``v_scale`` fp32 [pages, kv heads, page size]) where that is the cache's dtype.  Returns the rotated q: ``out``
-    (which may be q), or a new tensor, in which rows of no sequence are zero.
+    (q itself, or memory apart from q, k and v), or a new tensor, in which rows of no sequence are zero.
 
     k_cache, v_cache [pages, kv heads, page size, dim]; block_table int32 [B, pages], seq_lens int32 [B] with the new tokens,
     query_start int32 [B + 1] (None: one token per sequence).  See fmsmo_kv_store and fmsmo_kv_batch_t."""
@@ -1336,7 +1336,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, query_start=None
     ``qk_norm_rope_store`` for the cache and the batch): every token sees the keys up to its own, with ``window`` > 0 only the last
     ``window`` of them and the first ``sinks``.  ``scale`` defaults to dim ** -0.5.  ``max_query_len`` / ``max_seq_len``: the longest
     sequence's new tokens and keys, where the host knows them; the work is laid out for them (any length is right).  Returns
-    [T, heads, dim] in ``out`` (which may be q) or a new tensor; tokens that see nothing, and in a new tensor rows of no sequence, are zero.
+    [T, heads, dim] in ``out`` (q itself, or memory apart from it) or a new tensor; tokens that see nothing, and in a new tensor rows of no sequence, are zero.
     No gradients.  See fmsmo_paged_attn."""
     if not _COMPILING():
         r = (_H or _host()).paged_attention(q, k_cache, v_cache, block_table, seq_lens, query_start, scale, window or 0, sinks or 0, k_scale,

@@ -872,7 +872,7 @@ typedef struct {
 
 /*
  * New tokens: q [rows, q_heads, dim] and k [rows, cache heads, dim] are normalized per head, rotated by their position, q
- * written to q_out (which may be q), k and v to their places in the cache.  dtype (FMSMO_F16 or FMSMO_BF16) is that of q,
+ * written to q_out (q itself, or memory apart from q, k and v), k and v to their places in the cache.  dtype (FMSMO_F16 or FMSMO_BF16) is that of q,
  * k, v and q_out, and of a cache that is not e4m3; strides in elements, multiples of 8.
  *   y = x / sqrt(mean(x^2) + eps) * weight[dim]              (q_weight, k_weight: NULL for none; weight_dtype dtype or FMSMO_F32)
  *   (a, b) -> (a cos - b sin, b cos + a sin)   over the first `rotary` elements (0 or a multiple of 16), pairs (i, i + rotary / 2),
@@ -880,7 +880,8 @@ typedef struct {
  *   16-bit results are rounded once; e4m3: scale = max(max |y| / 448, 1e-12), code = e4m3(clamp(y / scale, -448, 448)) of
  *   the fp32 y, the recipe of fmsmo_quant_act_fp8_pertoken.
  * A position that the angle tables don't hold gives NaN; a row of q before position 0 is zero.  Rows of q_out
- * that belong to no sequence (behind the last one's) become zero with zero_rest, else they are left as they are.  A place in the cache that two rows of a call name holds one of them or a mixture.
+ * that belong to no sequence (behind the last one's) become zero with zero_rest, else they are left as they are.  A place in the
+ * cache that two rows of a call name holds one of them or a mixture.
  */
 int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, int dtype, int64_t rows, int q_heads,
                    const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
@@ -892,13 +893,14 @@ int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch,
  * out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j over the keys j that a row at position p sees:
  *   j <= p,  and with a window > 0 also j > p - window or j < sinks.
  * q heads h * g .. share key head h (g = q_heads / heads).  A row that sees nothing is zero; what a row doesn't see has no
- * influence on it, whatever it holds.  out may be q.  Sums are fp32; the probabilities are rounded to dtype before they meet the values
- * (e4m3 caches: times the values' scales, to bf16, for dtype fp16 to the sum of two bf16 numbers).  Rows of no
- * sequence: zero with zero_rest, else left as they are.
+ * influence on it, whatever it holds.  out is q or apart from it.  Sums are fp32; the probabilities are rounded to dtype before they meet the values
+ * (e4m3 caches: times the values' scales, to bf16, for dtype fp16 to the sum of two bf16 numbers; a few rows of a sequence:
+ * always to the sum of two where they are bf16).  Rows of no sequence: zero with zero_rest, else left as they are.
  * max_rows, max_keys: upper bounds of a sequence's rows and keys that the host knows (0: none); they choose the kernel and how
  * the work is split, and a sequence that exceeds them is still computed in full.
- * workspace: fmsmo_paged_attn_workspace_bytes(q_heads, heads, dim, dtype of the cache, seqs, rows, max_rows, max_keys) bytes, 16-byte aligned, private to the
- * call until it has finished; max_rows and max_keys as given there, at least 1 (max_rows 1 without query_start) and at most rows and table_width * page_size.
+ * workspace: fmsmo_paged_attn_workspace_bytes(q_heads, heads, dim, dtype of the cache, seqs, rows, max_rows, max_keys) bytes, 16-byte
+ * aligned, private to the call until it has finished; max_rows and max_keys as given there, at least 1 (max_rows 1 without
+ * query_start) and at most rows and table_width * page_size.
  */
 int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch, int dtype, int64_t rows, int q_heads,
                      const void* q, int64_t q_row, int64_t q_head, void* out, int64_t o_row, int64_t o_head, float scale,
