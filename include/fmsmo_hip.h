@@ -892,10 +892,11 @@ int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch,
 /*
  * out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j over the keys j that a row at position p sees:
  *   j <= p,  and with a window > 0 also j > p - window or j < sinks.
- * q heads h * g .. share key head h (g = q_heads / heads).  A row that sees nothing is zero; what a row doesn't see has no
- * influence on it, whatever it holds.  out is q or apart from it.  Sums are fp32; the probabilities are rounded to dtype before they meet the values
- * (e4m3 caches: times the values' scales, to bf16, for dtype fp16 to the sum of two bf16 numbers; a few rows of a sequence:
- * always to the sum of two where they are bf16).  Rows of no sequence: zero with zero_rest, else left as they are.
+ * q heads h * g .. share key head h (g = q_heads / heads).  A row that sees nothing, or nothing with a score above -inf, is zero;
+ * what a row doesn't see has no influence on it, whatever it holds.  out is q or apart from it.  Sums are fp32; the probabilities
+ * are rounded to dtype before they meet the values (e4m3 caches: times the values' scales, to bf16, for dtype fp16 to the sum
+ * of two bf16 numbers; a few rows of a sequence: always to the sum of two where they are bf16).  Rows of no sequence: zero with
+ * zero_rest, else left as they are.
  * max_rows, max_keys: upper bounds of a sequence's rows and keys that the host knows (0: none); they choose the kernel and how
  * the work is split, and a sequence that exceeds them is still computed in full.
  * workspace: fmsmo_paged_attn_workspace_bytes(q_heads, heads, dim, dtype of the cache, seqs, rows, max_rows, max_keys) bytes, 16-byte

@@ -190,3 +190,64 @@ def test_store_then_attend_as_a_model_does(dev):
         assert at == L and R.worst(y, ref, bound) <= 1.0
         want = torch.stack([R.turned(x[p, :heads], w[0], 1e-6, cos, sin, p, False)[0] for p in range(L)])
         assert ((q.double() - want).abs() <= R.eps_half(dt) * want.abs() * 1.01 + 2.0 ** -14).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_codes_are_those_of_a_division(dev, dt, D):
+    """Scale and codes bit for bit those of max / 448 and x / scale divided in fp32, over the types' whole range of scales (the values,
+    which neither norm nor rotation changes)."""
+    g = gen(D)
+    T, kv, size = 900, 2, 64
+    x = torch.randn(T, 3 * kv, D, generator=g)
+    top = 120 if dt == torch.bfloat16 else 12
+    x = (x * 2.0 ** torch.randint(-top, top, (T, 3 * kv, 1), generator=g)).to(dt)
+    x[::7] = x[::7].abs().clamp(max=1.0)
+    pages = -(-T // size)
+    k, v = (torch.zeros(pages, kv, size, D, dtype=torch.float8_e4m3fn, device=dev) for _ in range(2))
+    ks, vs = (torch.zeros(pages, kv, size, device=dev) for _ in range(2))
+    xd = x.to(dev)
+    K().qk_norm_rope_store(xd[:, :kv], xd[:, kv:2 * kv], xd[:, 2 * kv:], k, v, torch.arange(pages, dtype=torch.int32, device=dev)[None],
+                           torch.tensor([T], dtype=torch.int32, device=dev), torch.tensor([0, T], dtype=torch.int32, device=dev), k_scale=ks, v_scale=vs)
+    for part, codes, scales in ((x[:, kv:2 * kv], k, ks), (x[:, 2 * kv:], v, vs)):
+        f = part.float()
+        s = (f.abs().amax(-1) / 448).clamp(min=1e-12)
+        want = (f / s[..., None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+        have = codes.cpu().view(torch.uint8).transpose(1, 2).reshape(-1, kv, D)[:T]
+        assert torch.equal(scales.cpu().transpose(1, 2).reshape(-1, kv)[:T], s)
+        assert torch.equal(have, want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_a_captured_step_replays(dev, dtype):
+    """Store and attention of single tokens in one graph, replayed as the sequences grow, with eager steps on a second cache between."""
+    from fms_mo_amd.modules.attention import PagedKVCache
+
+    g = gen(5)
+    heads, kv, D, size, B = 8, 2, 128, 16, 3
+    caches = [PagedKVCache(40, size, kv, D, dtype, dev) for _ in range(2)]
+    table = torch.randperm(40, generator=g)[:36].reshape(B, 12).to(torch.int32).to(dev)
+    cos, sin = (t.to(dev) for t in tables(200, D // 2))
+    w = (1 + 0.1 * torch.randn(D, generator=g)).bfloat16().to(dev)
+    x = torch.zeros(B, heads + 2 * kv, D, dtype=torch.bfloat16, device=dev)
+    lens = torch.zeros(B, dtype=torch.int32, device=dev)
+
+    def step(cache):
+        q = cache.store(x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:], table, lens, cos=cos, sin=sin, q_weight=w, k_weight=w)
+        return cache.attend(q, table, lens, max_seq_len=192)
+    lens.copy_(torch.tensor([1, 15, 100], dtype=torch.int32))
+    for cache in caches:
+        step(cache)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step(caches[0])
+    for i in range(20):
+        lens += 1
+        x.copy_(torch.randn(x.shape, generator=g).bfloat16())
+        graph.replay()
+        want = step(caches[1])
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    for a, b in ((caches[0].k, caches[1].k), (caches[0].v, caches[1].v)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
