@@ -84,7 +84,8 @@ __device__ __forceinline__ uint32_t max_lanes(uint32_t v) {
 // It pays from about 768 tokens on: 512 tokens 6.9 us so and 6.6 with a block per group, 1024 tokens 9.7 and 11.1.  With the quotients and
 // the norm below (IEEE divisions before) the prompts take 75 us: 262 MB in and out, 3.5 TB/s, a large copy reaches 4.9.  A few tokens are
 // the launch: 3 us on the device for one.  Tried without gain: the first rows asked for before the sequence is looked up (79), weights and
-// angles multiplied once for all heads of a kind and places counted on from head to head (104: more registers, longer before the first row).
+// angles multiplied once for all heads of a kind and places counted on from head to head (104: more registers, longer before the first
+// row), the blocks' part of the places by the scalar unit (81: 78 registers, six waves per SIMD instead of seven), eight waves (111: spills).
 template <int T, bool E4M3, int D, int WT, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a, int per) {
   constexpr int LG = D / 8, ROWS = 256 / LG;
