@@ -75,6 +75,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
   // enters as the sum of two bf16 numbers and the product is made twice: the matrix units have nothing else to do.
   constexpr int PT = E4M3 ? FMSMO_BF16 : QT;
   constexpr bool TWO = PT == FMSMO_BF16;
+  // fp16 ends at 2^-24, and where one key stands out the many small probabilities beside it are what the result is made of: powers go
+  // up to 2^14, in the sums as well (it cancels in o / l and in the joins), so that what is lost of one is below 2^-39.
+  constexpr float LIFT = PT == FMSMO_F16 ? 14.0f : 0.0f;
   constexpr int KW = E4M3 ? D / 64 : D / 32;  // 16-byte loads per key and lane group
   constexpr int QS = D / 32;                  // steps of the reduction over D
   constexpr int VW = E4M3 ? ND / 4 : ND / 2;  // words of a lane's values per key
@@ -321,11 +324,12 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
         m = m_new;
       }
       float pr[8];
+      const float ml = ms - LIFT;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float x = exp2_hw(st[h][i] - ms);
+          const float x = exp2_hw(st[h][i] - ml);
           l += x;
           // (a key that the row does not see counts nothing, whatever its scale holds)
           pr[4 * h + i] = E4M3 ? (whole || st[h][i] != -__builtin_inff() ? x * vs[h][i] : 0.0f) : x;

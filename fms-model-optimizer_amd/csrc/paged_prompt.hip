@@ -31,6 +31,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
   // an fp16 result, of which bf16 would lose three bits, they are the sum of two bf16 numbers
   constexpr int PT = E4M3 ? FMSMO_BF16 : QT;
   constexpr bool TWO = E4M3 && QT == FMSMO_F16;
+  // The maximum is held back by up to HOLD, and powers are LIFT larger than it leaves them, in the sums as well.  fp16 ends at 2^-24
+  // and 2^16, and where one key stands out the many small probabilities beside it are what the result is made of: powers up to 2^15, of which
+  // less than 2^-36 of the largest one's share is lost.  bf16 has fp32's exponents.  (fp16, powers up to 2^8 that end at 2^-24: 6 prompts of
+  // up to 6001 tokens in a window of 1024 425 us, 430 so; 32768 keys at 2^-26 beside one without a value came out as zeros.)
+  constexpr bool HALF = PT == FMSMO_F16;
+  constexpr float HOLD = HALF ? 4.0f : 8.0f, LIFT = HALF ? 11.0f : 0.0f;
   constexpr int QS = D / 16, NV = D / 32;
   // Shared memory holds rows as they are in memory, D elements; 16-byte piece c of row r lies at place c ^ f(r), by which neither the keys
   // (16 bytes of 32 rows per instruction) nor the values (64 bytes of 8 rows) ask a bank for two things at once.
@@ -269,7 +275,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     // register 4 i + j of st[kt]: key kt * 32 + 8 i + 4 hl + j.  From here on as the exponents that the present maximum leaves.
-    const float ms = safe_max(m);
+    const float ms = safe_max(m), ml = ms - LIFT;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -277,7 +283,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
         v4f by = {c, c, c, c};
         if constexpr (E4M3) by = *(const v4f*)&sc[buf][0][kt * 32 + 8 * i + 4 * hl];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) st[kt][4 * i + j] = __fmaf_rn(st[kt][4 * i + j], by[j], -ms);
+        for (int j = 0; j < 4; ++j) st[kt][4 * i + j] = __fmaf_rn(st[kt][4 * i + j], by[j], -ml);
       }
     if (!whole) {
       // (one test at a time, and only those that the tile needs)
@@ -297,11 +303,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, st[0][i]), st[1][i]);
     top = max_x32(top);
-    // The maximum is held back: powers up to 2^8 are as good as powers up to 1, and O is rescaled a few times at all (8192 tokens 560 us,
+    // The maximum is held back: powers up to 2^HOLD are as good as powers up to 1, and O is rescaled a few times at all (8192 tokens 560 us,
     // 600 with O rescaled for every tile; e4m3, 2 x 2048 tokens behind 30000 keys, 2707 and 2795)
-    const bool grow = top > 8.0f || (m == -__builtin_inff() && top > m);
+    const bool grow = top > HOLD + LIFT || (m == -__builtin_inff() && top > m);
     const bool any = __any(grow);
-    const float step = grow ? top : 0.0f;
+    const float step = grow ? top - LIFT : 0.0f;
     if (any) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -310,13 +316,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
       }
     }
     if (any) {
-      const float m_new = grow ? ms + top : m, f = grow ? exp2_hw(m - m_new) : 1.0f;
+      const float m_new = grow ? ms + step : m, f = grow ? exp2_hw(m - m_new) : 1.0f;
 #pragma unroll
       for (int d = 0; d < NV; ++d) o[d] *= f;
       l *= f;
       m = m_new;
     }
     v4i pb[4], pl[4];
+    float sum = 0.0f;  // (a tile's first, so that what is small beside l is not rounded away one by one)
     const auto powers = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
@@ -326,7 +333,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             pr[j] = exp2_hw(st[kt][4 * i + j]);
-            l += pr[j];
+            sum += pr[j];
           }
           if constexpr (E4M3) {
             const v4f vs = *(const v4f*)&sc[buf][1][kt * 32 + 8 * i + 4 * hl];
@@ -346,6 +353,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
     };
     if (E4M3 && !whole) powers(std::true_type{});
     else powers(std::false_type{});
+    l += sum;
     // O^T: step k of the reduction has keys 16 k + 4 hl + (0..3) and those + 8, as the scores lie
     const auto values = [&](int d, int k) {
       const char* at = vl[buf] + (v_base ^ d * 64) + 16 * k * ROW;
