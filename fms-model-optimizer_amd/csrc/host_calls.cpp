@@ -903,7 +903,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Heads o;
   if (!result_of(args[13], q, &out, &o) || !here(q.t, c.k, c.v, c.ks, c.vs, b.table, b.lens, b.start, &out)) return none();
   const int64_t keys = b.b.table_width * c.c.page_size;
-  const int64_t max_rows = b.start ? std::min(most_rows ? most_rows : q.rows, q.rows) : 1, max_keys = std::min(most_keys ? most_keys : keys, keys);
+  const int64_t max_rows = b.start ? std::min(most_rows ? most_rows : q.rows, q.rows) : 1;
+  int64_t max_keys = std::min(most_keys ? most_keys : keys, keys);
+  if (window && window < keys && sinks < keys) max_keys = std::min(max_keys, window + sinks + std::min<int64_t>(max_rows, 128));  // (no tile of rows goes through more)
   const at::Tensor ws = workspace(p_fmsmo_paged_attn_workspace_bytes((int)q.heads, c.c.heads, c.c.dim, c.c.dtype, b.b.seqs, q.rows, max_rows, max_keys), *q.t);
   if (!LAUNCH(fmsmo_paged_attn, &c.c, &b.b, code_of(q.t->scalar_type()), q.rows, (int)q.heads, q.p, q.row, q.head, o.p, o.row, o.head, scale,
               window, sinks, max_rows, max_keys, (int)(args[13] == Py_None), ws.defined() ? ws.data_ptr() : nullptr,

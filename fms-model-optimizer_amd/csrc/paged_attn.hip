@@ -666,6 +666,10 @@ static void bounds(int64_t& max_rows, int64_t& max_keys, int64_t rows, int64_t c
   if (max_rows < 1 || max_rows > rows) max_rows = std::max<int64_t>(1, rows);
   if (max_keys < 1 || max_keys > cap) max_keys = std::max<int64_t>(1, cap);
 }
+// the keys that a tile of rows (one token at least) goes through
+static int64_t visited(int64_t max_rows, int64_t max_keys, int64_t window, int64_t sinks) {
+  return window ? std::min(max_keys, window + sinks + std::min<int64_t>(max_rows, PROMPT_ROWS)) : max_keys;
+}
 
 extern "C" int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int kv_heads, int dim, int cache_dtype, int64_t seqs, int64_t rows, int64_t max_rows,
                                                     int64_t max_keys) {
@@ -690,7 +694,7 @@ extern "C" int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_ba
   a.zero_rest = zero_rest && batch->query_start;
   bounds(max_rows, max_keys, rows, a.cap, batch->query_start != nullptr);
   const bool e4m3 = cache->dtype == FMSMO_KV_E4M3;
-  const Plan p = plan_of(a.group, a.kv_heads, cache->dim, e4m3, a.seqs, rows, max_rows, max_keys);
+  const Plan p = plan_of(a.group, a.kv_heads, cache->dim, e4m3, a.seqs, rows, max_rows, visited(max_rows, max_keys, a.window, a.sinks));
   const int64_t need = plan_bytes(p, cache->dim);
   if (need > workspace_bytes || (need && !workspace)) return FMSMO_ERR_SCRATCH;
   if (((uintptr_t)workspace) & 15) return FMSMO_ERR_ALIGN;

@@ -1274,6 +1274,8 @@ def _paged_attention_impl(q, k_cache, v_cache, block_table, seq_lens, query_star
     keys = batch.table_width * cache.page_size
     max_rows = 1 if query_start is None else min(max_query_len or rows, rows)
     max_keys = min(max_seq_len or keys, keys)
+    if window:  # (no tile of rows goes through more)
+        max_keys = min(max_keys, window + sinks + min(max_rows, 128))
     nbytes = L.load().fmsmo_paged_attn_workspace_bytes(heads, cache.heads, dim, cache.dtype, batch.seqs, rows, max_rows, max_keys)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes > 0 else None
     with _dev(q):
