@@ -634,6 +634,8 @@ static Plan plan_of(int group, int kv_heads, int dim, bool e4m3, int64_t seqs, i
     p.row_shift = 3;
     p.tiles = (int)(rows * group / PROMPT_ROWS + seqs);
     // Few tiles of rows: several blocks for each, as many as leave every one eight tiles of keys, up to two for a compute unit
+    // where rows fill their tiles.  (Many sequences of fewer rows than a tile get more, which evens them out: 64 single tokens, 20 heads on a key
+    // head, 16000 keys 125 us so, 138 with a tile counted for each; up to 16000 keys 68 and 73.)
     const int64_t blocks = std::max<int64_t>(rows * group / PROMPT_ROWS, 1) * kv_heads, key_tiles = (max_keys + PROMPT_KEYS - 1) / PROMPT_KEYS;
     p.cuts = (int64_t)p.tiles * kv_heads;  // (counted with the room between sequences: at most 2048 shares, 64 KiB each at 128 elements)
     p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({(dim > 128 ? 256 : 512) / blocks, key_tiles / 8, 2048 / p.cuts, 64}));
