@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a, int per) {
     if (b < 0) return none();
   }
   const Seq s = seq_of(p, b);
-  if (t >= s.row0 + s.n) return none();
+  if ((unsigned)t - (unsigned)s.row0 >= (unsigned)s.n) return none();  // (before the first one, too: descending starts)
   const int pos = s.pos0 + (t - s.row0);
   int page = pos >= 0 && pos < p.cap ? p.table[b * p.table_stride + (pos >> p.page_shift)] : -1;
   if ((unsigned)page >= (unsigned)p.pages) page = -1;

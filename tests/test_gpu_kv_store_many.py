@@ -130,3 +130,32 @@ def test_many_tokens_without_norm_or_rotation(dev, rotary, norm, interleaved):
     assert torch.equal(whole, parts)
     for a, b in zip(*caches):
         assert torch.equal(raw(a), raw(b))
+
+
+BIG = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("lens,start,last", [
+    ([BIG, -5], [0, 20, 40], 0), ([64, 64], [0, BIG, BIG], 0), ([64, 64], [30, 10, 40], 1), ([BIG, BIG], [-9, 5, -1], -1), ([64, 0], [60, 70, 80], -1),
+    ([64, 64], [50, 0, 40], 1), ([64, 64], [0, 40, 20], 0)])
+def test_nonsense_in_the_batch(dev, lens, start, last):
+    """Rows and lengths that the operands don't have, and descending starts: nothing around the tensors changes, rows that no sequence names
+    are zero, and a sequence's keys are written by its own rows only (`last`: the one sequence with rows)."""
+    g = gen(14)
+    table, pages = R.make_pages(g, [64, 64], 16)
+    caches = torch.full((2, pages + 2, 2, 16, 64), 5.0, dtype=torch.float16, device=dev)
+    kd, vd = caches[0, 1:-1], caches[1, 1:-1]
+    x = torch.randn(40, 8, 64, generator=g).half().to(dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for in_place in (False, True):
+        q = x[:, :4].clone() if in_place else x[:, :4]
+        room = torch.full((44, 4, 64), 3.0, dtype=torch.float16, device=dev)
+        out = K().qk_norm_rope_store(q, x[:, 4:6], x[:, 6:], kd, vd, table.to(dev), i32(lens), i32(start), out=room[2:42] if in_place else None)
+        torch.cuda.synchronize()
+        assert (room[:2] == 3).all() and (room[42:] == 3).all()
+        assert (caches[:, 0] == 5).all() and (caches[:, -1] == 5).all()
+        if last < 0:
+            assert (out == (3 if in_place else 0)).all()
+        theirs = [int(n) for n in table[1 - last] if 0 <= n < pages] if last >= 0 else range(pages)
+        for n in theirs:
+            assert (kd[n] == 5).all() and (vd[n] == 5).all()
