@@ -691,7 +691,7 @@ extern "C" int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_ba
   if (window < 0 || sinks < 0 || workspace_bytes < 0) return FMSMO_ERR_SHAPE;
   if (rows == 0 || batch->seqs == 0) return FMSMO_OK;
   a.c = scale * LOG2E;
-  a.window = (int)std::min<int64_t>(window, 1 << 30);
+  a.window = (int)std::min<int64_t>(window, 0x7fffffff);
   a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
   a.zero_rest = zero_rest && batch->query_start;
   bounds(max_rows, max_keys, rows, a.cap, batch->query_start != nullptr);

@@ -89,7 +89,7 @@ __device__ __forceinline__ Tiles tiles_of(const PagedArgs& a, int len, int p_lo,
   int end = p_hi + 1 < len ? p_hi + 1 : len;
   if (end < 0) end = 0;
   const int all = (end + TILE - 1) / TILE;
-  int lo = a.window ? p_lo - a.window + 1 : 0;
+  int lo = a.window ? (p_lo > 0 ? p_lo : 0) - a.window + 1 : 0;
   if (lo < 0) lo = 0;
   const int s = a.sinks < lo ? a.sinks : lo;
   t.sink_tiles = (s + TILE - 1) / TILE;
@@ -112,7 +112,9 @@ struct Bounds {
 __device__ __forceinline__ Bounds bounds_of(const PagedArgs& a, int p_lo, int p_hi, int len, int at) {
   Bounds b;
   b.hi = (p_hi < len - 1 ? p_hi : len - 1) - at;
-  b.lo = a.window ? p_lo - a.window - at : -(1 << 30);
+  // (a length beyond the table's keys may be any int, and so may a window: nothing here leaves 32 bits)
+  const int lo = (p_lo > 0 ? p_lo : 0) - a.window;
+  b.lo = a.window ? (lo > -1 ? lo : -1) - at : -(1 << 30);
   b.sink = a.sinks - at;
   return b;
 }
