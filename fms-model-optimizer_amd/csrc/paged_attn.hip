@@ -43,9 +43,11 @@ __device__ __forceinline__ Part part_of(const PagedArgs& a, const Seq& s, int un
   }
   return w;
 }
-// inclusive sums over the lanes of the wave: within rows of 16, then the rows before
+// inclusive sums over the lanes of the wave (HELD: that stop at 2^31 - 1): within rows of 16, then the rows before
+template <bool HELD = false>
 __device__ __forceinline__ int scan_lanes(int v) {
-#define FMSMO_DPP_ADD(ctrl, rows) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, true)
+  const auto add = [](int x, int y) { return HELD ? __builtin_elementwise_add_sat(x, y) : x + y; };
+#define FMSMO_DPP_ADD(ctrl, rows) v = add(v, __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, true))
   FMSMO_DPP_ADD(0x111, 0xf);  // row_shr 1, 2, 4, 8
   FMSMO_DPP_ADD(0x112, 0xf);
   FMSMO_DPP_ADD(0x114, 0xf);
@@ -100,11 +102,14 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
     scan = scan_lanes(part.pairs * part.units);
     kept = c;
   };
-  int total = 0;
+  int total = 0, given = 0;
   for (int c = 0; c < a.seqs; c += 64) {
     look(c);
     total += __builtin_amdgcn_readlane(scan, 63);
+    if constexpr (MULTI) given = __builtin_elementwise_add_sat(given, __builtin_amdgcn_readlane(scan_lanes<true>(seq.n), 63));
   }
+  // (starts that go up and down name rows again and again: more units than 31 bits hold, or than anybody waits for)
+  if (MULTI && given > a.rows) total = 0;
   const int workers = sa.workers < total ? sa.workers : total;  // (so that no worker is without work)
   const bool idle = (int)blockIdx.x >= workers;
   Cut* cut = (Cut*)sa.ws + blockIdx.x;

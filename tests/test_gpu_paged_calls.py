@@ -198,3 +198,24 @@ def test_nonsense_in_the_batch(dev, lens, start, defined):
                     ref, bound = R.attention(q.cpu(), k, v, table, lens, start, None, w, 2)
                     assert R.worst(y[named], ref[named], bound[named]) <= 1.0
     assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)
+
+
+@pytest.mark.parametrize("hint", [1, 4096])
+def test_starts_that_go_up_and_down(dev, hint):
+    """200 sequences that name the same 4096 rows, 2^24 units of work each: more rows than there are, of which nothing is computed by the kernel
+    of few rows; the prompt kernel's blocks are as many as rows have tiles."""
+    from fms_mo_amd import kernels as K
+
+    g = gen(22)
+    q = torch.randn(4096, 128, 64, generator=g).half().to(dev)
+    k, v = (torch.randn(4, 8, 16, 64, generator=g).half().to(dev) for _ in range(2))
+    seqs, P = 400, 4096
+    table = torch.randint(0, 4, (1, P), generator=g).to(torch.int32).to(dev).expand(seqs, P)
+    lens, start = i32([65536] * seqs, dev), i32([0, 4096] * (seqs // 2) + [0], dev)
+    out = torch.full((4098, 128, 64), 3.0, dtype=torch.float16, device=dev)
+    K.paged_attention(q, k, v, table, lens, start, max_query_len=hint, out=out[1:-1])
+    assert (out[0] == 3).all() and (out[-1] == 3).all()
+    if hint == 1:
+        assert (out == 3).all()
+    # what follows is as ever
+    compare(dev, torch.float16, False, 4, 2, 64, 16, [100, 65, 1, 0, 333], [2, 1, 1, 0, 3], seed=3)
