@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : E4M3 ? 3 : 4) vo
   const int pos = mine ? s.pos0 + tok : -1;
   const int w_lo = s.pos0 + (r0 + wr) / a.group, w_hi = wn > 0 ? s.pos0 + (r0 + wr + wn - 1) / a.group : w_lo;
   // exp2(c s - m) with c > 0, so that the maximum of c s is that of s: a negative scale turns the queries' sign
-  const float c = fmaxf(fabsf(a.c), 0x1p-126f);
+  const float c = fabsf(a.c) < 0x1p-126f ? 0x1p-126f : fabsf(a.c);  // (NaN stays)
   v4i q[QS];
   {
     const char* src = a.q + (s.row0 + tok) * a.q_row + head * a.q_head;

@@ -219,3 +219,17 @@ def test_starts_that_go_up_and_down(dev, hint):
         assert (out == 3).all()
     # what follows is as ever
     compare(dev, torch.float16, False, 4, 2, 64, 16, [100, 65, 1, 0, 333], [2, 1, 1, 0, 3], seed=3)
+
+
+@pytest.mark.parametrize("dt,e4m3", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 70])
+def test_a_scale_that_is_no_number(dev, dt, e4m3, new):
+    from fms_mo_amd import kernels as K
+
+    g = gen(23)
+    lens, start = [300, 77], None if new == 1 else i32([0, new, 2 * new], dev)
+    table, pages = R.make_pages(g, lens, 16)
+    kd, vd, ksd, vsd = on(dev, *R.make_cache(g, pages, 2, 16, 64, dt, e4m3))
+    q = torch.randn(2 * new, 4, 64, generator=g).to(dt).to(dev)
+    y = K.paged_attention(q, kd, vd, table.to(dev), i32(lens, dev), start, scale=float("nan"), k_scale=ksd, v_scale=vsd, max_query_len=new)
+    assert y.isnan().all()
