@@ -14,7 +14,8 @@
 //                 from which v_perm makes columns ND c + n of V^T for the ND instructions n.
 //
 // 64 sequences of up to 8000 keys, 32 + 8 heads of 128, bf16: 180 us, 6.1 TB/s, where a launch that only reads reaches 6.9.  Tried without
-// gain: tiles asked for two ahead, three waves per SIMD, eight waves a block, more blocks.
+// gain: tiles asked for two ahead, three waves per SIMD, eight waves a block, more blocks.  (All of it at 128 elements; 64 leave registers for
+// three or four blocks per compute unit, which have not been measured.)
 //
 // Work: all tiles of all sequences and heads in a row, cut into `workers` equal parts on the device from seq_lens, so a batch of
 // uneven lengths keeps every block busy for the same time and nothing about the lengths has to be known on the host.
@@ -479,7 +480,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
 // Joins the shares of the pairs that were cut: a block per cut and row, rows side by side, since neighbouring blocks go to different parts
 // of the chip and cuts may come in steps of eight (with the cuts side by side 32 pairs of 32 rows in 16 shares took 23 us, not 8).  The
 // weights of all shares first (a share per thread), then every group of D / 4 threads adds up every (1024 / D)-th share: loads that wait
-// for nothing but the weights.  Bound by those two dependent rounds of loads: 4 us for single tokens, 7 for 512 shares a row.
+// for nothing but the weights.  Bound by those two dependent rounds of loads, and with hundreds of shares by one block reading all of a
+// row's: a few shares of 128 elements 4 us, 64 of them 6.5 (131072 keys, 8 key heads), 512 of them 22 (one key head; 13 at 64 elements).
 template <int QT, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(SplitArgs sa) {
   constexpr int LG = D / 4, GROUPS = 256 / LG;

@@ -15,6 +15,10 @@
 // 2 x 2048 tokens behind 30000 keys 2415 us, 860 TFLOP/s.  Tried and slower, the one prompt (560 us then): the scores of the next tile
 // beside the softmax of this one (649; a third of the registers more and no better order), the values' reads ahead of their products
 // (621), s_setprio around the products (571), sums of the probabilities by dot products (587).
+//
+// Probabilities over 16-bit caches enter the second product once rounded to the cache's type: a second term would make half as many
+// matrix instructions again.  Error against 64 bits, in units of the result's size: bf16, 8192 tokens, 0.0021, where probabilities of fp32 leave
+// 0.0016; fp16 in a window 0.00026 and 0.00020; e4m3 with bf16 results 0.0023 and 0.0017.
 #include "paged_kv.hpp"
 
 #include <algorithm>

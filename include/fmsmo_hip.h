@@ -860,7 +860,8 @@ typedef struct {
  * the call's rows (ascending; query_start NULL: row b alone, and as many rows as sequences) and seq_lens[b] keys with
  * those of its rows, so its i-th of n rows stands at position seq_lens[b] - n + i.  Key j lies in row j % page_size of
  * page block_table[b * table_stride + j / page_size].  A page number outside of the cache's pages names no page: such keys are
- * neither written nor seen.  So are keys beyond the table's row.  Rows before position 0 see nothing.
+ * neither written nor seen.  So are keys beyond the table's row.  Rows before position 0 see nothing.  Arrays that descend, or name what
+ * is not there, give results without a meaning, but nothing outside of the operands is touched.  A call without sequences does nothing.
  */
 typedef struct {
   const int32_t* block_table;
@@ -895,8 +896,8 @@ int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch,
  * q heads h * g .. share key head h (g = q_heads / heads).  A row that sees nothing, or nothing with a score above -inf, is zero;
  * what a row doesn't see has no influence on it, whatever it holds.  out is q or apart from it.  Sums are fp32; the probabilities
  * are rounded to dtype before they meet the values (e4m3 caches: times the values' scales, to bf16, for dtype fp16 to the sum
- * of two bf16 numbers; a few rows of a sequence: always to the sum of two where they are bf16).  Rows of no sequence: zero with
- * zero_rest, else left as they are.
+ * of two bf16 numbers; a few rows of a sequence: always to the sum of two where they are bf16); of one in fp16 less than 2^-36 of the
+ * row's largest is lost.  Rows of no sequence: zero with zero_rest, else left as they are.
  * max_rows, max_keys: upper bounds of a sequence's rows and keys that the host knows (0: none); they choose the kernel and how
  * the work is split, and a sequence that exceeds them is still computed in full.
  * workspace: fmsmo_paged_attn_workspace_bytes(q_heads, heads, dim, dtype of the cache, seqs, rows, max_rows, max_keys) bytes, 16-byte
