@@ -74,10 +74,9 @@ template <int QT, bool E4M3, int D, bool MULTI, bool SHARED>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(SplitArgs sa) {
   constexpr int ND = D / 16;
   // Type of the probabilities and the values in the product.  e4m3 caches: the probabilities are multiplied by the values' scales before
-  // they are rounded, which takes the exponents of bf16.  A bf16 probability has lost as much as the rounded result may, so it
-  // enters as the sum of two bf16 numbers and the product is made twice: the matrix units have nothing else to do.
+  // they are rounded, which takes the exponents of bf16.  A probability of 16 bits has lost as much as the rounded result may, so it
+  // enters as the sum of two such numbers and the product is made twice: the matrix units have nothing else to do.
   constexpr int PT = E4M3 ? FMSMO_BF16 : QT;
-  constexpr bool TWO = PT == FMSMO_BF16;
   // fp16 ends at 2^-24, and where one key stands out the many small probabilities beside it are what the result is made of: powers go
   // up to 2^14, in the sums as well (it cancels in o / l and in the joins), so that what is lost of one is below 2^-39.
   constexpr float LIFT = PT == FMSMO_F16 ? 14.0f : 0.0f;
@@ -345,8 +344,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
       for (int i = 0; i < 4; ++i) {
         const uint32_t hi = pack2<PT>(pr[2 * i], pr[2 * i + 1]);
         pb[i] = (int)hi;
-        if constexpr (TWO)
-          pl[i] = (int)pack2<PT>(pr[2 * i] - __uint_as_float(hi << 16), pr[2 * i + 1] - __uint_as_float(hi & 0xffff0000u));
+        if constexpr (PT == FMSMO_F16) pl[i] = (int)pack2<PT>(pr[2 * i] - f16_to_f32((u16)hi), pr[2 * i + 1] - f16_to_f32((u16)(hi >> 16)));
+        else pl[i] = (int)pack2<PT>(pr[2 * i] - __uint_as_float(hi << 16), pr[2 * i + 1] - __uint_as_float(hi & 0xffff0000u));
       }
       // O^T
       uint32_t vw[8][ND / 2];
@@ -384,7 +383,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_split_kernel(Split
       for (int n = 0; n < ND; ++n) {
         const v4i f = {column(n, 0), column(n, 1), column(n, 2), column(n, 3)};
         o[n] = mfma16<PT>(f, pb, o[n]);
-        if constexpr (TWO) o[n] = mfma16<PT>(f, pl, o[n]);
+        o[n] = mfma16<PT>(f, pl, o[n]);
       }
       load_v(more, pg);
     }

@@ -896,7 +896,7 @@ int fmsmo_kv_store(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batch,
  * q heads h * g .. share key head h (g = q_heads / heads).  A row that sees nothing, or nothing with a score above -inf, is zero;
  * what a row doesn't see has no influence on it, whatever it holds.  out is q or apart from it.  Sums are fp32; the probabilities
  * are rounded to dtype before they meet the values (e4m3 caches: times the values' scales, to bf16, for dtype fp16 to the sum
- * of two bf16 numbers; a few rows of a sequence: always to the sum of two where they are bf16); of one in fp16 less than 2^-36 of the
+ * of two bf16 numbers; a few rows of a sequence: always to the sum of two); of one in fp16 less than 2^-36 of the
  * row's largest is lost.  Rows of no sequence: zero with zero_rest, else left as they are.
  * max_rows, max_keys: upper bounds of a sequence's rows and keys that the host knows (0: none); they choose the kernel and how
  * the work is split, and a sequence that exceeds them is still computed in full.

@@ -233,3 +233,21 @@ def test_a_scale_that_is_no_number(dev, dt, e4m3, new):
     q = torch.randn(2 * new, 4, 64, generator=g).to(dt).to(dev)
     y = K.paged_attention(q, kd, vd, table.to(dev), i32(lens, dev), start, scale=float("nan"), k_scale=ksd, v_scale=vsd, max_query_len=new)
     assert y.isnan().all()
+
+
+@pytest.mark.parametrize("rows,heads", [(1, 8), (3, 4)])
+def test_fp16_probabilities_of_few_rows_are_two_terms(dev, rows, heads):
+    """As for bf16: its own rounding and 2^-22 of the probabilities, not the 2^-11 of one fp16 number."""
+    from fms_mo_amd import kernels as K
+
+    g = gen(rows)
+    n, D = 70, 128
+    k, v = (t.view(n, D) for t in R.make_cache(g, n, 1, 1, D, torch.float16, False)[:2])
+    q = (0.1 * torch.randn(rows, heads, D, generator=g)).half()
+    ref, bound, w = against(q, k.double(), v.double(), n - rows + torch.arange(rows), D ** -0.5, 2.0 ** -22)
+    top = w.amax(-1, keepdim=True)
+    once = (w / top).half().double() * top @ v.double()
+    assert R.worst(once.half().view(q.shape), ref, bound) > 1.5
+    (kc, vc, _, _), table = paged(dev, k, v, 16)
+    y = K.paged_attention(q.to(dev), kc, vc, table, i32([n], dev), None if rows == 1 else i32([0, rows], dev))
+    assert R.worst(y, ref, bound) <= 1.0
