@@ -32,7 +32,8 @@ namespace {
   X(fmsmo_matmul_chunk_i8_dq_ws) X(fmsmo_matmul_chunk_fp_dq) X(fmsmo_matmul_chunk_workspace_bytes)    \
   X(fmsmo_quant_i8_affine_sums) X(fmsmo_quant_i8_affine_pair) X(fmsmo_affine_sum_parts) X(fmsmo_affine_parts_first) X(fmsmo_affine_add_parts) X(fmsmo_bmm_qa_ok)   \
   X(fmsmo_bmm_qa_i8) X(fmsmo_bmm_i8_zp)                                                                 \
-  X(fmsmo_kv_store) X(fmsmo_paged_attn) X(fmsmo_paged_attn_workspace_bytes)
+  X(fmsmo_kv_store) X(fmsmo_paged_attn) X(fmsmo_paged_attn_workspace_bytes)                                  \
+  X(fmsmo_add_rms_norm_quant) X(fmsmo_lora_add) X(fmsmo_lora_workspace_bytes) X(fmsmo_moe_few_tokens) X(fmsmo_moe_few_workspace_bytes)
 #define DECLARE(f) decltype(&::f) p_##f = nullptr;
 ENTRIES(DECLARE)
 #undef DECLARE
@@ -960,6 +961,153 @@ PyObject* kv_store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------ around the products of a served layer
+// a matrix of 16-bit elements with 16-byte aligned rows of multiples of eight, or none
+Mat mat16(PyObject* o, at::ScalarType st) {
+  Mat m = mat(o);
+  if (!m || m.t->scalar_type() != st || m.cols % 8 || m.ld % 8 || (uintptr_t)m.p % 16) return Mat{};
+  return m;
+}
+// what a call writes: `given` of the shape, or a new matrix
+bool matrix_of(PyObject* given, int64_t rows, int64_t cols, at::ScalarType st, const at::Tensor& like, at::Tensor* out, Mat* m) {
+  if (given == Py_None) {
+    *out = empty({rows, cols}, st, like);
+    *m = Mat{out, rows, cols, cols, (char*)out->data_ptr()};
+    return true;
+  }
+  *m = mat16(given, st);
+  if (!*m || m->rows != rows || m->cols != cols) return false;
+  *out = *m->t;
+  return true;
+}
+// (x, weight, residual | None, eps, dtype, scale | None, want_normed, residual_out | None) -> (q, scale, residual | None, normed | None)
+PyObject* add_rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  WANT(8);
+  const at::Tensor* xt = plain(args[0]);
+  if (!xt || (xt->scalar_type() != at::kHalf && xt->scalar_type() != at::kBFloat16)) return none();
+  const at::ScalarType st = xt->scalar_type();
+  const Mat x = mat16(args[0], st);
+  if (!x || x.rows == 0 || x.cols == 0 || !THPDtype_Check(args[4])) return none();
+  const at::ScalarType ct = ((THPDtype*)args[4])->scalar_type;
+  if (ct != at::kChar && ct != at::kFloat8_e4m3fn) return none();
+  const Opt w = opt_vec(args[1], x.cols, 16);
+  if (!w.ok || !w.p || (w.st != st && w.st != at::kFloat)) return none();
+  const double eps = REAL(3);
+  NUMBERS_OK;
+  const bool res = args[2] != Py_None, given = args[5] != Py_None;
+  Mat r, ro;
+  at::Tensor out, normed;
+  const at::Tensor* sc = nullptr;
+  if (res) {
+    r = mat16(args[2], st);
+    if (!r || r.rows != x.rows || r.cols != x.cols) return none();
+  } else if (args[7] != Py_None) {
+    return none();
+  }
+  if (given) {
+    sc = vec32(args[5], 1);
+    if (!sc) return none();
+  }
+  if (!here(x.t, w.t, r.t, sc)) return none();
+  if (res && (!matrix_of(args[7], x.rows, x.cols, st, *x.t, &out, &ro) || !here(&out))) return none();
+  const int want = PyObject_IsTrue(args[6]);
+  if (want) normed = empty({x.rows, x.cols}, st, *x.t);
+  at::Tensor q = empty({x.rows, x.cols}, ct, *x.t), s = given ? *sc : empty({x.rows}, at::kFloat, *x.t);
+  if (!LAUNCH(fmsmo_add_rms_norm_quant, x.p, code_of(st), x.ld, r.p, r.ld, w.p, w.dt, (float)eps, ct == at::kChar ? FMSMO_OP_I8 : FMSMO_OP_E4M3,
+              (int)given, q.data_ptr(), x.cols, (float*)s.data_ptr(), ro.p, ro.ld, want ? normed.data_ptr() : nullptr, x.cols, x.rows, x.cols,
+              stream_of(*x.t)))
+    return nullptr;
+  PyObject* t = PyTuple_New(4);
+  PyTuple_SET_ITEM(t, 0, wrap(std::move(q)));
+  if (given) Py_INCREF(args[5]);
+  PyTuple_SET_ITEM(t, 1, given ? args[5] : wrap(std::move(s)));
+  if (args[7] != Py_None) Py_INCREF(args[7]);
+  PyTuple_SET_ITEM(t, 2, args[7] != Py_None ? args[7] : res ? wrap(std::move(out)) : none());
+  PyTuple_SET_ITEM(t, 3, want ? wrap(std::move(normed)) : none());
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+// (y, x, a, b, adapters, query_start | None, scales | None, out | None) -> out
+PyObject* lora_add(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  WANT(8);
+  const at::Tensor *xt = plain(args[1]), *a = plain(args[2]), *b = plain(args[3]), *ids = plain(args[4]);
+  const at::Tensor *qs = args[5] == Py_None ? nullptr : plain(args[5]), *sc = args[6] == Py_None ? nullptr : plain(args[6]);
+  if (!xt || !a || !b || !ids || (!qs && args[5] != Py_None) || (!sc && args[6] != Py_None)) return none();
+  const at::ScalarType st = xt->scalar_type();
+  if (st != at::kHalf && st != at::kBFloat16) return none();
+  const Mat x = mat16(args[1], st), y = mat16(args[0], st);
+  if (!x || !y || x.rows == 0 || y.cols == 0 || x.rows != y.rows) return none();
+  if (a->dim() != 3 || b->dim() != 3 || a->scalar_type() != st || b->scalar_type() != st) return none();
+  const int64_t S = a->size(0), r = a->size(1), K = x.cols, N = y.cols;
+  if (S == 0 || r < 8 || r > 128 || r % 8 || a->size(2) != K || b->size(0) != S || b->size(1) != N || b->size(2) != r) return none();
+  const int64_t a_slot = step(*a, 0), a_row = a->stride(1), b_slot = step(*b, 0), b_row = N > 1 ? b->stride(1) : r;
+  if (a->stride(2) != 1 || b->stride(2) != 1 || a_slot % 8 || a_row % 8 || b_slot % 8 || b_row % 8 || a_row < K || b_row < r ||
+      (uintptr_t)a->data_ptr() % 16 || (uintptr_t)b->data_ptr() % 16)
+    return none();
+  if (ids->dim() != 1 || ids->scalar_type() != at::kInt || !ids->is_contiguous()) return none();
+  const int64_t seqs = ids->numel();
+  if (seqs == 0 || (qs ? qs->dim() != 1 || qs->numel() != seqs + 1 || qs->scalar_type() != at::kInt || !qs->is_contiguous() : seqs != x.rows)) return none();
+  if (sc && (sc->dim() != 1 || sc->numel() != S || sc->scalar_type() != at::kFloat || !sc->is_contiguous())) return none();
+  at::Tensor out;
+  Mat o;
+  if (!here(x.t, y.t, a, b, ids, qs, sc) || !matrix_of(args[7], x.rows, N, st, *x.t, &out, &o) || !here(&out)) return none();
+  const at::Tensor ws = workspace(p_fmsmo_lora_workspace_bytes(x.rows, seqs, qs != nullptr, (int)r, K), *x.t);
+  if (!ws.defined()) return none();
+  if (!LAUNCH(fmsmo_lora_add, code_of(st), x.p, x.ld, y.p, y.ld, o.p, o.ld, a->data_ptr(), a_slot, a_row, b->data_ptr(), b_slot, b_row, S, (int)r,
+              (const int32_t*)ids->data_ptr(), qs ? (const int32_t*)qs->data_ptr() : nullptr, seqs, sc ? (const float*)sc->data_ptr() : nullptr,
+              x.rows, N, K, ws.data_ptr(), ws.numel(), stream_of(*x.t)))
+    return nullptr;
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+// (a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, out_dtype, out | None) -> out
+PyObject* moe_few_tokens(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  WANT(11);
+  const Mat a = mat(args[0]), l = mat(args[2]);
+  const at::Tensor *w13 = plain(args[3]), *s13 = plain(args[4]), *w2 = plain(args[5]), *s2 = plain(args[6]);
+  if (!a || !l || !w13 || !s13 || !w2 || !s2) return none();
+  const at::ScalarType ct = a.t->scalar_type(), lt = l.t->scalar_type();
+  if ((ct != at::kChar && ct != at::kFloat8_e4m3fn) || w13->scalar_type() != ct || w2->scalar_type() != ct || code_of(lt) < 0) return none();
+  if (w13->dim() != 3 || w2->dim() != 3 || w13->size(1) % 2 || !w13->is_contiguous() || !w2->is_contiguous()) return none();
+  const int64_t T = a.rows, K = a.cols, E = w13->size(0), I = w13->size(1) / 2;
+  const int64_t top = WHOLE(7);
+  NUMBERS_OK;
+  if (T == 0 || T > 64 || K % 16 || I % 16 || K < 16 || I < 16 || E < 1 || E > 512 || top < 1 || top > 16 || top > E || w13->size(2) != K ||
+      w2->size(0) != E || w2->size(1) != K || w2->size(2) != I || l.rows != T || l.cols != E || a.ld % 16)
+    return none();
+  const at::Tensor* as = vec32(args[1], T);
+  if (!as) return none();
+  for (const at::Tensor* s : {s13, s2})
+    if (s->dim() != 2 || s->size(0) != E || s->size(1) != (s == s13 ? 2 * I : K) || s->scalar_type() != at::kFloat || !s->is_contiguous()) return none();
+  for (const void* p : {(const void*)a.p, (const void*)w13->data_ptr(), (const void*)w2->data_ptr(), (const void*)s13->data_ptr(), (const void*)s2->data_ptr()})
+    if ((uintptr_t)p % 16) return none();
+  at::ScalarType yt;
+  at::Tensor out;
+  Mat o;
+  if (args[10] == Py_None) {
+    if (!dtype_arg(args[9], &yt) || !here(a.t, l.t, w13, s13, w2, s2, as)) return none();
+    out = empty({T, K}, yt, *a.t);
+    o = Mat{&out, T, K, K, (char*)out.data_ptr()};
+  } else {
+    o = mat(args[10]);
+    if (!o || o.rows != T || o.cols != K || code_of(o.t->scalar_type()) < 0 || (uintptr_t)o.p % 16 || !here(a.t, l.t, w13, s13, w2, s2, as, o.t)) return none();
+    yt = o.t->scalar_type();
+    out = *o.t;
+  }
+  const int renorm = PyObject_IsTrue(args[8]);
+  const at::Tensor ws = workspace(p_fmsmo_moe_few_workspace_bytes(T, E, (int)top, K, I), *a.t);
+  if (!ws.defined()) return none();
+  if (!LAUNCH(fmsmo_moe_few_tokens, ct == at::kChar ? FMSMO_OP_I8 : FMSMO_OP_E4M3, a.p, a.ld, (const float*)as->data_ptr(), as->numel(), l.p,
+              code_of(lt), l.ld, w13->data_ptr(), (const float*)s13->data_ptr(), w2->data_ptr(), (const float*)s2->data_ptr(), T, E, (int)top,
+              renorm, o.p, code_of(yt), o.ld, K, I, ws.data_ptr(), ws.numel(), stream_of(*a.t)))
+    return nullptr;
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // ------------------------------------------------------------------ module
 // bind({entry point: address}, raise_status)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -993,7 +1141,8 @@ PyObject* entries(PyObject*, PyObject*) {
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(quant_i8), FAST(quant_i8_clips), FAST(quant_i8_static), FAST(quant_i8_static_t), FAST(quant_fp8), FAST(gemm_dq),
                          FAST(decode_i8), FAST(decode_fp8), FAST(grouped_i8), FAST(chunk_dq), FAST(bmm_quantized),
-                         FAST(deploy_i8), FAST(fp8_linear), FAST(paged_attention), FAST(kv_store), FAST(bind), {"entries", entries, METH_NOARGS, nullptr},
+                         FAST(deploy_i8), FAST(fp8_linear), FAST(paged_attention), FAST(kv_store),
+                         FAST(add_rms_norm_quant), FAST(lora_add), FAST(moe_few_tokens), FAST(bind), {"entries", entries, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fmsmo_host", nullptr, -1, methods};
 

@@ -107,6 +107,9 @@ SIGNATURES = {
     "fmsmo_bmm_fp8_dq": [_P, _L, _P, _L, _L, _P, _P, _P, _P, _I, _L, _L, _L, _L, _L, _P],
     "fmsmo_kv_store": [_P, _P, _I, _L, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _F, _P, _P, _L, _I, _I, _I, _P],
     "fmsmo_paged_attn": [_P, _P, _I, _L, _I, _P, _L, _L, _P, _L, _L, _F, _L, _L, _L, _L, _I, _P, _L, _P],
+    "fmsmo_add_rms_norm_quant": [_P, _I, _L, _P, _L, _P, _I, _F, _I, _I, _P, _L, _P, _P, _L, _P, _L, _L, _L, _P],
+    "fmsmo_lora_add": [_I, _P, _L, _P, _L, _P, _L, _P, _L, _L, _P, _L, _L, _L, _I, _P, _P, _L, _P, _L, _L, _L, _P, _L, _P],
+    "fmsmo_moe_few_tokens": [_I, _P, _L, _P, _L, _P, _I, _L, _P, _P, _P, _P, _L, _L, _I, _I, _P, _I, _L, _L, _L, _P, _L, _P],
     "fmsmo_zero_shift_bias": [_P, _L, _P, _L, _P, _F, _P, _I, _P, _L, _L, _P],
     "fmsmo_debug_clock_probe": [_P],
     "fmsmo_debug_stream_read": [_P, _L, _P, _P],
@@ -127,6 +130,8 @@ OTHER = {
     "fmsmo_gemm_fp8_workspace_bytes": ([c_int64, c_int64, c_int64], c_int64),
     "fmsmo_matmul_chunk_workspace_bytes": ([c_int, c_int64, c_int64, c_int64, c_int, c_int], c_int64),
     "fmsmo_paged_attn_workspace_bytes": ([c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64], c_int64),
+    "fmsmo_lora_workspace_bytes": ([c_int64, c_int64, c_int, c_int, c_int64], c_int64),
+    "fmsmo_moe_few_workspace_bytes": ([c_int64, c_int64, c_int, c_int64, c_int64], c_int64),
     "fmsmo_decode_linear_ok": ([c_int64, c_int64], c_int),
     "fmsmo_decode_linear_f32s_ok": ([c_int64, c_int64], c_int),
     "fmsmo_small_linear_static_ok": ([c_int64, c_int64, c_int64, _F, _F, _F, _F], c_int),

@@ -1361,3 +1361,249 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, query_start=None
     else:
         torch.ops.fms_mo_amd.paged_attention(*args)
     return out
+
+
+# ------------------------------------------------------------------ around the products of a served layer
+_CODES = {torch.int8: L.OP_I8, torch.float8_e4m3fn: L.OP_E4M3}
+
+
+def _rows16(t, name, shape, dtype, step=8):
+    """A matrix of the shape and dtype with unit inner stride, rows and address as the kernels load them (copied where they are not)."""
+    if t.dim() != 2 or t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.stride(1) != 1 or t.data_ptr() % 16 or (shape[0] > 1 and (t.stride(0) < shape[1] or t.stride(0) % step)):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _rows_out(out, name, shape, dtype, step=8):
+    """Checks a matrix that a call writes; its leading dimension."""
+    if out.shape != shape or out.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)}")
+    if out.stride(1) != 1 or (not _COMPILING() and out.data_ptr() % 16) or (shape[0] > 1 and (out.stride(0) < shape[1] or out.stride(0) % step)):
+        raise ValueError(f"the rows of {name} must be contiguous, 16-byte aligned and apart")
+
+
+def _add_rms_norm_quant_impl(x, weight, residual, eps, scale, q, scale_out, residual_out, normed):
+    _same_gpu(x, weight, residual, scale, q, scale_out, residual_out, normed)
+    M, K = x.shape
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if weight.shape != (K,) or weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"weight must be [{K}], {x.dtype} or float32")
+    if K % 8:
+        raise ValueError(f"rows must be a multiple of 8 elements, got {K}")
+    x = _rows16(x, "x", (M, K), x.dtype)
+    if residual is not None:
+        residual = _rows16(residual, "residual", (M, K), x.dtype)
+    if weight.data_ptr() % 16 or not weight.is_contiguous():
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    s = scale_out if scale is None else scale
+    with _dev(x):
+        L.call("fmsmo_add_rms_norm_quant", x.data_ptr(), _DT[x.dtype], _ld(x), _ptr(residual), 0 if residual is None else _ld(residual),
+               weight.data_ptr(), _DT[weight.dtype], float(eps), _CODES[q.dtype], int(scale is not None), q.data_ptr(), _ld(q), s.data_ptr(),
+               _ptr(residual_out), 0 if residual_out is None else _ld(residual_out), _ptr(normed), 0 if normed is None else _ld(normed), M, K,
+               _stream(x))
+
+
+def _lora_add_impl(y, x, a, b, adapters, query_start, scales, out):
+    _same_gpu(y, x, a, b, adapters, query_start, scales, out)
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if a.dim() != 3 or b.dim() != 3 or a.dtype != x.dtype or b.dtype != x.dtype:
+        raise ValueError(f"a and b must be [slots, rank, K] and [slots, N, rank] of {x.dtype}")
+    T, K = x.shape
+    S, r, _ = a.shape
+    N = y.shape[1]
+    if a.shape[2] != K or b.shape != (S, N, r):
+        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} do not fit x {tuple(x.shape)} and y {tuple(y.shape)}")
+    if r % 8 or not 8 <= r <= 128 or K % 8 or N % 8:
+        raise ValueError(f"rank must be a multiple of 8 up to 128 and rows of multiples of 8: rank {r}, {K} inputs, {N} outputs")
+    x = _rows16(x, "x", (T, K), x.dtype)
+    y = _rows16(y, "y", (T, N), x.dtype)
+    for name, t in (("a", a), ("b", b)):  # (a pool of adapters is not copied for a call)
+        slot, row = _strides(t, 2)
+        if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or slot % 8 or row % 8 or (t.shape[1] > 1 and row < t.shape[2])):
+            raise ValueError(f"the rows of {name} must be contiguous and 16-byte aligned")
+    if adapters.dim() != 1 or adapters.dtype != torch.int32 or (query_start is not None and query_start.dtype != torch.int32):
+        raise TypeError("adapters and query_start must be int32")
+    seqs = adapters.shape[0]
+    if query_start is None:
+        if seqs != T:
+            raise ValueError(f"without query_start every request has one row: {T} rows, {seqs} requests")
+    elif query_start.dim() != 1 or query_start.shape[0] != seqs + 1:
+        raise ValueError("query_start must be [requests + 1]")
+    else:
+        query_start = query_start.contiguous()
+    adapters = adapters.contiguous()
+    if scales is not None:
+        if scales.shape != (S,) or scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 [{S}]")
+        scales = scales.contiguous()
+    nbytes = L.load().fmsmo_lora_workspace_bytes(T, seqs, int(query_start is not None), r, K)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
+    (a_slot, a_row), (b_slot, b_row) = _strides(a, 2), _strides(b, 2)
+    with _dev(x):
+        L.call("fmsmo_lora_add", _DT[x.dtype], x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), out.data_ptr(), _ld(out), a.data_ptr(), a_slot,
+               a_row or K, b.data_ptr(), b_slot, b_row or r, S, r, adapters.data_ptr(), _ptr(query_start), seqs, _ptr(scales), T, N, K,
+               ws.data_ptr(), nbytes, _stream(x))
+
+
+def _moe_few_tokens_impl(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, out):
+    _same_gpu(a, a_scale, logits, w13, w13_scale, w2, w2_scale, out)
+    if a.dtype not in _CODES or w13.dtype != a.dtype or w2.dtype != a.dtype:
+        raise TypeError(f"a, w13 and w2 must all be int8 or all float8_e4m3fn, got {a.dtype}, {w13.dtype} and {w2.dtype}")
+    if a.dim() != 2 or w13.dim() != 3 or w2.dim() != 3 or w13.shape[1] % 2:
+        raise ValueError("a must be [T, K], w13 [E, 2 I, K] and w2 [E, K, I]")
+    T, K = a.shape
+    E, I = w13.shape[0], w13.shape[1] // 2
+    if w13.shape[2] != K or w2.shape != (E, K, I):
+        raise ValueError(f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not fit a {tuple(a.shape)}")
+    if K % 16 or I % 16 or min(K, I) < 16 or max(K, I) >= 1 << 20:
+        raise ValueError(f"K and I must be multiples of 16 below 2^20, got {K} and {I}")
+    if not 1 <= E <= 512 or not 1 <= top_k <= min(E, 16):
+        raise ValueError(f"top_k must be 1 to 16 of up to 512 experts, got {top_k} of {E}")
+    for name, t in (("w13", w13), ("w2", w2)):  # (weights are not copied for a call)
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+    for name, t, shape in (("w13_scale", w13_scale, (E, 2 * I)), ("w2_scale", w2_scale, (E, K))):
+        if t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be contiguous float32 {shape}, 16-byte aligned")
+    if logits.dim() != 2 or logits.shape != (T, E):
+        raise ValueError(f"logits must be {(T, E)}, got {tuple(logits.shape)}")
+    logits_dt = _dt(logits)
+    logits = _rows(logits)
+    a = _rows16(a.view(torch.int8), "a", (T, K), torch.int8, 16)
+    a_scale = _scale_vec(a_scale, T, a.device, "a_scale")
+    nbytes = L.load().fmsmo_moe_few_workspace_bytes(T, E, top_k, K, I)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=a.device)
+    with _dev(a):
+        L.call("fmsmo_moe_few_tokens", _CODES[w13.dtype], a.data_ptr(), _ld(a), a_scale.data_ptr(), a_scale.numel(), logits.data_ptr(), logits_dt,
+               _ld(logits), w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), T, E, top_k, int(renormalize),
+               out.data_ptr(), _DT[out.dtype], _ld(out), K, I, ws.data_ptr(), nbytes, _stream(a))
+
+
+_register(
+    "add_rms_norm_quant",
+    "(Tensor x, Tensor weight, Tensor? residual, float eps, Tensor? scale, Tensor(a!) q, Tensor(b!)? scale_out, Tensor(c!)? residual_out, "
+    "Tensor(d!)? normed) -> ()",
+    lambda *a: _add_rms_norm_quant_impl(*a),
+    lambda *a: None,
+)
+_register(
+    "lora_add",
+    "(Tensor y, Tensor x, Tensor a, Tensor b, Tensor adapters, Tensor? query_start, Tensor? scales, Tensor(a!) out) -> ()",
+    lambda *a: _lora_add_impl(*a),
+    lambda *a: None,
+)
+_register(
+    "moe_few_tokens",
+    "(Tensor a, Tensor a_scale, Tensor logits, Tensor w13, Tensor w13_scale, Tensor w2, Tensor w2_scale, int top_k, bool renormalize, "
+    "Tensor(a!) out) -> ()",
+    lambda *a: _moe_few_tokens_impl(*a),
+    lambda *a: None,
+)
+
+
+def add_rms_norm_quant(x, weight, residual=None, *, eps=1e-6, dtype=torch.int8, scale=None, want_normed=False, residual_out=None):
+    """What stands in front of an 8-bit product, in one launch: h = x + residual, n = h / sqrt(mean(h^2) + eps) * weight, and the codes of n
+    (``dtype`` int8 or float8_e4m3fn) with one scale per token, or with the given ``scale`` (fp32, one element).  x, residual [M, K] fp16 /
+    bf16, weight [K] of x's dtype or fp32.  Returns (q [M, K], scale fp32 [M] or the given one, h in x's dtype or None without a residual,
+    n in x's dtype where ``want_normed`` or None).  h goes to ``residual_out`` (x or residual itself, or memory apart from them) or a new
+    tensor.  A SmoothQuant divisor is divided out of the weight beforehand.  See fmsmo_add_rms_norm_quant."""
+    if not _COMPILING():
+        r = (_H or _host()).add_rms_norm_quant(x, weight, residual, eps, dtype, scale, want_normed, residual_out)
+        if r is not None:
+            return r
+    _need_gpu(x, weight, residual)
+    if x.dim() != 2 or (residual is not None and residual.shape != x.shape):
+        raise ValueError("x and residual must be [tokens, K]")
+    if dtype not in _CODES:
+        raise TypeError(f"codes are int8 or float8_e4m3fn, not {dtype}")
+    if residual_out is not None:
+        if residual is None:
+            raise ValueError("residual_out goes with a residual")
+        _rows_out(residual_out, "residual_out", x.shape, x.dtype)
+    if scale is not None:
+        scale = _as_scale(scale, x.device).detach()
+        if scale.numel() != 1 or scale.dtype != torch.float32:
+            raise ValueError("scale must be one fp32 number")
+        scale = scale.reshape(1)
+    M, K = x.shape
+    q = torch.empty((M, K), dtype=dtype, device=x.device)
+    made = torch.empty((M,), dtype=torch.float32, device=x.device) if scale is None else None
+    normed = torch.empty((M, K), dtype=x.dtype, device=x.device) if want_normed else None
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty((M, K), dtype=x.dtype, device=x.device)
+    args = (x, weight, residual, float(eps), scale, q, made, residual_out, normed)
+    if M == 0 or K == 0:
+        pass
+    elif _eager(*(t for t in args if torch.is_tensor(t))):
+        _add_rms_norm_quant_impl(*args)
+    else:
+        torch.ops.fms_mo_amd.add_rms_norm_quant(*args)
+    return q, made if scale is None else scale, residual_out, normed
+
+
+def lora_add(y, x, a, b, adapters, query_start=None, *, scales=None, out=None):
+    """Low-rank adapters of many requests beside a shared projection: y + scales[s] * b[s] (a[s] x) per row, s = ``adapters[request]``.
+    x [T, K] is what the projection took (in 16 bits), y [T, N] what it gave; a [slots, rank, K] and b [slots, N, rank] a pool of adapters
+    (smaller ranks padded with zeros; views of a larger pool need contiguous rows only), all fp16 or all bf16; adapters int32 [B], -1 for
+    none; query_start int32 [B + 1] as in ``paged_attention`` (None: one row per request); scales fp32 [slots].  Rows without an adapter
+    are y's.  Returns [T, N] in ``out`` (y itself, or memory apart from x and y) or a new tensor.  No gradients.  See fmsmo_lora_add."""
+    if not _COMPILING():
+        r = (_H or _host()).lora_add(y, x, a, b, adapters, query_start, scales, out)
+        if r is not None:
+            return r if out is None else out
+    _need_gpu(y, x)
+    if x.dim() != 2 or y.dim() != 2 or x.shape[0] != y.shape[0]:
+        raise ValueError("x and y must be [tokens, K] and [tokens, N]")
+    if out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    else:
+        _rows_out(out, "out", y.shape, y.dtype)
+    if y.numel() == 0:
+        return out
+    args = (y, x, a, b, adapters, query_start, scales, out)
+    if _eager(*(t for t in args if t is not None)):
+        _lora_add_impl(*args)
+    else:
+        torch.ops.fms_mo_amd.lora_add(*args)
+    return out
+
+
+def moe_few_tokens(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, *, renormalize=True, out_dtype=torch.bfloat16, out=None):
+    """A mixture-of-experts block for up to 64 tokens, from the router's logits to the weighted sum: the ``top_k`` experts of the largest
+    logits (of equal ones the lower index) with their softmax shares (``renormalize``: divided by their sum), gate and up products,
+    silu(gate) * up in 8 bits per token and expert, down products, sum.  a [T, K] int8 or float8_e4m3fn codes with a_scale [T] (as
+    ``add_rms_norm_quant`` and the quantizers make them), logits [T, E], w13 [E, 2 I, K] (gate rows, then up rows) and w2 [E, K, I] of a's dtype with
+    fp32 scales [E, 2 I] and [E, K].  Returns [T, K] in ``out`` or a new tensor of ``out_dtype``.  More tokens: ``grouped_gemm_i8_dq`` on
+    rows sorted by expert.  See fmsmo_moe_few_tokens."""
+    if not _COMPILING():
+        r = (_H or _host()).moe_few_tokens(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, out_dtype, out)
+        if r is not None:
+            return r if out is None else out
+    _need_gpu(a, logits, w13, w2)
+    if a.dim() != 2:
+        raise ValueError("a must be [tokens, K]")
+    T, K = a.shape
+    if T > 64:
+        raise ValueError(f"up to 64 tokens, got {T}: sort the rows by expert and use grouped_gemm_i8_dq")
+    if out is None:
+        if out_dtype not in _DT:
+            raise TypeError(f"unsupported floating dtype {out_dtype}")
+        out = torch.empty((T, K), dtype=out_dtype, device=a.device)
+    else:
+        if out.dtype not in _DT:
+            raise TypeError(f"unsupported floating dtype {out.dtype}")
+        _rows_out(out, "out", a.shape, out.dtype, 1)
+    if T == 0:
+        return out
+    args = (a, _as_scale(a_scale, a.device), logits, w13, w13_scale, w2, w2_scale, int(top_k), bool(renormalize), out)
+    if _eager(*(t for t in args if torch.is_tensor(t))):
+        _moe_few_tokens_impl(*args)
+    else:
+        torch.ops.fms_mo_amd.moe_few_tokens(*args)
+    return out

@@ -912,6 +912,65 @@ int fmsmo_paged_attn(const fmsmo_kv_cache_t* cache, const fmsmo_kv_batch_t* batc
 int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int heads, int dim, int cache_dtype, int64_t seqs, int64_t rows, int64_t max_rows,
                                          int64_t max_keys);
 
+/* ------------------------------------------------------------------------------------------
+ * 9. Around the products of a served decoder layer.  The reference leaves these to the model that its linears are swapped into; the
+ *    codes and scales made and taken here are those of sections 1 and 2.
+ * ------------------------------------------------------------------------------------------ */
+
+/*
+ * What stands in front of an 8-bit product, in one pass over the rows:
+ *   h = x + residual (residual NULL: x),  residual_out = h rounded to dtype        (NULL: not wanted; x or residual itself, or apart)
+ *   n = h / sqrt(mean(h^2) + eps) * weight[k],  normed = n rounded to dtype          (NULL: not wanted; apart from x and residual)
+ *   codes FMSMO_OP_I8:   s = max(max |n|, 1e-5) / 127,   q = rint(n / s)
+ *   codes FMSMO_OP_E4M3: s = max(max |n| / 448, 1e-12),  q = e4m3(n / s)              scale [M] receives s
+ *   with static_scale, scale [1] is read: q = rint(clamp(n / s, +-127)), e4m3(clamp(n / s, +-448)).
+ * Everything is fp32 up to the one rounding of each output; the recipes are those of fmsmo_quant_act_i8_pertoken with the compute dtype
+ * FMSMO_F32 and of fmsmo_quant_act_fp8_pertoken.  dtype FMSMO_F16 or FMSMO_BF16, weight_dtype the same or FMSMO_F32.  A row with a NaN
+ * or an infinity: scale NaN, e4m3 codes NaN, int8 codes not specified.
+ * K and leading dimensions multiples of 8, pointers 16-byte aligned (q: 8).
+ */
+int fmsmo_add_rms_norm_quant(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                             int weight_dtype, float eps, int codes, int static_scale, void* q, int64_t ldq, float* scale,
+                             void* residual_out, int64_t ldo, void* normed, int64_t ldn, int64_t M, int64_t K, fmsmo_stream_t stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   out[t] = y[t] + scales[s] * b[s] (a[s] x[t])          s = adapters[request of row t]
+ * x [rows, K], y and out [rows, N] (out: y itself, or apart from x and y), a [slots, rank, K], b [slots, N, rank], all of dtype FMSMO_F16 or FMSMO_BF16,
+ * with leading dimensions (slot and row strides) in elements; adapters of a smaller rank are padded with zeros.  scales fp32 [slots] or NULL.
+ * Request i has the rows query_start[i] .. query_start[i + 1] - 1 (ascending; query_start NULL: row i alone, and as many rows as requests).
+ * Rows of a request whose number is none of the slots (-1), and rows of no request: out = y.  Starts that descend give results without a
+ * meaning, but nothing outside of the operands is touched.  Sums are fp32; a[s] x is taken as the sum of two 16-bit numbers, the result is rounded once.
+ * rank a multiple of 8 up to 128; K, N, strides multiples of 8, operands 16-byte aligned.  workspace: fmsmo_lora_workspace_bytes(rows, seqs,
+ * query_start != NULL, rank, K) bytes, 16-byte aligned, private to the call until it has finished.
+ */
+int fmsmo_lora_add(int dtype, const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, const void* a, int64_t a_slot,
+                   int64_t a_row, const void* b, int64_t b_slot, int64_t b_row, int64_t slots, int rank, const int32_t* adapters,
+                   const int32_t* query_start, int64_t seqs, const float* scales, int64_t rows, int64_t N, int64_t K, void* workspace,
+                   int64_t workspace_bytes, fmsmo_stream_t stream);
+int64_t fmsmo_lora_workspace_bytes(int64_t rows, int64_t seqs, int ragged, int rank, int64_t K);
+
+/*
+ * A mixture-of-experts block for a few tokens (T <= 64), routing included:
+ *   p = softmax(logits[t]);  S = the `top` experts of the largest logits (of equal ones the lower index);  c_e = p_e / sum_S p (renormalize) or p_e
+ *   g, u = (a[t] . w13[e]^T) * a_scale[t] * w13_scale[e]     rows 0 .. I - 1 (gate) and I .. 2 I - 1 (up) of w13[e]
+ *   h = g / (1 + exp(-g)) * u,  as 8-bit codes per token and expert with the recipe of section 1 in fp32 (as in fmsmo_add_rms_norm_quant)
+ *   y[t] = sum over S of c_e * s * (codes . w2[e]^T) * w2_scale[e]
+ * codes: FMSMO_OP_I8 or FMSMO_OP_E4M3, of a [T, K], w13 [E, 2 I, K] and w2 [E, K, I], which are contiguous; a_scale fp32 [T] or [1],
+ * w13_scale fp32 [E, 2 I], w2_scale fp32 [E, K]; logits [T, E] and y [T, K] fp16, bf16 or fp32, any logits_dtype and y_dtype.
+ * Sums are int32 (int8) or fp32.  An expert whose share of a token is zero is not run for it (a logit of -infinity; a token whose logits all
+ * are has a result of zero).  A NaN among the logits counts as the largest (a negative one as the smallest), and the token's result is NaN
+ * where it is chosen.
+ * E <= 512, top <= 16, K and I multiples of 16 below 2^20, operands and w2_scale 16-byte aligned, lda a multiple of 16.  workspace:
+ * fmsmo_moe_few_workspace_bytes(T, E, top, K, I) bytes, 16-byte aligned, private to the call until it has finished.
+ * More tokens: fmsmo_grouped_gemm_i8_dq.
+ */
+int fmsmo_moe_few_tokens(int codes, const void* a, int64_t lda, const float* a_scale, int64_t a_scale_n, const void* logits, int logits_dtype,
+                         int64_t ldl, const void* w13, const float* w13_scale, const void* w2, const float* w2_scale, int64_t T, int64_t E,
+                         int top, int renormalize, void* y, int y_dtype, int64_t ldy, int64_t K, int64_t I, void* workspace,
+                         int64_t workspace_bytes, fmsmo_stream_t stream);
+int64_t fmsmo_moe_few_workspace_bytes(int64_t T, int64_t E, int top, int64_t K, int64_t I);
+
 #ifdef __cplusplus
 }
 #endif
