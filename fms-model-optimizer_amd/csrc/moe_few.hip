@@ -16,9 +16,6 @@ namespace fmsmo {
 
 constexpr int MOE_TOKENS = 64, MOE_EXPERTS = 512, MOE_TOP = 16;
 
-struct MoeEntry {  // an expert that some token chose
-  int e, off, cnt, pad;
-};
 struct MoeArgs {
   const uint8_t* a;     // [T, K] codes
   const float* a_scale; // [T] or [1]
@@ -31,15 +28,26 @@ struct MoeArgs {
   int64_t lda, ldl, ldy;
   int a_stride, logits_dtype, y_dtype;
   int T, E, top, K, I, renorm;
+  int down_group;   // tokens of a group of the down product, at most
   // workspace
-  int* count;       // [0]: entries, [1]: positions
-  MoeEntry* entry;  // [E]
-  int* token;       // [T top]: of a position
-  float* weight;
-  float* h;         // [T top][I]
+  int* ids;         // [T top] experts of a token, -1: a share of zero
+  float* share;     // [T top]
+  int* count;       // entries
+  uint32_t* entry;  // [MOE_ENTRIES]
+  int* token;       // [T top] of a position
+  float* weight;    // [T top] its share
   float* hs;        // [T top]
+  float* h;         // [T top][I]
   uint8_t* hq;      // [T top][I]
+  uint32_t* tops;   // [T top][I / 8] largest |h| of eight, as integers; NULL: not wanted
 };
+// A group of tokens of one expert: expert, tokens and first position in one number.
+constexpr int MOE_ENTRIES = MOE_EXPERTS + MOE_TOKENS * MOE_TOP / 8;
+__device__ __forceinline__ uint32_t entry_of(int e, int cnt, int off) { return (uint32_t)e | (uint32_t)cnt << 9 | (uint32_t)off << 16; }
+struct MoeGroup {
+  int e, cnt, off;
+};
+__device__ __forceinline__ MoeGroup group_of(uint32_t x) { return MoeGroup{(int)(x & 511u), (int)(x >> 9 & 127u), (int)(x >> 16)}; }
 
 // an order of floats as unsigned integers (both zeros are one number); 0 is none of them
 __device__ __forceinline__ uint32_t order_of(float v) {
@@ -48,105 +56,143 @@ __device__ __forceinline__ uint32_t order_of(float v) {
   return k ? k : 1u;
 }
 
-// One block.  A wave finds a token's experts, eight logits a lane, the largest by the largest; the rest is counting.
-__global__ __launch_bounds__(1024) void moe_route_kernel(MoeArgs a) {
-  constexpr int V = MOE_EXPERTS / 64;
-  __shared__ unsigned long long mask[MOE_EXPERTS];  // tokens of an expert
-  __shared__ int off[MOE_EXPERTS];
-  __shared__ short ids[MOE_TOKENS][MOE_TOP];
-  __shared__ float share[MOE_TOKENS][MOE_TOP];
-  __shared__ int wave_cnt[16], wave_act[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int e = threadIdx.x; e < a.E; e += 1024) mask[e] = 0;
-  __syncthreads();
-  for (int t = wave; t < a.T; t += 16) {
-    uint32_t key[V];
-    float val[V];
+// The choices of token t by one wave, V logits a lane, the largest by the largest: lane s returns the s-th expert and its share.
+template <int V>
+__device__ __forceinline__ void choose(const MoeArgs& a, int t, int& id, float& share) {
+  const int lane = threadIdx.x & 63;
+  uint32_t key[V];
+  float val[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 64 * i;
+    val[i] = scalar_f32(a.logits, a.logits_dtype, t * a.ldl + (e < a.E ? e : 0));
+    key[i] = e < a.E ? order_of(val[i]) : 0u;
+  }
+  float mine = 0.0f;  // lane s keeps the s-th choice
+  id = -1;
+  for (int s = 0; s < a.top; ++s) {
+    uint32_t m = key[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) m = m > key[i] ? m : key[i];
+    m = wave_max_u32(m);
+    int e = 0;
+    float v = 0.0f;
+    bool found = false;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = lane + 64 * i;
-      const bool in = e < a.E;
-      val[i] = in ? scalar_f32(a.logits, a.logits_dtype, t * a.ldl + e) : 0.0f;
-      key[i] = in ? order_of(val[i]) : 0u;
-    }
-    float first = 0.0f, sum = 0.0f, mine = 0.0f;
-    int id = -1;  // lane s keeps the s-th choice
-    for (int s = 0; s < a.top; ++s) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < V; ++i) m = m > key[i] ? m : key[i];
-      m = wave_max_u32(m);
-      int e = 0;
-      bool found = false;
-      float v = 0.0f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const uint64_t at = __ballot(key[i] == m);
-        if (!found && at) {
-          found = true;
-          const int l = __ffsll((unsigned long long)at) - 1;
-          e = l + 64 * i;
-          v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(val[i]), l));
-          if (lane == l) key[i] = 0;
-        }
-      }
-      if (s == 0) first = v;
-      const float p = first == -__builtin_inff() ? 0.0f : expf(v - first);
-      sum += p;
-      if (lane == s) {
-        id = e;
-        mine = p;
+      const uint64_t at = __ballot(key[i] == m);
+      if (!found && at) {
+        found = true;
+        const int l = __ffsll((unsigned long long)at) - 1;
+        e = l + 64 * i;
+        v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(val[i]), l));
+        if (lane == l) key[i] = 0;
       }
     }
-    if (!a.renorm) {
-      sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (lane + 64 * i < a.E && first != -__builtin_inff()) sum += expf(val[i] - first);
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-    }
-    if (lane < a.top) {
-      const float c = mine == 0.0f ? 0.0f : mine / sum;  // (a share of zero: the expert is not run)
-      share[t][lane] = c;
-      ids[t][lane] = (short)(c == 0.0f ? -1 : id);
-      if (c != 0.0f) atomicOr(&mask[id], 1ull << t);
+    if (lane == s) {
+      id = e;
+      mine = v;
     }
   }
-  __syncthreads();
-  const int e = threadIdx.x;
-  const int cnt = e < a.E ? __popcll(mask[e]) : 0;
-  int upto = cnt;
+  const float first = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), 0));
+  const bool some = first != -__builtin_inff();
+  const float p = lane < a.top && some ? expf(mine - first) : 0.0f;
+  float sum = p;
+  if (!a.renorm) {
+    sum = 0.0f;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(upto, d);
-    upto += lane >= d ? o : 0;
+    for (int i = 0; i < V; ++i)
+      if (lane + 64 * i < a.E && some) sum += expf(val[i] - first);
   }
-  const uint64_t act = __ballot(cnt > 0);
-  if (lane == 63) {
-    wave_cnt[wave] = upto;
-    wave_act[wave] = __popcll(act);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  share = p == 0.0f ? 0.0f : p / sum;
+  if (share == 0.0f) id = -1;  // (the expert is not run)
+}
+__device__ __forceinline__ void choose_any(const MoeArgs& a, int t, int& id, float& share) {
+  if (a.E <= 128) choose<2>(a, t, id, share);
+  else choose<MOE_EXPERTS / 64>(a, t, id, share);
+}
+
+// a wave per token
+__global__ __launch_bounds__(256) void moe_route_kernel(MoeArgs a) {
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= a.T) return;
+  int id;
+  float share;
+  choose_any(a, t, id, share);
+  if (lane < a.top) {
+    a.ids[t * a.top + lane] = id;
+    a.share[t * a.top + lane] = share;
+  }
+}
+
+// The choices sorted by expert, made by every block for itself: groups of up to 16 MT tokens and the tokens of the positions.
+struct MoeLists {
+  unsigned long long mask[MOE_EXPERTS];  // tokens of an expert
+  uint32_t entry[MOE_ENTRIES];
+  short off[MOE_EXPERTS], id[MOE_TOKENS * MOE_TOP];
+  uint8_t token[MOE_TOKENS * MOE_TOP];
+  int count;
+};
+// ROUTE: from the logits; else from what the routing kernel left.  Block 0 leaves all of it for the kernels behind.
+template <int NT, int MT, bool ROUTE>
+__device__ __forceinline__ void make_lists(const MoeArgs& a, MoeLists& l) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pairs = a.T * a.top;
+  for (int e = threadIdx.x; e < a.E; e += NT) l.mask[e] = 0;
+  __syncthreads();
+  if constexpr (ROUTE) {
+    for (int t = wave; t < a.T; t += NT / 64) {
+      int id;
+      float share;
+      choose_any(a, t, id, share);
+      if (lane < a.top) {
+        l.id[t * a.top + lane] = (short)id;
+        if (id >= 0) atomicOr(&l.mask[id], 1ull << t);
+        if (blockIdx.x == 0) a.share[t * a.top + lane] = share;
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < pairs; i += NT) {
+      const int id = a.ids[i];
+      l.id[i] = (short)id;
+      if (id >= 0) atomicOr(&l.mask[id], 1ull << (i / a.top));
+    }
   }
   __syncthreads();
-  int before = 0, rank = __popcll(act & ((1ull << lane) - 1));
-  for (int w = 0; w < wave; ++w) {
-    before += wave_cnt[w];
-    rank += wave_act[w];
-  }
-  if (e < a.E) off[e] = before + upto - cnt;
-  if (cnt > 0) a.entry[rank] = MoeEntry{e, before + upto - cnt, cnt, 0};
-  if (threadIdx.x == 1023) {
-    a.count[0] = rank + (cnt > 0);
-    a.count[1] = before + upto;
+  // groups and positions, by one wave; those of the down product by another one of block 0
+  const int size = wave == 0 ? 16 * MT : a.down_group;
+  if (wave == 0 || (wave == 1 && blockIdx.x == 0)) {
+    int pos = 0, groups = 0;
+    for (int e0 = 0; e0 < a.E; e0 += 64) {
+      const int e = e0 + lane, cnt = e < a.E ? __popcll(l.mask[e]) : 0, mine = (cnt + size - 1) / size;
+      int both = cnt | mine << 16;  // both sums at once (up to 1024 and 640)
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(both, d);
+        both += lane >= d ? o : 0;
+      }
+      const int off = pos + (both & 0xffff) - cnt, at = groups + (both >> 16) - mine;
+      if (wave == 0 && e < a.E) l.off[e] = (short)off;
+      for (int i = 0; i < mine; ++i) (wave ? a.entry : l.entry)[at + i] = entry_of(e, min(cnt - size * i, size), off + size * i);
+      const int total = __builtin_amdgcn_readlane(both, 63);
+      pos += total & 0xffff;
+      groups += total >> 16;
+    }
+    if (lane == 0) (wave ? a.count[0] : l.count) = groups;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.T * a.top; i += 1024) {
-    const int t = i / a.top, s = i % a.top, id = ids[t][s];
+  for (int i = threadIdx.x; i < pairs; i += NT) {
+    const int id = l.id[i], t = i / a.top;
     if (id < 0) continue;
-    const int pos = off[id] + __popcll(mask[id] & ((1ull << t) - 1));
-    a.token[pos] = t;
-    a.weight[pos] = share[t][s];
+    const int pos = l.off[id] + __popcll(l.mask[id] & ((1ull << t) - 1));
+    l.token[pos] = (uint8_t)t;
+    if (blockIdx.x == 0) {
+      a.token[pos] = t;
+      a.weight[pos] = a.share[i];
+    }
   }
+  __syncthreads();
 }
 
 // ------------------------------------------------------------------ streaming weights
@@ -184,61 +230,96 @@ __device__ __forceinline__ v4i stream16(const uint8_t* p, int64_t off, bool ther
   if (there) v = __builtin_nontemporal_load((const v4i*)(p + off));
   return v;
 }
+__device__ __forceinline__ v4i load_or_zero(const uint8_t* p, int64_t off, bool there) {
+  v4i v = {0, 0, 0, 0};
+  if (there) v = *(const v4i*)(p + off);
+  return v;
+}
 
-// h of the positions.  A unit: eight gate rows and the eight up rows that belong to them, over all of K, for one expert: the 16 rows of the
-// product.  KS = 1: each wave takes units of its own, one behind the other, D steps of 128 bytes a row on their way; KS = 4: the
-// four waves of a block share a unit's K.
-template <int OP, int MT, int KS, int D>
-__global__ __launch_bounds__(256) void moe_up_kernel(MoeArgs a) {
+// h of the positions.  A unit: eight gate rows and the eight up rows that belong to them, for one group of tokens: the 16 rows of the
+// product.  The four waves of a block share its K, every fourth step of 128 bytes each, D steps on their way, those of the next unit among
+// them; the waves' sums meet in shared memory, one barrier a unit, and a wave in turn finishes it.
+template <int OP, int MT, int D, bool ROUTE>
+__global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void moe_up_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
+  __shared__ MoeLists lists;
   __shared__ __attribute__((aligned(16))) uint8_t stage[4][2048];
-  __shared__ __attribute__((aligned(16))) Acc part[KS > 1 ? 3 : 1][MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ __attribute__((aligned(16))) Acc part[2][4][MT][64];
+  make_lists<256, MT, ROUTE>(a, lists);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4, drow = lane >> 3, dpos = lane & 7;
-  const int groups = a.I / 8, units = a.count[0] * groups, steps = (a.K + 127) / 128;
-  const int stride = KS == 1 ? gridDim.x * 4 : gridDim.x, first = KS == 1 ? wave * gridDim.x + blockIdx.x : blockIdx.x;
-  const int s0 = KS == 1 ? 0 : wave, ds = KS == 1 ? 1 : 4;
+  const int groups = a.I / 8, units = lists.count * groups;
+  const int steps = ((a.K + 511) / 512 + D - 1) / D * D;  // of a wave
   uint8_t* st = stage[wave];
   const int rr = r & 7;
-  for (int u = first; u < units; u += stride) {
-    const int en = u / groups, gi = u - en * groups;
-    const MoeEntry x = a.entry[en];
-    const int e = uniform(x.e), off = uniform(x.off), cnt = uniform(x.cnt);
-    const uint8_t* wg = a.w13 + ((int64_t)e * 2 * a.I + gi * 8 + drow) * a.K;
-    const uint8_t* wu = wg + (int64_t)a.I * a.K;
-    const uint8_t* xp[MT];
-    bool xv[MT];
-    int tok[MT];
+  struct Unit {
+    const uint8_t* w;  // the lane's gate row
+    const uint8_t* x[MT];
+    MoeGroup m;
+    int gi;
+    bool xv[MT], there;
+  };
+  const auto unit_of = [&](int u) {
+    Unit q;
+    q.there = u < units;
+    const int en = q.there ? u / groups : 0;
+    q.gi = q.there ? u - en * groups : 0;
+    q.m = group_of(uniform((int)lists.entry[en]));
+    if (!q.there) q.m.cnt = 0;
+    q.w = a.w13 + ((int64_t)q.m.e * 2 * a.I + q.gi * 8 + drow) * a.K + dpos * 16;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-      xv[j] = 16 * j + r < cnt;
-      tok[j] = xv[j] ? a.token[off + 16 * j + r] : 0;
-      xp[j] = a.a + tok[j] * a.lda;
+      q.xv[j] = 16 * j + r < q.m.cnt;
+      q.x[j] = a.a + (q.xv[j] ? (int)lists.token[q.m.off + 16 * j + r] : 0) * a.lda + g * 16;
     }
-    v4i wb[D][2], xb[D][MT][2];
-    const auto fetch = [&](int s, int d) {
-      const int k = s * 128;
-      const bool in = k + dpos * 16 < a.K;
-      wb[d][0] = stream16(wg, k + dpos * 16, in);
-      wb[d][1] = stream16(wu, k + dpos * 16, in);
+    return q;
+  };
+  const int64_t up = (int64_t)a.I * a.K;
+  v4i wb[D][2], xb[D][MT][2];
+  const auto fetch = [&](const Unit& q, int s, int d) {
+    const int k = (s * 4 + wave) * 128;
+    if (!q.there || k >= a.K) {  // (uniform)
+      wb[d][0] = wb[d][1] = v4i{0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        if (16 * j >= cnt) break;
-        xb[d][j][0] = xv[j] && k + g * 16 < a.K ? *(const v4i*)(xp[j] + k + g * 16) : v4i{0, 0, 0, 0};
-        xb[d][j][1] = xv[j] && k + 64 + g * 16 < a.K ? *(const v4i*)(xp[j] + k + 64 + g * 16) : v4i{0, 0, 0, 0};
+      for (int j = 0; j < MT; ++j) xb[d][j][0] = xb[d][j][1] = v4i{0, 0, 0, 0};
+      return;
+    }
+    const bool in = k + dpos * 16 < a.K;
+    wb[d][0] = stream16(q.w, k, in);
+    wb[d][1] = stream16(q.w + up, k, in);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      if (16 * j >= q.m.cnt) break;
+      xb[d][j][0] = load_or_zero(q.x[j], k, q.xv[j] && k + g * 16 < a.K);
+      xb[d][j][1] = load_or_zero(q.x[j], k + 64, q.xv[j] && k + 64 + g * 16 < a.K);
+    }
+  };
+  if ((int)blockIdx.x >= units) return;
+  Unit cur = unit_of(blockIdx.x);
+#pragma unroll
+  for (int d = 0; d < D; ++d) fetch(cur, d, d);
+  int turn = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x, ++turn) {
+    const Unit next = unit_of(u + gridDim.x);
+    const bool finish = (turn & 3) == wave;
+    float sg[4], su[4], as[MT];
+    if (finish) {  // asked for ahead of the products
+      const float* sc = a.s13 + (int64_t)cur.m.e * 2 * a.I + cur.gi * 8 + 4 * (g & 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sg[i] = sc[i];
+        su[i] = sc[a.I + i];
       }
-    };
 #pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (s0 + d * ds < steps) fetch(s0 + d * ds, d);
+      for (int j = 0; j < MT; ++j) as[j] = a.a_scale[cur.xv[j] ? (int)lists.token[cur.m.off + 16 * j + r] * a.a_stride : 0];
+    }
     Acc acc[MT];
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[j] = Acc{0, 0, 0, 0};
-    for (int s = s0; s < steps; s += D * ds) {
+    for (int s = 0; s < steps; s += D) {
+      const bool last = s + D >= steps;
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        const int at = s + d * ds;
-        if (at >= steps) break;
         *(v4i*)(st + drow * 128 + ((dpos ^ drow) * 16)) = wb[d][0];
         *(v4i*)(st + (8 + drow) * 128 + ((dpos ^ drow) * 16)) = wb[d][1];
         __builtin_amdgcn_wave_barrier();
@@ -247,49 +328,44 @@ __global__ __launch_bounds__(256) void moe_up_kernel(MoeArgs a) {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          if (16 * j >= cnt) break;
+          if (16 * j >= cur.m.cnt) break;
           moe_mfma<OP>(acc[j], w0, w1, xb[d][j][0], xb[d][j][1]);
         }
-        if (at + D * ds < steps) fetch(at + D * ds, d);
+        if (last) fetch(next, d, d);
+        else fetch(cur, s + D + d, d);
       }
     }
-    if constexpr (KS > 1) {
-      if (wave) {
+    Acc(*mine)[MT][64] = part[turn & 1];
 #pragma unroll
-        for (int j = 0; j < MT; ++j) part[wave - 1][j][lane] = acc[j];
+    for (int j = 0; j < MT; ++j) mine[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (finish) {
+      // lane (r, g): column r, rows 4 g .. + 3: gate rows in the lower half of the wave, their up rows 32 lanes on
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        if (16 * j >= cur.m.cnt) break;
+        const Acc sum = (mine[0][j][lane] + mine[1][j][lane]) + (mine[2][j][lane] + mine[3][j][lane]);
+        v4f h;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float own = (float)sum[i];
+          const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(own), __float_as_uint(own), false, false);
+          const float gate = __uint_as_float(both[0]) * (as[j] * sg[i]), upv = __uint_as_float(both[1]) * (as[j] * su[i]);
+          h[i] = gate / (1.0f + expf(-gate)) * upv;
+          const uint32_t m = __float_as_uint(h[i]) & 0x7fffffffu;  // (as integers: a NaN is larger than everything)
+          top = top > m ? top : m;
+        }
+        const int pos = cur.m.off + 16 * j + r;
+        if (cur.xv[j] && g < 2) *(v4f*)(a.h + (int64_t)pos * a.I + cur.gi * 8 + 4 * g) = h;
+        if (a.tops) {
+          const auto o = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+          top = o[0] > o[1] ? o[0] : o[1];
+          if (cur.xv[j] && g == 0) a.tops[(int64_t)pos * groups + cur.gi] = top;
+        }
       }
-      __syncthreads();
-      if (wave == 0) {
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-          for (int w = 0; w < 3; ++w) acc[j] += part[w][j][lane];
-      }
-      __syncthreads();
-      if (wave) continue;
     }
-    // lane (r, g): column r, rows 4 g .. + 3: gate rows in the lower half of the wave, their up rows 32 lanes on
-    const float* sc = a.s13 + (int64_t)e * 2 * a.I + gi * 8 + 4 * (g & 1);
-    float sg[4], su[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sg[i] = sc[i];
-      su[i] = sc[a.I + i];
-    }
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      if (16 * j >= cnt) break;
-      const float as = a.a_scale[tok[j] * a.a_stride];
-      v4f h;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float own = (float)acc[j][i];
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(own), __float_as_uint(own), false, false);
-        const float gate = __uint_as_float(both[0]) * (as * sg[i]), up = __uint_as_float(both[1]) * (as * su[i]);
-        h[i] = gate / (1.0f + expf(-gate)) * up;
-      }
-      if (xv[j] && g < 2) *(v4f*)(a.h + (int64_t)(off + 16 * j + r) * a.I + gi * 8 + 4 * g) = h;
-    }
+    cur = next;
   }
 }
 
@@ -319,21 +395,18 @@ __device__ __forceinline__ uint32_t moe_codes(v4f h, float s) {
     return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u), __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), 0x05040100u);
   }
 }
-// a block per position
+// 1024 elements of a position a block
+constexpr int MOE_QUANT = 1024;
 template <int OP>
 __global__ __launch_bounds__(256) void moe_quant_kernel(MoeArgs a) {
   __shared__ uint32_t tops[4];
-  const int pos = blockIdx.x;
-  if (pos >= a.count[1]) return;
-  const v4f* h = (const v4f*)(a.h + (int64_t)pos * a.I);
+  const int pos = blockIdx.x, groups = a.I / 8, i = blockIdx.y * (MOE_QUANT / 4) + threadIdx.x;
+  const bool in = 4 * i < a.I;
+  const v4f v = in ? ((const v4f*)(a.h + (int64_t)pos * a.I))[i] : v4f{0, 0, 0, 0};
   uint32_t top = 0;
-  for (int i = threadIdx.x; i < a.I / 4; i += 256) {
-    const v4f v = h[i];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t u = __float_as_uint(v[k]) & 0x7fffffffu;  // (as integers: a NaN is larger than everything)
-      top = top > u ? top : u;
-    }
+  for (int k = threadIdx.x; k < groups; k += 256) {
+    const uint32_t u = a.tops[(int64_t)pos * groups + k];
+    top = top > u ? top : u;
   }
   top = wave_max_u32(top);
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
@@ -341,97 +414,173 @@ __global__ __launch_bounds__(256) void moe_quant_kernel(MoeArgs a) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) top = top > tops[w] ? top : tops[w];
   const float s = moe_scale<OP>(top);
-  if (threadIdx.x == 0) a.hs[pos] = s;
-  for (int i = threadIdx.x; i < a.I / 4; i += 256) ((uint32_t*)(a.hq + (int64_t)pos * a.I))[i] = moe_codes<OP>(h[i], s);
+  if (threadIdx.x == 0 && blockIdx.y == 0) a.hs[pos] = s;
+  if (in) ((uint32_t*)(a.hq + (int64_t)pos * a.I))[i] = moe_codes<OP>(v, s);
 }
 
-// y.  A block owns ROWS outputs and goes through all chosen experts: their steps of 128 bytes in a row, cut into equal parts for the waves;
-// at the end of an expert a wave adds its products, with their scales and shares, to sums of its own, and the waves' sums are added in their order.
-template <int OP, int MT, int ROWS, int D>
-__global__ __launch_bounds__(512) void moe_down_kernel(MoeArgs a) {
+// y.  A block owns ROWS outputs and goes through all groups of tokens: their steps of 128 bytes one behind the other, cut into equal parts
+// for the waves, D steps on their way; at the end of a group a wave adds its products, with their scales and shares, to sums of its own, and the
+// waves' sums are added in their order.  ROWS = 8, groups of up to eight tokens: a product takes two steps, the first with its upper eight rows and
+// left eight columns, the second with the others, and the two blocks on its diagonal are added.  QUANT: few positions, whose codes every block makes for itself in shared memory.
+// Shared memory: sums [NW][T][ROWS], shares and scales [T top], entries, tokens; QUANT: codes.
+template <int OP, int MT, int ROWS, int NW, int D, bool QUANT>
+__global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
-  constexpr int NW = 8, L = ROWS / 8;
-  __shared__ __attribute__((aligned(16))) uint8_t stage[NW][ROWS * 128];
-  __shared__ __attribute__((aligned(16))) float sums[NW][16 * MT][ROWS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int NT = NW * 64;
+  constexpr bool PAIR = ROWS == 8;  // two steps a product
+  static_assert(!PAIR || MT == 1, "");
+  constexpr int STEP = PAIR ? 256 : 128;
+  __shared__ __attribute__((aligned(16))) uint8_t stage[NW][2048];
+  __shared__ uint32_t entry[MOE_ENTRIES];
+  __shared__ uint8_t token[MOE_TOKENS * MOE_TOP];
+  __shared__ float share[MOE_TOKENS * MOE_TOP];
+  extern __shared__ __attribute__((aligned(16))) char dyn[];
+  float* sums = (float*)dyn;  // [NW][T][ROWS]
+  uint8_t* codes = (uint8_t*)(sums + NW * a.T * ROWS);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4, drow = lane >> 3, dpos = lane & 7;
-  const int n0 = blockIdx.x * ROWS, steps = (a.I + 127) / 128, all = a.count[0] * steps;
-  for (int i = threadIdx.x; i < NW * 16 * MT * ROWS; i += 512) (&sums[0][0][0])[i] = 0.0f;
+  const int n0 = blockIdx.x * ROWS, steps = (a.I + STEP - 1) / STEP, pairs = a.T * a.top;
+  const int count = a.count[0], all = count * steps;
+  for (int i = threadIdx.x; i < count; i += NT) entry[i] = a.entry[i];
+  // (positions that no pair took hold what was there before: they are not in any group)
+  for (int i = threadIdx.x; i < pairs; i += NT) {
+    token[i] = (uint8_t)a.token[i];
+    share[i] = a.weight[i];
+    if (!QUANT) share[i] *= a.hs[i];
+  }
+  for (int i = threadIdx.x; i < NW * a.T * ROWS; i += NT) sums[i] = 0.0f;
   __syncthreads();
+  if constexpr (QUANT) {
+    const MoeGroup m = count ? group_of(entry[count - 1]) : MoeGroup{0, 0, 0};
+    for (int pos = wave; pos < m.off + m.cnt; pos += NW) {
+      const v4f* h = (const v4f*)(a.h + (int64_t)pos * a.I);
+      uint32_t top = 0;
+      for (int i = lane; i < a.I / 4; i += 64) {
+        const v4f v = h[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t u = __float_as_uint(v[k]) & 0x7fffffffu;
+          top = top > u ? top : u;
+        }
+      }
+      const float s = moe_scale<OP>(wave_max_u32(top));
+      if (lane == 0) share[pos] *= s;
+      for (int i = lane; i < a.I / 4; i += 64) ((uint32_t*)(codes + pos * a.I))[i] = moe_codes<OP>(h[i], s);
+    }
+    __syncthreads();
+  }
   const int from = (int)((int64_t)wave * all / NW), to = (int)((int64_t)(wave + 1) * all / NW);
   uint8_t* st = stage[wave];
   const int rr = r & 7;
-  int at = from;
-  while (at < to) {
-    const int en = at / steps, s_lo = at - en * steps, s_hi = min(steps, s_lo + to - at);
-    const MoeEntry x = a.entry[en];
-    const int e = uniform(x.e), off = uniform(x.off), cnt = uniform(x.cnt);
-    const uint8_t* wp = a.w2 + ((int64_t)e * a.K + n0 + drow) * a.I;
-    const uint8_t* xp = a.hq + (int64_t)(off + r) * a.I;
-    v4i wb[D][L], xb[D][MT][2];
-    const auto fetch = [&](int s, int d) {
-      const int k = s * 128;
-#pragma unroll
-      for (int l = 0; l < L; ++l) wb[d][l] = stream16(wp + (int64_t)l * 8 * a.I, k + dpos * 16, k + dpos * 16 < a.I);
+  int le = steps ? from / steps : 0, ls = from - le * steps, ce = le, cs = ls;  // what is loaded and what is multiplied next: group and step
+  MoeGroup lm = group_of(entry[0]), cm = lm;
+  const uint8_t* w = nullptr;
+  const uint8_t* x = nullptr;
+  // column r of a product: token col of tile j, and in a pair the step's half
+  const int col = PAIR ? rr : r, half = PAIR ? 128 * (r >> 3) : 0;
+  const auto load_from = [&] {
+    lm = group_of(uniform((int)entry[le]));
+    w = a.w2 + ((int64_t)lm.e * a.K + n0 + drow) * a.I + dpos * 16;
+    x = a.hq + (int64_t)(lm.off + col) * a.I + half + g * 16;
+  };
+  v4i wb[D][2], xb[QUANT ? 1 : D][MT][2];
+  const auto fetch = [&](int d) {
+    const int k = ls * STEP;
+    wb[d][0] = stream16(w, k, k + dpos * 16 < a.I);
+    wb[d][1] = PAIR ? stream16(w, k + 128, k + 128 + dpos * 16 < a.I) : stream16(w + (int64_t)8 * a.I, k, k + dpos * 16 < a.I);
+    if constexpr (!QUANT) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        if (16 * j >= cnt) break;
-        const bool v = 16 * j + r < cnt;
-        xb[d][j][0] = v && k + g * 16 < a.I ? *(const v4i*)(xp + (int64_t)16 * j * a.I + k + g * 16) : v4i{0, 0, 0, 0};
-        xb[d][j][1] = v && k + 64 + g * 16 < a.I ? *(const v4i*)(xp + (int64_t)16 * j * a.I + k + 64 + g * 16) : v4i{0, 0, 0, 0};
+        if (16 * j >= lm.cnt) break;
+        const bool v = 16 * j + col < lm.cnt;
+        xb[d][j][0] = load_or_zero(x + (int64_t)16 * j * a.I, k, v && k + half + g * 16 < a.I);
+        xb[d][j][1] = load_or_zero(x + (int64_t)16 * j * a.I, k + 64, v && k + half + 64 + g * 16 < a.I);
       }
-    };
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (s_lo + d < s_hi) fetch(s_lo + d, d);
-    Acc acc[MT];
+    }
+    if (++ls == steps) {
+      ls = 0;
+      ++le;
+      if (le < count) load_from();
+    }
+  };
+  Acc acc[MT];
+  v4f sc = {0, 0, 0, 0};
+  const int ng = PAIR ? g & 1 : g;  // the four outputs of this lane
+  const auto begin = [&] {  // a group's first step: its scales are asked for
+    cm = group_of(uniform((int)entry[ce]));
+    sc = *(const v4f*)(a.s2 + (int64_t)cm.e * a.K + n0 + 4 * ng);
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[j] = Acc{0, 0, 0, 0};
-    for (int s = s_lo; s < s_hi; s += D) {
+  };
+  const auto end = [&] {
+    if constexpr (PAIR) {  // rows 8 .. 15 of columns 8 .. 15 belong to rows 0 .. 7 of columns 0 .. 7: 32 + 8 lanes on
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[0][i] += __shfl(acc[0][i], (lane + 40) & 63);
+      if (lane >= 32) return;
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      if (16 * j + r >= cm.cnt) break;
+      const int pos = cm.off + 16 * j + r;
+      const float c = share[pos];
+      v4f* sum = (v4f*)(sums + (wave * a.T + token[pos]) * ROWS + 4 * ng);
+      v4f v = *sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __fmaf_rn((float)acc[j][i], c * sc[i], v[i]);
+      *sum = v;
+    }
+  };
+  if (from < to) {
+    load_from();
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (from + d < to) fetch(d);
+    begin();
+    for (int f = from; f < to; f += D) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        if (s + d >= s_hi) break;
-#pragma unroll
-        for (int l = 0; l < L; ++l) *(v4i*)(st + (8 * l + drow) * 128 + ((dpos ^ drow) * 16)) = wb[d][l];
+        if (f + d >= to) break;
+        *(v4i*)(st + drow * 128 + ((dpos ^ drow) * 16)) = wb[d][0];
+        *(v4i*)(st + (8 + drow) * 128 + ((dpos ^ drow) * 16)) = wb[d][1];
         __builtin_amdgcn_wave_barrier();
-        const int row = ROWS == 16 ? r : rr;  // (eight rows: twice)
-        const v4i w0 = *(const v4i*)(st + row * 128 + ((g ^ rr) * 16));
-        const v4i w1 = *(const v4i*)(st + row * 128 + (((4 + g) ^ rr) * 16));
+        const v4i w0 = *(const v4i*)(st + r * 128 + ((g ^ rr) * 16));
+        const v4i w1 = *(const v4i*)(st + r * 128 + (((4 + g) ^ rr) * 16));
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          if (16 * j >= cnt) break;
-          moe_mfma<OP>(acc[j], w0, w1, xb[d][j][0], xb[d][j][1]);
+          if (16 * j >= cm.cnt) break;
+          v4i x0, x1;
+          if constexpr (QUANT) {
+            const int k = cs * STEP + half + g * 16;
+            const bool v = 16 * j + col < cm.cnt;
+            x0 = x1 = v4i{0, 0, 0, 0};
+            if (v && k < a.I) x0 = *(const v4i*)(codes + (cm.off + 16 * j + col) * a.I + k);
+            if (v && k + 64 < a.I) x1 = *(const v4i*)(codes + (cm.off + 16 * j + col) * a.I + k + 64);
+          } else {
+            x0 = xb[d][j][0];
+            x1 = xb[d][j][1];
+          }
+          moe_mfma<OP>(acc[j], w0, w1, x0, x1);
         }
-        if (s + d + D < s_hi) fetch(s + d + D, d);
+        if (f + d + D < to) fetch(d);
+        if (++cs == steps || f + d + 1 == to) {
+          end();
+          cs = 0;
+          ++ce;
+          if (f + d + 1 < to) begin();
+        }
       }
     }
-    if (ROWS == 16 || g < 2) {
-      const v4f sc = *(const v4f*)(a.s2 + (int64_t)e * a.K + n0 + 4 * g);
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        if (16 * j + r >= cnt) break;
-        const int pos = off + 16 * j + r;
-        const float c = a.weight[pos] * a.hs[pos];
-        v4f* sum = (v4f*)&sums[wave][a.token[pos]][4 * g];
-        v4f v = *sum;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __fmaf_rn((float)acc[j][i], c * sc[i], v[i]);
-        *sum = v;
-      }
-    }
-    at += s_hi - s_lo;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.T * ROWS; i += 512) {
-    const int t = i / ROWS, n = i % ROWS;
-    float v = sums[0][t][n];
+  for (int i = threadIdx.x; i < a.T * ROWS; i += NT) {
+    float v = sums[i];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) v += sums[w][t][n];
-    const int64_t to_at = t * a.ldy + n0 + n;
-    if (a.y_dtype == FMSMO_F16) ((u16*)a.y)[to_at] = f32_to_f16(v);
-    else if (a.y_dtype == FMSMO_BF16) ((u16*)a.y)[to_at] = f32_to_bf16(v);
-    else ((float*)a.y)[to_at] = v;
+    for (int w = 1; w < NW; ++w) v += sums[w * a.T * ROWS + i];
+    const int64_t at = i / ROWS * a.ldy + n0 + i % ROWS;
+    if (a.y_dtype == FMSMO_F16) ((u16*)a.y)[at] = f32_to_f16(v);
+    else if (a.y_dtype == FMSMO_BF16) ((u16*)a.y)[at] = f32_to_bf16(v);
+    else ((float*)a.y)[at] = v;
   }
 }
 
@@ -445,37 +594,64 @@ static bool moe_sizes(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   return T >= 0 && T <= MOE_TOKENS && E >= 1 && E <= MOE_EXPERTS && top >= 1 && top <= MOE_TOP && top <= E && K >= 16 && I >= 16 && K % 16 == 0 &&
          I % 16 == 0 && K < 1 << 20 && I < 1 << 20;
 }
-// bytes up to each piece of the workspace: counts, entries, tokens, shares, scales, h, codes
+// bytes up to each piece of the workspace
 struct MoeSpace {
-  int64_t entry, token, weight, hs, h, hq, all;
+  int64_t ids, share, entry, token, weight, hs, h, hq, tops, all;
 };
-static MoeSpace moe_space(int64_t T, int64_t E, int top, int64_t I) {
+static MoeSpace moe_space(int64_t T, int top, int64_t I) {
   const int64_t P = T * top, p16 = (P + 3) / 4 * 16;
   MoeSpace s;
-  s.entry = 16;
-  s.token = s.entry + 16 * E;
+  s.ids = 16;
+  s.share = s.ids + p16;
+  s.entry = s.share + p16;
+  s.token = s.entry + 4 * MOE_ENTRIES;
   s.weight = s.token + p16;
   s.hs = s.weight + p16;
   s.h = s.hs + p16;
   s.hq = s.h + 4 * P * I;
-  s.all = s.hq + P * I;
+  s.tops = s.hq + P * I;
+  s.all = s.tops + P * I / 2;
   return s;
 }
 
 extern "C" int64_t fmsmo_moe_few_workspace_bytes(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
-  return moe_sizes(T, E, top, K, I) && T ? moe_space(T, E, top, I).all : 0;
+  return moe_sizes(T, E, top, K, I) && T ? moe_space(T, top, I).all : 0;
 }
 
+template <int OP, int MT, int ROWS, bool QUANT>
+static void run_down(const MoeArgs& a, hipStream_t s) {
+  constexpr int NW = 8, D = 4;
+  const size_t lds = (size_t)NW * a.T * ROWS * 4 + (QUANT ? (size_t)a.T * a.top * a.I : 0);
+  hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, QUANT>), dim3((unsigned)(a.K / ROWS)), dim3(NW * 64), lds, s, a);
+}
 template <int OP, int MT>
-static void run_moe(const MoeArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(moe_route_kernel, dim3(1), dim3(1024), 0, s, a);
-  // experts that may be chosen, at most; a wave to a unit where that gives every SIMD two of them
-  const int64_t units = (int64_t)std::min(a.E, a.T * a.top) * (a.I / 8);
-  if (units >= 2048) hipLaunchKernelGGL((moe_up_kernel<OP, MT, 1, 4>), dim3(512), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((moe_up_kernel<OP, MT, 4, 4>), dim3((unsigned)std::min<int64_t>(units, 1024)), dim3(256), 0, s, a);
-  hipLaunchKernelGGL((moe_quant_kernel<OP>), dim3((unsigned)(a.T * a.top)), dim3(256), 0, s, a);
-  if (a.K / 16 >= 256) hipLaunchKernelGGL((moe_down_kernel<OP, MT, 16, 4>), dim3((unsigned)(a.K / 16)), dim3(512), 0, s, a);
-  else hipLaunchKernelGGL((moe_down_kernel<OP, MT, 8, 4>), dim3((unsigned)(a.K / 8)), dim3(512), 0, s, a);
+static void run_moe(MoeArgs a, hipStream_t s) {
+  constexpr int QUANT_MOST = 8192;
+  const bool quant = MT == 1 && a.T * a.top * a.I <= QUANT_MOST, narrow = MT == 1 && a.K / 16 < 256;
+  if (quant) a.tops = nullptr;
+  a.down_group = narrow ? 8 : 16 * MT;
+  // groups of tokens, at most
+  const int64_t units = (int64_t)std::min(MT == 1 ? a.E + a.T * a.top / 16 : a.E, a.T * a.top) * (a.I / 8);
+  const dim3 grid((unsigned)std::min<int64_t>(units, MT == 1 ? 768 : 512));
+  if (a.T <= 8) {
+    if constexpr (MT == 1) hipLaunchKernelGGL((moe_up_kernel<OP, 1, 4, true>), grid, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((moe_up_kernel<OP, MT, MT == 1 ? 4 : 2, false>), grid, dim3(256), 0, s, a);
+  }
+  if (!quant) hipLaunchKernelGGL((moe_quant_kernel<OP>), dim3((unsigned)(a.T * a.top), (unsigned)div_up(a.I, MOE_QUANT)), dim3(256), 0, s, a);
+  if constexpr (MT == 1) {
+    if (narrow) {
+      if (quant) run_down<OP, 1, 8, true>(a, s);
+      else run_down<OP, 1, 8, false>(a, s);
+    } else if (quant) {
+      run_down<OP, 1, 16, true>(a, s);
+    } else {
+      run_down<OP, 1, 16, false>(a, s);
+    }
+  } else {
+    run_down<OP, MT, 16, false>(a, s);
+  }
 }
 
 extern "C" int fmsmo_moe_few_tokens(int codes, const void* a, int64_t lda, const float* a_scale, int64_t a_scale_n, const void* logits,
@@ -491,16 +667,16 @@ extern "C" int fmsmo_moe_few_tokens(int codes, const void* a, int64_t lda, const
   if ((a_scale_n != 1 && a_scale_n != T) || (T > 1 && (lda < K || ldl < E || ldy < K))) return FMSMO_ERR_SHAPE;
   const auto off = [](const void* p) { return (((uintptr_t)p) & 15) != 0; };
   if (off(a) || off(w13) || off(w2) || off(w2_scale) || off(workspace) || (T > 1 && lda % 16)) return FMSMO_ERR_ALIGN;
-  const MoeSpace sp = moe_space(T, E, top, I);
+  const MoeSpace sp = moe_space(T, top, I);
   if (workspace_bytes < sp.all) return FMSMO_ERR_SCRATCH;
   char* ws = (char*)workspace;
   MoeArgs g{(const uint8_t*)a, a_scale, logits, (const uint8_t*)w13, w13_scale, (const uint8_t*)w2, w2_scale, y, lda, ldl, ldy,
-            a_scale_n == 1 ? 0 : 1, logits_dtype, y_dtype, (int)T, (int)E, top, (int)K, (int)I, renormalize != 0,
-            (int*)ws, (MoeEntry*)(ws + sp.entry), (int*)(ws + sp.token), (float*)(ws + sp.weight), (float*)(ws + sp.h), (float*)(ws + sp.hs),
-            (uint8_t*)(ws + sp.hq)};
+            a_scale_n == 1 ? 0 : 1, logits_dtype, y_dtype, (int)T, (int)E, top, (int)K, (int)I, renormalize != 0, 0,
+            (int*)(ws + sp.ids), (float*)(ws + sp.share), (int*)ws, (uint32_t*)(ws + sp.entry), (int*)(ws + sp.token), (float*)(ws + sp.weight),
+            (float*)(ws + sp.hs), (float*)(ws + sp.h), (uint8_t*)(ws + sp.hq), (uint32_t*)(ws + sp.tops)};
   const auto tiles = [&](auto op) {
     constexpr int OP = decltype(op)::value;
-    if (T <= 16) run_moe<OP, 1>(g, (hipStream_t)stream);
+    if (T <= 16 || T * top <= 6 * E) run_moe<OP, 1>(g, (hipStream_t)stream);
     else if (T <= 32) run_moe<OP, 2>(g, (hipStream_t)stream);
     else run_moe<OP, 4>(g, (hipStream_t)stream);
   };
