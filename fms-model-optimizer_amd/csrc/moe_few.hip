@@ -110,7 +110,8 @@ __device__ __forceinline__ void choose(const MoeArgs& a, int t, int& id, float& 
   if (share == 0.0f) id = -1;  // (the expert is not run)
 }
 __device__ __forceinline__ void choose_any(const MoeArgs& a, int t, int& id, float& share) {
-  if (a.E <= 128) choose<2>(a, t, id, share);
+  if (a.E <= 64) choose<1>(a, t, id, share);
+  else if (a.E <= 128) choose<2>(a, t, id, share);
   else choose<MOE_EXPERTS / 64>(a, t, id, share);
 }
 
@@ -139,6 +140,31 @@ struct MoeLists {
 template <int NT, int MT, bool ROUTE>
 __device__ __forceinline__ void make_lists(const MoeArgs& a, MoeLists& l) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pairs = a.T * a.top;
+  if (ROUTE && a.T == 1) {  // a group per choice, in the order of the experts
+    if (wave == 0) {
+      int id, at = 0;
+      float share;
+      choose_any(a, 0, id, share);
+      for (int s = 0; s < a.top; ++s) {
+        const int o = __builtin_amdgcn_readlane(id, s);
+        at += o >= 0 && o < id;
+      }
+      if (lane < a.top) l.token[lane] = 0;
+      const int n = __popcll(__ballot(lane < a.top && id >= 0));
+      if (lane == 0) l.count = n;
+      if (lane < a.top && id >= 0) {
+        l.entry[at] = entry_of(id, 1, at);
+        if (blockIdx.x == 0) {
+          a.entry[at] = entry_of(id, 1, at);
+          a.token[at] = 0;
+          a.weight[at] = share;
+        }
+      }
+      if (blockIdx.x == 0 && lane == 0) a.count[0] = n;
+    }
+    __syncthreads();
+    return;
+  }
   for (int e = threadIdx.x; e < a.E; e += NT) l.mask[e] = 0;
   __syncthreads();
   if constexpr (ROUTE) {
@@ -240,7 +266,7 @@ __device__ __forceinline__ v4i load_or_zero(const uint8_t* p, int64_t off, bool 
 // product.  The four waves of a block share its K, every fourth step of 128 bytes each, D steps on their way, those of the next unit among
 // them; the waves' sums meet in shared memory, one barrier a unit, and a wave in turn finishes it.
 template <int OP, int MT, int D, bool ROUTE>
-__global__ __launch_bounds__(256, MT == 1 ? 3 : 2) void moe_up_kernel(MoeArgs a) {
+__global__ __launch_bounds__(256, MT == 1 ? 4 : 2) void moe_up_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
   __shared__ MoeLists lists;
   __shared__ __attribute__((aligned(16))) uint8_t stage[4][2048];
@@ -422,8 +448,9 @@ __global__ __launch_bounds__(256) void moe_quant_kernel(MoeArgs a) {
 // for the waves, D steps on their way; at the end of a group a wave adds its products, with their scales and shares, to sums of its own, and the
 // waves' sums are added in their order.  ROWS = 8, groups of up to eight tokens: a product takes two steps, the first with its upper eight rows and
 // left eight columns, the second with the others, and the two blocks on its diagonal are added.  QUANT: few positions, whose codes every block makes for itself in shared memory.
-// Shared memory: sums [NW][T][ROWS], shares and scales [T top], entries, tokens; QUANT: codes.
-template <int OP, int MT, int ROWS, int NW, int D, bool QUANT>
+// Up to TM tokens.
+constexpr int MOE_QUANT_MOST = 8192;
+template <int OP, int MT, int ROWS, int NW, int D, int TM, bool QUANT>
 __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
   constexpr int NT = NW * 64;
@@ -434,9 +461,8 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   __shared__ uint32_t entry[MOE_ENTRIES];
   __shared__ uint8_t token[MOE_TOKENS * MOE_TOP];
   __shared__ float share[MOE_TOKENS * MOE_TOP];
-  extern __shared__ __attribute__((aligned(16))) char dyn[];
-  float* sums = (float*)dyn;  // [NW][T][ROWS]
-  uint8_t* codes = (uint8_t*)(sums + NW * a.T * ROWS);
+  __shared__ __attribute__((aligned(16))) float sums[NW * TM * ROWS];
+  __shared__ __attribute__((aligned(16))) uint8_t codes[QUANT ? MOE_QUANT_MOST : 16];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4, drow = lane >> 3, dpos = lane & 7;
   const int n0 = blockIdx.x * ROWS, steps = (a.I + STEP - 1) / STEP, pairs = a.T * a.top;
@@ -450,25 +476,6 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   }
   for (int i = threadIdx.x; i < NW * a.T * ROWS; i += NT) sums[i] = 0.0f;
   __syncthreads();
-  if constexpr (QUANT) {
-    const MoeGroup m = count ? group_of(entry[count - 1]) : MoeGroup{0, 0, 0};
-    for (int pos = wave; pos < m.off + m.cnt; pos += NW) {
-      const v4f* h = (const v4f*)(a.h + (int64_t)pos * a.I);
-      uint32_t top = 0;
-      for (int i = lane; i < a.I / 4; i += 64) {
-        const v4f v = h[i];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t u = __float_as_uint(v[k]) & 0x7fffffffu;
-          top = top > u ? top : u;
-        }
-      }
-      const float s = moe_scale<OP>(wave_max_u32(top));
-      if (lane == 0) share[pos] *= s;
-      for (int i = lane; i < a.I / 4; i += 64) ((uint32_t*)(codes + pos * a.I))[i] = moe_codes<OP>(h[i], s);
-    }
-    __syncthreads();
-  }
   const int from = (int)((int64_t)wave * all / NW), to = (int)((int64_t)(wave + 1) * all / NW);
   uint8_t* st = stage[wave];
   const int rr = r & 7;
@@ -506,9 +513,12 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   Acc acc[MT];
   v4f sc = {0, 0, 0, 0};
   const int ng = PAIR ? g & 1 : g;  // the four outputs of this lane
-  const auto begin = [&] {  // a group's first step: its scales are asked for
+  v4f sn = sc;  // scales of the group that is multiplied, and of the next one
+  const auto ahead = [&](int i) { sn = *(const v4f*)(a.s2 + (int64_t)group_of(uniform((int)entry[i])).e * a.K + n0 + 4 * ng); };
+  const auto begin = [&] {
     cm = group_of(uniform((int)entry[ce]));
-    sc = *(const v4f*)(a.s2 + (int64_t)cm.e * a.K + n0 + 4 * ng);
+    sc = sn;
+    if (ce + 1 < count) ahead(ce + 1);
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[j] = Acc{0, 0, 0, 0};
   };
@@ -530,11 +540,33 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
       *sum = v;
     }
   };
-  if (from < to) {
+  if (from < to) {  // the first weights, ahead of the codes
     load_from();
 #pragma unroll
     for (int d = 0; d < D; ++d)
       if (from + d < to) fetch(d);
+    ahead(ce);
+  }
+  if constexpr (QUANT) {
+    const MoeGroup m = count ? group_of(entry[count - 1]) : MoeGroup{0, 0, 0};
+    for (int pos = wave; pos < m.off + m.cnt; pos += NW) {
+      const v4f* h = (const v4f*)(a.h + (int64_t)pos * a.I);
+      uint32_t top = 0;
+      for (int i = lane; i < a.I / 4; i += 64) {
+        const v4f v = h[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t u = __float_as_uint(v[k]) & 0x7fffffffu;
+          top = top > u ? top : u;
+        }
+      }
+      const float s = moe_scale<OP>(wave_max_u32(top));
+      if (lane == 0) share[pos] *= s;
+      for (int i = lane; i < a.I / 4; i += 64) ((uint32_t*)(codes + pos * a.I))[i] = moe_codes<OP>(h[i], s);
+    }
+    __syncthreads();
+  }
+  if (from < to) {
     begin();
     for (int f = from; f < to; f += D) {
 #pragma unroll
@@ -620,24 +652,26 @@ extern "C" int64_t fmsmo_moe_few_workspace_bytes(int64_t T, int64_t E, int top, 
 
 template <int OP, int MT, int ROWS, bool QUANT>
 static void run_down(const MoeArgs& a, hipStream_t s) {
-  constexpr int NW = 8, D = 4;
-  const size_t lds = (size_t)NW * a.T * ROWS * 4 + (QUANT ? (size_t)a.T * a.top * a.I : 0);
-  hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, QUANT>), dim3((unsigned)(a.K / ROWS)), dim3(NW * 64), lds, s, a);
+  // waves and steps on their way: eight rows want more waves (64 tokens over 128 experts: 41 us with 16 and 2, 43 with 12 and 4, 50 with 8 and 4,
+  // 54 with 16 and 4, whose registers do not suffice), sixteen are indifferent
+  constexpr int NW = ROWS == 8 ? 16 : 8, D = ROWS == 8 ? 2 : 4;
+  const dim3 grid((unsigned)(a.K / ROWS)), block(NW * 64);
+  if (MT > 1 || a.T > 16) hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, 64, QUANT>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((moe_down_kernel<OP, 1, ROWS, NW, D, 16, QUANT>), grid, block, 0, s, a);
 }
 template <int OP, int MT>
 static void run_moe(MoeArgs a, hipStream_t s) {
-  constexpr int QUANT_MOST = 8192;
-  const bool quant = MT == 1 && a.T * a.top * a.I <= QUANT_MOST, narrow = MT == 1 && a.K / 16 < 256;
+  const bool quant = MT == 1 && a.T * a.top <= 8 && a.T * a.top * a.I <= MOE_QUANT_MOST, narrow = MT == 1 && a.K / 16 < 256;
   if (quant) a.tops = nullptr;
   a.down_group = narrow ? 8 : 16 * MT;
   // groups of tokens, at most
   const int64_t units = (int64_t)std::min(MT == 1 ? a.E + a.T * a.top / 16 : a.E, a.T * a.top) * (a.I / 8);
-  const dim3 grid((unsigned)std::min<int64_t>(units, MT == 1 ? 768 : 512));
+  const dim3 grid((unsigned)std::min<int64_t>(units, MT == 1 ? 1024 : 512));
   if (a.T <= 8) {
-    if constexpr (MT == 1) hipLaunchKernelGGL((moe_up_kernel<OP, 1, 4, true>), grid, dim3(256), 0, s, a);
+    if constexpr (MT == 1) hipLaunchKernelGGL((moe_up_kernel<OP, 1, 2, true>), grid, dim3(256), 0, s, a);
   } else {
     hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((moe_up_kernel<OP, MT, MT == 1 ? 4 : 2, false>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((moe_up_kernel<OP, MT, 2, false>), grid, dim3(256), 0, s, a);
   }
   if (!quant) hipLaunchKernelGGL((moe_quant_kernel<OP>), dim3((unsigned)(a.T * a.top), (unsigned)div_up(a.I, MOE_QUANT)), dim3(256), 0, s, a);
   if constexpr (MT == 1) {
