@@ -6,7 +6,10 @@
 // A tile is up to 16 MT rows of one adapter.  One row per request: the rows of the requests that share an adapter, sixteen at a time, found by
 // counting; else 16 MT consecutive rows of a request.
 #include "paged_kv.hpp"
+#include "stream_loads.hpp"
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace fmsmo {
@@ -36,7 +39,7 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& a, int tile, int* 
   const int lane = threadIdx.x & 63;
   LoraTile t{0, 0, -1};
   if (!a.starts) {
-    const int slot = a.adapters[tile];
+    const int slot = uniform(a.adapters[tile]);
     if ((unsigned)slot >= (unsigned)a.slots) {  // on its own: the copy of its row
       t.n = 1;
       t.row0 = tile;
@@ -87,7 +90,7 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& a, int tile, int* 
       const int rn = __shfl(n, l) - at;
       t.row0 = uniform(__shfl(r0, l) + at);
       t.n = uniform(rn < TR ? rn : TR);
-      const int slot = req >= 0 && req < a.seqs ? a.adapters[req] : -1;
+      const int slot = uniform(req >= 0 && req < a.seqs ? a.adapters[req] : -1);
       t.slot = (unsigned)slot < (unsigned)a.slots ? slot : -1;
       return t;
     }
@@ -99,47 +102,35 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& a, int tile, int* 
 
 constexpr int LORA_STEP = 64;  // elements of K a step: 128 bytes of a row
 
-// 16 bytes at `off` behind `base`, or zeros
-__device__ __forceinline__ v4i load_or_zero(const char* base, int64_t off, bool there) {
-  v4i v = {0, 0, 0, 0};
-  if (there) v = *(const v4i*)(base + off);
-  return v;
-}
-
 // v of a tile over a part of K.  Rows of A (16 RT) and of x (16 MT) meet as the two operands of 16 x 16 x 32; the side with more bytes comes
-// through shared memory, eight rows of 128 bytes a load, the other one straight into the operands' layout.
-template <int T, int RT, int MT>
+// through shared memory, eight rows of 128 bytes a load, the other one straight into the operands' layout, D steps of a wave on their way.  Rows past
+// the rank and the tile's end are the last one again: what comes of them is not looked at.
+template <int T, int RT, int MT, int D>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs a) {
   constexpr bool X_STAGED = MT > 1;
   constexpr int S = X_STAGED ? MT : RT, O = X_STAGED ? RT : MT;  // tiles of 16 rows of the staged and the other side
   constexpr int SUMS = MT * 16 * (RT * 16 + 4) * 4;  // bytes of a wave's sums; they take the place of the staged rows
   __shared__ __attribute__((aligned(16))) char stage[S * 8192 > 2 * SUMS ? S * 8192 : 2 * SUMS];
   __shared__ int list[MT * 16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const LoraTile t = lora_tile<16 * MT>(a, blockIdx.x, list);
   if (t.n == 0 || t.slot < 0) return;
-  __syncthreads();
-  const char* A = a.a + (int64_t)t.slot * a.a_slot;
-  const int s0 = blockIdx.y * a.part_steps, s1 = min(s0 + a.part_steps, (a.K + LORA_STEP - 1) / LORA_STEP);
+  if (!a.starts) __syncthreads();
   const int r = lane & 15, g = lane >> 4, drow = lane >> 3, dpos = lane & 7;
-  const auto row_of = [&](int i) -> int64_t { return a.starts ? t.row0 + i : list[i]; };
-  // the staged side: rows drow, drow + 8, .. of this lane
-  const char* sp[2 * S];
-  bool sv[2 * S];
+  // rows of x are counted from the tile's first one (the host sees to it that offsets fit)
+  const Buf A = buf_of(a.a + (int64_t)t.slot * a.a_slot), X = buf_of(a.x + (int64_t)t.row0 * a.ldx);
+  const int s0 = blockIdx.y * a.part_steps, s1 = min(s0 + a.part_steps, (a.K + LORA_STEP - 1) / LORA_STEP);
+  const auto a_off = [&](int q) { return (uint32_t)min(q, a.rank - 1) * (uint32_t)a.a_row; };
+  const auto x_off = [&](int q) {
+    q = min(q, t.n - 1);
+    return (uint32_t)(a.starts ? q : list[q] - t.row0) * (uint32_t)a.ldx;
+  };
+  uint32_t so[2 * S], oo[O];
 #pragma unroll
-  for (int i = 0; i < 2 * S; ++i) {
-    const int q = 8 * i + drow;
-    sv[i] = q < (X_STAGED ? t.n : a.rank);
-    sp[i] = X_STAGED ? a.x + (sv[i] ? row_of(q) : 0) * a.ldx : A + (int64_t)(sv[i] ? q : 0) * a.a_row;
-  }
-  const char* op[O];
-  bool ov[O];
+  for (int i = 0; i < 2 * S; ++i) so[i] = (X_STAGED ? x_off(8 * i + drow) : a_off(8 * i + drow)) + dpos * 16;
 #pragma unroll
-  for (int i = 0; i < O; ++i) {
-    const int q = 16 * i + r;
-    ov[i] = q < (X_STAGED ? a.rank : t.n);
-    op[i] = X_STAGED ? A + (int64_t)(ov[i] ? q : 0) * a.a_row : a.x + (ov[i] ? row_of(q) : 0) * a.ldx;
-  }
+  for (int i = 0; i < O; ++i) oo[i] = (X_STAGED ? a_off(16 * i + r) : x_off(16 * i + r)) + g * 16;
+  const Buf sp = X_STAGED ? X : A, op = X_STAGED ? A : X;
   v4f acc[RT][MT];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -147,49 +138,41 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs a) {
     for (int j = 0; j < MT; ++j) acc[i][j] = v4f{0, 0, 0, 0};
   char* st = stage + wave * (S * 2048);
   const int rr = r & 7;
-  v4i sb[2 * S], ob[O][2];
-  const auto fetch_staged = [&](int s) {
-    const int e = s * LORA_STEP + dpos * 8;
+  v4i sb[D][2 * S], ob[D][O][2];
+  const auto fetch = [&](int s, int d) {  // (zeros past the part and past the row's end)
+    const uint32_t k = s * 2 * LORA_STEP;
+    const int left = s < s1 ? a.K - s * LORA_STEP : 0;
 #pragma unroll
-    for (int i = 0; i < 2 * S; ++i) sb[i] = load_or_zero(sp[i], 2 * e, sv[i] && e < a.K);
+    for (int i = 0; i < 2 * S; ++i)
+      sb[d][i] = X_STAGED ? buf_stream(sp, dpos * 8 < left ? so[i] : BUF_NONE, k) : buf_load(sp, dpos * 8 < left ? so[i] : BUF_NONE, k);
+#pragma unroll
+    for (int i = 0; i < O; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) ob[d][i][h] = buf_load(op, (4 * h + g) * 8 < left ? oo[i] + 64 * h : BUF_NONE, k);
   };
-  const auto fetch_other = [&](int s) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int e = s * LORA_STEP + (4 * h + g) * 8;
+  for (int d = 0; d < D; ++d) fetch(s0 + wave + 4 * d, d);
+  for (int s = s0 + wave; s < s1; s += 4 * D) {
 #pragma unroll
-      for (int i = 0; i < O; ++i) ob[i][h] = load_or_zero(op[i], 2 * e, ov[i] && e < a.K);
-    }
-  };
-  constexpr bool EARLY = O <= 2;  // the other side's next rows too are asked for ahead of the products (else: registers)
-  int s = s0 + wave;
-  if (s < s1) {
-    fetch_staged(s);
-    fetch_other(s);
-  }
-  for (; s < s1; s += 4) {
-    // chunk c of row q lies at position c ^ (q % 8)
+    for (int d = 0; d < D; ++d) {
+      // chunk c of row q lies at position c ^ (q % 8)
 #pragma unroll
-    for (int i = 0; i < 2 * S; ++i) *(v4i*)(st + (8 * i + drow) * 128 + ((dpos ^ drow) * 16)) = sb[i];
-    __builtin_amdgcn_wave_barrier();  // (the rows go to other lanes of the wave)
-    if (s + 4 < s1) fetch_staged(s + 4);
-    v4i o[O][2];
+      for (int i = 0; i < 2 * S; ++i) *(v4i*)(st + (8 * i + drow) * 128 + ((dpos ^ drow) * 16)) = sb[d][i];
+      __builtin_amdgcn_wave_barrier();  // (the rows go to other lanes of the wave)
 #pragma unroll
-    for (int i = 0; i < O; ++i) o[i][0] = ob[i][0], o[i][1] = ob[i][1];
-    if (EARLY && s + 4 < s1) fetch_other(s + 4);
+      for (int i = 0; i < S; ++i)
 #pragma unroll
-    for (int i = 0; i < S; ++i)
+        for (int h = 0; h < 2; ++h) {
+          const v4i w = *(const v4i*)(st + (16 * i + r) * 128 + (((4 * h + g) ^ rr) * 16));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const v4i w = *(const v4i*)(st + (16 * i + r) * 128 + (((4 * h + g) ^ rr) * 16));
-#pragma unroll
-        for (int j = 0; j < O; ++j) {
-          if constexpr (X_STAGED) acc[j][i] = mfma16<T>(o[j][h], w, acc[j][i]);
-          else acc[i][j] = mfma16<T>(w, o[j][h], acc[i][j]);
+          for (int j = 0; j < O; ++j) {
+            if constexpr (X_STAGED) acc[j][i] = mfma16<T>(ob[d][j][h], w, acc[j][i]);
+            else acc[i][j] = mfma16<T>(w, ob[d][j][h], acc[i][j]);
+          }
         }
-      }
-    if (!EARLY && s + 4 < s1) fetch_other(s + 4);
-    __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_wave_barrier();
+      fetch(s + 4 * (D + d), d);
+    }
   }
   // the waves' sums: (0 + 2) + (1 + 3)
   const auto put = [&](int at) {
@@ -220,33 +203,97 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs a) {
     for (int j = 0; j < MT; ++j) *(v4f*)(to + (16 * j + r) * 16 * RT + 16 * i + 4 * g) = acc[i][j];
 }
 
-// out = y + B v for a tile and `cols` groups of 64 outputs, one group a wave at a time
+// out = y + B v for a tile and `cols` groups of 64 outputs, a group a wave at a time: 64 rows of B as operands in registers, then the tile's rows,
+// sixteen by sixteen, whose products go through shared memory so that y is read and out is written in eight rows of 128 bytes.  The next group's y
+// (and B, where the rank leaves registers) are on their way meanwhile.
 template <int T, int RT, int MT>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs a) {
   constexpr int TR = 16 * MT, LD = 64 * RT + 16;  // bytes of a row of v: both halves of 16 RT numbers, and a step in banks
+  constexpr int KB = RT == 1 ? 1 : RT / 2;        // products over the rank; up to 16 both halves of v fill one
+  constexpr int NB = RT <= 4 ? 2 : 1;
+  constexpr int LT = 68;                          // numbers of a row of products
+  constexpr int GONE = 1 << 17;                   // no group: past any N
   __shared__ __attribute__((aligned(16))) char vs[TR][LD];
+  __shared__ __attribute__((aligned(16))) float turn[4][16 * LT];
   __shared__ float lift[TR];
   __shared__ int list[TR];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const LoraTile t = lora_tile<TR>(a, blockIdx.x, list);
   if (t.n == 0) return;
   if (t.slot < 0 && a.y == a.out) return;
-  const int r = lane & 15, g = lane >> 4;
-  const int c0 = blockIdx.y * a.cols, c1 = min(c0 + a.cols, (a.N + 63) / 64);
+  if (!a.starts) __syncthreads();
+  const int r = lane & 15, g = lane >> 4, drow = lane >> 3, dpos = lane & 7;
+  const int c0 = blockIdx.y * a.cols + wave, c1 = min((int)(blockIdx.y + 1) * a.cols, (a.N + 63) / 64);
   const int R = a.rank;
-  if (t.slot >= 0) {
+  const Buf B = buf_of(a.b + (int64_t)(t.slot < 0 ? 0 : t.slot) * a.b_slot);
+  const Buf Y = buf_of(a.y + (int64_t)t.row0 * a.ldy), O = buf_of(a.out + (int64_t)t.row0 * a.ldo);
+  // row 8 q + drow of the tile, eight outputs a lane
+  const auto row_of = [&](int q) { return a.starts ? q : list[q] - t.row0; };
+  v4i yv[MT][2], bw[NB][KB][4];
+  const auto fetch_y = [&](int c, int j) {
+    const bool in = c * 64 + 8 * dpos < a.N;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int q = 16 * j + 8 * h + drow;
+      yv[j][h] = buf_load(Y, in && q < t.n ? (uint32_t)row_of(q) * (uint32_t)a.ldy + dpos * 16 : BUF_NONE, (uint32_t)c * 128);
+    }
+  };
+  const auto put = [&](int c, int j, int h, v4i o) {
+    const int q = 16 * j + 8 * h + drow;
+    buf_store(O, o, q < t.n && c * 64 + 8 * dpos < a.N ? (uint32_t)row_of(q) * (uint32_t)a.ldo + dpos * 16 : BUF_NONE, (uint32_t)c * 128);
+  };
+  const auto fetch_b = [&](int c, v4i (&w)[KB][4]) {
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+      const int e = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = c * 64 + 16 * i + r;
+        w[k][i] = buf_load(B, n < a.N && e < R ? (uint32_t)n * (uint32_t)a.b_row + 2 * e : BUF_NONE);
+      }
+    }
+  };
+  if (t.slot < 0) {  // the bits of y
+    for (int c = c0; c < c1; c += 4)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        fetch_y(c, j);
+        put(c, j, 0, yv[j][0]);
+        put(c, j, 1, yv[j][1]);
+      }
+    return;
+  }
+  fetch_b(c0, bw[0]);
+#pragma unroll
+  for (int j = 0; j < MT; ++j) fetch_y(c0, j);
+  {
     const float scale = a.scales ? a.scales[t.slot] : 1.0f;
     const float* from = a.ws + (int64_t)blockIdx.x * (256 * MT * RT);
     const int64_t part = (int64_t)a.tiles * (256 * MT * RT);
     // In quadruples of a row: v, brought to a maximum of 1 to 4 by a power of two (fp16 holds neither large numbers nor the lower halves of
-    // small ones), its upper half at k, what that leaves at rank + k; zeros behind 2 rank.
-    for (int i = threadIdx.x; i < TR * 4 * RT; i += 256) {
-      const int c = i / (4 * RT), k = i % (4 * RT) * 4;
-      v4f v = {0, 0, 0, 0};
-      if (k < R && c < t.n) {
-        for (int p = 0; p < a.parts; ++p) v += *(const v4f*)(from + p * part + c * 16 * RT + k);
-        v *= scale;
+    // small ones), its upper half at k, what that leaves 16 RT numbers behind.  Rows past the tile's end and numbers past the rank are zero.
+    constexpr int QS = (TR * 4 * RT + 255) / 256;  // quadruples of a thread (of the first 64 or 128 threads alone, where there are few)
+    v4f sum[QS];
+#pragma unroll
+    for (int q = 0; q < QS; ++q) sum[q] = v4f{0, 0, 0, 0};
+    const int last = t.n * 4 * RT - 1;
+    int p = 0;
+    for (; p + 4 <= a.parts; p += 4) {  // (four loads on their way)
+#pragma unroll
+      for (int q = 0; q < QS; ++q) {
+        const float* at = from + p * part + 4 * min((int)threadIdx.x + 256 * q, last);
+        const v4f v0 = *(const v4f*)at, v1 = *(const v4f*)(at + part), v2 = *(const v4f*)(at + 2 * part), v3 = *(const v4f*)(at + 3 * part);
+        sum[q] += (v0 + v1) + (v2 + v3);
       }
+    }
+    for (; p < a.parts; ++p)
+#pragma unroll
+      for (int q = 0; q < QS; ++q) sum[q] += *(const v4f*)(from + p * part + 4 * min((int)threadIdx.x + 256 * q, last));
+#pragma unroll
+    for (int q = 0; q < QS; ++q) {
+      const int i = threadIdx.x + 256 * q, c = i / (4 * RT), k = i % (4 * RT) * 4;
+      if (i >= TR * 4 * RT) break;  // (whole waves)
+      const v4f v = c < t.n && k < R ? sum[q] * scale : v4f{0, 0, 0, 0};
       float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
       for (int d = 1; d < 4 * RT; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
@@ -254,82 +301,66 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs a) {
       e = e < 1 ? 1 : e > 253 ? 253 : e;
       const float down = __uint_as_float((uint32_t)(254 - e) << 23);
       if (k == 0) lift[c] = __uint_as_float((uint32_t)e << 23);
-      if (k < R) {
-        float hi[4], lo[4];
+      float hi[4], lo[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float s = v[j] * down;
-          hi[j] = round_to<T>(s);
-          lo[j] = fabsf(hi[j]) < 8.0f ? s - hi[j] : 0.0f;  // (infinities and NaN are in the upper half alone)
-        }
-        *(uint2*)(vs[c] + 2 * k) = make_uint2(pack2<T>(hi[0], hi[1]), pack2<T>(hi[2], hi[3]));
-        *(uint2*)(vs[c] + 2 * (R + k)) = make_uint2(pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]));
-      } else {  // (16 RT - rank numbers a row, half as many as 2 rank is short of 32 RT)
-        *(uint4*)(vs[c] + 2 * (2 * R + 2 * (k - R))) = make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < 4; ++j) {
+        const float s = v[j] * down;
+        hi[j] = round_to<T>(s);
+        lo[j] = fabsf(hi[j]) < 8.0f ? s - hi[j] : 0.0f;  // (infinities and NaN are in the upper half alone)
       }
+      *(uint2*)(vs[c] + 2 * k) = make_uint2(pack2<T>(hi[0], hi[1]), pack2<T>(hi[2], hi[3]));
+      *(uint2*)(vs[c] + 2 * (16 * RT + k)) = make_uint2(pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]));
     }
   }
   __syncthreads();
-  const char* B = a.b + (int64_t)(t.slot < 0 ? 0 : t.slot) * a.b_slot;
-  const auto row_of = [&](int i) -> int64_t { return a.starts ? t.row0 + i : list[i]; };
-  for (int c = c0 + wave; c < c1; c += 4) {
-    const int n0 = c * 64 + 16 * g;  // this lane's sixteen outputs
-    v4i yv[MT][2];
-    bool there[MT][2];
-    int64_t row[MT];
+  float* tw = turn[wave];
+  // (groups past the last one: zeros are loaded)
+  const auto group = [&](int c, v4i (&w)[KB][4], v4i (&next)[KB][4]) {
+    if constexpr (NB == 2) fetch_b(c + 4 < c1 ? c + 4 : GONE, next);
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-      const bool mine = 16 * j + r < t.n;
-      row[j] = mine ? row_of(16 * j + r) : 0;
+      v4f acc[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const v4i hi = *(const v4i*)(vs[16 * j + r] + 64 * k + 16 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = mfma16<T>(w[k][i], hi, acc[i]);
+        if constexpr (RT > 1) {
+          const v4i lo = *(const v4i*)(vs[16 * j + r] + 32 * RT + 64 * k + 16 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] = mfma16<T>(w[k][i], lo, acc[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *(v4f*)(tw + r * LT + 16 * i + 4 * g) = acc[i];
+      __builtin_amdgcn_wave_barrier();
+      v4i o[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        there[j][h] = mine && n0 + 8 * h < a.N;
-        yv[j][h] = load_or_zero(a.y + row[j] * a.ldy, 2 * (int64_t)(n0 + 8 * h), there[j][h]);
-      }
-    }
-    if (t.slot >= 0) {
-      // row 4 g' + j of part i of the product is output 16 g' + 4 i + j: a lane's results lie side by side
-      v4f acc[4][MT];
+        const int q = 8 * h + drow;
+        const float by = lift[16 * j + q];
+        const v4f d0 = *(const v4f*)(tw + q * LT + 8 * dpos), d1 = *(const v4f*)(tw + q * LT + 8 * dpos + 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = v4f{0, 0, 0, 0};
-      const int nb = c * 64 + 16 * (r >> 2) + (r & 3);
-      for (int k = 0; k < 2 * R; k += 32) {
-        const int kk = k + 8 * g, e = kk < R ? kk : kk - R;
-        v4i bw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bw[i] = load_or_zero(B, (int64_t)(nb + 4 * i) * a.b_row + 2 * e, nb + 4 * i < a.N && kk < 2 * R);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const v4i vv = *(const v4i*)(vs[16 * j + r] + 2 * kk);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i][j] = mfma16<T>(bw[i], vv, acc[i][j]);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t u = (uint32_t)yv[j][h][k];
+          const float lo = T == FMSMO_F16 ? f16_to_f32((u16)u) : bf16_to_f32((u16)u);
+          const float hi = T == FMSMO_F16 ? f16_to_f32((u16)(u >> 16)) : bf16_to_f32((u16)(u >> 16));
+          const v4f& d = k < 2 ? d0 : d1;
+          o[h][k] = (int)pack2<T>(__fmaf_rn(d[k % 2 * 2], by, lo), __fmaf_rn(d[k % 2 * 2 + 1], by, hi));
         }
       }
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const float by = lift[16 * j + r];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          v4i o;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t w = (uint32_t)yv[j][h][q];
-            const float lo = T == FMSMO_F16 ? f16_to_f32((u16)w) : bf16_to_f32((u16)w);
-            const float hi = T == FMSMO_F16 ? f16_to_f32((u16)(w >> 16)) : bf16_to_f32((u16)(w >> 16));
-            const v4f& d = acc[2 * h + q / 2][j];
-            o[q] = (int)pack2<T>(__fmaf_rn(d[q % 2 * 2], by, lo), __fmaf_rn(d[q % 2 * 2 + 1], by, hi));
-          }
-          yv[j][h] = o;
-        }
-      }
+      __builtin_amdgcn_wave_barrier();
+      fetch_y(c + 4 < c1 ? c + 4 : GONE, j);  // (out may be y: other columns)
+      put(c, j, 0, o[0]);
+      put(c, j, 1, o[1]);
     }
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (there[j][h]) *(v4i*)(a.out + row[j] * a.ldo + 2 * (int64_t)(n0 + 8 * h)) = yv[j][h];
+    if constexpr (NB == 1) fetch_b(c + 4 < c1 ? c + 4 : GONE, w);
+  };
+  for (int c = c0; c < c1; c += 8) {
+    group(c, bw[0], bw[NB - 1]);
+    if (c + 4 < c1) group(c + 4, bw[NB - 1], bw[0]);
   }
 }
 
@@ -339,8 +370,13 @@ using namespace fmsmo;
 
 int fmsmo_check_launch();
 
-// What a call is cut into.  Rows: tiles of 64 where a request has 32 on average, else of 16.  K: parts for about 512 blocks, a step of 64
-// elements for each of their four waves at least.  Outputs: blocks for about 1024.
+// Steps on their way of a wave of the first launch on tiles of 64 rows: what the registers hold.
+static constexpr int lora_depth(int rt) { return rt <= 2 ? 4 : rt == 4 ? 2 : 1; }
+// What a call is cut into.  Rows: tiles of 64 where a request has 32 on average, else of 16.  Few rows: parts of K for about 512 blocks, a step
+// of 64 elements for each of their four waves at least, and of the outputs for about 768.  Many: a compute unit takes in about 23 GB/s however
+// many blocks it has once 128 KB are on their way, so that what counts is how evenly the blocks fall on the units (8192 rows of 14336: 393 blocks with
+// two steps a wave 63 us, 512 50, 256 with four steps 45 and with two 73); a part more costs its share of v in memory, a block of the second
+// launch as much as one group of outputs.
 struct LoraPlan {
   int mt, rt, tiles, parts, part_steps, cols;
 };
@@ -350,28 +386,45 @@ static LoraPlan lora_plan(int64_t rows, int64_t seqs, bool ragged, int rank, int
   p.rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
   p.tiles = (int)(ragged ? rows / (16 * p.mt) + seqs + 2 : seqs);
   const int steps = div_up(K, LORA_STEP), groups = div_up(N, 64);
-  int parts = 512 / p.tiles;
-  parts = parts < 1 ? 1 : parts < div_up(steps, 4) ? parts : div_up(steps, 4);
-  p.part_steps = div_up(div_up(steps, parts), 4) * 4;
+  if (p.mt == 1) {
+    int parts = 512 / p.tiles;
+    parts = parts < 1 ? 1 : parts < div_up(steps, 4) ? parts : div_up(steps, 4);
+    p.part_steps = div_up(div_up(steps, parts), 4) * 4;
+    int blocks = 768 / p.tiles;
+    blocks = blocks < 1 ? 1 : blocks < div_up(groups, 4) ? blocks : div_up(groups, 4);
+    p.cols = div_up(div_up(groups, blocks), 4) * 4;
+  } else {
+    const double real = std::max(1.0, (double)rows / 64 + 0.5 * (double)(seqs - 1));  // tiles with rows in them, about
+    double best = 1e30;
+    for (int n = 1; n <= 16; ++n) {
+      const int each = div_up(div_up(steps, n), 4) * 4, parts = div_up(steps, each);
+      const double rounds = std::ceil(real * parts / 256), full = std::min(1.0, rounds * lora_depth(p.rt) / 4);
+      const double cost = rounds * each / full * (1.0 + parts * (0.01 + 64.0 * p.rt / (double)K));
+      if (cost < best) best = cost, p.part_steps = each;
+    }
+    best = 1e30;
+    for (int m = 1; m <= 16; ++m) {
+      const double cost = std::ceil(real * div_up(groups, 4 * m) / 256) * (m + 1.0);
+      if (cost < best) best = cost, p.cols = 4 * m;
+    }
+  }
   p.parts = div_up(steps, p.part_steps);
-  int blocks = 1024 / p.tiles;
-  blocks = blocks < 1 ? 1 : blocks < div_up(groups, 4) ? blocks : div_up(groups, 4);
-  p.cols = div_up(div_up(groups, blocks), 4) * 4;
   return p;
 }
 static bool lora_sizes(int64_t rows, int64_t seqs, int rank, int64_t K) {
-  return rows >= 0 && seqs >= 0 && rows < 1 << 30 && seqs < 1 << 29 && rank >= 8 && rank <= 128 && rank % 8 == 0 && K >= 8 && K < 1 << 28;
+  return rows >= 0 && seqs >= 0 && rows < 1 << 30 && seqs < 1 << 29 && rank >= 8 && rank <= 128 && rank % 8 == 0 && K >= 8 && K <= 1 << 22;
 }
 
 extern "C" int64_t fmsmo_lora_workspace_bytes(int64_t rows, int64_t seqs, int ragged, int rank, int64_t K) {
-  if (!lora_sizes(rows, seqs, rank, K) || rows == 0) return 0;
+  if (!lora_sizes(rows, seqs, rank, K) || rows == 0 || (!ragged && rows != seqs)) return 0;
   const LoraPlan p = lora_plan(rows, seqs, ragged != 0, rank, K, 64);
   return (int64_t)p.parts * p.tiles * (1024 * p.mt * p.rt);
 }
 
 template <int T, int RT, int MT>
 static void run_lora(const LoraArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((lora_shrink_kernel<T, RT, MT>), dim3((unsigned)a.tiles, (unsigned)a.parts), dim3(256), 0, s, a);
+  constexpr int D = MT == 4 ? lora_depth(RT) : 2;
+  hipLaunchKernelGGL((lora_shrink_kernel<T, RT, MT, D>), dim3((unsigned)a.tiles, (unsigned)a.parts), dim3(256), 0, s, a);
   hipLaunchKernelGGL((lora_expand_kernel<T, RT, MT>), dim3((unsigned)a.tiles, (unsigned)div_up(div_up(a.N, 64), a.cols)), dim3(256), 0, s, a);
 }
 
@@ -384,18 +437,28 @@ extern "C" int fmsmo_lora_add(int dtype, const void* x, int64_t ldx, const void*
   if (rows == 0 || N == 0) return FMSMO_OK;
   if (!x || !y || !out || (slots && (!a || !b)) || (seqs && !adapters)) return FMSMO_ERR_NULL;
   if (!query_start && rows != seqs) return FMSMO_ERR_SHAPE;
-  if (!lora_sizes(rows, seqs, rank, K) || N >= 1 << 28 || slots > 0x7fffffff) return FMSMO_ERR_UNSUPPORTED;
+  if (!lora_sizes(rows, seqs, rank, K) || N > 1 << 22 || slots > 0x7fffffff) return FMSMO_ERR_UNSUPPORTED;
   if ((rows > 1 && (ldx < K || ldy < N || ldo < N)) || a_row < K || b_row < rank || a_slot < 0 || b_slot < 0) return FMSMO_ERR_SHAPE;
   const auto off = [](const void* p) { return (((uintptr_t)p) & 15) != 0; };
   if (K % 8 || N % 8 || off(x) || off(y) || off(out) || off(a) || off(b) || (rows > 1 && (ldx % 8 || ldy % 8 || ldo % 8)) || a_slot % 8 ||
       a_row % 8 || b_slot % 8 || b_row % 8 || off(workspace))
     return FMSMO_ERR_ALIGN;
-  const LoraPlan p = lora_plan(rows, seqs, query_start != nullptr, rank, K, N);
+  // the kernels count 32 bits from a tile's first row, from an adapter and from its B
+  constexpr int64_t MOST = 0x7f000000;
+  if (64 * (2 * a_row) > MOST || 128 * (2 * a_row) > MOST || N * (2 * b_row) > MOST) return FMSMO_ERR_UNSUPPORTED;
+  const int64_t widest = 2 * std::max(ldx, std::max(ldy, ldo));
+  if (rows > 1 && 64 * widest + 2 * std::max(K, N) > MOST) return FMSMO_ERR_UNSUPPORTED;
   if (!workspace) return FMSMO_ERR_NULL;
+  const LoraPlan p = lora_plan(rows, seqs, query_start != nullptr, rank, K, N);
   if (workspace_bytes < (int64_t)p.parts * p.tiles * (1024 * p.mt * p.rt)) return FMSMO_ERR_SCRATCH;
-  LoraArgs g{(const char*)x, (const char*)y, (char*)out, (const char*)a, (const char*)b, adapters, query_start, scales, (float*)workspace,
-             2 * ldx, 2 * ldy, 2 * ldo, 2 * a_slot, 2 * a_row, 2 * b_slot, 2 * b_row, (int)rows, (int)seqs, (int)slots, rank, (int)K, (int)N,
-             p.parts, p.part_steps, p.tiles, p.cols};
+  // rows of one adapter may lie anywhere among the requests of one row: as many of them at a time as 32 bits reach
+  const int64_t most = query_start || rows == 1 ? rows : (MOST - 2 * std::max(K, N)) / widest;
+  for (int64_t from = 0; from < rows; from += most) {
+  const int64_t some = std::min(most, rows - from);
+  LoraArgs g{(const char*)x + 2 * from * ldx, (const char*)y + 2 * from * ldy, (char*)out + 2 * from * ldo, (const char*)a, (const char*)b,
+             adapters + from, query_start, scales, (float*)workspace, 2 * ldx, 2 * ldy, 2 * ldo, 2 * a_slot, 2 * a_row, 2 * b_slot, 2 * b_row,
+             (int)some, (int)(query_start ? seqs : some), (int)slots, rank, (int)K, (int)N, p.parts, p.part_steps, (int)(query_start ? p.tiles : some),
+             p.cols};
   const auto go = [&](auto t, auto rt) {
     constexpr int T = decltype(t)::value, RT = decltype(rt)::value;
     if (p.mt == 4) run_lora<T, RT, 4>(g, (hipStream_t)stream);
@@ -409,5 +472,6 @@ extern "C" int fmsmo_lora_add(int dtype, const void* x, int64_t ldx, const void*
   };
   if (dtype == FMSMO_F16) ranks(std::integral_constant<int, FMSMO_F16>{});
   else ranks(std::integral_constant<int, FMSMO_BF16>{});
+  }
   return fmsmo_check_launch();
 }

@@ -1,5 +1,6 @@
 """Argument checks and workspace sizes of the operators around a layer's products: rejected before any launch, so no GPU is needed."""
 import ctypes
+import random
 
 import pytest
 import torch
@@ -81,6 +82,17 @@ def test_lora_workspace_holds_every_tile(lib, rank, K):
             tiles = rows // tile + seqs + 2 if ragged else seqs
             assert n % 16 == 0 and n >= 4 * tiles * tile * rank
     assert lib.fmsmo_lora_workspace_bytes(0, 4, 1, rank, K) == 0 and lib.fmsmo_lora_workspace_bytes(4, 4, 0, 12, K) == 0
+
+
+def test_lora_workspace_of_any_sizes(lib):
+    """No sizes, a caller's mistakes among them, end in anything but a number."""
+    r = random.Random(1)
+    for _ in range(50000):
+        rows = int(2 ** r.uniform(0, 30))
+        seqs = r.choice([0, 1, 2, rows // 64, rows // 33, rows, int(2 ** r.uniform(0, 29))])
+        n = lib.fmsmo_lora_workspace_bytes(rows, seqs, r.randint(0, 1), 8 * r.randint(1, 16), 8 * int(2 ** r.uniform(0, 19)))
+        assert n >= 0 and n % 16 == 0
+    assert lib.fmsmo_lora_workspace_bytes(3, 0, 1, 16, 64) > 0 and lib.fmsmo_lora_workspace_bytes(3, 0, 0, 16, 64) == 0
 
 
 def test_moe(lib, p):
