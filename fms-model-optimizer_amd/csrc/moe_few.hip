@@ -9,6 +9,7 @@
 // The chosen (token, expert) pairs are sorted by expert: a `position` each.  The weights stream past once, eight rows of 128 bytes a load,
 // and are turned into matrix operands in shared memory; an expert's tokens are the columns of the product.
 #include "paged_kv.hpp"
+#include "stream_loads.hpp"
 
 #include <type_traits>
 
@@ -251,22 +252,11 @@ __device__ __forceinline__ void moe_mfma(typename MoeAcc<OP>::type& c, v4i w0, v
     }
   }
 }
-__device__ __forceinline__ v4i stream16(const uint8_t* p, int64_t off, bool there) {
-  v4i v = {0, 0, 0, 0};
-  if (there) v = __builtin_nontemporal_load((const v4i*)(p + off));
-  return v;
-}
-__device__ __forceinline__ v4i load_or_zero(const uint8_t* p, int64_t off, bool there) {
-  v4i v = {0, 0, 0, 0};
-  if (there) v = *(const v4i*)(p + off);
-  return v;
-}
-
 // h of the positions.  A unit: eight gate rows and the eight up rows that belong to them, for one group of tokens: the 16 rows of the
 // product.  The four waves of a block share its K, every fourth step of 128 bytes each, D steps on their way, those of the next unit among
 // them; the waves' sums meet in shared memory, one barrier a unit, and a wave in turn finishes it.
 template <int OP, int MT, int D, bool ROUTE>
-__global__ __launch_bounds__(256, MT == 1 ? 4 : 2) void moe_up_kernel(MoeArgs a) {
+__global__ __launch_bounds__(256, MT == 1 && D == 2 ? 4 : 2) void moe_up_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
   __shared__ MoeLists lists;
   __shared__ __attribute__((aligned(16))) uint8_t stage[4][2048];
@@ -279,45 +269,39 @@ __global__ __launch_bounds__(256, MT == 1 ? 4 : 2) void moe_up_kernel(MoeArgs a)
   uint8_t* st = stage[wave];
   const int rr = r & 7;
   struct Unit {
-    const uint8_t* w;  // the lane's gate row
-    const uint8_t* x[MT];
+    Buf w;             // of the expert
+    uint32_t wo;       // the lane's gate row
+    uint32_t xo[MT];   // and tokens
     MoeGroup m;
     int gi;
-    bool xv[MT], there;
   };
-  const auto unit_of = [&](int u) {
+  const Buf xb_of = buf_of(a.a);
+  const auto unit_of = [&](int u) {  // (past the last one: nothing is loaded)
     Unit q;
-    q.there = u < units;
-    const int en = q.there ? u / groups : 0;
-    q.gi = q.there ? u - en * groups : 0;
+    const bool there = u < units;
+    const int en = there ? u / groups : 0;
+    q.gi = there ? u - en * groups : 0;
     q.m = group_of(uniform((int)lists.entry[en]));
-    if (!q.there) q.m.cnt = 0;
-    q.w = a.w13 + ((int64_t)q.m.e * 2 * a.I + q.gi * 8 + drow) * a.K + dpos * 16;
+    q.w = buf_of(a.w13 + (int64_t)q.m.e * 2 * a.I * a.K);
+    q.wo = there ? (uint32_t)(q.gi * 8 + drow) * (uint32_t)a.K + dpos * 16 : BUF_NONE;
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      q.xv[j] = 16 * j + r < q.m.cnt;
-      q.x[j] = a.a + (q.xv[j] ? (int)lists.token[q.m.off + 16 * j + r] : 0) * a.lda + g * 16;
-    }
+    for (int j = 0; j < MT; ++j)
+      q.xo[j] = there && 16 * j + r < q.m.cnt ? lists.token[q.m.off + 16 * j + r] * (uint32_t)a.lda + g * 16 : BUF_NONE;
     return q;
   };
-  const int64_t up = (int64_t)a.I * a.K;
+  const uint32_t up = (uint32_t)a.I * (uint32_t)a.K;
   v4i wb[D][2], xb[D][MT][2];
   const auto fetch = [&](const Unit& q, int s, int d) {
-    const int k = (s * 4 + wave) * 128;
-    if (!q.there || k >= a.K) {  // (uniform)
-      wb[d][0] = wb[d][1] = v4i{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < MT; ++j) xb[d][j][0] = xb[d][j][1] = v4i{0, 0, 0, 0};
-      return;
-    }
-    const bool in = k + dpos * 16 < a.K;
-    wb[d][0] = stream16(q.w, k, in);
-    wb[d][1] = stream16(q.w + up, k, in);
+    const uint32_t k = (s * 4 + wave) * 128;
+    const int left = a.K - (int)k;
+    const uint32_t wo = dpos * 16 < left ? q.wo : BUF_NONE;
+    wb[d][0] = buf_stream(q.w, wo, k);
+    wb[d][1] = buf_stream(q.w, wo, k + up);
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-      if (16 * j >= q.m.cnt) break;
-      xb[d][j][0] = load_or_zero(q.x[j], k, q.xv[j] && k + g * 16 < a.K);
-      xb[d][j][1] = load_or_zero(q.x[j], k + 64, q.xv[j] && k + 64 + g * 16 < a.K);
+      if (MT > 1 && 16 * j >= q.m.cnt) break;
+      xb[d][j][0] = buf_load(xb_of, g * 16 < left ? q.xo[j] : BUF_NONE, k);
+      xb[d][j][1] = buf_load(xb_of, g * 16 + 64 < left ? q.xo[j] : BUF_NONE, k + 64);
     }
   };
   if ((int)blockIdx.x >= units) return;
@@ -337,7 +321,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 4 : 2) void moe_up_kernel(MoeArgs a)
         su[i] = sc[a.I + i];
       }
 #pragma unroll
-      for (int j = 0; j < MT; ++j) as[j] = a.a_scale[cur.xv[j] ? (int)lists.token[cur.m.off + 16 * j + r] * a.a_stride : 0];
+      for (int j = 0; j < MT; ++j) as[j] = a.a_scale[16 * j + r < cur.m.cnt ? (int)lists.token[cur.m.off + 16 * j + r] * a.a_stride : 0];
     }
     Acc acc[MT];
 #pragma unroll
@@ -354,11 +338,10 @@ __global__ __launch_bounds__(256, MT == 1 ? 4 : 2) void moe_up_kernel(MoeArgs a)
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          if (16 * j >= cur.m.cnt) break;
+          if (MT > 1 && 16 * j >= cur.m.cnt) break;
           moe_mfma<OP>(acc[j], w0, w1, xb[d][j][0], xb[d][j][1]);
         }
-        if (last) fetch(next, d, d);
-        else fetch(cur, s + D + d, d);
+        fetch(last ? next : cur, last ? d : s + D + d, d);
       }
     }
     Acc(*mine)[MT][64] = part[turn & 1];
@@ -383,11 +366,11 @@ __global__ __launch_bounds__(256, MT == 1 ? 4 : 2) void moe_up_kernel(MoeArgs a)
           top = top > m ? top : m;
         }
         const int pos = cur.m.off + 16 * j + r;
-        if (cur.xv[j] && g < 2) *(v4f*)(a.h + (int64_t)pos * a.I + cur.gi * 8 + 4 * g) = h;
+        if (16 * j + r < cur.m.cnt && g < 2) *(v4f*)(a.h + (int64_t)pos * a.I + cur.gi * 8 + 4 * g) = h;
         if (a.tops) {
           const auto o = __builtin_amdgcn_permlane16_swap(top, top, false, false);
           top = o[0] > o[1] ? o[0] : o[1];
-          if (cur.xv[j] && g == 0) a.tops[(int64_t)pos * groups + cur.gi] = top;
+          if (16 * j + r < cur.m.cnt && g == 0) a.tops[(int64_t)pos * groups + cur.gi] = top;
         }
       }
     }
@@ -481,29 +464,34 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   const int rr = r & 7;
   int le = steps ? from / steps : 0, ls = from - le * steps, ce = le, cs = ls;  // what is loaded and what is multiplied next: group and step
   MoeGroup lm = group_of(entry[0]), cm = lm;
-  const uint8_t* w = nullptr;
-  const uint8_t* x = nullptr;
   // column r of a product: token col of tile j, and in a pair the step's half
   const int col = PAIR ? rr : r, half = PAIR ? 128 * (r >> 3) : 0;
+  Buf w = buf_of(a.w2);
+  const Buf xb_of = buf_of(a.hq);
+  uint32_t wo = BUF_NONE, xo[MT];
   const auto load_from = [&] {
     lm = group_of(uniform((int)entry[le]));
-    w = a.w2 + ((int64_t)lm.e * a.K + n0 + drow) * a.I + dpos * 16;
-    x = a.hq + (int64_t)(lm.off + col) * a.I + half + g * 16;
+    w = buf_of(a.w2 + (int64_t)lm.e * a.K * a.I);
+    wo = (uint32_t)(n0 + drow) * (uint32_t)a.I + dpos * 16;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) xo[j] = 16 * j + col < lm.cnt ? (uint32_t)(lm.off + 16 * j + col) * (uint32_t)a.I + half + g * 16 : BUF_NONE;
   };
   v4i wb[D][2], xb[QUANT ? 1 : D][MT][2];
+  int loads = to - from;  // steps that are not on their way yet; behind the last one zeros are loaded
   const auto fetch = [&](int d) {
-    const int k = ls * STEP;
-    wb[d][0] = stream16(w, k, k + dpos * 16 < a.I);
-    wb[d][1] = PAIR ? stream16(w, k + 128, k + 128 + dpos * 16 < a.I) : stream16(w + (int64_t)8 * a.I, k, k + dpos * 16 < a.I);
+    const uint32_t k = ls * STEP;
+    const int left = loads > 0 ? a.I - (int)k : 0;
+    wb[d][0] = buf_stream(w, dpos * 16 < left ? wo : BUF_NONE, k);
+    wb[d][1] = PAIR ? buf_stream(w, dpos * 16 + 128 < left ? wo : BUF_NONE, k + 128) : buf_stream(w, dpos * 16 < left ? wo : BUF_NONE, k + 8 * a.I);
     if constexpr (!QUANT) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        if (16 * j >= lm.cnt) break;
-        const bool v = 16 * j + col < lm.cnt;
-        xb[d][j][0] = load_or_zero(x + (int64_t)16 * j * a.I, k, v && k + half + g * 16 < a.I);
-        xb[d][j][1] = load_or_zero(x + (int64_t)16 * j * a.I, k + 64, v && k + half + 64 + g * 16 < a.I);
+        if (MT > 1 && 16 * j >= lm.cnt) break;
+        xb[d][j][0] = buf_load(xb_of, half + g * 16 < left ? xo[j] : BUF_NONE, k);
+        xb[d][j][1] = buf_load(xb_of, half + g * 16 + 64 < left ? xo[j] : BUF_NONE, k + 64);
       }
     }
+    --loads;
     if (++ls == steps) {
       ls = 0;
       ++le;
@@ -543,8 +531,7 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   if (from < to) {  // the first weights, ahead of the codes
     load_from();
 #pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (from + d < to) fetch(d);
+    for (int d = 0; d < D; ++d) fetch(d);
     ahead(ce);
   }
   if constexpr (QUANT) {
@@ -571,7 +558,6 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
     for (int f = from; f < to; f += D) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        if (f + d >= to) break;
         *(v4i*)(st + drow * 128 + ((dpos ^ drow) * 16)) = wb[d][0];
         *(v4i*)(st + (8 + drow) * 128 + ((dpos ^ drow) * 16)) = wb[d][1];
         __builtin_amdgcn_wave_barrier();
@@ -580,7 +566,7 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          if (16 * j >= cm.cnt) break;
+          if (MT > 1 && 16 * j >= cm.cnt) break;
           v4i x0, x1;
           if constexpr (QUANT) {
             const int k = cs * STEP + half + g * 16;
@@ -594,8 +580,8 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
           }
           moe_mfma<OP>(acc[j], w0, w1, x0, x1);
         }
-        if (f + d + D < to) fetch(d);
-        if (++cs == steps || f + d + 1 == to) {
+        fetch(d);
+        if (f + d < to && (++cs == steps || f + d + 1 == to)) {
           end();
           cs = 0;
           ++ce;
@@ -624,7 +610,7 @@ int fmsmo_check_launch();
 
 static bool moe_sizes(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   return T >= 0 && T <= MOE_TOKENS && E >= 1 && E <= MOE_EXPERTS && top >= 1 && top <= MOE_TOP && top <= E && K >= 16 && I >= 16 && K % 16 == 0 &&
-         I % 16 == 0 && K < 1 << 20 && I < 1 << 20;
+         I % 16 == 0 && K < 1 << 20 && I < 1 << 20 && 2 * I * K <= 0x7f000000;  // (an expert's weights are counted in 32 bits)
 }
 // bytes up to each piece of the workspace
 struct MoeSpace {
@@ -664,14 +650,22 @@ static void run_moe(MoeArgs a, hipStream_t s) {
   const bool quant = MT == 1 && a.T * a.top <= 8 && a.T * a.top * a.I <= MOE_QUANT_MOST, narrow = MT == 1 && a.K / 16 < 256;
   if (quant) a.tops = nullptr;
   a.down_group = narrow ? 8 : 16 * MT;
-  // groups of tokens, at most
+  // Groups of tokens, at most.  Eight steps on their way where a wave has a multiple of eight for a unit (K = 4096, 16 tokens over 8 experts of
+  // 14336: 150 us, 156 with two; 2048 has four, 91 and 67 us with 64 tokens over 128 experts of 768).
   const int64_t units = (int64_t)std::min(MT == 1 ? a.E + a.T * a.top / 16 : a.E, a.T * a.top) * (a.I / 8);
-  const dim3 grid((unsigned)std::min<int64_t>(units, MT == 1 ? 1024 : 512));
-  if (a.T <= 8) {
-    if constexpr (MT == 1) hipLaunchKernelGGL((moe_up_kernel<OP, 1, 2, true>), grid, dim3(256), 0, s, a);
+  const bool deep = MT == 1 && div_up(a.K, 512) % 8 == 0;
+  const dim3 grid((unsigned)std::min<int64_t>(units, MT > 1 || deep ? 512 : 1024)), block(256);
+  if (a.T > 8) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), block, 0, s, a);
+  if constexpr (MT == 1) {
+    if (a.T <= 8) {
+      if (deep) hipLaunchKernelGGL((moe_up_kernel<OP, 1, 8, true>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((moe_up_kernel<OP, 1, 2, true>), grid, block, 0, s, a);
+    } else {
+      if (deep) hipLaunchKernelGGL((moe_up_kernel<OP, 1, 8, false>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((moe_up_kernel<OP, 1, 2, false>), grid, block, 0, s, a);
+    }
   } else {
-    hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((moe_up_kernel<OP, MT, 2, false>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((moe_up_kernel<OP, MT, 2, false>), grid, block, 0, s, a);
   }
   if (!quant) hipLaunchKernelGGL((moe_quant_kernel<OP>), dim3((unsigned)(a.T * a.top), (unsigned)div_up(a.I, MOE_QUANT)), dim3(256), 0, s, a);
   if constexpr (MT == 1) {
@@ -700,6 +694,7 @@ extern "C" int fmsmo_moe_few_tokens(int codes, const void* a, int64_t lda, const
   if (!a || !a_scale || !logits || !w13 || !w13_scale || !w2 || !w2_scale || !y || !workspace) return FMSMO_ERR_NULL;
   if ((a_scale_n != 1 && a_scale_n != T) || (T > 1 && (lda < K || ldl < E || ldy < K))) return FMSMO_ERR_SHAPE;
   const auto off = [](const void* p) { return (((uintptr_t)p) & 15) != 0; };
+  if (T > 1 && lda > 1 << 24) return FMSMO_ERR_UNSUPPORTED;
   if (off(a) || off(w13) || off(w2) || off(w2_scale) || off(workspace) || (T > 1 && lda % 16)) return FMSMO_ERR_ALIGN;
   const MoeSpace sp = moe_space(T, top, I);
   if (workspace_bytes < sp.all) return FMSMO_ERR_SCRATCH;
