@@ -40,25 +40,62 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// eight elements as they lie in memory, and widened
+template <int T>
+struct Raw {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const void* p, size_t piece) {
+    if constexpr (T == FMSMO_F32) {
+      a = ((const uint4*)p)[2 * piece];
+      b = ((const uint4*)p)[2 * piece + 1];
+    } else {
+      a = ((const uint4*)p)[piece];
+    }
+  }
+  __device__ __forceinline__ void widen(float (&v)[8]) const {
+    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+    if constexpr (T == FMSMO_F32) {
+      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = __uint_as_float(u[i]);
+        v[4 + i] = __uint_as_float(w[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = cvt16<T>((u16)(u[i] & 0xffff));
+        v[2 * i + 1] = cvt16<T>((u16)(u[i] >> 16));
+      }
+    }
+  }
+};
 // h of eight elements
 template <int T>
-__device__ __forceinline__ void load_h(const NormArgs& a, int64_t row, int c, float (&h)[8]) {
-  load8<T>(a.x + row * a.ldx, (size_t)c * AQ_VEC, h);
+__device__ __forceinline__ void sum_h(const NormArgs& a, const Raw<T>& x, const Raw<T>& r, float (&h)[8]) {
+  x.widen(h);
   if (a.residual) {
-    float r[8];
-    load8<T>(a.residual + row * a.ldr, (size_t)c * AQ_VEC, r);
+    float v[8];
+    r.widen(v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] += r[i];
+    for (int i = 0; i < 8; ++i) h[i] += v[i];
   }
+}
+template <int T>
+__device__ __forceinline__ void load_h(const NormArgs& a, int64_t row, int c, float (&h)[8]) {
+  Raw<T> x, r;
+  x.load(a.x + row * a.ldx, c);
+  if (a.residual) r.load(a.residual + row * a.ldr, c);
+  sum_h<T>(a, x, r, h);
 }
 template <int T>
 __device__ __forceinline__ void put16(u16* at, const float (&v)[8]) {
   *(uint4*)at = make_uint4(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]), pack16<T>(v[4], v[5]), pack16<T>(v[6], v[7]));
 }
 template <int WT>
-__device__ __forceinline__ void times_weight(const NormArgs& a, int c, float r, float (&h)[8]) {
+__device__ __forceinline__ void times_weight(const Raw<WT>& weight, float r, float (&h)[8]) {
   float w[8];
-  load8<WT>(a.weight, (size_t)c * AQ_VEC, w);
+  weight.widen(w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) h[i] = __fmul_rn(__fmul_rn(h[i], r), w[i]);
 }
@@ -130,19 +167,32 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void norm_quant_kernel(Nor
   const int at = NW == 1 ? lane : (int)threadIdx.x, pieces = a.K / AQ_VEC;
   float h[HELD][8];
   float ss = 0.0f;
+  Raw<WT> w[HELD];
   const auto add_squares = [&](const float (&v)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) ss = __fmaf_rn(v[k], v[k], ss);
   };
   if constexpr (CH > 0) {
+    // all loads at once, the weight's too; a lane past the row's end loads the last piece again (a branch around a load makes the
+    // others wait for it: one token of 4096 3.6 us so, 2.5 with one piece a lane and no branch taken)
+    Raw<T> x[CH], res[CH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int c = at + i * NT;
-      if (c < pieces) load_h<T>(a, row, c, h[i]);
+    for (int i = 0; i < CH; ++i) x[i].load(a.x + row * a.ldx, min(at + i * NT, pieces - 1));
+    if (a.residual) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) res[i].load(a.residual + row * a.ldr, min(at + i * NT, pieces - 1));
     }
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (at + i * NT < pieces) add_squares(h[i]);
+    for (int i = 0; i < CH; ++i) w[i].load(a.weight, min(at + i * NT, pieces - 1));
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      sum_h<T>(a, x[i], res[i], h[i]);
+      if (at + i * NT >= pieces) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[i][k] = 0.0f;
+      }
+      add_squares(h[i]);
+    }
   } else {
     for (int c = at; c < pieces; c += NT) {
       load_h<T>(a, row, c, h[0]);
@@ -163,16 +213,17 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void norm_quant_kernel(Nor
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = at + i * NT;
-      if (c >= pieces) continue;
-      if (a.residual_out) put16<T>(a.residual_out + row * a.ldo + (size_t)c * AQ_VEC, h[i]);
-      times_weight<WT>(a, c, r, h[i]);
-      if (a.normed) put16<T>(a.normed + row * a.ldn + (size_t)c * AQ_VEC, h[i]);
-      top = max8(h[i], top);
+      const bool in = c < pieces;
+      if (a.residual_out && in) put16<T>(a.residual_out + row * a.ldo + (size_t)c * AQ_VEC, h[i]);
+      times_weight<WT>(w[i], r, h[i]);
+      if (a.normed && in) put16<T>(a.normed + row * a.ldn + (size_t)c * AQ_VEC, h[i]);
+      if (in) top = max8(h[i], top);
     }
   } else if (!a.given) {
     for (int c = at; c < pieces; c += NT) {
+      w[0].load(a.weight, c);
       load_h<T>(a, row, c, h[0]);
-      times_weight<WT>(a, c, r, h[0]);
+      times_weight<WT>(w[0], r, h[0]);
       top = max8(h[0], top);
     }
   }
@@ -202,9 +253,10 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void norm_quant_kernel(Nor
     }
   } else {
     for (int c = at; c < pieces; c += NT) {  // (each piece is read by the thread that writes it: residual_out may be x or residual)
+      w[0].load(a.weight, c);
       load_h<T>(a, row, c, h[0]);
       if (a.residual_out) put16<T>(a.residual_out + row * a.ldo + (size_t)c * AQ_VEC, h[0]);
-      times_weight<WT>(a, c, r, h[0]);
+      times_weight<WT>(w[0], r, h[0]);
       if (a.normed) put16<T>(a.normed + row * a.ldn + (size_t)c * AQ_VEC, h[0]);
       *(uint2*)(q + (size_t)c * AQ_VEC) = codes8<E4M3>(h[0], s, inverse, given);
     }
@@ -225,13 +277,24 @@ static void run_norm(const NormArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((norm_quant_kernel<T, WT, E4M3, NW, CH>), grid, block, 0, s, a);
   };
 #define GO(nw, ch) go(std::integral_constant<int, nw>{}, std::integral_constant<int, ch>{})
+  // Few rows: a piece a lane, which is the shortest way through a row (one token of 4096: 2.4 us, 3.2 with two pieces, 4.3 with four; 64 tokens
+  // 3.9, 4.6, 5.8).  Many: two, with which more rows are on their way (8192 tokens 39.5, 37.6, 38.4; 1777 of 12800: 19.8 with two, 18.2 with four).
+  const bool many = a.rows >= 1024;
   if (a.K <= 512) GO(1, 1);
-  else if (a.K <= 1024) GO(1, 2);
+  else if (a.K <= 1024) GO(2, 1);
   else if (a.K <= 2048) GO(4, 1);
-  else if (a.K <= 4096) GO(4, 2);
-  else if (a.K <= 8192) GO(8, 2);
-  else if (a.K <= 16384) GO(8, 4);
-  else GO(16, 0);
+  else if (a.K <= 4096) {
+    if (many) GO(4, 2);
+    else GO(8, 1);
+  } else if (a.K <= 8192) {
+    if (many) GO(8, 2);
+    else GO(16, 1);
+  } else if (a.K <= 16384) {
+    if (many) GO(8, 4);
+    else GO(16, 2);
+  } else {
+    GO(16, 0);
+  }
 #undef GO
 }
 

@@ -40,7 +40,7 @@ def check(x, w, res, got, code, eps, scale=None):
 
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("code", [I8, E4M3])
-@pytest.mark.parametrize("T,cols", [(1, 8), (1, 4096), (3, 64), (5, 72), (7, 512), (4, 520), (9, 1024), (2, 1032), (6, 2048), (33, 4096), (3, 4104),
+@pytest.mark.parametrize("T,cols", [(1030, 264), (1100, 4096), (1025, 5120), (1024, 9000), (1, 8), (1, 4096), (3, 64), (5, 72), (7, 512), (4, 520), (9, 1024), (2, 1032), (6, 2048), (33, 4096), (3, 4104),
                                     (2, 8192), (3, 12800), (1, 16384), (2, 16392), (1, 40000)])
 def test_rows(dev, dt, code, T, cols):
     g = gen(T * cols)
