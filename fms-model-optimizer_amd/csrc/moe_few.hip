@@ -11,6 +11,8 @@
 #include "paged_kv.hpp"
 #include "stream_loads.hpp"
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace fmsmo {
@@ -40,6 +42,7 @@ struct MoeArgs {
   float* hs;        // [T top]
   float* h;         // [T top][I]
   uint8_t* hq;      // [T top][I]
+  float* parts;     // [splits][T][K] of the down product, where blocks share outputs
   uint32_t* tops;   // [T top][I / 8] largest |h| of eight, as integers; NULL: not wanted
 };
 // A group of tokens of one expert: expert, tokens and first position in one number.
@@ -252,20 +255,40 @@ __device__ __forceinline__ void moe_mfma(typename MoeAcc<OP>::type& c, v4i w0, v
     }
   }
 }
+// Weights are loaded as 16 rows of 256 bytes, four rows a load.  Where rows are no multiples of 128 bytes, the lines at the ends of a piece are
+// its neighbours' too, and weights stay in the caches (KEEP: 16 tokens over 8 experts of 4112 x 14352 gate and up 194 us, 203 streamed; 47 over 32 of
+// 656 x 3264 48 and 53); else they are read past them (64 tokens over 128 experts of 2048 x 768 67 us, 77 kept).
+constexpr int MOE_STEP = 256;
+template <bool KEEP>
+__device__ __forceinline__ v4i moe_weights(Buf b, uint32_t off, uint32_t uniform_off) {
+  return KEEP ? buf_load(b, off, uniform_off) : buf_stream(b, off, uniform_off);
+}
+// Four loads into shared memory, the first 128 bytes of the 16 rows and then the others, chunk c of row q at position c ^ (q % 8)
+__device__ __forceinline__ void moe_stage(uint8_t* st, const v4i (&w)[4]) {
+  const int lane = threadIdx.x & 63, row = lane >> 4, c = lane & 15;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int q = 4 * i + row;
+    *(v4i*)(st + (c >> 3) * 2048 + q * 128 + (((c ^ q) & 7) * 16)) = w[i];
+  }
+  __builtin_amdgcn_wave_barrier();  // (the rows go to other lanes of the wave)
+}
+
 // h of the positions.  A unit: eight gate rows and the eight up rows that belong to them, for one group of tokens: the 16 rows of the
-// product.  The four waves of a block share its K, every fourth step of 128 bytes each, D steps on their way, those of the next unit among
-// them; the waves' sums meet in shared memory, one barrier a unit, and a wave in turn finishes it.
-template <int OP, int MT, int D, bool ROUTE>
-__global__ __launch_bounds__(256, MT == 1 && D == 2 ? 4 : 2) void moe_up_kernel(MoeArgs a) {
+// product.  D steps of 256 bytes a row are on their way, those of the next unit among them.  SHARE: the four waves of a block share a unit's K,
+// every fourth step each; their sums meet in shared memory, one barrier a unit, and a wave in turn finishes it.  Else each wave has units of its own.
+template <int OP, int MT, int D, bool ROUTE, bool SHARE, bool KEEP>
+__global__ __launch_bounds__(256, MT == 1 && D < 4 ? 4 : 2) void moe_up_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
   __shared__ MoeLists lists;
-  __shared__ __attribute__((aligned(16))) uint8_t stage[4][2048];
-  __shared__ __attribute__((aligned(16))) Acc part[2][4][MT][64];
+  __shared__ __attribute__((aligned(16))) uint8_t stage[4][4096];
+  __shared__ __attribute__((aligned(16))) Acc part[SHARE ? 2 : 1][SHARE ? 4 : 1][MT][64];
   make_lists<256, MT, ROUTE>(a, lists);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4, drow = lane >> 3, dpos = lane & 7;
+  const int r = lane & 15, g = lane >> 4;  // operands: row or column r, 16-byte pieces g and 4 + g; loads: rows g, 4 + g, .., piece r
   const int groups = a.I / 8, units = lists.count * groups;
-  const int steps = ((a.K + 511) / 512 + D - 1) / D * D;  // of a wave
+  constexpr int KS = SHARE ? 4 : 1;
+  const int steps = ((a.K + MOE_STEP * KS - 1) / (MOE_STEP * KS) + D - 1) / D * D;  // of a wave
   uint8_t* st = stage[wave];
   const int rr = r & 7;
   struct Unit {
@@ -283,35 +306,36 @@ __global__ __launch_bounds__(256, MT == 1 && D == 2 ? 4 : 2) void moe_up_kernel(
     q.gi = there ? u - en * groups : 0;
     q.m = group_of(uniform((int)lists.entry[en]));
     q.w = buf_of(a.w13 + (int64_t)q.m.e * 2 * a.I * a.K);
-    q.wo = there ? (uint32_t)(q.gi * 8 + drow) * (uint32_t)a.K + dpos * 16 : BUF_NONE;
+    q.wo = there ? (uint32_t)(q.gi * 8 + g) * (uint32_t)a.K + r * 16 : BUF_NONE;
 #pragma unroll
     for (int j = 0; j < MT; ++j)
       q.xo[j] = there && 16 * j + r < q.m.cnt ? lists.token[q.m.off + 16 * j + r] * (uint32_t)a.lda + g * 16 : BUF_NONE;
     return q;
   };
   const uint32_t up = (uint32_t)a.I * (uint32_t)a.K;
-  v4i wb[D][2], xb[D][MT][2];
+  v4i wb[D][4], xb[D][MT][4];
   const auto fetch = [&](const Unit& q, int s, int d) {
-    const uint32_t k = (s * 4 + wave) * 128;
+    const uint32_t k = (SHARE ? s * 4 + wave : s) * MOE_STEP;
     const int left = a.K - (int)k;
-    const uint32_t wo = dpos * 16 < left ? q.wo : BUF_NONE;
-    wb[d][0] = buf_stream(q.w, wo, k);
-    wb[d][1] = buf_stream(q.w, wo, k + up);
+    const uint32_t wo = r * 16 < left ? q.wo : BUF_NONE;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wb[d][i] = moe_weights<KEEP>(q.w, wo, k + (i & 1) * 4 * a.K + (i >> 1) * up);
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       if (MT > 1 && 16 * j >= q.m.cnt) break;
-      xb[d][j][0] = buf_load(xb_of, g * 16 < left ? q.xo[j] : BUF_NONE, k);
-      xb[d][j][1] = buf_load(xb_of, g * 16 + 64 < left ? q.xo[j] : BUF_NONE, k + 64);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xb[d][j][i] = buf_load(xb_of, g * 16 + 64 * i < left ? q.xo[j] : BUF_NONE, k + 64 * i);
     }
   };
-  if ((int)blockIdx.x >= units) return;
-  Unit cur = unit_of(blockIdx.x);
+  const int first = SHARE ? blockIdx.x : blockIdx.x * 4 + wave, stride = SHARE ? gridDim.x : gridDim.x * 4;
+  if (first >= units) return;
+  Unit cur = unit_of(first);
 #pragma unroll
   for (int d = 0; d < D; ++d) fetch(cur, d, d);
   int turn = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x, ++turn) {
-    const Unit next = unit_of(u + gridDim.x);
-    const bool finish = (turn & 3) == wave;
+  for (int u = first; u < units; u += stride, ++turn) {
+    const Unit next = unit_of(u + stride);
+    const bool finish = !SHARE || (turn & 3) == wave;
     float sg[4], su[4], as[MT];
     if (finish) {  // asked for ahead of the products
       const float* sc = a.s13 + (int64_t)cur.m.e * 2 * a.I + cur.gi * 8 + 4 * (g & 1);
@@ -330,30 +354,34 @@ __global__ __launch_bounds__(256, MT == 1 && D == 2 ? 4 : 2) void moe_up_kernel(
       const bool last = s + D >= steps;
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        *(v4i*)(st + drow * 128 + ((dpos ^ drow) * 16)) = wb[d][0];
-        *(v4i*)(st + (8 + drow) * 128 + ((dpos ^ drow) * 16)) = wb[d][1];
-        __builtin_amdgcn_wave_barrier();
-        const v4i w0 = *(const v4i*)(st + r * 128 + ((g ^ rr) * 16));
-        const v4i w1 = *(const v4i*)(st + r * 128 + (((4 + g) ^ rr) * 16));
-        __builtin_amdgcn_wave_barrier();
+        moe_stage(st, wb[d]);
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          if (MT > 1 && 16 * j >= cur.m.cnt) break;
-          moe_mfma<OP>(acc[j], w0, w1, xb[d][j][0], xb[d][j][1]);
+        for (int h = 0; h < 2; ++h) {
+          const v4i w0 = *(const v4i*)(st + h * 2048 + r * 128 + ((g ^ rr) * 16));
+          const v4i w1 = *(const v4i*)(st + h * 2048 + r * 128 + (((4 + g) ^ rr) * 16));
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            if (MT > 1 && 16 * j >= cur.m.cnt) break;
+            moe_mfma<OP>(acc[j], w0, w1, xb[d][j][2 * h], xb[d][j][2 * h + 1]);
+          }
         }
+        __builtin_amdgcn_wave_barrier();
         fetch(last ? next : cur, last ? d : s + D + d, d);
       }
     }
-    Acc(*mine)[MT][64] = part[turn & 1];
+    Acc(*mine)[MT][64] = part[SHARE ? turn & 1 : 0];
+    if constexpr (SHARE) {
 #pragma unroll
-    for (int j = 0; j < MT; ++j) mine[wave][j][lane] = acc[j];
-    __syncthreads();
+      for (int j = 0; j < MT; ++j) mine[wave][j][lane] = acc[j];
+      __syncthreads();
+    }
     if (finish) {
       // lane (r, g): column r, rows 4 g .. + 3: gate rows in the lower half of the wave, their up rows 32 lanes on
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
         if (16 * j >= cur.m.cnt) break;
-        const Acc sum = (mine[0][j][lane] + mine[1][j][lane]) + (mine[2][j][lane] + mine[3][j][lane]);
+        Acc sum = acc[j];
+        if constexpr (SHARE) sum = (mine[0][j][lane] + mine[1][j][lane]) + (mine[2][j][lane] + mine[3][j][lane]);
         v4f h;
         uint32_t top = 0;
 #pragma unroll
@@ -427,28 +455,35 @@ __global__ __launch_bounds__(256) void moe_quant_kernel(MoeArgs a) {
   if (in) ((uint32_t*)(a.hq + (int64_t)pos * a.I))[i] = moe_codes<OP>(v, s);
 }
 
-// y.  A block owns ROWS outputs and goes through all groups of tokens: their steps of 128 bytes one behind the other, cut into equal parts
+__device__ __forceinline__ void moe_put(const MoeArgs& a, int tok, int n, float v) {
+  const int64_t at = tok * a.ldy + n;
+  if (a.y_dtype == FMSMO_F16) ((u16*)a.y)[at] = f32_to_f16(v);
+  else if (a.y_dtype == FMSMO_BF16) ((u16*)a.y)[at] = f32_to_bf16(v);
+  else ((float*)a.y)[at] = v;
+}
+// y.  A block owns ROWS outputs and goes through all groups of tokens: their steps of 256 bytes one behind the other, cut into equal parts
 // for the waves, D steps on their way; at the end of a group a wave adds its products, with their scales and shares, to sums of its own, and the
-// waves' sums are added in their order.  ROWS = 8, groups of up to eight tokens: a product takes two steps, the first with its upper eight rows and
+// waves' sums are added in their order.  Where few outputs leave units without a block, several blocks share the steps of the same outputs
+// and a kernel behind adds what they leave.  ROWS = 8, groups of up to eight tokens: a product takes two steps, the first with its upper eight rows and
 // left eight columns, the second with the others, and the two blocks on its diagonal are added.  QUANT: few positions, whose codes every block makes for itself in shared memory.
 // Up to TM tokens.
 constexpr int MOE_QUANT_MOST = 8192;
-template <int OP, int MT, int ROWS, int NW, int D, int TM, bool QUANT>
+template <int OP, int MT, int ROWS, int NW, int D, int TM, bool QUANT, bool KEEP>
 __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
   constexpr int NT = NW * 64;
   constexpr bool PAIR = ROWS == 8;  // two steps a product
   static_assert(!PAIR || MT == 1, "");
-  constexpr int STEP = PAIR ? 256 : 128;
-  __shared__ __attribute__((aligned(16))) uint8_t stage[NW][2048];
+  constexpr int WL = PAIR ? 2 : 4;  // loads of a step
+  __shared__ __attribute__((aligned(16))) uint8_t stage[NW][1024 * WL];
   __shared__ uint32_t entry[MOE_ENTRIES];
   __shared__ uint8_t token[MOE_TOKENS * MOE_TOP];
   __shared__ float share[MOE_TOKENS * MOE_TOP];
   __shared__ __attribute__((aligned(16))) float sums[NW * TM * ROWS];
   __shared__ __attribute__((aligned(16))) uint8_t codes[QUANT ? MOE_QUANT_MOST : 16];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4, drow = lane >> 3, dpos = lane & 7;
-  const int n0 = blockIdx.x * ROWS, steps = (a.I + STEP - 1) / STEP, pairs = a.T * a.top;
+  const int r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * ROWS, steps = (a.I + MOE_STEP - 1) / MOE_STEP, pairs = a.T * a.top;
   const int count = a.count[0], all = count * steps;
   for (int i = threadIdx.x; i < count; i += NT) entry[i] = a.entry[i];
   // (positions that no pair took hold what was there before: they are not in any group)
@@ -459,7 +494,8 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   }
   for (int i = threadIdx.x; i < NW * a.T * ROWS; i += NT) sums[i] = 0.0f;
   __syncthreads();
-  const int from = (int)((int64_t)wave * all / NW), to = (int)((int64_t)(wave + 1) * all / NW);
+  const int part = blockIdx.y * NW + wave, parts = gridDim.y * NW;
+  const int from = (int)((int64_t)part * all / parts), to = (int)((int64_t)(part + 1) * all / parts);
   uint8_t* st = stage[wave];
   const int rr = r & 7;
   int le = steps ? from / steps : 0, ls = from - le * steps, ce = le, cs = ls;  // what is loaded and what is multiplied next: group and step
@@ -472,23 +508,24 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   const auto load_from = [&] {
     lm = group_of(uniform((int)entry[le]));
     w = buf_of(a.w2 + (int64_t)lm.e * a.K * a.I);
-    wo = (uint32_t)(n0 + drow) * (uint32_t)a.I + dpos * 16;
+    wo = (uint32_t)(n0 + g) * (uint32_t)a.I + r * 16;
 #pragma unroll
     for (int j = 0; j < MT; ++j) xo[j] = 16 * j + col < lm.cnt ? (uint32_t)(lm.off + 16 * j + col) * (uint32_t)a.I + half + g * 16 : BUF_NONE;
   };
-  v4i wb[D][2], xb[QUANT ? 1 : D][MT][2];
+  constexpr int XL = PAIR ? 2 : 4;
+  v4i wb[D][WL], xb[QUANT ? 1 : D][MT][XL];
   int loads = to - from;  // steps that are not on their way yet; behind the last one zeros are loaded
   const auto fetch = [&](int d) {
-    const uint32_t k = ls * STEP;
+    const uint32_t k = ls * MOE_STEP;
     const int left = loads > 0 ? a.I - (int)k : 0;
-    wb[d][0] = buf_stream(w, dpos * 16 < left ? wo : BUF_NONE, k);
-    wb[d][1] = PAIR ? buf_stream(w, dpos * 16 + 128 < left ? wo : BUF_NONE, k + 128) : buf_stream(w, dpos * 16 < left ? wo : BUF_NONE, k + 8 * a.I);
+#pragma unroll
+    for (int i = 0; i < WL; ++i) wb[d][i] = moe_weights<KEEP>(w, r * 16 < left ? wo : BUF_NONE, k + i * 4 * a.I);
     if constexpr (!QUANT) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
         if (MT > 1 && 16 * j >= lm.cnt) break;
-        xb[d][j][0] = buf_load(xb_of, half + g * 16 < left ? xo[j] : BUF_NONE, k);
-        xb[d][j][1] = buf_load(xb_of, half + g * 16 + 64 < left ? xo[j] : BUF_NONE, k + 64);
+#pragma unroll
+        for (int i = 0; i < XL; ++i) xb[d][j][i] = buf_load(xb_of, half + g * 16 + 64 * i < left ? xo[j] : BUF_NONE, k + 64 * i);
       }
     }
     --loads;
@@ -558,28 +595,38 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
     for (int f = from; f < to; f += D) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        *(v4i*)(st + drow * 128 + ((dpos ^ drow) * 16)) = wb[d][0];
-        *(v4i*)(st + (8 + drow) * 128 + ((dpos ^ drow) * 16)) = wb[d][1];
-        __builtin_amdgcn_wave_barrier();
-        const v4i w0 = *(const v4i*)(st + r * 128 + ((g ^ rr) * 16));
-        const v4i w1 = *(const v4i*)(st + r * 128 + (((4 + g) ^ rr) * 16));
-        __builtin_amdgcn_wave_barrier();
+        if constexpr (PAIR) {  // rows 0 .. 7 of the product: the first 128 bytes of the eight rows, rows 8 .. 15: the others
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          if (MT > 1 && 16 * j >= cm.cnt) break;
-          v4i x0, x1;
-          if constexpr (QUANT) {
-            const int k = cs * STEP + half + g * 16;
-            const bool v = 16 * j + col < cm.cnt;
-            x0 = x1 = v4i{0, 0, 0, 0};
-            if (v && k < a.I) x0 = *(const v4i*)(codes + (cm.off + 16 * j + col) * a.I + k);
-            if (v && k + 64 < a.I) x1 = *(const v4i*)(codes + (cm.off + 16 * j + col) * a.I + k + 64);
-          } else {
-            x0 = xb[d][j][0];
-            x1 = xb[d][j][1];
+          for (int i = 0; i < 2; ++i) {
+            const int q = 4 * i + g;
+            *(v4i*)(st + (r >> 3) * 1024 + q * 128 + (((r ^ q) & 7) * 16)) = wb[d][i];
           }
-          moe_mfma<OP>(acc[j], w0, w1, x0, x1);
+          __builtin_amdgcn_wave_barrier();
+        } else {
+          moe_stage(st, wb[d]);
         }
+#pragma unroll
+        for (int h = 0; h < WL / 2; ++h) {
+          const v4i w0 = *(const v4i*)(st + h * 2048 + r * 128 + ((g ^ rr) * 16));
+          const v4i w1 = *(const v4i*)(st + h * 2048 + r * 128 + (((4 + g) ^ rr) * 16));
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            if (MT > 1 && 16 * j >= cm.cnt) break;
+            v4i x0, x1;
+            if constexpr (QUANT) {
+              const int k = cs * MOE_STEP + 128 * h + half + g * 16;
+              const bool v = 16 * j + col < cm.cnt;
+              x0 = x1 = v4i{0, 0, 0, 0};
+              if (v && k < a.I) x0 = *(const v4i*)(codes + (cm.off + 16 * j + col) * a.I + k);
+              if (v && k + 64 < a.I) x1 = *(const v4i*)(codes + (cm.off + 16 * j + col) * a.I + k + 64);
+            } else {
+              x0 = xb[d][j][2 * h];
+              x1 = xb[d][j][2 * h + 1];
+            }
+            moe_mfma<OP>(acc[j], w0, w1, x0, x1);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
         fetch(d);
         if (f + d < to && (++cs == steps || f + d + 1 == to)) {
           end();
@@ -595,11 +642,17 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
     float v = sums[i];
 #pragma unroll
     for (int w = 1; w < NW; ++w) v += sums[w * a.T * ROWS + i];
-    const int64_t at = i / ROWS * a.ldy + n0 + i % ROWS;
-    if (a.y_dtype == FMSMO_F16) ((u16*)a.y)[at] = f32_to_f16(v);
-    else if (a.y_dtype == FMSMO_BF16) ((u16*)a.y)[at] = f32_to_bf16(v);
-    else ((float*)a.y)[at] = v;
+    const int tok = i / ROWS, n = n0 + i % ROWS;
+    if (gridDim.y > 1) a.parts[((int64_t)blockIdx.y * a.T + tok) * a.K + n] = v;
+    else moe_put(a, tok, n, v);
   }
+}
+__global__ __launch_bounds__(256) void moe_join_kernel(MoeArgs a, int splits) {
+  const int n = blockIdx.x * 256 + threadIdx.x, tok = blockIdx.y;
+  if (n >= a.K) return;
+  float v = 0.0f;
+  for (int s = 0; s < splits; ++s) v += a.parts[((int64_t)s * a.T + tok) * a.K + n];
+  moe_put(a, tok, n, v);
 }
 
 }  // namespace fmsmo
@@ -612,11 +665,45 @@ static bool moe_sizes(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   return T >= 0 && T <= MOE_TOKENS && E >= 1 && E <= MOE_EXPERTS && top >= 1 && top <= MOE_TOP && top <= E && K >= 16 && I >= 16 && K % 16 == 0 &&
          I % 16 == 0 && K < 1 << 20 && I < 1 << 20 && 2 * I * K <= 0x7f000000;  // (an expert's weights are counted in 32 bits)
 }
+// What a call is cut into.
+struct MoePlan {
+  int mt;       // tiles of 16 tokens of a group
+  bool narrow;  // the down product's blocks have eight outputs
+  bool quant;   // and make the codes of h themselves
+  bool share;   // the waves of a block share a unit of the gate and up products
+  bool deep;    // eight steps on their way there
+  int splits;   // blocks for the same outputs
+};
+static MoePlan moe_plan(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
+  MoePlan p;
+  // (with up to six tokens an expert on average, few have more than sixteen: those stream their weights twice)
+  p.mt = T <= 16 || T * top <= 6 * E ? 1 : T <= 32 ? 2 : 4;
+  const int64_t used = std::min(E, T * top);
+  // Waves with units of their own where rows are short and units many (13 tokens over 32 experts of 1024 x 14080: 160 us, 176 shared; 16 over 8 of
+  // 4096 x 14336: 159 and 151; one token over 128 of 2048 x 768: 12.4 and 9.5).  Four steps on their way where a wave has a multiple of four for a
+  // unit (K = 4096: 151 us, 177 with one).
+  p.share = K >= 2048 || used * (I / 8) < 4096;
+  p.deep = p.mt == 1 && p.share && div_up(K, 1024) % 4 == 0;
+  // The down product: a compute unit takes in 23 GB/s, a little less on eight rows, so that what counts is how evenly the blocks fall on the units
+  // (8 experts, 14336 -> 4096 columns, 256 blocks: 71 us, 4112 columns, 257 blocks: 137); a split is a launch more.
+  const double bytes = (double)used * K * I;
+  double best = 1e30;
+  p.narrow = false;
+  p.splits = 1;
+  for (int narrow = p.mt == 1; narrow >= 0; --narrow)
+    for (int n = 1; n <= 8; ++n) {
+      const double blocks = (double)n * (double)(K / (narrow ? 8 : 16));
+      const double cost = std::ceil(blocks / 256) * bytes / blocks / (narrow ? 21e9 : 23e9) + (n > 1 ? 4e-6 : 0.0);
+      if (cost < best * 0.98) best = cost, p.narrow = narrow, p.splits = n;
+    }
+  p.quant = p.mt == 1 && T * top <= 8 && T * top * I <= MOE_QUANT_MOST;
+  return p;
+}
 // bytes up to each piece of the workspace
 struct MoeSpace {
-  int64_t ids, share, entry, token, weight, hs, h, hq, tops, all;
+  int64_t ids, share, entry, token, weight, hs, h, hq, tops, parts, all;
 };
-static MoeSpace moe_space(int64_t T, int top, int64_t I) {
+static MoeSpace moe_space(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   const int64_t P = T * top, p16 = (P + 3) / 4 * 16;
   MoeSpace s;
   s.ids = 16;
@@ -628,58 +715,65 @@ static MoeSpace moe_space(int64_t T, int top, int64_t I) {
   s.h = s.hs + p16;
   s.hq = s.h + 4 * P * I;
   s.tops = s.hq + P * I;
-  s.all = s.tops + P * I / 2;
+  s.parts = s.tops + P * I / 2;
+  const int splits = moe_plan(T, E, top, K, I).splits;
+  s.all = s.parts + (splits > 1 ? 4 * splits * T * K : 0);
   return s;
 }
 
 extern "C" int64_t fmsmo_moe_few_workspace_bytes(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
-  return moe_sizes(T, E, top, K, I) && T ? moe_space(T, top, I).all : 0;
+  return moe_sizes(T, E, top, K, I) && T ? moe_space(T, E, top, K, I).all : 0;
 }
 
-template <int OP, int MT, int ROWS, bool QUANT>
-static void run_down(const MoeArgs& a, hipStream_t s) {
-  // waves and steps on their way: eight rows want more waves (64 tokens over 128 experts: 41 us with 16 and 2, 43 with 12 and 4, 50 with 8 and 4,
-  // 54 with 16 and 4, whose registers do not suffice), sixteen are indifferent
-  constexpr int NW = ROWS == 8 ? 16 : 8, D = ROWS == 8 ? 2 : 4;
-  const dim3 grid((unsigned)(a.K / ROWS)), block(NW * 64);
-  if (MT > 1 || a.T > 16) hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, 64, QUANT>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((moe_down_kernel<OP, 1, ROWS, NW, D, 16, QUANT>), grid, block, 0, s, a);
+template <int OP, int MT, int ROWS, bool QUANT, bool KEEP>
+static void run_down(const MoeArgs& a, int splits, hipStream_t s) {
+  // waves and steps on their way: eight rows want more waves (64 tokens over 128 experts: 41 us with 16 and 2, 50 with 8 and 4, 54 with 16 and 4,
+  // whose registers do not suffice), sixteen are indifferent
+  constexpr int NW = ROWS == 8 ? 16 : 8, D = 2;
+  const dim3 grid((unsigned)(a.K / ROWS), (unsigned)splits), block(NW * 64);
+  if (MT > 1 || a.T > 16) hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, 64, QUANT, KEEP>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((moe_down_kernel<OP, 1, ROWS, NW, D, 16, QUANT, KEEP>), grid, block, 0, s, a);
 }
-template <int OP, int MT>
-static void run_moe(MoeArgs a, hipStream_t s) {
-  const bool quant = MT == 1 && a.T * a.top <= 8 && a.T * a.top * a.I <= MOE_QUANT_MOST, narrow = MT == 1 && a.K / 16 < 256;
-  if (quant) a.tops = nullptr;
-  a.down_group = narrow ? 8 : 16 * MT;
-  // Groups of tokens, at most.  Eight steps on their way where a wave has a multiple of eight for a unit (K = 4096, 16 tokens over 8 experts of
-  // 14336: 150 us, 156 with two; 2048 has four, 91 and 67 us with 64 tokens over 128 experts of 768).
+template <int OP, int MT, int D, bool SHARE, bool KEEP>
+static void run_up(const MoeArgs& a, hipStream_t s) {
+  // groups of tokens, at most
   const int64_t units = (int64_t)std::min(MT == 1 ? a.E + a.T * a.top / 16 : a.E, a.T * a.top) * (a.I / 8);
-  const bool deep = MT == 1 && div_up(a.K, 512) % 8 == 0;
-  const dim3 grid((unsigned)std::min<int64_t>(units, MT > 1 || deep ? 512 : 1024)), block(256);
-  if (a.T > 8) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), block, 0, s, a);
+  const dim3 grid((unsigned)std::min<int64_t>(SHARE ? units : div_up(units, 4), MT > 1 || D > 1 ? 512 : 1024)), block(256);
   if constexpr (MT == 1) {
     if (a.T <= 8) {
-      if (deep) hipLaunchKernelGGL((moe_up_kernel<OP, 1, 8, true>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((moe_up_kernel<OP, 1, 2, true>), grid, block, 0, s, a);
-    } else {
-      if (deep) hipLaunchKernelGGL((moe_up_kernel<OP, 1, 8, false>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((moe_up_kernel<OP, 1, 2, false>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((moe_up_kernel<OP, 1, D, true, SHARE, KEEP>), grid, block, 0, s, a);
+      return;
     }
-  } else {
-    hipLaunchKernelGGL((moe_up_kernel<OP, MT, 2, false>), grid, block, 0, s, a);
   }
-  if (!quant) hipLaunchKernelGGL((moe_quant_kernel<OP>), dim3((unsigned)(a.T * a.top), (unsigned)div_up(a.I, MOE_QUANT)), dim3(256), 0, s, a);
-  if constexpr (MT == 1) {
-    if (narrow) {
-      if (quant) run_down<OP, 1, 8, true>(a, s);
-      else run_down<OP, 1, 8, false>(a, s);
-    } else if (quant) {
-      run_down<OP, 1, 16, true>(a, s);
-    } else {
-      run_down<OP, 1, 16, false>(a, s);
+  hipLaunchKernelGGL((moe_up_kernel<OP, MT, D, false, SHARE, KEEP>), grid, block, 0, s, a);
+}
+template <int OP, int MT>
+static void run_moe(MoeArgs a, const MoePlan& p, hipStream_t s) {
+  if (p.quant) a.tops = nullptr;
+  a.down_group = p.narrow ? 8 : 16 * MT;
+  if (a.T > 8) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), dim3(256), 0, s, a);
+  const auto up = [&](auto keep) {
+    constexpr bool KEEP = decltype(keep)::value;
+    if (!p.share) return run_up<OP, MT, 1, false, KEEP>(a, s);
+    if constexpr (MT == 1) {
+      if (p.deep) return run_up<OP, 1, 4, true, KEEP>(a, s);
     }
-  } else {
-    run_down<OP, MT, 16, false>(a, s);
-  }
+    run_up<OP, MT, 1, true, KEEP>(a, s);
+  };
+  const auto down = [&](auto keep) {
+    constexpr bool KEEP = decltype(keep)::value;
+    if constexpr (MT == 1) {
+      if (p.narrow) return p.quant ? run_down<OP, 1, 8, true, KEEP>(a, p.splits, s) : run_down<OP, 1, 8, false, KEEP>(a, p.splits, s);
+      if (p.quant) return run_down<OP, 1, 16, true, KEEP>(a, p.splits, s);
+    }
+    run_down<OP, MT, 16, false, KEEP>(a, p.splits, s);
+  };
+  if (a.K % 128) up(std::true_type{});
+  else up(std::false_type{});
+  if (!p.quant) hipLaunchKernelGGL((moe_quant_kernel<OP>), dim3((unsigned)(a.T * a.top), (unsigned)div_up(a.I, MOE_QUANT)), dim3(256), 0, s, a);
+  if (a.I % 128) down(std::true_type{});
+  else down(std::false_type{});
+  if (p.splits > 1) hipLaunchKernelGGL(moe_join_kernel, dim3((unsigned)div_up(a.K, 256), (unsigned)a.T), dim3(256), 0, s, a, p.splits);
 }
 
 extern "C" int fmsmo_moe_few_tokens(int codes, const void* a, int64_t lda, const float* a_scale, int64_t a_scale_n, const void* logits,
@@ -696,18 +790,19 @@ extern "C" int fmsmo_moe_few_tokens(int codes, const void* a, int64_t lda, const
   const auto off = [](const void* p) { return (((uintptr_t)p) & 15) != 0; };
   if (T > 1 && lda > 1 << 24) return FMSMO_ERR_UNSUPPORTED;
   if (off(a) || off(w13) || off(w2) || off(w2_scale) || off(workspace) || (T > 1 && lda % 16)) return FMSMO_ERR_ALIGN;
-  const MoeSpace sp = moe_space(T, top, I);
+  const MoeSpace sp = moe_space(T, E, top, K, I);
   if (workspace_bytes < sp.all) return FMSMO_ERR_SCRATCH;
   char* ws = (char*)workspace;
   MoeArgs g{(const uint8_t*)a, a_scale, logits, (const uint8_t*)w13, w13_scale, (const uint8_t*)w2, w2_scale, y, lda, ldl, ldy,
             a_scale_n == 1 ? 0 : 1, logits_dtype, y_dtype, (int)T, (int)E, top, (int)K, (int)I, renormalize != 0, 0,
             (int*)(ws + sp.ids), (float*)(ws + sp.share), (int*)ws, (uint32_t*)(ws + sp.entry), (int*)(ws + sp.token), (float*)(ws + sp.weight),
-            (float*)(ws + sp.hs), (float*)(ws + sp.h), (uint8_t*)(ws + sp.hq), (uint32_t*)(ws + sp.tops)};
+            (float*)(ws + sp.hs), (float*)(ws + sp.h), (uint8_t*)(ws + sp.hq), (float*)(ws + sp.parts), (uint32_t*)(ws + sp.tops)};
+  const MoePlan p = moe_plan(T, E, top, K, I);
   const auto tiles = [&](auto op) {
     constexpr int OP = decltype(op)::value;
-    if (T <= 16 || T * top <= 6 * E) run_moe<OP, 1>(g, (hipStream_t)stream);
-    else if (T <= 32) run_moe<OP, 2>(g, (hipStream_t)stream);
-    else run_moe<OP, 4>(g, (hipStream_t)stream);
+    if (p.mt == 1) run_moe<OP, 1>(g, p, (hipStream_t)stream);
+    else if (p.mt == 2) run_moe<OP, 2>(g, p, (hipStream_t)stream);
+    else run_moe<OP, 4>(g, p, (hipStream_t)stream);
   };
   if (codes == FMSMO_OP_I8) tiles(std::integral_constant<int, FMSMO_OP_I8>{});
   else tiles(std::integral_constant<int, FMSMO_OP_E4M3>{});
