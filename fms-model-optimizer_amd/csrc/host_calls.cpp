@@ -1053,7 +1053,7 @@ PyObject* lora_add(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   at::Tensor out;
   Mat o;
   if (!here(x.t, y.t, a, b, ids, qs, sc) || !matrix_of(args[7], x.rows, N, st, *x.t, &out, &o) || !here(&out)) return none();
-  const at::Tensor ws = workspace(p_fmsmo_lora_workspace_bytes(x.rows, seqs, qs != nullptr, (int)r, K), *x.t);
+  const at::Tensor ws = workspace(p_fmsmo_lora_workspace_bytes(x.rows, seqs, qs != nullptr, S, (int)r, K), *x.t);
   if (!ws.defined()) return none();
   if (!LAUNCH(fmsmo_lora_add, code_of(st), x.p, x.ld, y.p, y.ld, o.p, o.ld, a->data_ptr(), a_slot, a_row, b->data_ptr(), b_slot, b_row, S, (int)r,
               (const int32_t*)ids->data_ptr(), qs ? (const int32_t*)qs->data_ptr() : nullptr, seqs, sc ? (const float*)sc->data_ptr() : nullptr,

@@ -372,39 +372,43 @@ int fmsmo_check_launch();
 
 // Steps on their way of a wave of the first launch on tiles of 64 rows: what the registers hold.
 static constexpr int lora_depth(int rt) { return rt <= 2 ? 4 : rt == 4 ? 2 : 1; }
-// What a call is cut into.  Rows: tiles of 64 where a request has 32 on average, else of 16.  Few rows: parts of K for about 512 blocks, a step
-// of 64 elements for each of their four waves at least, and of the outputs for about 768.  Many: a compute unit takes in about 23 GB/s however
-// many blocks it has once 128 KB are on their way, so that what counts is how evenly the blocks fall on the units (8192 rows of 14336: 393 blocks with
-// two steps a wave 63 us, 512 50, 256 with four steps 45 and with two 73); a part more costs its share of v in memory, a block of the second
-// launch as much as one group of outputs.
+// What a call is cut into.  Rows: tiles of 64 where a request has 32 on average, else of 16.
 struct LoraPlan {
   int mt, rt, tiles, parts, part_steps, cols;
 };
-static LoraPlan lora_plan(int64_t rows, int64_t seqs, bool ragged, int rank, int64_t K, int64_t N) {
+static LoraPlan lora_plan(int64_t rows, int64_t seqs, bool ragged, int64_t slots, int rank, int64_t K, int64_t N) {
   LoraPlan p;
   p.mt = ragged && rows >= 32 * seqs ? 4 : 1;
   p.rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
   p.tiles = (int)(ragged ? rows / (16 * p.mt) + seqs + 2 : seqs);
   const int steps = div_up(K, LORA_STEP), groups = div_up(N, 64);
   if (p.mt == 1) {
-    int parts = 512 / p.tiles;
-    parts = parts < 1 ? 1 : parts < div_up(steps, 4) ? parts : div_up(steps, 4);
-    p.part_steps = div_up(div_up(steps, parts), 4) * 4;
-    int blocks = 768 / p.tiles;
-    blocks = blocks < 1 ? 1 : blocks < div_up(groups, 4) ? blocks : div_up(groups, 4);
+    // Few rows: parts of K for about 512 blocks, a step of 64 elements for each of their four waves at least (and 64 MB of sums at most), and of the
+    // outputs for about 768.  Of requests of one row, those of an adapter are one tile (196 requests of 32 adapters, rank 64, 8872 -> 8376: 52 us
+    // with the parts that as many tiles as requests would have).
+    const int real = (int)(ragged ? p.tiles : std::min(seqs, slots + seqs / 16 + 1));
+    int parts = std::min({512 / real, div_up(steps, 4), (int)((64 << 10) / ((int64_t)p.tiles * p.rt))});
+    p.part_steps = div_up(div_up(steps, std::max(parts, 1)), 4) * 4;
+    const int blocks = std::max(1, std::min(768 / real, div_up(groups, 4)));
     p.cols = div_up(div_up(groups, blocks), 4) * 4;
   } else {
-    const double real = std::max(1.0, (double)rows / 64 + 0.5 * (double)(seqs - 1));  // tiles with rows in them, about
+    // Many: a compute unit takes in about 23 GB/s however many blocks it has once 128 KB are on their way, so that what counts is how evenly the
+    // blocks fall on the units (8192 rows of 14336, rank 32: 393 blocks with two steps a wave 63 us, 512 50, 256 with four steps 45 and with two 73).
+    // A part's sums are read by every block of the second launch (4096 rows, rank 128, 4096 -> 4096: 94 us with 16 parts).  Seconds:
+    const double real = std::max(1.0, (double)rows / 64 + 0.5 * (double)(seqs - 1)), rate = 23e9;  // tiles with rows in them, about
+    const double sums = 64 * 16 * p.rt * 4 / 40e9, way = 4.0 * lora_depth(p.rt) * (8 + 2 * p.rt) / 128;
+    const double again = std::ceil(real * std::max(1.0, std::floor(256 / real)) / 256);
     double best = 1e30;
     for (int n = 1; n <= 16; ++n) {
       const int each = div_up(div_up(steps, n), 4) * 4, parts = div_up(steps, each);
-      const double rounds = std::ceil(real * parts / 256), full = std::min(1.0, rounds * lora_depth(p.rt) / 4);
-      const double cost = rounds * each / full * (1.0 + parts * (0.01 + 64.0 * p.rt / (double)K));
+      const double rounds = std::ceil(real * parts / 256);
+      const double cost = rounds * (each * (64 + 16 * p.rt) * 128 / rate / std::min(1.0, rounds * way) + 1e-6) + parts * sums * again;
       if (cost < best) best = cost, p.part_steps = each;
     }
+    const double before = div_up(steps, p.part_steps) * sums + 2e-6;
     best = 1e30;
     for (int m = 1; m <= 16; ++m) {
-      const double cost = std::ceil(real * div_up(groups, 4 * m) / 256) * (m + 1.0);
+      const double cost = std::ceil(real * div_up(groups, 4 * m) / 256) * (m * 4 * (16384 + 2048 * p.rt) / rate + before);
       if (cost < best) best = cost, p.cols = 4 * m;
     }
   }
@@ -415,9 +419,9 @@ static bool lora_sizes(int64_t rows, int64_t seqs, int rank, int64_t K) {
   return rows >= 0 && seqs >= 0 && rows < 1 << 30 && seqs < 1 << 29 && rank >= 8 && rank <= 128 && rank % 8 == 0 && K >= 8 && K <= 1 << 22;
 }
 
-extern "C" int64_t fmsmo_lora_workspace_bytes(int64_t rows, int64_t seqs, int ragged, int rank, int64_t K) {
-  if (!lora_sizes(rows, seqs, rank, K) || rows == 0 || (!ragged && rows != seqs)) return 0;
-  const LoraPlan p = lora_plan(rows, seqs, ragged != 0, rank, K, 64);
+extern "C" int64_t fmsmo_lora_workspace_bytes(int64_t rows, int64_t seqs, int ragged, int64_t slots, int rank, int64_t K) {
+  if (!lora_sizes(rows, seqs, rank, K) || rows == 0 || slots < 0 || (!ragged && rows != seqs)) return 0;
+  const LoraPlan p = lora_plan(rows, seqs, ragged != 0, std::min<int64_t>(slots, 1 << 29), rank, K, 64);
   return (int64_t)p.parts * p.tiles * (1024 * p.mt * p.rt);
 }
 
@@ -449,7 +453,7 @@ extern "C" int fmsmo_lora_add(int dtype, const void* x, int64_t ldx, const void*
   const int64_t widest = 2 * std::max(ldx, std::max(ldy, ldo));
   if (rows > 1 && 64 * widest + 2 * std::max(K, N) > MOST) return FMSMO_ERR_UNSUPPORTED;
   if (!workspace) return FMSMO_ERR_NULL;
-  const LoraPlan p = lora_plan(rows, seqs, query_start != nullptr, rank, K, N);
+  const LoraPlan p = lora_plan(rows, seqs, query_start != nullptr, std::min<int64_t>(slots, 1 << 29), rank, K, N);
   if (workspace_bytes < (int64_t)p.parts * p.tiles * (1024 * p.mt * p.rt)) return FMSMO_ERR_SCRATCH;
   // rows of one adapter may lie anywhere among the requests of one row: as many of them at a time as 32 bits reach
   const int64_t most = query_start || rows == 1 ? rows : (MOST - 2 * std::max(K, N)) / widest;

@@ -278,7 +278,7 @@ __device__ __forceinline__ void moe_stage(uint8_t* st, const v4i (&w)[4]) {
 // product.  D steps of 256 bytes a row are on their way, those of the next unit among them.  SHARE: the four waves of a block share a unit's K,
 // every fourth step each; their sums meet in shared memory, one barrier a unit, and a wave in turn finishes it.  Else each wave has units of its own.
 template <int OP, int MT, int D, bool ROUTE, bool SHARE, bool KEEP>
-__global__ __launch_bounds__(256, MT == 1 && D < 4 ? 4 : 2) void moe_up_kernel(MoeArgs a) {
+__global__ __launch_bounds__(256, MT == 1 && D < 4 ? 4 : D < 4 ? 3 : 2) void moe_up_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
   __shared__ MoeLists lists;
   __shared__ __attribute__((aligned(16))) uint8_t stage[4][4096];
@@ -676,8 +676,10 @@ struct MoePlan {
 };
 static MoePlan moe_plan(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   MoePlan p;
-  // (with up to six tokens an expert on average, few have more than sixteen: those stream their weights twice)
-  p.mt = T <= 16 || T * top <= 6 * E ? 1 : T <= 32 ? 2 : 4;
+  // Groups of 16 tokens, 32 or 64: experts with more stream their weights again.  With up to six tokens an expert on average few have more than 16,
+  // with up to twenty few have more than 32 (64 tokens, two of 8 experts of 4096 x 14336: gate and up 219 us in groups of 32, 252 of 64; 40, four of
+  // 16: 21 and 28; 64, two of 4: 180 and 157).
+  p.mt = T <= 16 || T * top <= 6 * E ? 1 : T <= 32 || T * top <= 20 * E ? 2 : 4;
   const int64_t used = std::min(E, T * top);
   // Waves with units of their own where rows are short and units many (13 tokens over 32 experts of 1024 x 14080: 160 us, 176 shared; 16 over 8 of
   // 4096 x 14336: 159 and 151; one token over 128 of 2048 x 768: 12.4 and 9.5).  Four steps on their way where a wave has a multiple of four for a
@@ -737,8 +739,8 @@ static void run_down(const MoeArgs& a, int splits, hipStream_t s) {
 template <int OP, int MT, int D, bool SHARE, bool KEEP>
 static void run_up(const MoeArgs& a, hipStream_t s) {
   // groups of tokens, at most
-  const int64_t units = (int64_t)std::min(MT == 1 ? a.E + a.T * a.top / 16 : a.E, a.T * a.top) * (a.I / 8);
-  const dim3 grid((unsigned)std::min<int64_t>(SHARE ? units : div_up(units, 4), MT > 1 || D > 1 ? 512 : 1024)), block(256);
+  const int64_t units = (int64_t)std::min(a.E + a.T * a.top / (16 * MT), a.T * a.top) * (a.I / 8);
+  const dim3 grid((unsigned)std::min<int64_t>(SHARE ? units : div_up(units, 4), MT == 1 && D > 1 ? 512 : MT > 1 ? 768 : 1024)), block(256);
   if constexpr (MT == 1) {
     if (a.T <= 8) {
       hipLaunchKernelGGL((moe_up_kernel<OP, 1, D, true, SHARE, KEEP>), grid, block, 0, s, a);

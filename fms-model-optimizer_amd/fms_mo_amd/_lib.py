@@ -130,7 +130,7 @@ OTHER = {
     "fmsmo_gemm_fp8_workspace_bytes": ([c_int64, c_int64, c_int64], c_int64),
     "fmsmo_matmul_chunk_workspace_bytes": ([c_int, c_int64, c_int64, c_int64, c_int, c_int], c_int64),
     "fmsmo_paged_attn_workspace_bytes": ([c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64], c_int64),
-    "fmsmo_lora_workspace_bytes": ([c_int64, c_int64, c_int, c_int, c_int64], c_int64),
+    "fmsmo_lora_workspace_bytes": ([c_int64, c_int64, c_int, c_int64, c_int, c_int64], c_int64),
     "fmsmo_moe_few_workspace_bytes": ([c_int64, c_int64, c_int, c_int64, c_int64], c_int64),
     "fmsmo_decode_linear_ok": ([c_int64, c_int64], c_int),
     "fmsmo_decode_linear_f32s_ok": ([c_int64, c_int64], c_int),

@@ -1442,7 +1442,7 @@ def _lora_add_impl(y, x, a, b, adapters, query_start, scales, out):
         if scales.shape != (S,) or scales.dtype != torch.float32:
             raise ValueError(f"scales must be float32 [{S}]")
         scales = scales.contiguous()
-    nbytes = L.load().fmsmo_lora_workspace_bytes(T, seqs, int(query_start is not None), r, K)
+    nbytes = L.load().fmsmo_lora_workspace_bytes(T, seqs, int(query_start is not None), S, r, K)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
     (a_slot, a_row), (b_slot, b_row) = _strides(a, 2), _strides(b, 2)
     with _dev(x):

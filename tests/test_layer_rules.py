@@ -47,7 +47,7 @@ def test_norm(lib, p):
 
 
 def test_lora(lib, p):
-    size = lib.fmsmo_lora_workspace_bytes(4, 4, 0, 16, 64)
+    size = lib.fmsmo_lora_workspace_bytes(4, 4, 0, 2, 16, 64)
     assert 0 < size < 65536
 
     def call(**k):
@@ -76,12 +76,12 @@ def test_lora_workspace_holds_every_tile(lib, rank, K):
         for ragged in (0, 1):
             if not ragged:
                 seqs = rows
-            n = lib.fmsmo_lora_workspace_bytes(rows, seqs, ragged, rank, K)
+            n = lib.fmsmo_lora_workspace_bytes(rows, seqs, ragged, 3, rank, K)
             # a tile per 64 rows (16 where requests are short), one more per request and for the rows of none; fp32
             tile = 64 if ragged and rows >= 32 * seqs else 16
             tiles = rows // tile + seqs + 2 if ragged else seqs
             assert n % 16 == 0 and n >= 4 * tiles * tile * rank
-    assert lib.fmsmo_lora_workspace_bytes(0, 4, 1, rank, K) == 0 and lib.fmsmo_lora_workspace_bytes(4, 4, 0, 12, K) == 0
+    assert lib.fmsmo_lora_workspace_bytes(0, 4, 1, 3, rank, K) == 0 and lib.fmsmo_lora_workspace_bytes(4, 4, 0, 3, 12, K) == 0
 
 
 def test_lora_workspace_of_any_sizes(lib):
@@ -90,9 +90,9 @@ def test_lora_workspace_of_any_sizes(lib):
     for _ in range(50000):
         rows = int(2 ** r.uniform(0, 30))
         seqs = r.choice([0, 1, 2, rows // 64, rows // 33, rows, int(2 ** r.uniform(0, 29))])
-        n = lib.fmsmo_lora_workspace_bytes(rows, seqs, r.randint(0, 1), 8 * r.randint(1, 16), 8 * int(2 ** r.uniform(0, 19)))
+        n = lib.fmsmo_lora_workspace_bytes(rows, seqs, r.randint(0, 1), int(2 ** r.uniform(0, 40)) - 1, 8 * r.randint(1, 16), 8 * int(2 ** r.uniform(0, 19)))
         assert n >= 0 and n % 16 == 0
-    assert lib.fmsmo_lora_workspace_bytes(3, 0, 1, 16, 64) > 0 and lib.fmsmo_lora_workspace_bytes(3, 0, 0, 16, 64) == 0
+    assert lib.fmsmo_lora_workspace_bytes(3, 0, 1, 2, 16, 64) > 0 and lib.fmsmo_lora_workspace_bytes(3, 0, 0, 2, 16, 64) == 0
 
 
 def test_moe(lib, p):
