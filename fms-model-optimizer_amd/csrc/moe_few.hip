@@ -18,6 +18,8 @@
 namespace fmsmo {
 
 constexpr int MOE_TOKENS = 64, MOE_EXPERTS = 512, MOE_TOP = 16;
+constexpr int MOE_ROUTED = 8;  // tokens up to which every block of the gate and up products routes for itself (16 tokens over 128 experts: 80 us so, 72 with
+                               // a launch of its own; ten over 8 experts, small ones: 15.2 and 16.2)
 
 struct MoeArgs {
   const uint8_t* a;     // [T, K] codes
@@ -467,7 +469,7 @@ __device__ __forceinline__ void moe_put(const MoeArgs& a, int tok, int n, float 
 // and a kernel behind adds what they leave.  ROWS = 8, groups of up to eight tokens: a product takes two steps, the first with its upper eight rows and
 // left eight columns, the second with the others, and the two blocks on its diagonal are added.  QUANT: few positions, whose codes every block makes for itself in shared memory.
 // Up to TM tokens.
-constexpr int MOE_QUANT_MOST = 8192;
+constexpr int MOE_QUANT_MOST = 16384;
 template <int OP, int MT, int ROWS, int NW, int D, int TM, bool QUANT, bool KEEP>
 __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   const int r = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * ROWS, steps = (a.I + MOE_STEP - 1) / MOE_STEP, pairs = a.T * a.top;
   const int count = a.count[0], all = count * steps;
-  for (int i = threadIdx.x; i < count; i += NT) entry[i] = a.entry[i];
+  for (int i = threadIdx.x; i < min(a.E, pairs) + pairs / 8; i += NT) entry[i] = a.entry[i];  // (as many as there may be: not after the count)
   // (positions that no pair took hold what was there before: they are not in any group)
   for (int i = threadIdx.x; i < pairs; i += NT) {
     token[i] = (uint8_t)a.token[i];
@@ -575,18 +577,29 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
     const MoeGroup m = count ? group_of(entry[count - 1]) : MoeGroup{0, 0, 0};
     for (int pos = wave; pos < m.off + m.cnt; pos += NW) {
       const v4f* h = (const v4f*)(a.h + (int64_t)pos * a.I);
-      uint32_t top = 0;
-      for (int i = lane; i < a.I / 4; i += 64) {
-        const v4f v = h[i];
+      const auto max4 = [](v4f v, uint32_t top) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t u = __float_as_uint(v[k]) & 0x7fffffffu;
           top = top > u ? top : u;
         }
-      }
+        return top;
+      };
+      constexpr int HELD = 4;  // 1024 elements of a row stay in registers, the others are read again
+      v4f v[HELD];
+      uint32_t top = 0;
+#pragma unroll
+      for (int q = 0; q < HELD; ++q) v[q] = h[min(lane + 64 * q, a.I / 4 - 1)];
+#pragma unroll
+      for (int q = 0; q < HELD; ++q) top = max4(v[q], top);
+      for (int i = lane + 64 * HELD; i < a.I / 4; i += 64) top = max4(h[i], top);
       const float s = moe_scale<OP>(wave_max_u32(top));
       if (lane == 0) share[pos] *= s;
-      for (int i = lane; i < a.I / 4; i += 64) ((uint32_t*)(codes + pos * a.I))[i] = moe_codes<OP>(h[i], s);
+      uint32_t* to = (uint32_t*)(codes + pos * a.I);
+#pragma unroll
+      for (int q = 0; q < HELD; ++q)
+        if (lane + 64 * q < a.I / 4) to[lane + 64 * q] = moe_codes<OP>(v[q], s);
+      for (int i = lane + 64 * HELD; i < a.I / 4; i += 64) to[i] = moe_codes<OP>(h[i], s);
     }
     __syncthreads();
   }
@@ -698,7 +711,8 @@ static MoePlan moe_plan(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
       const double cost = std::ceil(blocks / 256) * bytes / blocks / (narrow ? 21e9 : 23e9) + (n > 1 ? 4e-6 : 0.0);
       if (cost < best * 0.98) best = cost, p.narrow = narrow, p.splits = n;
     }
-  p.quant = p.mt == 1 && T * top <= 8 && T * top * I <= MOE_QUANT_MOST;
+  // (a launch or so many rows for every block: 2 tokens, eight of 128 experts of 2048 x 768 23.4 us and 24.3, 4 tokens 34.9 and 31.9)
+  p.quant = p.mt == 1 && T * top <= 16 && T * top * I <= MOE_QUANT_MOST;
   return p;
 }
 // bytes up to each piece of the workspace
@@ -742,7 +756,7 @@ static void run_up(const MoeArgs& a, hipStream_t s) {
   const int64_t units = (int64_t)std::min(a.E + a.T * a.top / (16 * MT), a.T * a.top) * (a.I / 8);
   const dim3 grid((unsigned)std::min<int64_t>(SHARE ? units : div_up(units, 4), MT == 1 && D > 1 ? 512 : MT > 1 ? 768 : 1024)), block(256);
   if constexpr (MT == 1) {
-    if (a.T <= 8) {
+    if (a.T <= MOE_ROUTED) {
       hipLaunchKernelGGL((moe_up_kernel<OP, 1, D, true, SHARE, KEEP>), grid, block, 0, s, a);
       return;
     }
@@ -753,7 +767,7 @@ template <int OP, int MT>
 static void run_moe(MoeArgs a, const MoePlan& p, hipStream_t s) {
   if (p.quant) a.tops = nullptr;
   a.down_group = p.narrow ? 8 : 16 * MT;
-  if (a.T > 8) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), dim3(256), 0, s, a);
+  if (a.T > MOE_ROUTED) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), dim3(256), 0, s, a);
   const auto up = [&](auto keep) {
     constexpr bool KEEP = decltype(keep)::value;
     if (!p.share) return run_up<OP, MT, 1, false, KEEP>(a, s);
