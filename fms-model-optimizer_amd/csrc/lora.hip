@@ -105,8 +105,10 @@ constexpr int LORA_STEP = 64;  // elements of K a step: 128 bytes of a row
 // v of a tile over a part of K.  Rows of A (16 RT) and of x (16 MT) meet as the two operands of 16 x 16 x 32; the side with more bytes comes
 // through shared memory, eight rows of 128 bytes a load, the other one straight into the operands' layout, D steps of a wave on their way.  Rows past
 // the rank and the tile's end are the last one again: what comes of them is not looked at.
+// (From rank 33 on the sums stay in the registers that the products are made in: two waves a SIMD are asked for.  Rank 128, 4096 rows of 4096: 30 us
+// without, 22 with; at rank 32 that leaves too few, 45 and 79 us.)
 template <int T, int RT, int MT, int D>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs a) {
+__global__ __launch_bounds__(256, RT >= 4 ? 2 : 1) void lora_shrink_kernel(LoraArgs a) {
   constexpr bool X_STAGED = MT > 1;
   constexpr int S = X_STAGED ? MT : RT, O = X_STAGED ? RT : MT;  // tiles of 16 rows of the staged and the other side
   constexpr int SUMS = MT * 16 * (RT * 16 + 4) * 4;  // bytes of a wave's sums; they take the place of the staged rows
@@ -372,45 +374,52 @@ int fmsmo_check_launch();
 
 // Steps on their way of a wave of the first launch on tiles of 64 rows: what the registers hold.
 static constexpr int lora_depth(int rt) { return rt <= 2 ? 4 : rt == 4 ? 2 : 1; }
-// What a call is cut into.  Rows: tiles of 64 where a request has 32 on average, else of 16.
+// What a call is cut into.  Rows: tiles of 64 where a request has 32 on average, else of 16.  (Tiles of 128 rows read half of A and B and hold half as
+// many waves' rows: rank 64, 6972 rows, 4096 -> 6144 79 us and 66.)
 struct LoraPlan {
   int mt, rt, tiles, parts, part_steps, cols;
 };
+// Many rows: a compute unit takes in about 23 GB/s however many blocks it has once 128 KB are on their way, so that what counts is how evenly the
+// blocks fall on the units (8192 rows of 14336, rank 32: 393 blocks with two steps a wave 63 us, 512 50, 256 with four steps 45 and with two 73),
+// and what they read of A and B beside the rows.  A part's sums are read by every block of the second launch (4096 rows, rank 128, 4096 -> 4096:
+// 94 us with 16 parts, 65 with those chosen here).
+static void lora_many(LoraPlan& p, double rows, double seqs, int steps, int groups) {
+  constexpr int R = 64;
+  const double real = std::max(1.0, rows / R + 0.5 * (seqs - 1)), rate = 23e9;  // tiles with rows in them, about
+  const double sums = R * 16 * p.rt * 4 / 40e9, way = 4.0 * lora_depth(p.rt) * (8 + 2 * p.rt) / 128;  // seconds; of what is on its way
+  const double again = std::ceil(real * std::max(1.0, std::floor(256 / real)) / 256);
+  double first = 1e30, second = 1e30;
+  for (int n = 1; n <= 16; ++n) {
+    const int each = div_up(div_up(steps, n), 4) * 4, parts = div_up(steps, each);
+    const double rounds = std::ceil(real * parts / 256);
+    const double cost = rounds * (each * (R + 16 * p.rt) * 128 / rate / std::min(1.0, rounds * way) + 1e-6) + parts * sums * again;
+    if (cost < first) first = cost, p.part_steps = each;
+  }
+  const double before = div_up(steps, p.part_steps) * sums + 2e-6;
+  for (int m = 1; m <= 16; ++m) {
+    const double cost = std::ceil(real * div_up(groups, 4 * m) / 256) * (m * 4 * (256 * R + 2048 * p.rt) / rate + before);
+    if (cost < second) second = cost, p.cols = 4 * m;
+  }
+}
 static LoraPlan lora_plan(int64_t rows, int64_t seqs, bool ragged, int64_t slots, int rank, int64_t K, int64_t N) {
   LoraPlan p;
-  p.mt = ragged && rows >= 32 * seqs ? 4 : 1;
   p.rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
-  p.tiles = (int)(ragged ? rows / (16 * p.mt) + seqs + 2 : seqs);
   const int steps = div_up(K, LORA_STEP), groups = div_up(N, 64);
-  if (p.mt == 1) {
+  if (!ragged || rows < 32 * seqs) {
     // Few rows: parts of K for about 512 blocks, a step of 64 elements for each of their four waves at least (and 64 MB of sums at most), and of the
     // outputs for about 768.  Of requests of one row, those of an adapter are one tile (196 requests of 32 adapters, rank 64, 8872 -> 8376: 52 us
-    // with the parts that as many tiles as requests would have).
+    // with the parts that as many tiles as requests would have, 33 so).
+    p.mt = 1;
+    p.tiles = (int)(ragged ? rows / 16 + seqs + 2 : seqs);
     const int real = (int)(ragged ? p.tiles : std::min(seqs, slots + seqs / 16 + 1));
-    int parts = std::min({512 / real, div_up(steps, 4), (int)((64 << 10) / ((int64_t)p.tiles * p.rt))});
+    const int parts = std::min({512 / real, div_up(steps, 4), (int)((64 << 10) / ((int64_t)p.tiles * p.rt))});
     p.part_steps = div_up(div_up(steps, std::max(parts, 1)), 4) * 4;
     const int blocks = std::max(1, std::min(768 / real, div_up(groups, 4)));
     p.cols = div_up(div_up(groups, blocks), 4) * 4;
   } else {
-    // Many: a compute unit takes in about 23 GB/s however many blocks it has once 128 KB are on their way, so that what counts is how evenly the
-    // blocks fall on the units (8192 rows of 14336, rank 32: 393 blocks with two steps a wave 63 us, 512 50, 256 with four steps 45 and with two 73).
-    // A part's sums are read by every block of the second launch (4096 rows, rank 128, 4096 -> 4096: 94 us with 16 parts).  Seconds:
-    const double real = std::max(1.0, (double)rows / 64 + 0.5 * (double)(seqs - 1)), rate = 23e9;  // tiles with rows in them, about
-    const double sums = 64 * 16 * p.rt * 4 / 40e9, way = 4.0 * lora_depth(p.rt) * (8 + 2 * p.rt) / 128;
-    const double again = std::ceil(real * std::max(1.0, std::floor(256 / real)) / 256);
-    double best = 1e30;
-    for (int n = 1; n <= 16; ++n) {
-      const int each = div_up(div_up(steps, n), 4) * 4, parts = div_up(steps, each);
-      const double rounds = std::ceil(real * parts / 256);
-      const double cost = rounds * (each * (64 + 16 * p.rt) * 128 / rate / std::min(1.0, rounds * way) + 1e-6) + parts * sums * again;
-      if (cost < best) best = cost, p.part_steps = each;
-    }
-    const double before = div_up(steps, p.part_steps) * sums + 2e-6;
-    best = 1e30;
-    for (int m = 1; m <= 16; ++m) {
-      const double cost = std::ceil(real * div_up(groups, 4 * m) / 256) * (m * 4 * (16384 + 2048 * p.rt) / rate + before);
-      if (cost < best) best = cost, p.cols = 4 * m;
-    }
+    p.mt = 4;
+    lora_many(p, (double)rows, (double)seqs, steps, groups);
+    p.tiles = (int)(rows / 64 + seqs + 2);
   }
   p.parts = div_up(steps, p.part_steps);
   return p;
@@ -427,7 +436,7 @@ extern "C" int64_t fmsmo_lora_workspace_bytes(int64_t rows, int64_t seqs, int ra
 
 template <int T, int RT, int MT>
 static void run_lora(const LoraArgs& a, hipStream_t s) {
-  constexpr int D = MT == 4 ? lora_depth(RT) : 2;
+  constexpr int D = MT > 1 ? lora_depth(RT) : 2;
   hipLaunchKernelGGL((lora_shrink_kernel<T, RT, MT, D>), dim3((unsigned)a.tiles, (unsigned)a.parts), dim3(256), 0, s, a);
   hipLaunchKernelGGL((lora_expand_kernel<T, RT, MT>), dim3((unsigned)a.tiles, (unsigned)div_up(div_up(a.N, 64), a.cols)), dim3(256), 0, s, a);
 }
