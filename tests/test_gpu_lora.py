@@ -143,6 +143,39 @@ def test_many_requests(dev):
     check(dev, y, x, a, b, torch.randint(-1, 5, (300,), generator=g).tolist(), [0] + start + [700], scales)
 
 
+def test_rows_far_apart(dev):
+    """One-row requests whose rows lie over more than 2 GB: what 32 bits reach at a time; an adapter's rows among both pieces."""
+    g = gen(13)
+    T, far = 300, 1 << 22
+    y, x, a, b, scales = make(g, T, 64, 72, 8, 3, torch.float16)
+    ids = torch.randint(-1, 3, (T,), generator=g).tolist()
+    want = check(dev, y, x, a, b, ids, None, scales)
+    room = torch.empty(T * far, dtype=torch.float16, device=dev)
+    apart = room.as_strided((T, 64), (far, 1))
+    apart.copy_(x)
+    args = (a.to(dev), b.to(dev), torch.tensor(ids, dtype=torch.int32, device=dev))
+    assert torch.equal(K().lora_add(y.to(dev), apart, *args, scales=scales.to(dev)), want)
+    out = room.as_strided((T, 72), (far, 1), 128)
+    assert K().lora_add(y.to(dev), x.to(dev), *args, scales=scales.to(dev), out=out) is out and torch.equal(out, want)
+    start = torch.arange(0, T + 1, 2, dtype=torch.int32, device=dev)
+    two = K().lora_add(y.to(dev), x.to(dev), *args[:2], args[2][:150], start, scales=scales.to(dev))
+    assert torch.equal(K().lora_add(y.to(dev), apart, *args[:2], args[2][:150], start, scales=scales.to(dev)), two)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rank,cols,rows,new", [(128, 4104, 264, [700]), (24, 72, 4104, [90, 333]), (64, 2056, 1032, [64, 128, 1, 500]), (16, 9000, 136, [1030]),
+                                                (32, 264, 2056, [2000])])
+def test_longer_requests(dev, dt, rank, cols, rows, new):
+    g = gen(rank + cols)
+    start = [0]
+    for n in new:
+        start.append(start[-1] + n)
+    y, x, a, b, scales = make(g, start[-1] + 3, cols, rows, rank, 4, dt)
+    ids = torch.randint(0, 4, (len(new),), generator=g).tolist()
+    first = check(dev, y, x, a, b, ids, start, scales)
+    assert torch.equal(check(dev, y, x, a, b, ids, start, scales), first)
+
+
 def test_nothing_to_do(dev):
     k = K()
     z = torch.empty(0, 64, device=dev).half()

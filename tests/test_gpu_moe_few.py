@@ -59,6 +59,29 @@ def test_larger(dev, code, T, E, top, hidden, inter):
     check(dev, args, top, out_dtype=torch.float16)
 
 
+@pytest.mark.parametrize("code", [I8, E4M3])
+@pytest.mark.parametrize("T,E,top,hidden,inter", [
+    (13, 32, 8, 528, 1040),   # waves with units of their own, rows that share lines, blocks that share outputs
+    (9, 40, 2, 1024, 2048),   # the same with whole lines
+    (33, 8, 4, 512, 1024),    # groups of 32, more than one an expert
+    (64, 4, 2, 272, 1040),    # groups of 64
+    (40, 3, 2, 640, 512),     # and blocks that share outputs
+    (8, 4, 2, 4096, 128),     # four steps on their way
+    (20, 64, 2, 4096, 16),    # the same behind a routing launch
+    (17, 6, 2, 4112, 32),     # more blocks than units
+    (2, 20, 8, 256, 1024),    # as many positions as the down kernel makes codes for
+    (3, 20, 6, 256, 896),     # and more
+    (1, 16, 16, 1008, 1008),
+    (64, 200, 16, 48, 32),
+])
+def test_each_way_of_cutting(dev, code, T, E, top, hidden, inter):
+    args = make(gen(T + E + hidden), T, E, hidden, inter, code, torch.float32)
+    ref = R.moe(*args, top, True)
+    first = check(dev, args, top, out_dtype=torch.float32, ref=ref)
+    for _ in range(3):
+        assert torch.equal(check(dev, args, top, out_dtype=torch.float32, ref=ref), first)
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_types_of_logits_and_shares(dev, dt, renormalize):
