@@ -39,7 +39,18 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& a, int tile, int* 
   const int lane = threadIdx.x & 63;
   LoraTile t{0, 0, -1};
   if (!a.starts) {
-    const int slot = uniform(a.adapters[tile]);
+    // The adapters of the first 256 requests at once, the others 64 by 64. One load behind the other for the first too:
+    // 256 requests of rank 16 8.9 + 8.3 us, 7.8 + 7.4 so.
+    constexpr int Q = 4;
+    int held[Q] = {a.adapters[min(lane, a.seqs - 1)], -1, -1, -1}, slot = 0;
+    if (a.seqs > 64) {
+#pragma unroll
+      for (int q = 1; q < Q; ++q) held[q] = a.adapters[min(64 * q + lane, a.seqs - 1)];
+    }
+    if (tile >= 64 * Q) slot = a.adapters[tile];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) slot = tile >> 6 == q ? __builtin_amdgcn_readlane(held[q], tile & 63) : slot;
+    slot = uniform(slot);
     if ((unsigned)slot >= (unsigned)a.slots) {  // on its own: the copy of its row
       t.n = 1;
       t.row0 = tile;
@@ -48,16 +59,21 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& a, int tile, int* 
     }
     // the requests of this adapter before this one; a tile starts at each TR-th of them
     int before = 0, mine = 0;
-    for (int i = 0; i < tile; i += 64) before += __popcll(__ballot(i + lane < tile && a.adapters[i + lane] == slot));
+#pragma unroll
+    for (int q = 0; q < Q; ++q) before += __popcll(__ballot(64 * q + lane < tile && held[q] == slot));
+    for (int i = 64 * Q; i < tile; i += 64) before += __popcll(__ballot(i + lane < tile && a.adapters[i + lane] == slot));
     before = uniform(before);
     if (before % TR) return t;
-    for (int i = tile & ~63; i < a.seqs && mine < TR; i += 64) {
-      const bool same = i + lane >= tile && i + lane < a.seqs && a.adapters[i + lane] == slot;
+    const auto take = [&](int i, int id) {
+      const bool same = i + lane >= tile && i + lane < a.seqs && id == slot;
       const uint64_t m = __ballot(same);
       const int at = mine + __popcll(m & ((1ull << lane) - 1));
       if (same && at < TR && threadIdx.x < 64) list[at] = i + lane;
       mine += __popcll(m);
-    }
+    };
+#pragma unroll
+    for (int q = 0; q < Q; ++q) take(64 * q, held[q]);
+    for (int i = max(tile & ~63, 64 * Q); i < a.seqs && mine < TR; i += 64) take(i, a.adapters[min(i + lane, a.seqs - 1)]);
     mine = uniform(mine);
     t.n = mine < TR ? mine : TR;
     t.row0 = tile;
@@ -68,10 +84,11 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& a, int tile, int* 
   int seen = 0;
   for (int i = -1; i <= a.seqs; i += 64) {
     const int b = i + lane;
-    int r0 = 0, r1 = 0;
+    int r0 = 0, r1 = 0, id = -1;
     if (b <= a.seqs) {
       r0 = b < 0 ? 0 : a.starts[b];
       r1 = b >= a.seqs ? a.rows : a.starts[b + 1];
+      if (b >= 0 && b < a.seqs) id = a.adapters[b];
       r0 = r0 < 0 ? 0 : r0 < a.rows ? r0 : a.rows;
       r1 = r1 < 0 ? 0 : r1 < a.rows ? r1 : a.rows;
     }
@@ -86,11 +103,11 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraArgs& a, int tile, int* 
     const uint64_t hit = __ballot(tile >= first && tile < first + mine);
     if (hit) {
       const int l = __ffsll((unsigned long long)hit) - 1;
-      const int at = (tile - __shfl(first, l)) * TR, req = i + l;
+      const int at = (tile - __shfl(first, l)) * TR;
       const int rn = __shfl(n, l) - at;
       t.row0 = uniform(__shfl(r0, l) + at);
       t.n = uniform(rn < TR ? rn : TR);
-      const int slot = uniform(req >= 0 && req < a.seqs ? a.adapters[req] : -1);
+      const int slot = uniform(__shfl(id, l));
       t.slot = (unsigned)slot < (unsigned)a.slots ? slot : -1;
       return t;
     }
@@ -467,24 +484,24 @@ extern "C" int fmsmo_lora_add(int dtype, const void* x, int64_t ldx, const void*
   // rows of one adapter may lie anywhere among the requests of one row: as many of them at a time as 32 bits reach
   const int64_t most = query_start || rows == 1 ? rows : (MOST - 2 * std::max(K, N)) / widest;
   for (int64_t from = 0; from < rows; from += most) {
-  const int64_t some = std::min(most, rows - from);
-  LoraArgs g{(const char*)x + 2 * from * ldx, (const char*)y + 2 * from * ldy, (char*)out + 2 * from * ldo, (const char*)a, (const char*)b,
-             adapters + from, query_start, scales, (float*)workspace, 2 * ldx, 2 * ldy, 2 * ldo, 2 * a_slot, 2 * a_row, 2 * b_slot, 2 * b_row,
-             (int)some, (int)(query_start ? seqs : some), (int)slots, rank, (int)K, (int)N, p.parts, p.part_steps, (int)(query_start ? p.tiles : some),
-             p.cols};
-  const auto go = [&](auto t, auto rt) {
-    constexpr int T = decltype(t)::value, RT = decltype(rt)::value;
-    if (p.mt == 4) run_lora<T, RT, 4>(g, (hipStream_t)stream);
-    else run_lora<T, RT, 1>(g, (hipStream_t)stream);
-  };
-  const auto ranks = [&](auto t) {
-    if (p.rt == 1) go(t, std::integral_constant<int, 1>{});
-    else if (p.rt == 2) go(t, std::integral_constant<int, 2>{});
-    else if (p.rt == 4) go(t, std::integral_constant<int, 4>{});
-    else go(t, std::integral_constant<int, 8>{});
-  };
-  if (dtype == FMSMO_F16) ranks(std::integral_constant<int, FMSMO_F16>{});
-  else ranks(std::integral_constant<int, FMSMO_BF16>{});
+    const int64_t some = std::min(most, rows - from);
+    LoraArgs g{(const char*)x + 2 * from * ldx, (const char*)y + 2 * from * ldy, (char*)out + 2 * from * ldo, (const char*)a, (const char*)b,
+               adapters + from, query_start, scales, (float*)workspace, 2 * ldx, 2 * ldy, 2 * ldo, 2 * a_slot, 2 * a_row, 2 * b_slot, 2 * b_row,
+               (int)some, (int)(query_start ? seqs : some), (int)slots, rank, (int)K, (int)N, p.parts, p.part_steps, (int)(query_start ? p.tiles : some),
+               p.cols};
+    const auto go = [&](auto t, auto rt) {
+      constexpr int T = decltype(t)::value, RT = decltype(rt)::value;
+      if (p.mt == 4) run_lora<T, RT, 4>(g, (hipStream_t)stream);
+      else run_lora<T, RT, 1>(g, (hipStream_t)stream);
+    };
+    const auto ranks = [&](auto t) {
+      if (p.rt == 1) go(t, std::integral_constant<int, 1>{});
+      else if (p.rt == 2) go(t, std::integral_constant<int, 2>{});
+      else if (p.rt == 4) go(t, std::integral_constant<int, 4>{});
+      else go(t, std::integral_constant<int, 8>{});
+    };
+    if (dtype == FMSMO_F16) ranks(std::integral_constant<int, FMSMO_F16>{});
+    else ranks(std::integral_constant<int, FMSMO_BF16>{});
   }
   return fmsmo_check_launch();
 }
