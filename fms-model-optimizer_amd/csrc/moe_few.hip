@@ -466,9 +466,9 @@ __device__ __forceinline__ void moe_put(const MoeArgs& a, int tok, int n, float 
 // y.  A block owns ROWS outputs and goes through all groups of tokens: their steps of 256 bytes one behind the other, cut into equal parts
 // for the waves, D steps on their way; at the end of a group a wave adds its products, with their scales and shares, to sums of its own, and the
 // waves' sums are added in their order.  Where few outputs leave units without a block, several blocks share the steps of the same outputs
-// and a kernel behind adds what they leave.  ROWS = 8, groups of up to eight tokens: a product takes two steps, the first with its upper eight rows and
-// left eight columns, the second with the others, and the two blocks on its diagonal are added.  QUANT: few positions, whose codes every block makes for itself in shared memory.
-// Up to TM tokens.
+// and a kernel behind adds what they leave.  ROWS = 8, groups of up to eight tokens: a product takes two steps, the first with its upper eight
+// rows and left eight columns, the second with the others, and the two blocks on its diagonal are added.  QUANT: few positions, whose codes every
+// block makes for itself in shared memory.  Up to TM tokens.
 constexpr int MOE_QUANT_MOST = 16384;
 template <int OP, int MT, int ROWS, int NW, int D, int TM, bool QUANT, bool KEEP>
 __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
@@ -676,7 +676,7 @@ int fmsmo_check_launch();
 
 static bool moe_sizes(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   return T >= 0 && T <= MOE_TOKENS && E >= 1 && E <= MOE_EXPERTS && top >= 1 && top <= MOE_TOP && top <= E && K >= 16 && I >= 16 && K % 16 == 0 &&
-         I % 16 == 0 && K < 1 << 20 && I < 1 << 20 && 2 * I * K <= 0x7f000000;  // (an expert's weights are counted in 32 bits)
+         I % 16 == 0 && K < 1 << 17 && I < 1 << 17 && 2 * I * K <= 0x7f000000;  // (sums of products, and offsets into an expert's weights, in 32 bits)
 }
 // What a call is cut into.
 struct MoePlan {

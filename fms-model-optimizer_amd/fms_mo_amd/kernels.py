@@ -1461,8 +1461,8 @@ def _moe_few_tokens_impl(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k
     E, I = w13.shape[0], w13.shape[1] // 2
     if w13.shape[2] != K or w2.shape != (E, K, I):
         raise ValueError(f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not fit a {tuple(a.shape)}")
-    if K % 16 or I % 16 or min(K, I) < 16 or max(K, I) >= 1 << 20:
-        raise ValueError(f"K and I must be multiples of 16 below 2^20, got {K} and {I}")
+    if K % 16 or I % 16 or min(K, I) < 16 or max(K, I) >= 1 << 17:
+        raise ValueError(f"K and I must be multiples of 16 below 2^17, got {K} and {I}")
     if not 1 <= E <= 512 or not 1 <= top_k <= min(E, 16):
         raise ValueError(f"top_k must be 1 to 16 of up to 512 experts, got {top_k} of {E}")
     for name, t in (("w13", w13), ("w2", w2)):  # (weights are not copied for a call)
@@ -1512,7 +1512,8 @@ def add_rms_norm_quant(x, weight, residual=None, *, eps=1e-6, dtype=torch.int8, 
     (``dtype`` int8 or float8_e4m3fn) with one scale per token, or with the given ``scale`` (fp32, one element).  x, residual [M, K] fp16 /
     bf16, weight [K] of x's dtype or fp32.  Returns (q [M, K], scale fp32 [M] or the given one, h in x's dtype or None without a residual,
     n in x's dtype where ``want_normed`` or None).  h goes to ``residual_out`` (x or residual itself, or memory apart from them) or a new
-    tensor.  A SmoothQuant divisor is divided out of the weight beforehand.  See fmsmo_add_rms_norm_quant."""
+    tensor.  A SmoothQuant divisor is divided out of the weight beforehand.  No gradients.  See
+    fmsmo_add_rms_norm_quant."""
     if not _COMPILING():
         r = (_H or _host()).add_rms_norm_quant(x, weight, residual, eps, dtype, scale, want_normed, residual_out)
         if r is not None:
@@ -1579,8 +1580,8 @@ def moe_few_tokens(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, *, r
     logits (of equal ones the lower index) with their softmax shares (``renormalize``: divided by their sum), gate and up products,
     silu(gate) * up in 8 bits per token and expert, down products, sum.  a [T, K] int8 or float8_e4m3fn codes with a_scale [T] (as
     ``add_rms_norm_quant`` and the quantizers make them), logits [T, E], w13 [E, 2 I, K] (gate rows, then up rows) and w2 [E, K, I] of a's dtype with
-    fp32 scales [E, 2 I] and [E, K].  Returns [T, K] in ``out`` or a new tensor of ``out_dtype``.  More tokens: ``grouped_gemm_i8_dq`` on
-    rows sorted by expert.  See fmsmo_moe_few_tokens."""
+    fp32 scales [E, 2 I] and [E, K].  Returns [T, K] in ``out`` (apart from the operands) or a new tensor of ``out_dtype``.  More tokens:
+    ``grouped_gemm_i8_dq`` on rows sorted by expert.  No gradients.  See fmsmo_moe_few_tokens."""
     if not _COMPILING():
         r = (_H or _host()).moe_few_tokens(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, out_dtype, out)
         if r is not None:

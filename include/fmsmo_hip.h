@@ -941,9 +941,9 @@ int fmsmo_add_rms_norm_quant(const void* x, int dtype, int64_t ldx, const void* 
  * Request i has the rows query_start[i] .. query_start[i + 1] - 1 (ascending; query_start NULL: row i alone, and as many rows as requests).
  * Rows of a request whose number is none of the slots (-1), and rows of no request: out = y.  Starts that descend give results without a
  * meaning, but nothing outside of the operands is touched.  Sums are fp32; a[s] x is taken as the sum of two 16-bit numbers, the result is rounded once.
- * rank a multiple of 8 up to 128; K, N up to 2^22 and strides multiples of 8, operands 16-byte aligned; 64 rows of x, y or out, 128 of an adapter's a and
- * all of its b within 2 GB.  workspace: fmsmo_lora_workspace_bytes(rows, seqs,
- * query_start != NULL, slots, rank, K) bytes, 16-byte aligned, private to the call until it has finished.
+ * rank a multiple of 8 up to 128; K, N up to 2^22 and strides multiples of 8, operands 16-byte aligned; 64 rows of x, y or out, 128 of an
+ * adapter's a and all of its b within 2 GB.  workspace: fmsmo_lora_workspace_bytes(rows, seqs, query_start != NULL, slots, rank, K) bytes,
+ * 16-byte aligned, private to the call until it has finished.
  */
 int fmsmo_lora_add(int dtype, const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, const void* a, int64_t a_slot,
                    int64_t a_row, const void* b, int64_t b_slot, int64_t b_row, int64_t slots, int rank, const int32_t* adapters,
@@ -962,8 +962,9 @@ int64_t fmsmo_lora_workspace_bytes(int64_t rows, int64_t seqs, int ragged, int64
  * Sums are int32 (int8) or fp32.  An expert whose share of a token is zero is not run for it (a logit of -infinity; a token whose logits all
  * are has a result of zero).  A NaN among the logits counts as the largest (a negative one as the smallest), and the token's result is NaN
  * where it is chosen.
- * E <= 512, top <= 16, K and I multiples of 16 below 2^20, operands and w2_scale 16-byte aligned, lda a multiple of 16.  workspace:
- * fmsmo_moe_few_workspace_bytes(T, E, top, K, I) bytes, 16-byte aligned, private to the call until it has finished.
+ * E <= 512, top <= 16, K and I multiples of 16 below 2^17, w13[e] within 2 GB; operands and w2_scale 16-byte aligned, lda a multiple of 16
+ * up to 2^24; y apart from the operands.  workspace: fmsmo_moe_few_workspace_bytes(T, E, top, K, I) bytes, 16-byte aligned, private to the call
+ * until it has finished.
  * More tokens: fmsmo_grouped_gemm_i8_dq.
  */
 int fmsmo_moe_few_tokens(int codes, const void* a, int64_t lda, const float* a_scale, int64_t a_scale_n, const void* logits, int logits_dtype,

@@ -82,6 +82,14 @@ def test_each_way_of_cutting(dev, code, T, E, top, hidden, inter):
         assert torch.equal(check(dev, args, top, out_dtype=torch.float32, ref=ref), first)
 
 
+@pytest.mark.parametrize("hidden,inter", [(131056, 16), (16, 131056)])
+def test_the_largest_sums_of_codes(dev, hidden, inter):
+    """All codes the lowest: sums just below 2^31 (down: codes of h, all 127, times the lowest)."""
+    a, w13, w2 = (torch.full(s, -128, dtype=I8) for s in ((2, hidden), (1, 2 * inter, hidden), (1, hidden, inter)))
+    s13, s2 = torch.full((1, 2 * inter), 2.0 ** -30), torch.full((1, hidden), 2.0 ** -24)
+    check(dev, (a, torch.ones(2), torch.zeros(2, 1), w13, s13, w2, s2), 1)
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_types_of_logits_and_shares(dev, dt, renormalize):

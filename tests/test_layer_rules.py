@@ -110,7 +110,8 @@ def test_moe(lib, p):
         assert call(**{name: None}) == NULL
     assert call(T=-1) == SHAPE and call(sn=3) == SHAPE and call(lda=16) == SHAPE and call(ldl=3) == SHAPE and call(ldy=16) == SHAPE
     for bad in (dict(T=65), dict(E=513), dict(E=0), dict(top=0), dict(top=5), dict(top=17, E=32), dict(K=24), dict(I=24), dict(K=0), dict(codes=2),
-                dict(ldt=3), dict(ydt=7), dict(K=1 << 20)):
+                dict(ldt=3), dict(ydt=7), dict(K=1 << 20),
+                dict(K=1 << 17, lda=1 << 17, ldy=1 << 17), dict(I=1 << 17)):
         assert call(**bad) == UNSUPPORTED
     for bad in (dict(a=p + 8), dict(w13=p + 1), dict(w2=p + 1), dict(s2=p + 4), dict(ws=p + 4), dict(lda=40)):
         assert call(**bad) == ALIGN
