@@ -276,19 +276,20 @@ __device__ __forceinline__ void moe_stage(uint8_t* st, const v4i (&w)[4]) {
   __builtin_amdgcn_wave_barrier();  // (the rows go to other lanes of the wave)
 }
 
-// h of the positions.  A unit: eight gate rows and the eight up rows that belong to them, for one group of tokens: the 16 rows of the
-// product.  D steps of 256 bytes a row are on their way, those of the next unit among them.  SHARE: the four waves of a block share a unit's K,
-// every fourth step each; their sums meet in shared memory, one barrier a unit, and a wave in turn finishes it.  Else each wave has units of its own.
-template <int OP, int MT, int D, bool ROUTE, bool SHARE, bool KEEP>
-__global__ __launch_bounds__(256, MT == 1 && D < 4 ? 4 : D < 4 ? 3 : 2) void moe_up_kernel(MoeArgs a) {
+// h of the positions.  A unit: 8 RW gate rows and the up rows that belong to them, for one group of tokens: RW products' 16 rows, each eight
+// gate rows and their up rows.  D steps of 256 bytes a row are on their way, those of the next unit among them.  SHARE: the four waves of a block
+// share a unit's K, every fourth step each; their sums meet in shared memory, one barrier a unit, and a wave in turn finishes it.  Else each wave
+// has units of its own.
+template <int OP, int MT, int RW, int D, bool ROUTE, bool SHARE, bool KEEP>
+__global__ __launch_bounds__(256, RW * D >= 2 ? 2 : MT == 1 ? 4 : 3) void moe_up_kernel(MoeArgs a) {
   typedef typename MoeAcc<OP>::type Acc;
   __shared__ MoeLists lists;
-  __shared__ __attribute__((aligned(16))) uint8_t stage[4][4096];
-  __shared__ __attribute__((aligned(16))) Acc part[SHARE ? 2 : 1][SHARE ? 4 : 1][MT][64];
+  __shared__ __attribute__((aligned(16))) uint8_t stage[4][4096 * RW];
+  __shared__ __attribute__((aligned(16))) Acc part[SHARE ? 2 : 1][SHARE ? 4 : 1][RW * MT][64];
   make_lists<256, MT, ROUTE>(a, lists);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;  // operands: row or column r, 16-byte pieces g and 4 + g; loads: rows g, 4 + g, .., piece r
-  const int groups = a.I / 8, units = lists.count * groups;
+  const int groups = a.I / (8 * RW), units = lists.count * groups;
   constexpr int KS = SHARE ? 4 : 1;
   const int steps = ((a.K + MOE_STEP * KS - 1) / (MOE_STEP * KS) + D - 1) / D * D;  // of a wave
   uint8_t* st = stage[wave];
@@ -308,20 +309,22 @@ __global__ __launch_bounds__(256, MT == 1 && D < 4 ? 4 : D < 4 ? 3 : 2) void moe
     q.gi = there ? u - en * groups : 0;
     q.m = group_of(uniform((int)lists.entry[en]));
     q.w = buf_of(a.w13 + (int64_t)q.m.e * 2 * a.I * a.K);
-    q.wo = there ? (uint32_t)(q.gi * 8 + g) * (uint32_t)a.K + r * 16 : BUF_NONE;
+    q.wo = there ? (uint32_t)(q.gi * 8 * RW + g) * (uint32_t)a.K + r * 16 : BUF_NONE;
 #pragma unroll
     for (int j = 0; j < MT; ++j)
       q.xo[j] = there && 16 * j + r < q.m.cnt ? lists.token[q.m.off + 16 * j + r] * (uint32_t)a.lda + g * 16 : BUF_NONE;
     return q;
   };
   const uint32_t up = (uint32_t)a.I * (uint32_t)a.K;
-  v4i wb[D][4], xb[D][MT][4];
+  v4i wb[D][RW][4], xb[D][MT][4];
   const auto fetch = [&](const Unit& q, int s, int d) {
     const uint32_t k = (SHARE ? s * 4 + wave : s) * MOE_STEP;
     const int left = a.K - (int)k;
     const uint32_t wo = r * 16 < left ? q.wo : BUF_NONE;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) wb[d][i] = moe_weights<KEEP>(q.w, wo, k + (i & 1) * 4 * a.K + (i >> 1) * up);
+    for (int w = 0; w < RW; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wb[d][w][i] = moe_weights<KEEP>(q.w, wo, k + (2 * w + (i & 1)) * 4 * a.K + (i >> 1) * up);
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       if (MT > 1 && 16 * j >= q.m.cnt) break;
@@ -338,43 +341,54 @@ __global__ __launch_bounds__(256, MT == 1 && D < 4 ? 4 : D < 4 ? 3 : 2) void moe
   for (int u = first; u < units; u += stride, ++turn) {
     const Unit next = unit_of(u + stride);
     const bool finish = !SHARE || (turn & 3) == wave;
-    float sg[4], su[4], as[MT];
+    float sg[RW][4], su[RW][4], as[MT];
     if (finish) {  // asked for ahead of the products
-      const float* sc = a.s13 + (int64_t)cur.m.e * 2 * a.I + cur.gi * 8 + 4 * (g & 1);
+      const float* sc = a.s13 + (int64_t)cur.m.e * 2 * a.I + cur.gi * 8 * RW + 4 * (g & 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sg[i] = sc[i];
-        su[i] = sc[a.I + i];
-      }
+      for (int w = 0; w < RW; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sg[w][i] = sc[8 * w + i];
+          su[w][i] = sc[a.I + 8 * w + i];
+        }
 #pragma unroll
       for (int j = 0; j < MT; ++j) as[j] = a.a_scale[16 * j + r < cur.m.cnt ? (int)lists.token[cur.m.off + 16 * j + r] * a.a_stride : 0];
     }
-    Acc acc[MT];
+    Acc acc[RW][MT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[j] = Acc{0, 0, 0, 0};
+    for (int w = 0; w < RW; ++w)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[w][j] = Acc{0, 0, 0, 0};
     for (int s = 0; s < steps; s += D) {
       const bool last = s + D >= steps;
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        moe_stage(st, wb[d]);
+#pragma unroll
+        for (int w = 0; w < RW; ++w) moe_stage(st + w * 4096, wb[d][w]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const v4i w0 = *(const v4i*)(st + h * 2048 + r * 128 + ((g ^ rr) * 16));
-          const v4i w1 = *(const v4i*)(st + h * 2048 + r * 128 + (((4 + g) ^ rr) * 16));
+          v4i wv[RW][2];
+#pragma unroll
+          for (int w = 0; w < RW; ++w)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) wv[w][i] = *(const v4i*)(st + w * 4096 + h * 2048 + r * 128 + (((4 * i + g) ^ rr) * 16));
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
             if (MT > 1 && 16 * j >= cur.m.cnt) break;
-            moe_mfma<OP>(acc[j], w0, w1, xb[d][j][2 * h], xb[d][j][2 * h + 1]);
+#pragma unroll
+            for (int w = 0; w < RW; ++w) moe_mfma<OP>(acc[w][j], wv[w][0], wv[w][1], xb[d][j][2 * h], xb[d][j][2 * h + 1]);
           }
         }
         __builtin_amdgcn_wave_barrier();
         fetch(last ? next : cur, last ? d : s + D + d, d);
       }
     }
-    Acc(*mine)[MT][64] = part[SHARE ? turn & 1 : 0];
+    Acc(*mine)[RW * MT][64] = part[SHARE ? turn & 1 : 0];
     if constexpr (SHARE) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) mine[wave][j][lane] = acc[j];
+      for (int w = 0; w < RW; ++w)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) mine[wave][w * MT + j][lane] = acc[w][j];
       __syncthreads();
     }
     if (finish) {
@@ -382,25 +396,30 @@ __global__ __launch_bounds__(256, MT == 1 && D < 4 ? 4 : D < 4 ? 3 : 2) void moe
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
         if (16 * j >= cur.m.cnt) break;
-        Acc sum = acc[j];
-        if constexpr (SHARE) sum = (mine[0][j][lane] + mine[1][j][lane]) + (mine[2][j][lane] + mine[3][j][lane]);
-        v4f h;
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float own = (float)sum[i];
-          const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(own), __float_as_uint(own), false, false);
-          const float gate = __uint_as_float(both[0]) * (as[j] * sg[i]), upv = __uint_as_float(both[1]) * (as[j] * su[i]);
-          h[i] = gate / (1.0f + expf(-gate)) * upv;
-          const uint32_t m = __float_as_uint(h[i]) & 0x7fffffffu;  // (as integers: a NaN is larger than everything)
-          top = top > m ? top : m;
-        }
         const int pos = cur.m.off + 16 * j + r;
-        if (16 * j + r < cur.m.cnt && g < 2) *(v4f*)(a.h + (int64_t)pos * a.I + cur.gi * 8 + 4 * g) = h;
-        if (a.tops) {
-          const auto o = __builtin_amdgcn_permlane16_swap(top, top, false, false);
-          top = o[0] > o[1] ? o[0] : o[1];
-          if (16 * j + r < cur.m.cnt && g == 0) a.tops[(int64_t)pos * groups + cur.gi] = top;
+        const bool there = 16 * j + r < cur.m.cnt;
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+          Acc sum = acc[w][j];
+          if constexpr (SHARE) sum = (mine[0][w * MT + j][lane] + mine[1][w * MT + j][lane]) + (mine[2][w * MT + j][lane] + mine[3][w * MT + j][lane]);
+          v4f h;
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float own = (float)sum[i];
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(own), __float_as_uint(own), false, false);
+            const float gate = __uint_as_float(both[0]) * (as[j] * sg[w][i]), upv = __uint_as_float(both[1]) * (as[j] * su[w][i]);
+            h[i] = gate / (1.0f + expf(-gate)) * upv;
+            const uint32_t m = __float_as_uint(h[i]) & 0x7fffffffu;  // (as integers: a NaN is larger than everything)
+            top = top > m ? top : m;
+          }
+          const int at = cur.gi * RW + w;
+          if (there && g < 2) *(v4f*)(a.h + (int64_t)pos * a.I + at * 8 + 4 * g) = h;
+          if (a.tops) {
+            const auto o = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+            top = o[0] > o[1] ? o[0] : o[1];
+            if (there && g == 0) a.tops[(int64_t)pos * (a.I / 8) + at] = top;
+          }
         }
       }
     }
@@ -467,8 +486,9 @@ __device__ __forceinline__ void moe_put(const MoeArgs& a, int tok, int n, float 
 // for the waves, D steps on their way; at the end of a group a wave adds its products, with their scales and shares, to sums of its own, and the
 // waves' sums are added in their order.  Where few outputs leave units without a block, several blocks share the steps of the same outputs
 // and a kernel behind adds what they leave.  ROWS = 8, groups of up to eight tokens: a product takes two steps, the first with its upper eight
-// rows and left eight columns, the second with the others, and the two blocks on its diagonal are added.  QUANT: few positions, whose codes every
-// block makes for itself in shared memory.  Up to TM tokens.
+// rows and left eight columns, the second with the others, and the two blocks on its diagonal are added.  ROWS = 32, groups of more than 16 tokens:
+// two products, so that tokens are read half as often (64 tokens, two of 8 experts of 4096 x 14336 90 us and 5 of the join, 116 with 16 rows; two of
+// 4 of 4096 x 8192 37 + 5 and 50).  QUANT: few positions, whose codes every block makes for itself in shared memory.  Up to TM tokens.
 constexpr int MOE_QUANT_MOST = 16384;
 template <int OP, int MT, int ROWS, int NW, int D, int TM, bool QUANT, bool KEEP>
 __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
@@ -476,8 +496,8 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   constexpr int NT = NW * 64;
   constexpr bool PAIR = ROWS == 8;  // two steps a product
   static_assert(!PAIR || MT == 1, "");
-  constexpr int WL = PAIR ? 2 : 4;  // loads of a step
-  __shared__ __attribute__((aligned(16))) uint8_t stage[NW][1024 * WL];
+  constexpr int WL = PAIR ? 2 : 4, RW = PAIR ? 1 : ROWS / 16;  // loads of a step for a product's rows, products beside each other
+  __shared__ __attribute__((aligned(16))) uint8_t stage[NW][1024 * WL * RW];
   __shared__ uint32_t entry[MOE_ENTRIES];
   __shared__ uint8_t token[MOE_TOKENS * MOE_TOP];
   __shared__ float share[MOE_TOKENS * MOE_TOP];
@@ -506,22 +526,25 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
   const int col = PAIR ? rr : r, half = PAIR ? 128 * (r >> 3) : 0;
   Buf w = buf_of(a.w2);
   const Buf xb_of = buf_of(a.hq);
-  uint32_t wo = BUF_NONE, xo[MT];
+  uint32_t wo[RW], xo[MT];
   const auto load_from = [&] {
     lm = group_of(uniform((int)entry[le]));
     w = buf_of(a.w2 + (int64_t)lm.e * a.K * a.I);
-    wo = (uint32_t)(n0 + g) * (uint32_t)a.I + r * 16;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) wo[w] = RW == 1 || n0 + 16 * w < a.K ? (uint32_t)(n0 + 16 * w + g) * (uint32_t)a.I + r * 16 : BUF_NONE;
 #pragma unroll
     for (int j = 0; j < MT; ++j) xo[j] = 16 * j + col < lm.cnt ? (uint32_t)(lm.off + 16 * j + col) * (uint32_t)a.I + half + g * 16 : BUF_NONE;
   };
   constexpr int XL = PAIR ? 2 : 4;
-  v4i wb[D][WL], xb[QUANT ? 1 : D][MT][XL];
+  v4i wb[D][RW][WL], xb[QUANT ? 1 : D][MT][XL];
   int loads = to - from;  // steps that are not on their way yet; behind the last one zeros are loaded
   const auto fetch = [&](int d) {
     const uint32_t k = ls * MOE_STEP;
     const int left = loads > 0 ? a.I - (int)k : 0;
 #pragma unroll
-    for (int i = 0; i < WL; ++i) wb[d][i] = moe_weights<KEEP>(w, r * 16 < left ? wo : BUF_NONE, k + i * 4 * a.I);
+    for (int v = 0; v < RW; ++v)
+#pragma unroll
+      for (int i = 0; i < WL; ++i) wb[d][v][i] = moe_weights<KEEP>(w, r * 16 < left ? wo[v] : BUF_NONE, k + i * 4 * a.I);
     if constexpr (!QUANT) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
@@ -537,22 +560,28 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
       if (le < count) load_from();
     }
   };
-  Acc acc[MT];
-  v4f sc = {0, 0, 0, 0};
+  Acc acc[RW][MT];
   const int ng = PAIR ? g & 1 : g;  // the four outputs of this lane
-  v4f sn = sc;  // scales of the group that is multiplied, and of the next one
-  const auto ahead = [&](int i) { sn = *(const v4f*)(a.s2 + (int64_t)group_of(uniform((int)entry[i])).e * a.K + n0 + 4 * ng); };
+  v4f sc[RW], sn[RW];  // scales of the group that is multiplied, and of the next one
+  const auto ahead = [&](int i) {
+    const float* of = a.s2 + (int64_t)group_of(uniform((int)entry[i])).e * a.K + n0 + 4 * ng;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) sn[w] = *(const v4f*)(of + (n0 + 16 * w < a.K ? 16 * w : 0));
+  };
   const auto begin = [&] {
     cm = group_of(uniform((int)entry[ce]));
-    sc = sn;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) sc[w] = sn[w];
     if (ce + 1 < count) ahead(ce + 1);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[j] = Acc{0, 0, 0, 0};
+    for (int w = 0; w < RW; ++w)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[w][j] = Acc{0, 0, 0, 0};
   };
   const auto end = [&] {
     if constexpr (PAIR) {  // rows 8 .. 15 of columns 8 .. 15 belong to rows 0 .. 7 of columns 0 .. 7: 32 + 8 lanes on
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[0][i] += __shfl(acc[0][i], (lane + 40) & 63);
+      for (int i = 0; i < 4; ++i) acc[0][0][i] += __shfl(acc[0][0][i], (lane + 40) & 63);
       if (lane >= 32) return;
     }
 #pragma unroll
@@ -560,11 +589,14 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
       if (16 * j + r >= cm.cnt) break;
       const int pos = cm.off + 16 * j + r;
       const float c = share[pos];
-      v4f* sum = (v4f*)(sums + (wave * a.T + token[pos]) * ROWS + 4 * ng);
-      v4f v = *sum;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __fmaf_rn((float)acc[j][i], c * sc[i], v[i]);
-      *sum = v;
+      for (int w = 0; w < RW; ++w) {
+        v4f* sum = (v4f*)(sums + (wave * a.T + token[pos]) * ROWS + 16 * w + 4 * ng);
+        v4f v = *sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __fmaf_rn((float)acc[w][j][i], c * sc[w][i], v[i]);
+        *sum = v;
+      }
     }
   };
   if (from < to) {  // the first weights, ahead of the codes
@@ -612,16 +644,20 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int q = 4 * i + g;
-            *(v4i*)(st + (r >> 3) * 1024 + q * 128 + (((r ^ q) & 7) * 16)) = wb[d][i];
+            *(v4i*)(st + (r >> 3) * 1024 + q * 128 + (((r ^ q) & 7) * 16)) = wb[d][0][i];
           }
           __builtin_amdgcn_wave_barrier();
         } else {
-          moe_stage(st, wb[d]);
+#pragma unroll
+          for (int w = 0; w < RW; ++w) moe_stage(st + 4096 * w, wb[d][w]);
         }
 #pragma unroll
         for (int h = 0; h < WL / 2; ++h) {
-          const v4i w0 = *(const v4i*)(st + h * 2048 + r * 128 + ((g ^ rr) * 16));
-          const v4i w1 = *(const v4i*)(st + h * 2048 + r * 128 + (((4 + g) ^ rr) * 16));
+          v4i wv[RW][2];
+#pragma unroll
+          for (int w = 0; w < RW; ++w)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) wv[w][i] = *(const v4i*)(st + w * 4096 + h * 2048 + r * 128 + (((4 * i + g) ^ rr) * 16));
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
             if (MT > 1 && 16 * j >= cm.cnt) break;
@@ -636,7 +672,8 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
               x0 = xb[d][j][2 * h];
               x1 = xb[d][j][2 * h + 1];
             }
-            moe_mfma<OP>(acc[j], w0, w1, x0, x1);
+#pragma unroll
+            for (int w = 0; w < RW; ++w) moe_mfma<OP>(acc[w][j], wv[w][0], wv[w][1], x0, x1);
           }
         }
         __builtin_amdgcn_wave_barrier();
@@ -656,6 +693,7 @@ __global__ __launch_bounds__(NW * 64) void moe_down_kernel(MoeArgs a) {
 #pragma unroll
     for (int w = 1; w < NW; ++w) v += sums[w * a.T * ROWS + i];
     const int tok = i / ROWS, n = n0 + i % ROWS;
+    if (n >= a.K) continue;
     if (gridDim.y > 1) a.parts[((int64_t)blockIdx.y * a.T + tok) * a.K + n] = v;
     else moe_put(a, tok, n, v);
   }
@@ -684,14 +722,15 @@ struct MoePlan {
   bool narrow;  // the down product's blocks have eight outputs
   bool quant;   // and make the codes of h themselves
   bool share;   // the waves of a block share a unit of the gate and up products
-  bool deep;    // eight steps on their way there
+  bool deep;    // four steps on their way there
+  bool wide;    // two products' rows a unit there
   int splits;   // blocks for the same outputs
 };
 static MoePlan moe_plan(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   MoePlan p;
   // Groups of 16 tokens, 32 or 64: experts with more stream their weights again.  With up to six tokens an expert on average few have more than 16,
-  // with up to twenty few have more than 32 (64 tokens, two of 8 experts of 4096 x 14336: gate and up 219 us in groups of 32, 252 of 64; 40, four of
-  // 16: 21 and 28; 64, two of 4: 180 and 157).
+  // with up to twenty few have more than 32 (one product's rows a unit: 64 tokens, two of 8 experts of 4096 x 14336: gate and up 219 us in groups of 32, 252 of 64;
+  // 40, four of 16: 21 and 28; 64, two of 4: 180 and 157).
   p.mt = T <= 16 || T * top <= 6 * E ? 1 : T <= 32 || T * top <= 20 * E ? 2 : 4;
   const int64_t used = std::min(E, T * top);
   // Waves with units of their own where rows are short and units many (13 tokens over 32 experts of 1024 x 14080: 160 us, 176 shared; 16 over 8 of
@@ -699,6 +738,10 @@ static MoePlan moe_plan(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   // unit (K = 4096: 151 us, 177 with one).
   p.share = K >= 2048 || used * (I / 8) < 4096;
   p.deep = p.mt == 1 && p.share && div_up(K, 1024) % 4 == 0;
+  // Two products' rows a unit, so that tokens are read half as often (a compute unit takes in about 33 GB/s of both), where it leaves enough of them
+  // and tokens weigh: 64 tokens, two of 8 experts of 4096 x 14336 197 us, 222 with one; two of 4 of 4096 x 8192 80 and 110; 64 over 128 experts 64
+  // and 68; but 27, all of 4 experts of 2784 x 352, 9.2 and 7.6, 32 over 64 experts of 2048 x 1408 58 and 57.
+  p.wide = p.mt > 1 ? used * (I / 8) >= 1024 : p.share && !p.deep && T * top >= 4 * used && used * (I / 8) >= 4096;
   // The down product: a compute unit takes in 23 GB/s, a little less on eight rows, so that what counts is how evenly the blocks fall on the units
   // (8 experts, 14336 -> 4096 columns, 256 blocks: 71 us, 4112 columns, 257 blocks: 137); a split is a launch more.
   const double bytes = (double)used * K * I;
@@ -707,7 +750,7 @@ static MoePlan moe_plan(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   p.splits = 1;
   for (int narrow = p.mt == 1; narrow >= 0; --narrow)
     for (int n = 1; n <= 8; ++n) {
-      const double blocks = (double)n * (double)(K / (narrow ? 8 : 16));
+      const double blocks = (double)n * (double)(p.mt > 1 ? div_up(K, 32) : K / (narrow ? 8 : 16));
       const double cost = std::ceil(blocks / 256) * bytes / blocks / (narrow ? 21e9 : 23e9) + (n > 1 ? 4e-6 : 0.0);
       if (cost < best * 0.98) best = cost, p.narrow = narrow, p.splits = n;
     }
@@ -745,23 +788,28 @@ template <int OP, int MT, int ROWS, bool QUANT, bool KEEP>
 static void run_down(const MoeArgs& a, int splits, hipStream_t s) {
   // waves and steps on their way: eight rows want more waves (64 tokens over 128 experts: 41 us with 16 and 2, 50 with 8 and 4, 54 with 16 and 4,
   // whose registers do not suffice), sixteen are indifferent
-  constexpr int NW = ROWS == 8 ? 16 : 8, D = 2;
-  const dim3 grid((unsigned)(a.K / ROWS), (unsigned)splits), block(NW * 64);
-  if (MT > 1 || a.T > 16) hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, 64, QUANT, KEEP>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((moe_down_kernel<OP, 1, ROWS, NW, D, 16, QUANT, KEEP>), grid, block, 0, s, a);
-}
-template <int OP, int MT, int D, bool SHARE, bool KEEP>
-static void run_up(const MoeArgs& a, hipStream_t s) {
-  // groups of tokens, at most
-  const int64_t units = (int64_t)std::min(a.E + a.T * a.top / (16 * MT), a.T * a.top) * (a.I / 8);
-  const dim3 grid((unsigned)std::min<int64_t>(SHARE ? units : div_up(units, 4), MT == 1 && D > 1 ? 512 : MT > 1 ? 768 : 1024)), block(256);
+    constexpr int NW = ROWS == 8 ? 16 : 8, D = MT == 4 ? 1 : 2;
+  const dim3 grid((unsigned)div_up(a.K, ROWS), (unsigned)splits), block(NW * 64);
   if constexpr (MT == 1) {
-    if (a.T <= MOE_ROUTED) {
-      hipLaunchKernelGGL((moe_up_kernel<OP, 1, D, true, SHARE, KEEP>), grid, block, 0, s, a);
+    if (a.T <= 16) {
+      hipLaunchKernelGGL((moe_down_kernel<OP, 1, ROWS, NW, D, 16, QUANT, KEEP>), grid, block, 0, s, a);
       return;
     }
   }
-  hipLaunchKernelGGL((moe_up_kernel<OP, MT, D, false, SHARE, KEEP>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, 64, QUANT, KEEP>), grid, block, 0, s, a);
+}
+template <int OP, int MT, int RW, int D, bool SHARE, bool KEEP>
+static void run_up(const MoeArgs& a, hipStream_t s) {
+  // groups of tokens, at most
+  const int64_t units = (int64_t)std::min(a.E + a.T * a.top / (16 * MT), a.T * a.top) * (a.I / (8 * RW));
+  const dim3 grid((unsigned)std::min<int64_t>(SHARE ? units : div_up(units, 4), RW * D > 1 ? 512 : MT > 1 ? 768 : 1024)), block(256);
+  if constexpr (MT == 1) {
+    if (a.T <= MOE_ROUTED) {
+      hipLaunchKernelGGL((moe_up_kernel<OP, 1, RW, D, true, SHARE, KEEP>), grid, block, 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((moe_up_kernel<OP, MT, RW, D, false, SHARE, KEEP>), grid, block, 0, s, a);
 }
 template <int OP, int MT>
 static void run_moe(MoeArgs a, const MoePlan& p, hipStream_t s) {
@@ -770,11 +818,13 @@ static void run_moe(MoeArgs a, const MoePlan& p, hipStream_t s) {
   if (a.T > MOE_ROUTED) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)div_up(a.T, 4)), dim3(256), 0, s, a);
   const auto up = [&](auto keep) {
     constexpr bool KEEP = decltype(keep)::value;
-    if (!p.share) return run_up<OP, MT, 1, false, KEEP>(a, s);
     if constexpr (MT == 1) {
-      if (p.deep) return run_up<OP, 1, 4, true, KEEP>(a, s);
+      if (!p.share) return run_up<OP, 1, 1, 1, false, KEEP>(a, s);
+      if (p.deep) return run_up<OP, 1, 1, 4, true, KEEP>(a, s);
+    } else {
+      if (!p.share) return p.wide ? run_up<OP, MT, 2, 1, false, KEEP>(a, s) : run_up<OP, MT, 1, 1, false, KEEP>(a, s);
     }
-    run_up<OP, MT, 1, true, KEEP>(a, s);
+    p.wide ? run_up<OP, MT, 2, 1, true, KEEP>(a, s) : run_up<OP, MT, 1, 1, true, KEEP>(a, s);
   };
   const auto down = [&](auto keep) {
     constexpr bool KEEP = decltype(keep)::value;
@@ -782,7 +832,7 @@ static void run_moe(MoeArgs a, const MoePlan& p, hipStream_t s) {
       if (p.narrow) return p.quant ? run_down<OP, 1, 8, true, KEEP>(a, p.splits, s) : run_down<OP, 1, 8, false, KEEP>(a, p.splits, s);
       if (p.quant) return run_down<OP, 1, 16, true, KEEP>(a, p.splits, s);
     }
-    run_down<OP, MT, 16, false, KEEP>(a, p.splits, s);
+    run_down<OP, MT, (MT > 1 ? 32 : 16), false, KEEP>(a, p.splits, s);
   };
   if (a.K % 128) up(std::true_type{});
   else up(std::false_type{});

@@ -107,10 +107,10 @@ def moe(a, a_scale, logits, w13, s13, w2, s2, top, renormalize=True):
             D, S2 = w2[e].double(), s2[e].double()
             part, sums = D @ q, D.abs() @ q.abs()
             y[t] += c * s * S2 * part
-            # Eight waves share the experts' reductions: each wave's part of a sum (in int32 for int8) is multiplied by its scales and added in fp32,
-            # then the waves' sums are.  No part and no running sum is larger than the sum of magnitudes, so an expert's parts (at most 8)
-            # cost a rounding for the conversion, the product and the addition each only where they are cut, 18 in all with the waves' sums,
-            # and every expert of the token one more for its addition.
-            wrong = D.abs() @ either + part.abs() * (ds + 10 * up) + sums * up * (18 + top + (I if code != torch.int8 else 0))
+            # Up to sixteen waves of up to eight blocks share the experts' reductions: each wave's part of a sum (in int32 for int8) is converted,
+            # multiplied by its scales and added in fp32 to what the wave has, then the waves' sums and the blocks' are added.  Running sums are no
+            # larger than the magnitudes in them, so that is a rounding of the sum of magnitudes for the conversions, two for the products, one for each
+            # addition on the longest way: `top` in a wave, 16 over the waves, 8 over the blocks.
+            wrong = D.abs() @ either + part.abs() * (ds + 10 * up) + sums * up * (27 + top + (I if code != torch.int8 else 0))
             slack[t] += c * s * S2.abs() * wrong
     return y, slack

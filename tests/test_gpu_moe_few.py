@@ -73,6 +73,9 @@ def test_larger(dev, code, T, E, top, hidden, inter):
     (3, 20, 6, 256, 896),     # and more
     (1, 16, 16, 1008, 1008),
     (64, 200, 16, 48, 32),
+    (20, 4, 2, 272, 2048),    # groups of 32, two products a unit
+    (20, 8, 4, 144, 4096),    # the same, waves with units of their own
+    (48, 2, 2, 272, 4096),    # groups of 64
 ])
 def test_each_way_of_cutting(dev, code, T, E, top, hidden, inter):
     args = make(gen(T + E + hidden), T, E, hidden, inter, code, torch.float32)
@@ -80,6 +83,10 @@ def test_each_way_of_cutting(dev, code, T, E, top, hidden, inter):
     first = check(dev, args, top, out_dtype=torch.float32, ref=ref)
     for _ in range(3):
         assert torch.equal(check(dev, args, top, out_dtype=torch.float32, ref=ref), first)
+
+
+def test_two_products_a_unit_for_groups_of_16(dev):
+    check(dev, make(gen(64), 64, 64, 2064, 512, E4M3), 5)
 
 
 @pytest.mark.parametrize("hidden,inter", [(131056, 16), (16, 131056)])
