@@ -259,7 +259,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs a) {
   };
   const auto put = [&](int c, int j, int h, v4i o) {
     const int q = 16 * j + 8 * h + drow;
-    buf_store(O, o, q < t.n && c * 64 + 8 * dpos < a.N ? (uint32_t)row_of(q) * (uint32_t)a.ldo + dpos * 16 : BUF_NONE, (uint32_t)c * 128);
+    buf_store(O, o, q < t.n && c * 64 + 8 * dpos < a.N ? (uint32_t)row_of(q) * (uint32_t)a.ldo + dpos * 16 + (uint32_t)c * 128 : BUF_NONE);
   };
   const auto fetch_b = [&](int c, v4i (&w)[KB][4]) {
 #pragma unroll

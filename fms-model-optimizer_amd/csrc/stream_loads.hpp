@@ -20,8 +20,10 @@ __device__ __forceinline__ v4i buf_stream(Buf b, uint32_t off, uint32_t uniform_
   return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(b, off, uniform_off, 2));
 }
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void buf_store(Buf b, v4i v, uint32_t off, uint32_t uniform_off = 0) {
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), b, off, uniform_off, 0);
+// The whole offset in the lane's register: behind a 16-byte store with an offset in a scalar register the compiler puts no wait states before the
+// data's registers are written again, and gfx950 has then now and then stored what they were written with (seen in the lowest four bytes).
+__device__ __forceinline__ void buf_store(Buf b, v4i v, uint32_t off) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), b, off, 0, 0);
 }
 
 }  // namespace fmsmo

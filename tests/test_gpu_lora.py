@@ -74,6 +74,22 @@ def test_rows_of_no_request(dev):
     assert got.data_ptr() == d.data_ptr() and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rank", [16, 32, 64, 128])
+def test_rows_of_no_request_are_copied_whole(dev, dt, rank):
+    """Many outputs of few rows without a request, again and again: each store leaves with the data that it was given."""
+    g = gen(rank)
+    y, x, a, b, scales = (t.to(dev) for t in make(g, 426, 72, 4104, rank, 2, dt))
+    ids, start = torch.tensor([0, 1], dtype=torch.int32, device=dev), torch.tensor([0, 90, 423], dtype=torch.int32, device=dev)
+    first = K().lora_add(y, x, a, b, ids, start, scales=scales)
+    for _ in range(20):
+        got = K().lora_add(y, x, a, b, ids, start, scales=scales)
+        assert torch.equal(got[423:], y[423:]) and torch.equal(got, first)
+    alone = torch.full((426,), -1, dtype=torch.int32, device=dev)
+    for _ in range(5):
+        assert torch.equal(K().lora_add(y, x, a, b, alone), y)
+
+
 def test_no_adapter_keeps_the_bits(dev):
     y = torch.tensor([[-0.0, float("nan"), float("inf"), 1.0] * 4], device=dev).half()
     x = torch.full((1, 16), float("nan"), device=dev).half()
