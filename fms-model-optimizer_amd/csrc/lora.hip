@@ -391,7 +391,8 @@ int fmsmo_check_launch();
 
 // Steps on their way of a wave of the first launch on tiles of 64 rows: what the registers hold.
 static constexpr int lora_depth(int rt) { return rt <= 2 ? 4 : rt == 4 ? 2 : 1; }
-// What a call is cut into.  Rows: tiles of 64 where a request has 32 on average, else of 16.  (Tiles of 128 rows read half of A and B and hold half as
+// What a call is cut into.  Rows: tiles of 64 where a request has 32 on average and they are so many that A and B, read for every tile, weigh, else
+// of 16.  (Tiles of 128 rows read half of A and B and hold half as
 // many waves' rows: rank 64, 6972 rows, 4096 -> 6144 79 us and 66.)
 struct LoraPlan {
   int mt, rt, tiles, parts, part_steps, cols;
@@ -422,7 +423,9 @@ static LoraPlan lora_plan(int64_t rows, int64_t seqs, bool ragged, int64_t slots
   LoraPlan p;
   p.rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
   const int steps = div_up(K, LORA_STEP), groups = div_up(N, 64);
-  if (!ragged || rows < 32 * seqs) {
+  // (tiles of 64 rows and of 16: rank 128, 156 rows of 2088 -> 1280 26.4 us and 14.3; 4096 -> 4096 of rank 32, 100 rows 16.0 and 10.3, 3000 24.7
+  // and 17.6, 8192 40.7 and 50.4; rank 64, 3000 31.2 and 26.2, 4096 31.1 and 32.6; rank 128, 2048 39.4 and 38.6)
+  if (!ragged || rows < 32 * seqs || rows < (p.rt == 8 ? 2048 : 4096)) {
     // Few rows: parts of K for about 512 blocks, a step of 64 elements for each of their four waves at least (and 64 MB of sums at most), and of the
     // outputs for about 768.  Of requests of one row, those of an adapter are one tile (196 requests of 32 adapters, rank 64, 8872 -> 8376: 52 us
     // with the parts that as many tiles as requests would have, 33 so).
@@ -453,7 +456,7 @@ extern "C" int64_t fmsmo_lora_workspace_bytes(int64_t rows, int64_t seqs, int ra
 
 template <int T, int RT, int MT>
 static void run_lora(const LoraArgs& a, hipStream_t s) {
-  constexpr int D = MT > 1 ? lora_depth(RT) : 2;
+  constexpr int D = MT > 1 ? lora_depth(RT) : RT == 8 ? 1 : 2;  // (rank 128 and 16 rows: two steps leave the registers, 6.9 us and 5.5)
   hipLaunchKernelGGL((lora_shrink_kernel<T, RT, MT, D>), dim3((unsigned)a.tiles, (unsigned)a.parts), dim3(256), 0, s, a);
   hipLaunchKernelGGL((lora_expand_kernel<T, RT, MT>), dim3((unsigned)a.tiles, (unsigned)div_up(div_up(a.N, 64), a.cols)), dim3(256), 0, s, a);
 }

@@ -192,6 +192,33 @@ def test_longer_requests(dev, dt, rank, cols, rows, new):
     assert torch.equal(check(dev, y, x, a, b, ids, start, scales), first)
 
 
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rank,cols,rows", [(8, 136, 72), (16, 1032, 136), (24, 72, 1096), (64, 200, 264), (104, 264, 136), (128, 2056, 64)])
+def test_tiles_of_64_rows(dev, dt, rank, cols, rows):
+    """Enough rows, requests that end beside tiles and empty ones among them, rows of no request in front and behind; in place; a row of NaN, and
+    infinities in one without an adapter, which is y's."""
+    g = gen(rank + cols)
+    start = [5]
+    for n in (1200, 0, 63, 64, 65, 1, 128, 0, 2600):
+        start.append(start[-1] + n)
+    y, x, a, b, scales = make(g, start[-1] + 70, cols, rows, rank, 4, dt)
+    ids = [3, 0, 1, -1, 2, 0, 4, 1, 0]
+    x[40] = float("nan")
+    x[1300] = float("inf")
+    args = [t.to(dev) for t in (a, b)] + [torch.tensor(ids, dtype=torch.int32, device=dev), torch.tensor(start, dtype=torch.int32, device=dev)]
+    got = K().lora_add(y.to(dev), x.to(dev), *args, scales=scales.to(dev))
+    assert got[40].isnan().all() and torch.equal(got[1300].cpu(), y[1300])
+    d = y.to(dev)
+    K().lora_add(d, x.to(dev), *args, scales=scales.to(dev), out=d)
+    assert torch.equal(d.view(torch.int16), got.view(torch.int16))
+    x[40] = x[1300] = 0
+    clean = check(dev, y, x, a, b, ids, start, scales)
+    keep = [t for t in range(y.shape[0]) if t not in (40, 1300)]
+    assert torch.equal(got[keep], clean[keep])
+    for part in (slice(0, 5), slice(start[-1], None), slice(start[3], start[4])):
+        assert torch.equal(got[part].cpu().view(torch.int16), y[part].view(torch.int16))
+
+
 def test_nothing_to_do(dev):
     k = K()
     z = torch.empty(0, 64, device=dev).half()
