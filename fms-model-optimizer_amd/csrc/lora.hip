@@ -432,7 +432,11 @@ static LoraPlan lora_plan(int64_t rows, int64_t seqs, bool ragged, int64_t slots
     p.mt = 1;
     p.tiles = (int)(ragged ? rows / 16 + seqs + 2 : seqs);
     const int real = (int)(ragged ? p.tiles : std::min(seqs, slots + seqs / 16 + 1));
-    const int parts = std::min({512 / real, div_up(steps, 4), (int)((64 << 10) / ((int64_t)p.tiles * p.rt))});
+    // What a block of the first launch takes in falls with the parts, what one of the second adds up grows with them: the sum is least at the root of
+    // steps (2 rt + 2) KB / 23 GB/s over rt KB / 33 GB/s (one row, 14336 inputs, rank 16: 56 parts 8.2 + 3.8 us, 36 6.0 + 3.8; 72 rows of 4 adapters,
+    // rank 128, 10592 -> 3352: 14.4 + 15.8 and 12.8 + 12.5).
+    const int even = (int)std::sqrt(2.9 * steps * (p.rt + 1) / p.rt);
+    const int parts = std::min({512 / real, div_up(steps, 4), even, (int)((64 << 10) / ((int64_t)p.tiles * p.rt))});
     p.part_steps = div_up(div_up(steps, std::max(parts, 1)), 4) * 4;
     const int blocks = std::max(1, std::min(768 / real, div_up(groups, 4)));
     p.cols = div_up(div_up(groups, blocks), 4) * 4;
