@@ -1540,7 +1540,8 @@ def add_rms_norm_quant(x, weight, residual=None, *, eps=1e-6, dtype=torch.int8, 
         residual_out = torch.empty((M, K), dtype=x.dtype, device=x.device)
     args = (x, weight, residual, float(eps), scale, q, made, residual_out, normed)
     if M == 0 or K == 0:
-        pass
+        if made is not None:  # (tokens of no elements: the scale of rows of zeros)
+            made.fill_(1e-5 / 127 if dtype == torch.int8 else 1e-12)
     elif _eager(*(t for t in args if torch.is_tensor(t))):
         _add_rms_norm_quant_impl(*args)
     else:

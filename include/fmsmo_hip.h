@@ -926,7 +926,8 @@ int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int heads, int dim, int ca
  *   with static_scale, scale [1] is read: q = rint(clamp(n / s, +-127)), e4m3(clamp(n / s, +-448)).
  * Everything is fp32 up to the one rounding of each output; the recipes are those of fmsmo_quant_act_i8_pertoken with the compute dtype
  * FMSMO_F32 and of fmsmo_quant_act_fp8_pertoken.  dtype FMSMO_F16 or FMSMO_BF16, weight_dtype the same or FMSMO_F32.  A row with a NaN
- * or an infinity: scale NaN, e4m3 codes NaN, int8 codes not specified.
+ * or an infinity: scale NaN, e4m3 codes NaN, int8 codes not specified; one whose sum of squares leaves fp32: n = 0.
+ * M = 0 or K = 0: nothing is written.
  * K and leading dimensions multiples of 8, pointers 16-byte aligned (q: 8).
  */
 int fmsmo_add_rms_norm_quant(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
