@@ -1582,7 +1582,7 @@ def moe_few_tokens(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, *, r
     silu(gate) * up in 8 bits per token and expert, down products, sum.  a [T, K] int8 or float8_e4m3fn codes with a_scale [T] (as
     ``add_rms_norm_quant`` and the quantizers make them), logits [T, E], w13 [E, 2 I, K] (gate rows, then up rows) and w2 [E, K, I] of a's dtype with
     fp32 scales [E, 2 I] and [E, K].  Returns [T, K] in ``out`` (apart from the operands) or a new tensor of ``out_dtype``.  More tokens:
-    ``grouped_gemm_i8_dq`` on rows sorted by expert.  No gradients.  See fmsmo_moe_few_tokens."""
+    64 at a time, or for int8 ``grouped_gemm_i8_dq`` on rows sorted by expert.  No gradients.  See fmsmo_moe_few_tokens."""
     if not _COMPILING():
         r = (_H or _host()).moe_few_tokens(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, out_dtype, out)
         if r is not None:
@@ -1592,7 +1592,8 @@ def moe_few_tokens(a, a_scale, logits, w13, w13_scale, w2, w2_scale, top_k, *, r
         raise ValueError("a must be [tokens, K]")
     T, K = a.shape
     if T > 64:
-        raise ValueError(f"up to 64 tokens, got {T}: sort the rows by expert and use grouped_gemm_i8_dq")
+        raise ValueError(f"up to 64 tokens, got {T}: call it for 64 at a time"
+                         + (", or sort the rows by expert and use grouped_gemm_i8_dq" if a.dtype == torch.int8 else ""))
     if out is None:
         if out_dtype not in _DT:
             raise TypeError(f"unsupported floating dtype {out_dtype}")

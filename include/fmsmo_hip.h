@@ -966,7 +966,7 @@ int64_t fmsmo_lora_workspace_bytes(int64_t rows, int64_t seqs, int ragged, int64
  * E <= 512, top <= 16, K and I multiples of 16 below 2^17, w13[e] within 2 GB; operands and w2_scale 16-byte aligned, lda a multiple of 16
  * up to 2^24; y apart from the operands.  workspace: fmsmo_moe_few_workspace_bytes(T, E, top, K, I) bytes, 16-byte aligned, private to the call
  * until it has finished.
- * More tokens: fmsmo_grouped_gemm_i8_dq.
+ * More tokens: 64 at a time, or, int8, fmsmo_grouped_gemm_i8_dq on rows sorted by expert.
  */
 int fmsmo_moe_few_tokens(int codes, const void* a, int64_t lda, const float* a_scale, int64_t a_scale_n, const void* logits, int logits_dtype,
                          int64_t ldl, const void* w13, const float* w13_scale, const void* w2, const float* w2_scale, int64_t T, int64_t E,
