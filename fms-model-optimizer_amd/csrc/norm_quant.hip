@@ -8,6 +8,7 @@
 // The recipes are those of the per-token quantizers in fp32, so a product takes these codes as it takes theirs.
 #include "quant_math.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace fmsmo {
@@ -315,9 +316,7 @@ extern "C" int fmsmo_add_rms_norm_quant(const void* x, int dtype, int64_t ldx, c
   if (K % 8 || off(x, ldx) || off(residual, ldr) || off(residual_out, ldo) || off(normed, ldn) || ((uintptr_t)weight & 15) ||
       ((uintptr_t)q & 7) || (M > 1 && ldq % 8) || ((uintptr_t)scale & 3))
     return FMSMO_ERR_ALIGN;
-  NormArgs a{(const u16*)x, (const u16*)residual, weight, (u16*)residual_out, (u16*)normed, (uint8_t*)q, scale, ldx, ldr, ldo, ldn, ldq,
-             M, (int)K, eps, 1.0f / (float)K, static_scale != 0};
-  const auto types = [&](auto t) {
+  const auto types = [&](auto t, const NormArgs& a) {
     constexpr int T = decltype(t)::value;
     if (weight_dtype == FMSMO_F32) {
       if (codes == FMSMO_OP_E4M3) run_norm<T, FMSMO_F32, true>(a, (hipStream_t)stream);
@@ -327,7 +326,15 @@ extern "C" int fmsmo_add_rms_norm_quant(const void* x, int dtype, int64_t ldx, c
       else run_norm<T, T, false>(a, (hipStream_t)stream);
     }
   };
-  if (dtype == FMSMO_F16) types(std::integral_constant<int, FMSMO_F16>{});
-  else types(std::integral_constant<int, FMSMO_BF16>{});
+  // A launch has fewer than 2^32 threads, and a row up to 1024 of them.
+  constexpr int64_t MOST = 1 << 21;
+  for (int64_t from = 0; from < M; from += MOST) {
+    const NormArgs a{(const u16*)x + from * ldx, residual ? (const u16*)residual + from * ldr : nullptr, weight,
+                     residual_out ? (u16*)residual_out + from * ldo : nullptr, normed ? (u16*)normed + from * ldn : nullptr, (uint8_t*)q + from * ldq,
+                     static_scale ? scale : scale + from, ldx, ldr, ldo, ldn, ldq, std::min(MOST, M - from), (int)K, eps, 1.0f / (float)K,
+                     static_scale != 0};
+    if (dtype == FMSMO_F16) types(std::integral_constant<int, FMSMO_F16>{}, a);
+    else types(std::integral_constant<int, FMSMO_BF16>{}, a);
+  }
   return fmsmo_check_launch();
 }

@@ -48,3 +48,32 @@ def test_more_tokens_than_the_expert_block_takes(dev, code):
     got = torch.cat([call(slice(i, i + 64)) for i in range(0, T, 64)])
     want, slack = R.moe(*(t.cpu() for t in (a, sa, l, w13, s13, w2, s2)), 2)
     assert ((got.cpu().double() - want).abs() <= R.rounding(want, torch.float32) + slack * (1 + R.HALF[torch.float32])).all()
+
+
+def test_rows_of_several_launches(dev):
+    """2^26 rows and more, which no launch has threads for: the results of calls on pieces of them."""
+    T, some = (1 << 26) + 5, 1 << 20
+    g = torch.Generator(dev).manual_seed(5)
+    x, w = torch.empty(T, 8, device=dev, dtype=torch.bfloat16).normal_(generator=g), torch.randn(8, device=dev).bfloat16()
+    q, s, _, _ = K().add_rms_norm_quant(x, w, dtype=I8)
+    q2, s2, _, _ = K().add_rms_norm_quant(x, w, dtype=E4M3, scale=0.01)
+    for i in range(0, T, some):
+        t = slice(i, min(i + some, T))
+        a, b, _, _ = K().add_rms_norm_quant(x[t], w, dtype=I8)
+        assert torch.equal(q[t], a) and torch.equal(s[t], b)
+        assert torch.equal(q2[t].view(torch.uint8), K().add_rms_norm_quant(x[t], w, dtype=E4M3, scale=s2)[0].view(torch.uint8))
+
+
+def test_residuals_of_several_launches(dev):
+    """Rows on both sides of what one launch takes, with everything that a call can write, in place and apart."""
+    T, some = (1 << 22) + 3, (1 << 21) - 7
+    g = torch.Generator(dev).manual_seed(6)
+    x, r = (torch.empty(T, 16, device=dev, dtype=torch.float16).normal_(generator=g) for _ in range(2))
+    w = torch.randn(16, device=dev)
+    got = K().add_rms_norm_quant(x, w, r, dtype=E4M3, want_normed=True)
+    for i in range(0, T, some):
+        t = slice(i, min(i + some, T))
+        for a, b in zip(got, K().add_rms_norm_quant(x[t], w, r[t], dtype=E4M3, want_normed=True)):
+            assert torch.equal(a[t].view(torch.uint8), b.view(torch.uint8))
+    h = K().add_rms_norm_quant(x, w, r, dtype=E4M3, residual_out=r)
+    assert h[2] is r and torch.equal(r, got[2]) and torch.equal(h[1], got[1])
