@@ -430,7 +430,9 @@ static LoraPlan lora_plan(int64_t rows, int64_t seqs, bool ragged, int64_t slots
     // outputs for about 768.  Of requests of one row, those of an adapter are one tile (196 requests of 32 adapters, rank 64, 8872 -> 8376: 52 us
     // with the parts that as many tiles as requests would have, 33 so).
     p.mt = 1;
-    p.tiles = (int)(ragged ? rows / 16 + seqs + 2 : seqs);
+    // (Requests of one row 8192 at a time: each counts those before it, and 64 MB hold their sums.  64 -> 64 of rank 16, 65536 requests: 6.7 ms at
+    // once, 0.92 so; of rank 128: 16.2 and 2.0.)
+    p.tiles = (int)(ragged ? rows / 16 + seqs + 2 : std::min<int64_t>(seqs, 8192));
     const int real = (int)(ragged ? p.tiles : std::min(seqs, slots + seqs / 16 + 1));
     // What a block of the first launch takes in falls with the parts, what one of the second adds up grows with them: the sum is least at the root of
     // steps (2 rt + 2) KB / 23 GB/s over rt KB / 33 GB/s (one row, 14336 inputs, rank 16: 56 parts 8.2 + 3.8 us, 36 6.0 + 3.8; 72 rows of 4 adapters,
@@ -487,9 +489,10 @@ extern "C" int fmsmo_lora_add(int dtype, const void* x, int64_t ldx, const void*
   if (rows > 1 && 64 * widest + 2 * std::max(K, N) > MOST) return FMSMO_ERR_UNSUPPORTED;
   if (!workspace) return FMSMO_ERR_NULL;
   const LoraPlan p = lora_plan(rows, seqs, query_start != nullptr, std::min<int64_t>(slots, 1 << 29), rank, K, N);
+  if (p.tiles >= 1 << 24) return FMSMO_ERR_UNSUPPORTED;  // (a launch has fewer than 2^32 threads)
   if (workspace_bytes < (int64_t)p.parts * p.tiles * (1024 * p.mt * p.rt)) return FMSMO_ERR_SCRATCH;
   // rows of one adapter may lie anywhere among the requests of one row: as many of them at a time as 32 bits reach
-  const int64_t most = query_start || rows == 1 ? rows : (MOST - 2 * std::max(K, N)) / widest;
+  const int64_t most = query_start || rows == 1 ? rows : std::min<int64_t>(p.tiles, (MOST - 2 * std::max(K, N)) / widest);
   for (int64_t from = 0; from < rows; from += most) {
     const int64_t some = std::min(most, rows - from);
     LoraArgs g{(const char*)x + 2 * from * ldx, (const char*)y + 2 * from * ldy, (char*)out + 2 * from * ldo, (const char*)a, (const char*)b,

@@ -943,8 +943,9 @@ int fmsmo_add_rms_norm_quant(const void* x, int dtype, int64_t ldx, const void* 
  * Rows of a request whose number is none of the slots (-1), and rows of no request: out = y.  Starts that descend give results without a
  * meaning, but nothing outside of the operands is touched.  Sums are fp32; a[s] x is taken as the sum of two 16-bit numbers, the result is rounded once.
  * rank a multiple of 8 up to 128; K, N up to 2^22 and strides multiples of 8, operands 16-byte aligned; 64 rows of x, y or out, 128 of an
- * adapter's a and all of its b within 2 GB.  workspace: fmsmo_lora_workspace_bytes(rows, seqs, query_start != NULL, slots, rank, K) bytes,
- * 16-byte aligned, private to the call until it has finished.
+ * adapter's a and all of its b within 2 GB; fewer than 2^30 rows, with query_start rows / 16 + seqs below 2^24 - 2.
+ * workspace: fmsmo_lora_workspace_bytes(rows, seqs, query_start != NULL, slots, rank, K) bytes, 16-byte aligned, private to the call until it has
+ * finished.
  */
 int fmsmo_lora_add(int dtype, const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, const void* a, int64_t a_slot,
                    int64_t a_row, const void* b, int64_t b_slot, int64_t b_row, int64_t slots, int rank, const int32_t* adapters,

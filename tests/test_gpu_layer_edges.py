@@ -77,3 +77,21 @@ def test_residuals_of_several_launches(dev):
             assert torch.equal(a[t].view(torch.uint8), b.view(torch.uint8))
     h = K().add_rms_norm_quant(x, w, r, dtype=E4M3, residual_out=r)
     assert h[2] is r and torch.equal(r, got[2]) and torch.equal(h[1], got[1])
+
+
+@pytest.mark.parametrize("rank,T", [(128, 20001), (64, 40000)])
+def test_one_row_requests_of_several_launches(dev, rank, T):
+    g = torch.Generator().manual_seed(rank)
+    x, y = torch.randn(T, 64, generator=g).bfloat16(), torch.randn(T, 64, generator=g).bfloat16()
+    a, b = (0.125 * torch.randn(5, rank, 64, generator=g)).bfloat16(), torch.randn(5, 64, rank, generator=g).bfloat16()
+    ids, scales = torch.randint(-1, 6, (T,), generator=g), 0.5 + torch.rand(5, generator=g)
+    args = [t.to(dev) for t in (y, x, a, b, ids.to(torch.int32))]
+    got = K().lora_add(*args, scales=scales.to(dev))
+    # the rows of each adapter as one request of the reference
+    order = ids.argsort(stable=True)
+    start = [0] + torch.bincount(ids + 1, minlength=7).cumsum(0).tolist()
+    want, slack = R.lora(y[order], x[order], a, b, list(range(-1, 6)), start, scales)
+    bound = R.rounding(want, y.dtype) + slack * (1 + R.HALF[y.dtype]) + 2.0 ** -24 * want.abs()
+    assert ((got.cpu()[order].double() - want).abs() <= bound).all()
+    d = args[0].clone()
+    assert K().lora_add(d, *args[1:], scales=scales.to(dev), out=d) is d and torch.equal(d, got)
