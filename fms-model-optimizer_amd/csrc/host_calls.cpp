@@ -10,6 +10,7 @@
 // gets its error messages there).  Nothing is kept from one call to the next.
 #include <ATen/ATen.h>
 #include <cmath>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -1035,6 +1036,9 @@ PyObject* lora_add(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor *xt = plain(args[1]), *a = plain(args[2]), *b = plain(args[3]), *ids = plain(args[4]);
   const at::Tensor *qs = args[5] == Py_None ? nullptr : plain(args[5]), *sc = args[6] == Py_None ? nullptr : plain(args[6]);
   if (!xt || !a || !b || !ids || (!qs && args[5] != Py_None) || (!sc && args[6] != Py_None)) return none();
+  if (c10::GradMode::is_enabled())
+    for (const at::Tensor* t : {xt, a, b, sc, plain(args[0]), args[7] == Py_None ? nullptr : plain(args[7])})
+      if (t && t->requires_grad()) return none();
   const at::ScalarType st = xt->scalar_type();
   if (st != at::kHalf && st != at::kBFloat16) return none();
   const Mat x = mat16(args[1], st), y = mat16(args[0], st);

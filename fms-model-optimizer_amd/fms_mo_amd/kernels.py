@@ -1554,11 +1554,14 @@ def lora_add(y, x, a, b, adapters, query_start=None, *, scales=None, out=None):
     x [T, K] is what the projection took (in 16 bits), y [T, N] what it gave; a [slots, rank, K] and b [slots, N, rank] a pool of adapters
     (smaller ranks padded with zeros; views of a larger pool need contiguous rows only), all fp16 or all bf16; adapters int32 [B], -1 for
     none; query_start int32 [B + 1] as in ``paged_attention`` (None: one row per request); scales fp32 [slots].  Rows without an adapter
-    are y's.  Returns [T, N] in ``out`` (y itself, or memory apart from x and y) or a new tensor.  No gradients.  See fmsmo_lora_add."""
+    are y's.  Returns [T, N] in ``out`` (y itself, or memory apart from x and y) or a new tensor.  No gradients: refused where one would be
+    expected (operands that require them, outside of ``torch.no_grad``).  See fmsmo_lora_add."""
     if not _COMPILING():
         r = (_H or _host()).lora_add(y, x, a, b, adapters, query_start, scales, out)
         if r is not None:
             return r if out is None else out
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, x, a, b, scales, out)):
+        raise RuntimeError("lora_add has no gradients: call it under torch.no_grad(), or with operands that require none")
     _need_gpu(y, x)
     if x.dim() != 2 or y.dim() != 2 or x.shape[0] != y.shape[0]:
         raise ValueError("x and y must be [tokens, K] and [tokens, N]")

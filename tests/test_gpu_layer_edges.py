@@ -95,3 +95,25 @@ def test_one_row_requests_of_several_launches(dev, rank, T):
     assert ((got.cpu()[order].double() - want).abs() <= bound).all()
     d = args[0].clone()
     assert K().lora_add(d, *args[1:], scales=scales.to(dev), out=d) is d and torch.equal(d, got)
+
+
+def test_adapters_that_require_gradients(dev):
+    """Refused where the native host call would take them; under no_grad parameters are operands like others."""
+    g = torch.Generator().manual_seed(2)
+    x, y = (torch.randn(3, 64, generator=g).half().to(dev) for _ in range(2))
+    a, b = torch.randn(2, 8, 64, generator=g).half().to(dev), torch.randn(2, 64, 8, generator=g).half().to(dev)
+    ids, scales = torch.tensor([1, -1, 0], dtype=torch.int32, device=dev), torch.rand(2, generator=g).to(dev)
+    want = K().lora_add(y, x, a, b, ids, scales=scales)
+    for i in range(5):
+        d = [y, x, a, b, scales]
+        d[i] = torch.nn.Parameter(d[i])
+
+        def call(y, x, a, b, scales):
+            return K().lora_add(y, x, a, b, ids, scales=scales)
+
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call(*d)
+        with torch.no_grad():
+            assert torch.equal(call(*d), want) and torch.equal(torch.compile(call, backend="aot_eager", fullgraph=True)(*d), want)
+        with torch.inference_mode():
+            assert torch.equal(call(*d), want)

@@ -1,5 +1,6 @@
 """Sizes at which calls of the operators around a layer's products are cut or refused: no GPU is needed."""
 import pytest
+import torch
 
 from test_layer_rules import SCRATCH, UNSUPPORTED, lib, p  # noqa: F401
 
@@ -17,3 +18,20 @@ def test_adapters_of_more_tiles_than_a_launch_has_threads_for(lib, p):  # noqa: 
 
     assert call(4, (1 << 24) - 3) == SCRATCH and call(4, (1 << 24) - 2) == UNSUPPORTED and call(4, 1 << 28) == UNSUPPORTED
     assert call((1 << 28) - 64, 1 << 23) == UNSUPPORTED and call(1 << 28, 2) == SCRATCH and call((1 << 30) - 64, 1) == UNSUPPORTED
+
+
+def test_adapters_have_no_gradients():
+    """Where a gradient would be expected the call is refused (and goes on to the next check where none is)."""
+    from fms_mo_amd import kernels as k
+
+    h, ids = torch.zeros(2, 64).half(), torch.zeros(2, dtype=torch.int32)
+    given = dict(y=h, x=h, a=torch.zeros(1, 8, 64).half(), b=torch.zeros(1, 64, 8).half(), scales=torch.ones(1), out=torch.zeros(2, 64).half())
+    for name in given:
+        d = dict(given)
+        d[name] = torch.nn.Parameter(d[name])
+        with pytest.raises(RuntimeError, match="no gradients"):
+            k.lora_add(adapters=ids, **d)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            k.lora_add(adapters=ids, **d)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        k.lora_add(adapters=ids, **given)
