@@ -1,13 +1,13 @@
-// A mixture-of-experts block for a few tokens (up to 64), whose weights are read once and bound it: routing, gate and up products, gated
-// silu in 8 bits, down products and the weighted sum.
+// A mixture-of-experts block for a few tokens (up to 64), whose weights bound it: routing, gate and up products, gated silu in 8 bits, down
+// products and the weighted sum.
 //
 //   p = softmax(logits[t]); S = the `top` experts of the largest logits (of equal ones the lower index); c_e = p_e / sum_S p, or p_e
 //   g, u = (a[t] . w13[e]^T) a_scale[t] w13_scale[e]  (rows 0 .. I - 1 and I .. 2I - 1),  h = g / (1 + exp(-g)) u  in fp32
 //   codes of h per token and expert: int8 s = max(max|h|, 1e-5) / 127, e4m3 s = max(max|h| / 448, 1e-12), as the per-token quantizers in fp32
 //   y[t] = sum_S c_e s (codes . w2[e]^T) w2_scale[e]
 //
-// The chosen (token, expert) pairs are sorted by expert: a `position` each.  The weights stream past once, eight rows of 128 bytes a load,
-// and are turned into matrix operands in shared memory; an expert's tokens are the columns of the product.
+// The chosen (token, expert) pairs are sorted by expert: a `position` each.  The weights stream past, once for a group of up to 8 to 64 tokens of an
+// expert (by the plan; mostly all of them), and are turned into matrix operands in shared memory; a group's tokens are the columns of the product.
 #include "paged_kv.hpp"
 #include "stream_loads.hpp"
 
@@ -743,15 +743,19 @@ static MoePlan moe_plan(int64_t T, int64_t E, int top, int64_t K, int64_t I) {
   // and 68; but 27, all of 4 experts of 2784 x 352, 9.2 and 7.6, 32 over 64 experts of 2048 x 1408 58 and 57.
   p.wide = p.mt > 1 ? used * (I / 8) >= 1024 : p.share && !p.deep && T * top >= 4 * used && used * (I / 8) >= 4096;
   // The down product: a compute unit takes in 23 GB/s, a little less on eight rows, so that what counts is how evenly the blocks fall on the units
-  // (8 experts, 14336 -> 4096 columns, 256 blocks: 71 us, 4112 columns, 257 blocks: 137); a split is a launch more.
+  // (8 experts, 14336 -> 4096 columns, 256 blocks: 71 us, 4112 columns, 257 blocks: 137); a split is a launch more.  On eight rows an expert's
+  // tokens are groups of eight, and its weights stream past for each of them: m tokens an expert on average are about m / 8 + 0.5 groups.
+  // Sixteen rows and eight, the whole block: 16 tokens, all of 2 experts of 2048 x 16384 58 us and 67, all of 8 of 2048 x 7168 90 and 103; 12, six of 8 of
+  // 2048 x 5632 63 and 71; 64, six of 64 of 2048 x 1408 108 and 114; but 32, four of 32 of 2048 x 2048 79 and 77.
   const double bytes = (double)used * K * I;
+  const double again = std::min(std::max((double)(T * top) / (8.0 * used) + 0.5, 1.0), (double)div_up(T, 8));
   double best = 1e30;
   p.narrow = false;
   p.splits = 1;
   for (int narrow = p.mt == 1; narrow >= 0; --narrow)
     for (int n = 1; n <= 8; ++n) {
       const double blocks = (double)n * (double)(p.mt > 1 ? div_up(K, 32) : K / (narrow ? 8 : 16));
-      const double cost = std::ceil(blocks / 256) * bytes / blocks / (narrow ? 21e9 : 23e9) + (n > 1 ? 4e-6 : 0.0);
+      const double cost = std::ceil(blocks / 256) * bytes * (narrow ? again : 1.0) / blocks / (narrow ? 21e9 : 23e9) + (n > 1 ? 4e-6 : 0.0);
       if (cost < best * 0.98) best = cost, p.narrow = narrow, p.splits = n;
     }
   // (a launch or so many rows for every block: 2 tokens, eight of 128 experts of 2048 x 768 23.4 us and 24.3, 4 tokens 34.9 and 31.9)

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import layer_reference as R
+from test_gpu_moe_few import check, gen, make
 
 pytestmark = pytest.mark.gpu
 I8, E4M3 = torch.int8, torch.float8_e4m3fn
@@ -117,3 +118,12 @@ def test_adapters_that_require_gradients(dev):
             assert torch.equal(call(*d), want) and torch.equal(torch.compile(call, backend="aot_eager", fullgraph=True)(*d), want)
         with torch.inference_mode():
             assert torch.equal(call(*d), want)
+
+
+@pytest.mark.parametrize("code", [I8, E4M3])
+@pytest.mark.parametrize("T,E,top,hidden,inter", [(16, 2, 2, 2048, 528), (12, 8, 6, 1040, 272), (64, 64, 6, 528, 144), (10, 4, 4, 2048, 80), (16, 2, 1, 1024, 512),
+                                                  (48, 12, 1, 256, 1024)])
+def test_experts_of_nine_tokens_and_more(dev, code, T, E, top, hidden, inter):
+    args = make(gen(T + E), T, E, hidden, inter, code, torch.float32)
+    first = check(dev, args, top)
+    assert torch.equal(check(dev, args, top), first)

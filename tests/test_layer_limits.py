@@ -35,3 +35,13 @@ def test_adapters_have_no_gradients():
             k.lora_add(adapters=ids, **d)
     with pytest.raises(RuntimeError, match="no CPU path"):
         k.lora_add(adapters=ids, **given)
+
+
+@pytest.mark.parametrize("T,E,top,K,I,blocks", [(16, 2, 2, 2048, 16384, 2), (16, 8, 8, 2048, 7168, 2), (12, 8, 6, 2048, 5632, 2), (64, 64, 6, 2048, 1408, 2),
+                                                (10, 4, 4, 2048, 5632, 2), (64, 128, 8, 2048, 768, 1), (32, 32, 4, 2048, 2048, 1), (8, 4, 4, 2048, 5632, 1)])
+def test_experts_of_more_than_eight_tokens(lib, T, E, top, K, I, blocks):  # noqa: F811
+    """The down product's blocks of eight outputs read an expert's weights for every eight of its tokens.  Where that is more than once for most
+    experts, blocks of sixteen go two for the same outputs, whose sums need room in the workspace."""
+    rest = 5 * T * top * I + T * top * I // 2 + 24 * T * top + 8192  # codes, h, its maxima, numbers of a choice, groups
+    n = lib.fmsmo_moe_few_workspace_bytes(T, E, top, K, I)
+    assert (n > rest) == (blocks > 1) and (blocks == 1 or n >= 4 * blocks * T * K + 5 * T * top * I)
