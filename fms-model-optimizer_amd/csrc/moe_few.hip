@@ -792,15 +792,15 @@ template <int OP, int MT, int ROWS, bool QUANT, bool KEEP>
 static void run_down(const MoeArgs& a, int splits, hipStream_t s) {
   // waves and steps on their way: eight rows want more waves (64 tokens over 128 experts: 41 us with 16 and 2, 50 with 8 and 4, 54 with 16 and 4,
   // whose registers do not suffice), sixteen are indifferent
-    constexpr int NW = ROWS == 8 ? 16 : 8, D = MT == 4 ? 1 : 2;
+  constexpr int NW = ROWS == 8 ? 16 : 8, D = MT == 4 ? 1 : 2;
   const dim3 grid((unsigned)div_up(a.K, ROWS), (unsigned)splits), block(NW * 64);
   if constexpr (MT == 1) {
-    if (a.T <= 16) {
+    if (QUANT || a.T <= 16) {  // (up to 16 positions where QUANT, so no more tokens)
       hipLaunchKernelGGL((moe_down_kernel<OP, 1, ROWS, NW, D, 16, QUANT, KEEP>), grid, block, 0, s, a);
       return;
     }
   }
-  hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, 64, QUANT, KEEP>), grid, block, 0, s, a);
+  if constexpr (!QUANT) hipLaunchKernelGGL((moe_down_kernel<OP, MT, ROWS, NW, D, 64, false, KEEP>), grid, block, 0, s, a);
 }
 template <int OP, int MT, int RW, int D, bool SHARE, bool KEEP>
 static void run_up(const MoeArgs& a, hipStream_t s) {
@@ -826,7 +826,7 @@ static void run_moe(MoeArgs a, const MoePlan& p, hipStream_t s) {
       if (!p.share) return run_up<OP, 1, 1, 1, false, KEEP>(a, s);
       if (p.deep) return run_up<OP, 1, 1, 4, true, KEEP>(a, s);
     } else {
-      if (!p.share) return p.wide ? run_up<OP, MT, 2, 1, false, KEEP>(a, s) : run_up<OP, MT, 1, 1, false, KEEP>(a, s);
+      if (!p.share) return run_up<OP, MT, 2, 1, false, KEEP>(a, s);  // (so many units that it is the wide form)
     }
     p.wide ? run_up<OP, MT, 2, 1, true, KEEP>(a, s) : run_up<OP, MT, 1, 1, true, KEEP>(a, s);
   };
