@@ -423,9 +423,11 @@ static LoraPlan lora_plan(int64_t rows, int64_t seqs, bool ragged, int64_t slots
   LoraPlan p;
   p.rt = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
   const int steps = div_up(K, LORA_STEP), groups = div_up(N, 64);
-  // (tiles of 64 rows and of 16: rank 128, 156 rows of 2088 -> 1280 26.4 us and 14.3; 4096 -> 4096 of rank 32, 100 rows 16.0 and 10.3, 3000 24.7
-  // and 17.6, 8192 40.7 and 50.4; rank 64, 3000 31.2 and 26.2, 4096 31.1 and 32.6; rank 128, 2048 39.4 and 38.6)
-  if (!ragged || rows < 32 * seqs || rows < (p.rt == 8 ? 2048 : 4096)) {
+  // (Tiles of 64 rows and of 16: rank 128, 156 rows of 2088 -> 1280 26.4 us and 14.3; 4096 -> 4096 of rank 32, 100 rows 16.0 and 10.3, 3000 24.7
+  // and 17.6, 8192 40.7 and 50.4; rank 64, 3000 31.2 and 26.2, 4096 31.1 and 32.6.  Rank 128 has less to gain from few rows, its A and B being
+  // most of what they read: the sum of 15 calls, 4096 -> 4096 to 14336 -> 4096 for one to nine requests, 2048 rows 814 and 767, 2800 913 and 898, 3200 942
+  // and 1018, 4095 1102 and 1257; but rank 72, padded to as many products, 2800 819 and 675, 3200 845 and 732, 4095 973 and 957.)
+  if (!ragged || rows < 32 * seqs || rows < (rank >= 120 ? 3000 : 4096)) {
     // Few rows: parts of K for about 512 blocks, a step of 64 elements for each of their four waves at least (and 64 MB of sums at most), and of the
     // outputs for about 768.  Of requests of one row, those of an adapter are one tile (196 requests of 32 adapters, rank 64, 8872 -> 8376: 52 us
     // with the parts that as many tiles as requests would have, 33 so).

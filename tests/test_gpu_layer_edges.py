@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import layer_reference as R
+import test_gpu_lora as lora
 from test_gpu_moe_few import check, gen, make
 
 pytestmark = pytest.mark.gpu
@@ -127,3 +128,10 @@ def test_experts_of_nine_tokens_and_more(dev, code, T, E, top, hidden, inter):
     args = make(gen(T + E), T, E, hidden, inter, code, torch.float32)
     first = check(dev, args, top)
     assert torch.equal(check(dev, args, top), first)
+
+
+@pytest.mark.parametrize("rank,T", [(128, 2999), (128, 3000), (72, 3500), (72, 4095), (72, 4096), (16, 4096)])
+def test_rows_about_the_larger_tiles(dev, rank, T):
+    g = gen(rank + T)
+    y, x, a, b, scales = lora.make(g, T, 136, 72, rank, 3, torch.float16)
+    lora.check(dev, y, x, a, b, [2, -1, 0, 1], [3, 1500, 1501, 2000, T - 1], scales)

@@ -1,4 +1,6 @@
 """Sizes at which calls of the operators around a layer's products are cut or refused: no GPU is needed."""
+import random
+
 import pytest
 import torch
 
@@ -45,3 +47,36 @@ def test_experts_of_more_than_eight_tokens(lib, T, E, top, K, I, blocks):  # noq
     rest = 5 * T * top * I + T * top * I // 2 + 24 * T * top + 8192  # codes, h, its maxima, numbers of a choice, groups
     n = lib.fmsmo_moe_few_workspace_bytes(T, E, top, K, I)
     assert (n > rest) == (blocks > 1) and (blocks == 1 or n >= 4 * blocks * T * K + 5 * T * top * I)
+
+
+def few(rows, seqs, ragged, rank):
+    return not ragged or rows < 32 * seqs or rows < (3000 if rank >= 120 else 4096)
+
+
+@pytest.mark.parametrize("rank", [8, 24, 40, 72, 128])
+@pytest.mark.parametrize("K", [8, 64, 1000, 14336])
+def test_lora_workspace_holds_the_tiles_of_any_starts(lib, rank, K):  # noqa: F811
+    """The sums of every tile of ascending starts, rows in front of the first request and behind the last among them, for tiles of 16 rows and
+    of 64; with one step of K they are all that there is."""
+    r, padded = random.Random(rank), 16 if rank <= 16 else 32 if rank <= 32 else 64 if rank <= 64 else 128
+    seen = set()
+    for rows, seqs in ((1, 1), (1, 3), (5, 700), (100, 2), (2047, 1), (2999, 2), (3000, 2), (4095, 1), (4096, 1), (4096, 128), (4096, 129), (8192, 1),
+                       (8192, 256), (8192, 257), (50000, 3)):
+        tile = 16 if few(rows, seqs, True, rank) else 64
+        seen.add(tile)
+        n = lib.fmsmo_lora_workspace_bytes(rows, seqs, 1, 3, rank, K)
+        assert n % 16 == 0
+        if K <= 64:
+            assert n == 4 * padded * tile * (rows // tile + seqs + 2)
+        for _ in range(20):
+            at = sorted(r.randint(0, rows) for _ in range(seqs + 1))
+            tiles = sum(-(-(b - a) // tile) for a, b in zip([0] + at, at + [rows]))
+            assert n >= 4 * padded * tile * tiles
+    assert seen == {16, 64}
+
+
+@pytest.mark.parametrize("rank", [8, 24, 40, 128])
+def test_lora_workspace_of_one_row_requests(lib, rank):  # noqa: F811
+    padded = 16 if rank <= 16 else 32 if rank <= 32 else 64 if rank <= 64 else 128
+    for rows in (1, 7, 100, 8192):
+        assert lib.fmsmo_lora_workspace_bytes(rows, rows, 0, 3, rank, 64) == 4 * padded * 16 * rows
