@@ -135,3 +135,45 @@ def test_rows_about_the_larger_tiles(dev, rank, T):
     g = gen(rank + T)
     y, x, a, b, scales = lora.make(g, T, 136, 72, rank, 3, torch.float16)
     lora.check(dev, y, x, a, b, [2, -1, 0, 1], [3, 1500, 1501, 2000, T - 1], scales)
+
+
+@pytest.mark.parametrize("T", [60, 4300])
+@pytest.mark.parametrize("start,same", [([0, 0, 0, 0], None), ([60, 40, 20, 0], None), ([-9, 30, 2000000000, 60], [0, 30, 60, 60]), ([0, 50, 20, 60], False),
+                                        ([2147483647, -2147483648, 5, 60], False), ([60, 0, 0, 60], False)])
+def test_starts_of_any_values(dev, T, start, same):
+    """Batches of 16-row and of 64-row tiles.  Rows that no request names are y's, starts outside of the rows end at them; where starts descend
+    nothing but the rows of out is written."""
+    k, g = K(), gen(T)
+    y, x, a, b, scales = lora.make(g, T, 64, 72, 16, 2, torch.float16)
+    by = T / 60
+    given = [s if abs(s) > 100 else int(s * by) for s in start]
+    if given[3] == int(60 * by):
+        given[3] = T
+    d = [t.to(dev) for t in (y, x, a, b, torch.tensor([0, 1, 0], dtype=torch.int32))]
+    room = torch.full((T + 200, 72), 7.0, device=dev).half()
+    out = k.lora_add(*d, torch.tensor(given, dtype=torch.int32, device=dev), scales=scales.to(dev), out=room[100:T + 100])
+    torch.cuda.synchronize()
+    assert (room[:100] == 7).all() and (room[T + 100:] == 7).all()
+    if same is None:
+        assert torch.equal(out, d[0])
+    elif same:
+        plain = [min(int(s * by), T) for s in same[:2]] + [T, T]
+        assert torch.equal(out, k.lora_add(*d, torch.tensor(plain, dtype=torch.int32, device=dev), scales=scales.to(dev)))
+        lora.check(dev, y, x, a, b, [0, 1, 0], plain, scales)
+
+
+@pytest.mark.parametrize("T", [1, 4, 20, 64])
+@pytest.mark.parametrize("which", [0, 3, 5])
+def test_e4m3_codes_of_no_number_stay_with_their_tokens(dev, T, which):
+    """In a token: its result alone; in an expert's weights: those of the tokens that it is run for."""
+    args = list(make(gen(T), T, 4, 64, 32, E4M3, torch.float32))
+    clean = check(dev, args, 2)
+    args[which] = args[which].clone()
+    if which == 0:
+        args[0].view(torch.uint8)[T // 2, 3] = 0x7f
+        odd = torch.arange(T) == T // 2
+    else:
+        args[which].view(torch.uint8)[1, 5, 7] = 0xff
+        odd = torch.tensor([1 in row for row in R.route(args[2], 2, True)[0]])
+    got = K().moe_few_tokens(*[t.to(dev) for t in args], 2, out_dtype=torch.float32).cpu()
+    assert torch.equal(got[~odd], clean.cpu()[~odd]) and got[odd].isnan().any(1).all()
