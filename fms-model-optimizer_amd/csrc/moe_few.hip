@@ -18,8 +18,9 @@
 namespace fmsmo {
 
 constexpr int MOE_TOKENS = 64, MOE_EXPERTS = 512, MOE_TOP = 16;
-constexpr int MOE_ROUTED = 8;  // tokens up to which every block of the gate and up products routes for itself (16 tokens over 128 experts: 80 us so, 72 with
-                               // a launch of its own; ten over 8 experts, small ones: 15.2 and 16.2)
+// Tokens up to which every block of the gate and up products routes for itself (16 tokens over 128 experts: 80 us so, 72 with a launch of its own).
+// The number of tokens alone decides, though over few experts ten tokens would gain yet (small ones, of 8: 15.2 us so, 16.2 with the launch).
+constexpr int MOE_ROUTED = 8;
 
 struct MoeArgs {
   const uint8_t* a;     // [T, K] codes

@@ -120,7 +120,7 @@ __device__ __forceinline__ uint2 codes8(const float (&n)[8], float s, float inve
   float q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    q[i] = given ? n[i] / s : quotient(n[i], s, inverse);  // (a given scale may have no reciprocal)
+    q[i] = given ? n[i] / s : quotient(n[i], s, inverse);  // (a given scale may have no reciprocal; 8192 tokens of 4096, int8: 40.9 us, 39.2 else)
     if (given) {
       constexpr float MOST = E4M3 ? 448.0f : 127.0f;
       q[i] = q[i] > MOST ? MOST : q[i] < -MOST ? -MOST : q[i];  // (a NaN stays)
@@ -156,7 +156,7 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
 }
 
 // NW waves a row, CH pieces of eight elements a lane, held in registers between the sum and the codes; a block of one-wave rows takes four.
-// CH = 0: rows longer than that, read three times.
+// CH = 0: rows longer than that, read three times, twice with a scale that is given (4096 tokens of 16392 118 us and 104, floor 96; of 16384 87).
 template <int T, int WT, bool E4M3, int NW, int CH>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void norm_quant_kernel(NormArgs a) {
   constexpr int NT = NW * 64, HELD = CH ? CH : 1;
