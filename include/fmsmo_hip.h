@@ -928,7 +928,7 @@ int64_t fmsmo_paged_attn_workspace_bytes(int q_heads, int heads, int dim, int ca
  * FMSMO_F32 and of fmsmo_quant_act_fp8_pertoken.  dtype FMSMO_F16 or FMSMO_BF16, weight_dtype the same or FMSMO_F32.  A row with a NaN
  * or an infinity: scale NaN, e4m3 codes NaN, int8 codes not specified; one whose sum of squares leaves fp32: n = 0.
  * M = 0 or K = 0: nothing is written.
- * K and leading dimensions multiples of 8, pointers 16-byte aligned (q: 8).
+ * K and leading dimensions multiples of 8, pointers 16-byte aligned (q: 8); M below 2^31, K up to 2^31 - 16.
  */
 int fmsmo_add_rms_norm_quant(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
                              int weight_dtype, float eps, int codes, int static_scale, void* q, int64_t ldq, float* scale,

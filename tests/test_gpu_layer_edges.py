@@ -177,3 +177,37 @@ def test_e4m3_codes_of_no_number_stay_with_their_tokens(dev, T, which):
         odd = torch.tensor([1 in row for row in R.route(args[2], 2, True)[0]])
     got = K().moe_few_tokens(*[t.to(dev) for t in args], 2, out_dtype=torch.float32).cpu()
     assert torch.equal(got[~odd], clean.cpu()[~odd]) and got[odd].isnan().any(1).all()
+
+
+def test_several_launches_captured(dev):
+    """Calls that are cut into several launches, replayed on new inputs with eager work and synchronizations between."""
+    k, T, M = K(), 9000, (1 << 21) + 9
+    g = torch.Generator(dev).manual_seed(4)
+
+    def fresh():
+        return (torch.empty(T, 64, device=dev, dtype=torch.float16).normal_(generator=g), torch.randint(-1, 3, (T,), device=dev, generator=g, dtype=torch.int32),
+                torch.empty(M, 8, device=dev, dtype=torch.float16).normal_(generator=g))
+
+    x, ids, rows = fresh()
+    y = torch.empty(T, 72, device=dev, dtype=torch.float16).normal_(generator=g)
+    a, b = (torch.empty(s, device=dev, dtype=torch.float16).normal_(generator=g) for s in ((3, 104, 64), (3, 72, 104)))
+    w = torch.ones(8, device=dev).half()
+
+    def call():
+        return k.lora_add(y, x, a, b, ids), *k.add_rms_norm_quant(rows, w, dtype=I8)[:2]
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        for t, new in zip((x, ids, rows), fresh()):
+            t.copy_(new)
+        want = [t.clone() for t in call()]
+        graph.replay()
+        torch.empty(1 << 20, device=dev).normal_()
+        if i % 2:
+            torch.cuda.synchronize()
+        for o, v in zip(out, want):
+            assert torch.equal(o, v)
